@@ -49,6 +49,30 @@ class DecoderLayer(ctypes.Structure):
                 ("moe", c_void_p), ("dense", c_void_p)]
 
 
+class RopeDesc(ctypes.Structure):
+    _fields_ = [("rot_dim", c_size_t), ("interleaved", c_int), ("scaling", c_int), ("freq_base", ctypes.c_double),
+                ("factor", ctypes.c_double), ("original_positions", ctypes.c_double),
+                ("low_rotations", ctypes.c_double), ("high_rotations", ctypes.c_double), ("magnitude", c_float)]
+
+
+class PagedSeqs(ctypes.Structure):
+    _fields_ = [("n_seqs", c_size_t), ("max_pages", c_size_t), ("table_stride", c_size_t), ("page_table", c_void_p),
+                ("lens", c_void_p)]
+
+
+class PagedTokens(ctypes.Structure):
+    _fields_ = [("n_tokens", c_size_t), ("dtype", c_uint32), ("k", c_void_p), ("v", c_void_p), ("k_stride", c_size_t),
+                ("v_stride", c_size_t), ("q", c_void_p), ("q_out", c_void_p), ("n_heads", c_size_t),
+                ("q_stride", c_size_t), ("q_out_stride", c_size_t), ("q_norm", c_void_p), ("k_norm", c_void_p),
+                ("eps", c_float), ("pos", c_void_p), ("seq_start", c_void_p)]
+
+
+class PagedQuery(ctypes.Structure):
+    _fields_ = [("dtype", c_uint32), ("q", c_void_p), ("out", c_void_p), ("n_heads", c_size_t),
+                ("q_stride", c_size_t), ("out_stride", c_size_t), ("scale", c_float), ("window", c_size_t),
+                ("lse", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
 class GgufTensorInfo(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char_p), ("n_dims", c_uint32), ("dims", P(ctypes.c_uint64)),
                 ("ggml_type", c_uint32), ("offset", ctypes.c_uint64), ("data_start", ctypes.c_uint64),
@@ -124,6 +148,18 @@ _SIGS = {
     "bb_model_run_layers": (c_int, [c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p, c_int]),
     "bb_model_forward_step": (c_int, [c_void_p, c_void_p, c_uint32, c_void_p, c_void_p, c_int]),
     "bb_model_absorb": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_size_t]),
+    "bb_rope_plan_create": (c_int, [c_void_p, P(RopeDesc), P(c_void_p)]),
+    "bb_rope_plan_destroy": (c_int, [c_void_p]),
+    "bb_rope": (c_int, [c_void_p, c_void_p, c_uint32, c_void_p, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t,
+                        c_void_p, c_void_p, c_size_t, c_size_t, c_int]),
+    "bb_paged_kv_create": (c_int, [c_void_p, c_uint32, c_size_t, c_size_t, c_size_t, c_size_t, P(c_void_p)]),
+    "bb_paged_kv_view": (c_int, [c_void_p, c_uint32, c_void_p, c_void_p, c_size_t, c_size_t, c_size_t, c_size_t,
+                                 c_size_t, c_size_t, c_size_t, P(c_void_p)]),
+    "bb_paged_kv_destroy": (c_int, [c_void_p]),
+    "bb_paged_kv_pages": (c_int, [c_void_p, P(c_void_p), P(c_void_p)]),
+    "bb_paged_append": (c_int, [c_void_p, c_void_p, c_void_p, P(PagedSeqs), P(PagedTokens), c_int]),
+    "bb_paged_attention_workspace": (c_int, [c_void_p, c_void_p, c_size_t, c_size_t, P(c_size_t)]),
+    "bb_paged_attention": (c_int, [c_void_p, c_void_p, P(PagedSeqs), P(PagedQuery), c_int]),
     "bb_gguf_open": (c_int, [ctypes.c_char_p, P(c_void_p)]),
     "bb_gguf_open_bytes": (c_int, [c_void_p, c_size_t, P(c_void_p)]),
     "bb_gguf_close": (c_int, [c_void_p]),

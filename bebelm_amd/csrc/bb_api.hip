@@ -917,6 +917,22 @@ struct bb_cache {
   size_t pos = 0;
 };
 
+struct bb_rope_plan {
+  bb_ctx* ctx;
+  int device;
+  size_t rot_dim;
+  bb::RopeTurns turns;
+  double* dev;
+};
+
+struct bb_paged_kv {
+  bb_ctx* ctx;
+  int device;
+  uint32_t dtype;
+  bb::PagedView view;
+  uint8_t* own = nullptr;  // the pool, when the library allocated it
+};
+
 void bb::free_owned(bb::ModelOwned& o) {
   for (bb_conv_op* p : o.conv) (void)bb_conv_op_destroy(p);
   for (bb_attn_op* p : o.attn) (void)bb_attn_op_destroy(p);
@@ -2539,6 +2555,455 @@ int bb_model_absorb(bb_ctx* c, bb_model* m, bb_cache* k, const uint32_t* tokens,
       }
     }
     check_hip(hipStreamSynchronize(c->stream), "hipStreamSynchronize");
+  });
+}
+
+}  // extern "C"
+
+// ---- paged cache (bb_paged.hip) ------------------------------------------------------------------
+namespace {
+
+constexpr size_t PAGED_SEQS_MAX = 65536;
+constexpr size_t STRIDE_MAX = (size_t)1 << 40;  // elements; with counts below 2^20 no product passes 64 bits
+
+// Bytes of an element of the paged operators' types.
+size_t elem_bytes(uint32_t dt, const char* what) {
+  if (dt == BB_F32) return 4;
+  if (dt == BB_F16 || dt == BB_BF16) return 2;
+  fail(BB_ERR_DTYPE, std::string(what) + ": dtype must be F32, F16 or BF16");
+}
+
+bool capturing(bb_ctx* c) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  check_hip(hipStreamIsCapturing(c->stream, &st), "hipStreamIsCapturing");
+  return st != hipStreamCaptureStatusNone;
+}
+
+// The launch wrapper for calls that may be captured: a captured launch is not timed.
+template <class F>
+void launch_paged(bb_ctx* c, bool captured, int id, F&& f) {
+  if (captured) check_hip(f(), bb::kernel_name(id));
+  else launch(c, id, f);
+}
+
+// Bytes from the first to past the last element of n rows of `row` elements `stride` apart.
+size_t span_bytes(size_t n, size_t stride, size_t row, size_t elem) {
+  return n == 0 ? 0 : ((n - 1) * stride + row) * elem;
+}
+
+bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return na > 0 && nb > 0 && x < y + nb && y < x + na;
+}
+
+void need_out_apart(const void* x, size_t nx, const void* out, size_t nout, bool same_layout, const char* what) {
+  if (x == out && same_layout) return;
+  need(!overlap(x, nx, out, nout), BB_ERR_ARG, std::string(what) + " overlaps its input");
+}
+
+void need_plan(const bb_ctx* c, const bb_rope_plan* p, size_t head_dim) {
+  need(p->device == c->device, BB_ERR_ARG, "the rotary plan is of another device");
+  need(p->rot_dim <= head_dim, BB_ERR_SHAPE, "rot_dim exceeds head_dim");
+}
+
+// The page table and lengths of a batch, checked; with BB_LOC_HOST what they hold too, the pages from
+// the one of position first(s, length) on.
+template <class F>
+void need_seqs(const bb_paged_kv* kv, const bb_paged_seqs* q, int loc, F&& first) {
+  need(q->n_seqs <= PAGED_SEQS_MAX, BB_ERR_RANGE, "more than 65536 sequences");
+  need(q->max_pages >= 1 && q->max_pages * (size_t)kv->view.page_size < ((size_t)1 << 31) && q->max_pages < ((size_t)1 << 31),
+       BB_ERR_RANGE, "max_pages * page_size must be below 2^31");
+  need(q->table_stride >= q->max_pages && q->table_stride < STRIDE_MAX, BB_ERR_ARG, "table_stride below max_pages");
+  if (q->n_seqs == 0) return;
+  need(q->page_table && q->lens, BB_ERR_ARG, "null page table or lengths");
+  if (loc != BB_LOC_HOST) return;
+  const size_t ps = (size_t)kv->view.page_size;
+  for (size_t s = 0; s < q->n_seqs; ++s) {
+    const int64_t n = q->lens[s];
+    need(n >= 0 && (size_t)n <= q->max_pages * ps, BB_ERR_RANGE,
+         "sequence " + std::to_string(s) + ": length " + std::to_string(n) + " is not in its pages");
+    for (size_t i = (size_t)first(s, n) / ps; i < ((size_t)n + ps - 1) / ps; ++i) {
+      const int32_t pg = q->page_table[s * q->table_stride + i];
+      need(pg >= 0 && pg < kv->view.n_pages, BB_ERR_RANGE,
+           "sequence " + std::to_string(s) + ": page " + std::to_string(pg) + " is not in the pool");
+    }
+  }
+}
+
+bb::PagedSeqs seqs_of(const bb_paged_seqs* q, const void* table, const void* lens) {
+  return {static_cast<const int32_t*>(table), static_cast<const int32_t*>(lens), q->table_stride, (int)q->n_seqs,
+          (int)q->max_pages};
+}
+
+void need_pool(const bb_ctx* c, const bb_paged_kv* kv) {
+  need(kv != nullptr, BB_ERR_ARG, "null paged cache");
+  need(kv->device == c->device, BB_ERR_ARG, "the paged cache is of another device");
+}
+
+bb_paged_kv* new_pool(bb_ctx* c, uint32_t dtype, void* k, void* v, size_t n_pages, size_t page_size, size_t n_kv,
+                      size_t hd, size_t page_stride, size_t pos_stride, size_t head_stride, uint8_t* own) {
+  auto* p = new bb_paged_kv();
+  p->ctx = c;
+  p->device = c->device;
+  p->dtype = dtype;
+  p->view = {k, v, page_stride, pos_stride, head_stride, (int)n_pages, (int)page_size, (int)n_kv, (int)hd};
+  p->own = own;
+  return p;
+}
+
+void need_pool_sizes(size_t n_pages, size_t page_size, size_t n_kv, size_t hd) {
+  need(n_pages >= 1 && page_size >= 1 && n_kv >= 1 && hd >= 1, BB_ERR_ARG, "sizes must be >= 1");
+  need(hd % 8 == 0 && hd <= (size_t)bb::OPS_HD_MAX, BB_ERR_SHAPE, "head_dim must be a multiple of 8, at most 256");
+  need(n_pages < ((size_t)1 << 31) && page_size < ((size_t)1 << 20) && n_kv <= 4096, BB_ERR_RANGE,
+       "pool sizes beyond 2^31 pages, 2^20 positions a page or 4096 heads");
+}
+
+size_t paged_ws(bb_ctx* c, const bb_paged_kv* kv, size_t n_heads, size_t n_seqs) {
+  need(n_heads >= 1 && n_heads % (size_t)kv->view.n_kv == 0, BB_ERR_ARG, "n_heads must be a multiple of n_kv_heads");
+  need(n_heads < ((size_t)1 << 16), BB_ERR_RANGE, "n_heads must be below 65536");
+  need(n_seqs <= PAGED_SEQS_MAX, BB_ERR_RANGE, "more than 65536 sequences");
+  return bb::paged_attn_ws(c->n_cu, (int)n_seqs, (int)n_heads, kv->view.n_kv, kv->view.hd);
+}
+
+}  // namespace
+
+extern "C" {
+
+int bb_rope_plan_create(bb_ctx* c, const bb_rope_desc* d, bb_rope_plan** out) {
+  return guard([&] {
+    need_ctx(c);
+    need(d && out, BB_ERR_ARG, "null argument");
+    const size_t rot = d->rot_dim;
+    need(rot >= 2 && rot % 2 == 0 && rot <= (size_t)bb::OPS_HD_MAX, BB_ERR_SHAPE, "rot_dim must be even and in 2..256");
+    need(d->scaling >= BB_ROPE_NONE && d->scaling <= BB_ROPE_PARTS, BB_ERR_ARG, "unknown rotary scaling");
+    need(std::isfinite(d->freq_base) && d->freq_base > 0, BB_ERR_ARG, "freq_base must be positive");
+    need(std::isfinite(d->magnitude), BB_ERR_ARG, "magnitude must be finite");
+    const bool scaled = d->scaling != BB_ROPE_NONE;
+    if (scaled) need(std::isfinite(d->factor) && d->factor > 0, BB_ERR_ARG, "factor must be positive");
+    if (d->scaling == BB_ROPE_BASE) need(rot >= 4, BB_ERR_SHAPE, "BB_ROPE_BASE needs rot_dim >= 4");
+    if (d->scaling == BB_ROPE_PARTS)
+      need(std::isfinite(d->original_positions) && d->original_positions > 0 && std::isfinite(d->low_rotations) &&
+               std::isfinite(d->high_rotations) && d->low_rotations < d->high_rotations,
+           BB_ERR_ARG, "BB_ROPE_PARTS needs original_positions > 0 and low_rotations < high_rotations");
+    const double two_pi = 6.283185307179586476925286766559;
+    double log_base = std::log(d->freq_base);
+    if (d->scaling == BB_ROPE_BASE) log_base += std::log(d->factor) * ((double)rot / (double)(rot - 2));
+    std::vector<double> turns(rot / 2);
+    for (size_t i = 0; i < rot / 2; ++i) {
+      double f = std::exp(-2.0 * (double)i / (double)rot * log_base);
+      if (d->scaling == BB_ROPE_LINEAR) f /= d->factor;
+      if (d->scaling == BB_ROPE_PARTS) {
+        const double g = std::min(1.0, std::max(0.0, (d->original_positions * f / two_pi - d->low_rotations) /
+                                                         (d->high_rotations - d->low_rotations)));
+        f *= g + (1.0 - g) / d->factor;
+      }
+      turns[i] = f / two_pi;
+      // (2^31 positions times the turns must leave the f64 reduction a finite value)
+      need(std::isfinite(turns[i]) && turns[i] < 1e18, BB_ERR_RANGE, "a frequency is out of range");
+    }
+    set_device(c);
+    auto* dev = static_cast<double*>(dev_alloc(turns.size() * sizeof(double)));
+    try {
+      copy_to_dev(c, dev, turns.data(), turns.size() * sizeof(double), "rotary frequencies upload");
+      auto* p = new bb_rope_plan();
+      p->ctx = c;
+      p->device = c->device;
+      p->rot_dim = rot;
+      p->dev = dev;
+      p->turns.turns = dev;
+      p->turns.half = (int)(rot / 2);
+      p->turns.interleaved = d->interleaved != 0;
+      p->turns.magnitude = d->magnitude;
+      *out = p;
+    } catch (...) {
+      (void)hipFree(dev);
+      throw;
+    }
+  });
+}
+
+int bb_rope_plan_destroy(bb_rope_plan* p) {
+  return guard([&] {
+    if (!p) return;
+    check_hip(hipSetDevice(p->device), "hipSetDevice");
+    (void)hipFree(p->dev);
+    delete p;
+  });
+}
+
+int bb_rope(bb_ctx* c, const bb_rope_plan* plan, uint32_t dtype, const void* x, size_t token_stride, size_t head_stride,
+            size_t n_tokens, size_t n_heads, size_t head_dim, const int32_t* pos, void* out, size_t out_token_stride,
+            size_t out_head_stride, int loc) {
+  return guard([&] {
+    need_ctx(c);
+    need_loc(loc);
+    need(plan != nullptr, BB_ERR_ARG, "null rotary plan");
+    const size_t eb = elem_bytes(dtype, "x");
+    need(head_dim >= 1 && head_dim <= (size_t)bb::OPS_HD_MAX, BB_ERR_SHAPE, "head_dim must be in 1..256");
+    need_plan(c, plan, head_dim);
+    need(n_heads >= 1 && n_heads < ((size_t)1 << 16), BB_ERR_RANGE, "n_heads must be in 1..65535");
+    need(n_tokens < ((size_t)1 << 22), BB_ERR_RANGE, "n_tokens must be below 2^22");
+    if (n_tokens == 0) return;
+    need(x && pos && out, BB_ERR_ARG, "null argument");
+    for (const size_t st : {token_stride, head_stride, out_token_stride, out_head_stride})
+      need(st < STRIDE_MAX, BB_ERR_RANGE, "stride beyond 2^40 elements");
+    // every element of out has a place of its own: the smaller stride holds a head vector, the larger one all of
+    // the smaller's
+    const bool tok_major = out_token_stride >= out_head_stride;
+    const size_t lo = tok_major ? out_head_stride : out_token_stride, n_lo = tok_major ? n_heads : n_tokens;
+    const size_t hi = tok_major ? out_token_stride : out_head_stride, n_hi = tok_major ? n_tokens : n_heads;
+    need((n_lo == 1 || lo >= head_dim) && (n_hi == 1 || hi >= (n_lo - 1) * (n_lo == 1 ? 0 : lo) + head_dim), BB_ERR_ARG,
+         "out's strides put two elements in one place");
+    const size_t nx = ((n_tokens - 1) * token_stride + (n_heads - 1) * head_stride + head_dim) * eb;
+    const size_t no = ((n_tokens - 1) * out_token_stride + (n_heads - 1) * out_head_stride + head_dim) * eb;
+    need_out_apart(x, nx, out, no,
+                   (n_tokens == 1 || token_stride == out_token_stride) && (n_heads == 1 || head_stride == out_head_stride),
+                   "out");
+    set_device(c);
+    const bool cap = capturing(c);
+    need(!(cap && loc == BB_LOC_HOST), BB_ERR_ARG, "a call on host memory cannot be captured");
+    // (host memory: out's span goes in too, what lies between its rows stays as it is)
+    with_io(c, loc, {{x, nx, true, false}, {pos, n_tokens * 4, true, false}, {out, no, true, true}},
+            [&](std::vector<void*>& d) {
+              bb::RopeRows r{};
+              r.T = n_tokens;
+              r.hd = (int)head_dim;
+              r.n_q = (int)n_heads;
+              r.q = d[0];
+              r.q_ts = token_stride;
+              r.q_hs = head_stride;
+              r.pos = static_cast<const int32_t*>(d[1]);
+              r.q_out = d[2];
+              r.qo_ts = out_token_stride;
+              r.qo_hs = out_head_stride;
+              launch_paged(c, cap, bb::K_ROPE, [&] {
+                return bb::launch_rope_rows(c->stream, (int)dtype, 0, r, plan->turns, bb::PagedView{}, bb::PagedSeqs{});
+              });
+            });
+  });
+}
+
+int bb_paged_kv_create(bb_ctx* c, uint32_t dtype, size_t n_pages, size_t page_size, size_t n_kv_heads, size_t head_dim,
+                       bb_paged_kv** out) {
+  return guard([&] {
+    need_ctx(c);
+    need(out != nullptr, BB_ERR_ARG, "out is null");
+    const size_t eb = elem_bytes(dtype, "pool");
+    need_pool_sizes(n_pages, page_size, n_kv_heads, head_dim);
+    const size_t page = page_size * n_kv_heads * head_dim;
+    need(n_pages * (page >> 10) < ((size_t)1 << 40), BB_ERR_RANGE, "pool too large");  // (below 2^61)
+    const size_t half = round_up(n_pages * page * eb, 256);
+    set_device(c);
+    auto* dev = static_cast<uint8_t*>(dev_alloc(2 * half));
+    try {
+      clear_dev(c, dev, 2 * half);
+      *out = new_pool(c, dtype, dev, dev + half, n_pages, page_size, n_kv_heads, head_dim, page, n_kv_heads * head_dim,
+                      head_dim, dev);
+    } catch (...) {
+      (void)hipFree(dev);
+      throw;
+    }
+  });
+}
+
+int bb_paged_kv_view(bb_ctx* c, uint32_t dtype, void* k, void* v, size_t n_pages, size_t page_size, size_t n_kv_heads,
+                     size_t head_dim, size_t page_stride, size_t pos_stride, size_t head_stride, bb_paged_kv** out) {
+  return guard([&] {
+    need_ctx(c);
+    need(out != nullptr, BB_ERR_ARG, "out is null");
+    const size_t eb = elem_bytes(dtype, "pool");
+    need_pool_sizes(n_pages, page_size, n_kv_heads, head_dim);
+    need_aligned(k, "keys");
+    need_aligned(v, "values");
+    need(k != v, BB_ERR_ARG, "keys and values must not be the same memory");
+    std::pair<size_t, size_t> dims[3] = {{page_stride, n_pages}, {pos_stride, page_size}, {head_stride, n_kv_heads}};
+    for (auto& d : dims) {
+      if (d.second == 1) d.first = 0;  // never stepped
+      need(d.first < STRIDE_MAX, BB_ERR_RANGE, "stride beyond 2^40 elements");
+      need(d.first * eb % 16 == 0, BB_ERR_ARG, "strides must be whole 16-byte pieces");
+    }
+    std::sort(dims, dims + 3);
+    size_t span = head_dim;
+    for (const auto& d : dims) {
+      if (d.second == 1) continue;
+      need(d.first >= span, BB_ERR_ARG, "strides put two elements in one place");
+      need(d.second - 1 < ((size_t)1 << 62) / d.first, BB_ERR_RANGE, "pool too large");
+      span += (d.second - 1) * d.first;
+    }
+    *out = new_pool(c, dtype, k, v, n_pages, page_size, n_kv_heads, head_dim, page_stride, pos_stride, head_stride,
+                    nullptr);
+  });
+}
+
+int bb_paged_kv_destroy(bb_paged_kv* kv) {
+  return guard([&] {
+    if (!kv) return;
+    if (kv->own) {
+      check_hip(hipSetDevice(kv->device), "hipSetDevice");
+      (void)hipFree(kv->own);
+    }
+    delete kv;
+  });
+}
+
+int bb_paged_kv_pages(const bb_paged_kv* kv, void** k, void** v) {
+  return guard([&] {
+    need(kv && k && v, BB_ERR_ARG, "null argument");
+    *k = kv->view.k;
+    *v = kv->view.v;
+  });
+}
+
+int bb_paged_append(bb_ctx* c, bb_paged_kv* kv, const bb_rope_plan* plan, const bb_paged_seqs* sq,
+                    const bb_paged_tokens* tk, int loc) {
+  return guard([&] {
+    need_ctx(c);
+    need_loc(loc);
+    need_pool(c, kv);
+    need(sq && tk, BB_ERR_ARG, "null argument");
+    const size_t T = tk->n_tokens, B = sq->n_seqs, hd = (size_t)kv->view.hd, row = (size_t)kv->view.n_kv * hd;
+    const size_t eb = elem_bytes(tk->dtype, "tokens");
+    need(T < ((size_t)1 << 22), BB_ERR_RANGE, "n_tokens must be below 2^22");
+    if (loc == BB_LOC_HOST && tk->seq_start && B > 0) {
+      need(B <= PAGED_SEQS_MAX, BB_ERR_RANGE, "more than 65536 sequences");
+      need(tk->seq_start[0] == 0, BB_ERR_RANGE, "seq_start must start at 0");
+      for (size_t s = 0; s < B; ++s)
+        need(tk->seq_start[s + 1] >= tk->seq_start[s] && (size_t)tk->seq_start[s + 1] <= T, BB_ERR_RANGE,
+             "seq_start must ascend, up to n_tokens");
+    }
+    need_seqs(kv, sq, loc, [&](size_t s, int64_t n) {
+      const int64_t bring = tk->seq_start ? tk->seq_start[s + 1] - tk->seq_start[s] : std::min<int64_t>(n, 1);
+      need(bring <= n, BB_ERR_RANGE, "a sequence is shorter than its tokens");
+      return n - bring;
+    });
+    if (plan) need_plan(c, plan, hd);
+    if (!tk->seq_start) need(T == B, BB_ERR_SHAPE, "without seq_start every sequence has one token");
+    if (T == 0 || B == 0) return;
+    need(tk->k && tk->v, BB_ERR_ARG, "null keys or values");
+    need(T == 1 || (tk->k_stride >= row && tk->v_stride >= row), BB_ERR_ARG, "k_stride or v_stride below a token's row");
+    need(tk->k_stride < STRIDE_MAX && tk->v_stride < STRIDE_MAX, BB_ERR_RANGE, "stride beyond 2^40 elements");
+    const size_t nk = span_bytes(T, tk->k_stride, row, eb), nv = span_bytes(T, tk->v_stride, row, eb);
+    size_t nq = 0, nqo = 0;
+    if (tk->q) {
+      need(tk->q_out != nullptr, BB_ERR_ARG, "q without q_out");
+      need(tk->n_heads >= 1 && tk->n_heads < ((size_t)1 << 16), BB_ERR_RANGE, "n_heads must be in 1..65535");
+      const size_t qr = tk->n_heads * hd;
+      need(T == 1 || (tk->q_stride >= qr && tk->q_out_stride >= qr), BB_ERR_ARG, "q_stride or q_out_stride below a token's row");
+      need(tk->q_stride < STRIDE_MAX && tk->q_out_stride < STRIDE_MAX, BB_ERR_RANGE, "stride beyond 2^40 elements");
+      nq = span_bytes(T, tk->q_stride, qr, eb);
+      nqo = span_bytes(T, tk->q_out_stride, qr, eb);
+      need_out_apart(tk->q, nq, tk->q_out, nqo, T == 1 || tk->q_stride == tk->q_out_stride, "q_out");
+      need(!overlap(tk->k, nk, tk->q_out, nqo) && !overlap(tk->v, nv, tk->q_out, nqo), BB_ERR_ARG,
+           "q_out overlaps the keys or values");
+    } else {
+      need(!tk->q_norm && !tk->q_out, BB_ERR_ARG, "q_norm or q_out without q");
+    }
+    if (tk->q_norm || tk->k_norm) need(tk->eps >= 0.0f && std::isfinite(tk->eps), BB_ERR_ARG, "eps must not be negative");
+    set_device(c);
+    const bool cap = capturing(c);
+    need(!(cap && loc == BB_LOC_HOST), BB_ERR_ARG, "a call on host memory cannot be captured");
+    const size_t nt = span_bytes(B, sq->table_stride, sq->max_pages, 4);
+    with_io(c, loc,
+            {{sq->page_table, nt, true, false},
+             {sq->lens, B * 4, true, false},
+             {tk->k, nk, true, false},
+             {tk->v, nv, true, false},
+             {tk->q, nq, true, false},
+             {tk->q_out, nqo, true, true},
+             {tk->q_norm, tk->q_norm ? hd * 4 : 0, true, false},
+             {tk->k_norm, tk->k_norm ? hd * 4 : 0, true, false},
+             {tk->pos, tk->pos ? T * 4 : 0, true, false},
+             {tk->seq_start, tk->seq_start ? (B + 1) * 4 : 0, true, false}},
+            [&](std::vector<void*>& d) {
+              bb::RopeRows r{};
+              r.T = T;
+              r.hd = (int)hd;
+              r.n_q = tk->q ? (int)tk->n_heads : 0;
+              r.n_kv = kv->view.n_kv;
+              r.k = d[2];
+              r.v = d[3];
+              r.k_ts = tk->k_stride;
+              r.v_ts = tk->v_stride;
+              r.q = tk->q ? d[4] : nullptr;
+              r.q_out = tk->q ? d[5] : nullptr;
+              r.q_ts = tk->q_stride;
+              r.qo_ts = tk->q_out_stride;
+              r.q_hs = r.qo_hs = hd;
+              r.q_norm = tk->q_norm ? static_cast<const float*>(d[6]) : nullptr;
+              r.k_norm = tk->k_norm ? static_cast<const float*>(d[7]) : nullptr;
+              r.eps = tk->eps;
+              r.pos = tk->pos ? static_cast<const int32_t*>(d[8]) : nullptr;
+              r.seq_start = tk->seq_start ? static_cast<const int32_t*>(d[9]) : nullptr;
+              launch_paged(c, cap, bb::K_PAGED_APPEND, [&] {
+                return bb::launch_rope_rows(c->stream, (int)tk->dtype, (int)kv->dtype, r,
+                                            plan ? plan->turns : bb::RopeTurns{}, kv->view, seqs_of(sq, d[0], d[1]));
+              });
+            });
+  });
+}
+
+int bb_paged_attention_workspace(bb_ctx* c, const bb_paged_kv* kv, size_t n_heads, size_t n_seqs, size_t* bytes) {
+  return guard([&] {
+    need_ctx(c);
+    need_pool(c, kv);
+    need(bytes != nullptr, BB_ERR_ARG, "bytes is null");
+    *bytes = paged_ws(c, kv, n_heads, n_seqs);
+  });
+}
+
+int bb_paged_attention(bb_ctx* c, const bb_paged_kv* kv, const bb_paged_seqs* sq, const bb_paged_query* pq, int loc) {
+  return guard([&] {
+    need_ctx(c);
+    need_loc(loc);
+    need_pool(c, kv);
+    need(sq && pq, BB_ERR_ARG, "null argument");
+    const size_t B = sq->n_seqs, hd = (size_t)kv->view.hd, nh = pq->n_heads, row = nh * hd;
+    const size_t eb = elem_bytes(pq->dtype, "query");
+    const size_t want = paged_ws(c, kv, nh, B);
+    need_seqs(kv, sq, loc, [&](size_t, int64_t n) {
+      return pq->window > 0 && pq->window < (size_t)n ? n - (int64_t)pq->window : 0;
+    });
+    need(std::isfinite(pq->scale), BB_ERR_ARG, "scale must be finite");
+    if (B == 0) return;
+    need(pq->q && pq->out, BB_ERR_ARG, "null query or output");
+    need(B == 1 || (pq->q_stride >= row && pq->out_stride >= row), BB_ERR_ARG, "q_stride or out_stride below a sequence's row");
+    need(pq->q_stride < STRIDE_MAX && pq->out_stride < STRIDE_MAX, BB_ERR_RANGE, "stride beyond 2^40 elements");
+    const size_t nq = span_bytes(B, pq->q_stride, row, eb), no = span_bytes(B, pq->out_stride, row, eb);
+    need(!overlap(pq->q, nq, pq->out, no), BB_ERR_ARG, "out overlaps the query");
+    const size_t nl = pq->lse ? B * nh * 4 : 0;
+    need(!overlap(pq->lse, nl, pq->out, no) && !overlap(pq->lse, nl, pq->q, nq), BB_ERR_ARG, "lse overlaps the query or out");
+    set_device(c);
+    const bool cap = capturing(c);
+    need(!(cap && loc == BB_LOC_HOST), BB_ERR_ARG, "a call on host memory cannot be captured");
+    if (pq->workspace) {
+      need_aligned(pq->workspace, "workspace");
+      need(pq->workspace_bytes >= want, BB_ERR_RANGE, "workspace smaller than bb_paged_attention_workspace's answer");
+    } else {
+      need(!cap, BB_ERR_ARG, "a captured call needs a workspace of its own");
+    }
+    const size_t nt = span_bytes(B, sq->table_stride, sq->max_pages, 4);
+    with_io(c, loc,
+            {{sq->page_table, nt, true, false},
+             {sq->lens, B * 4, true, false},
+             {pq->q, nq, true, false},
+             {pq->out, no, true, true},
+             {pq->lse, nl, false, true}},
+            [&](std::vector<void*>& d) {
+              bb::PagedQuery q{};
+              q.q = d[2];
+              q.out = d[3];
+              q.q_stride = pq->q_stride;
+              q.out_stride = pq->out_stride;
+              q.n_heads = (int)nh;
+              q.window = pq->window < ((size_t)1 << 31) ? (int)pq->window : 0;  // (lengths are below 2^31)
+              q.scale = pq->scale != 0.0f ? pq->scale : 1.0f / std::sqrt((float)hd);
+              q.lse = nl ? static_cast<float*>(d[4]) : nullptr;
+              q.ws = pq->workspace ? pq->workspace : ensure_ws(c, want);
+              launch_paged(c, cap, bb::K_PAGED_ATTN, [&] {
+                return bb::launch_paged_attn(c->stream, c->n_cu, (int)pq->dtype, (int)kv->dtype, q, kv->view,
+                                             seqs_of(sq, d[0], d[1]));
+              });
+            });
   });
 }
 

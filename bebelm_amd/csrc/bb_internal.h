@@ -95,6 +95,9 @@ enum KernelId : int {
   K_ATTN_PV,
   K_SOFTMAX,
   K_EMBED,
+  K_ROPE,
+  K_PAGED_APPEND,
+  K_PAGED_ATTN,
   K_COUNT
 };
 const char* kernel_name(int id);
@@ -359,6 +362,54 @@ hipError_t launch_zero(hipStream_t s, float* x, size_t n);
 // out [T][H] = rows tokens[t] (device) of an embedding table in F32 / F16 / Q4_K / Q6_K rows.
 hipError_t launch_embed(hipStream_t s, const uint8_t* te, int dtype, size_t row_bytes, const uint32_t* tokens, int T,
                         int H, float* out);
+
+// ---- paged cache (bb_paged.hip) ----
+// A pool: element (page, position, head, d) of keys and values at page·page_stride + position·pos_stride
+// + head·head_stride + d.
+struct PagedView {
+  void *k, *v;
+  size_t page_stride, pos_stride, head_stride;
+  int n_pages, page_size, n_kv, hd;
+};
+// The sequences of a batch (lens null: none, rows are only turned).
+struct PagedSeqs {
+  const int32_t *table, *lens;
+  size_t table_stride;
+  int n_seqs, max_pages;
+};
+// Frequencies of a rotation: f_i / 2pi (turns per position) of half pairs.
+struct RopeTurns {
+  const double* turns = nullptr;
+  int half = 0;
+  int interleaved = 0;
+  float magnitude = 1.0f;
+};
+// Rows of tokens: n_q query heads (q to q_out) and n_kv key and value heads (to the pool) each.
+struct RopeRows {
+  size_t T;
+  int hd, n_q, n_kv;
+  const void *q, *k, *v;
+  void* q_out;
+  size_t q_ts, q_hs, qo_ts, qo_hs, k_ts, v_ts;
+  const float *q_norm, *k_norm;
+  float eps;
+  const int32_t *pos, *seq_start;
+};
+// dtype of q, k, v and q_out; cache: the pool's dtype (n_kv > 0).
+hipError_t launch_rope_rows(hipStream_t s, int dtype, int cache, const RopeRows& r, const RopeTurns& t,
+                            const PagedView& kv, const PagedSeqs& seqs);
+struct PagedQuery {
+  const void* q;
+  void* out;
+  size_t q_stride, out_stride;
+  int n_heads, window;
+  float scale;
+  float* lse;
+  void* ws;
+};
+size_t paged_attn_ws(int n_cu, int n_seqs, int n_heads, int n_kv, int hd);
+hipError_t launch_paged_attn(hipStream_t s, int n_cu, int dtype, int cache, const PagedQuery& q, const PagedView& kv,
+                             const PagedSeqs& seqs);
 
 }  // namespace bb
 #endif

@@ -316,6 +316,109 @@ class KvCache:
             self.handle = None
 
 
+F32, F16, BF16 = 0, 1, 30  # element types of the paged-cache operators
+_DTYPES = {"float32": F32, "float16": F16, "bfloat16": BF16}
+
+
+def _dtype(a):
+    """The type code of an array's elements."""
+    code = _DTYPES.get(str(a.dtype).replace("torch.", ""))
+    if code is None:
+        raise ValueError(f"elements must be float32, float16 or bfloat16, not {a.dtype}")
+    return code
+
+
+def _on(ctx, *arrays):
+    """The torch tensors among the arrays are in host memory or on the context's GPU."""
+    for a in arrays:
+        if a is not None and getattr(a, "is_cuda", False) and a.device.index != ctx.device:
+            raise ValueError(f"tensor on {a.device}, context on GPU {ctx.device}")
+
+
+class RopePlan:
+    """The frequencies of a rotary position rule in device memory (bb_rope_plan): made once, used by
+    any number of kernels.rope and kernels.paged_append calls on the context's GPU."""
+
+    SCALINGS = ("none", "linear", "base", "parts")
+
+    def __init__(self, ctx, rot_dim, freq_base, interleaved=False, scaling="none", factor=1.0, original_positions=0.0,
+                 low_rotations=1.0, high_rotations=32.0, magnitude=1.0):
+        if scaling not in self.SCALINGS:
+            raise ValueError(f"scaling must be one of {self.SCALINGS}")
+        self.ctx, self.rot_dim, self.handle = ctx, rot_dim, None
+        d = _lib.RopeDesc(rot_dim, int(bool(interleaved)), self.SCALINGS.index(scaling), freq_base, factor,
+                          original_positions, low_rotations, high_rotations, magnitude)
+        h = ctypes.c_void_p()
+        check(lib().bb_rope_plan_create(ctx.handle, ctypes.byref(d), ctypes.byref(h)))
+        self.handle = h
+
+    def close(self):
+        if self.handle:
+            check(lib().bb_rope_plan_destroy(self.handle))
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class PagedKv:
+    """A pool of pages of keys and values (bb_paged_kv) over two torch CUDA tensors of one shape and
+    strides, [n_pages, page_size, n_kv_heads, head_dim] with adjacent elements of a head (a permuted
+    view of another order will do). The tensors are kept; whoever holds them sees what is stored."""
+
+    def __init__(self, ctx, k, v):
+        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
+            raise ValueError("keys and values must be of one type, shape [pages, positions, heads, head_dim] and strides")
+        if not (k.is_cuda and v.is_cuda):
+            raise ValueError("the pool must be in device memory")
+        if k.stride(3) != 1 and k.shape[3] > 1:
+            raise ValueError("the elements of a head must be adjacent")
+        _on(ctx, k, v)
+        self.ctx, self.k, self.v, self.handle = ctx, k, v, None
+        self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = k.shape
+        h = ctypes.c_void_p()
+        check(lib().bb_paged_kv_view(ctx.handle, _dtype(k), k.data_ptr(), v.data_ptr(), *k.shape, *k.stride()[:3],
+                                     ctypes.byref(h)))
+        self.handle = h
+
+    @classmethod
+    def create(cls, ctx, dtype, n_pages, page_size, n_kv_heads, head_dim):
+        """A pool in device memory of the library's (dtype F32, F16 or BF16), zeroed; k and v are None."""
+        self = cls.__new__(cls)
+        self.ctx, self.k, self.v, self.handle = ctx, None, None, None
+        self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = n_pages, page_size, n_kv_heads, head_dim
+        h = ctypes.c_void_p()
+        check(lib().bb_paged_kv_create(ctx.handle, dtype, n_pages, page_size, n_kv_heads, head_dim, ctypes.byref(h)))
+        self.handle = h
+        return self
+
+    def pages(self):
+        """The device addresses of the keys and the values."""
+        k, v = ctypes.c_void_p(), ctypes.c_void_p()
+        check(lib().bb_paged_kv_pages(self.handle, ctypes.byref(k), ctypes.byref(v)))
+        return k.value, v.value
+
+    def attention_workspace(self, n_heads, n_seqs):
+        """Bytes of device memory that kernels.paged_attention needs (its workspace argument)."""
+        n = ctypes.c_size_t()
+        check(lib().bb_paged_attention_workspace(self.ctx.handle, self.handle, n_heads, n_seqs, ctypes.byref(n)))
+        return n.value
+
+    def close(self):
+        if self.handle:
+            check(lib().bb_paged_kv_destroy(self.handle))
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class AttnOp:
     """The GQA attention operator of one layer (model.rs:430-456 / :222-259)."""
 

@@ -11,7 +11,7 @@
  *     message in bb_last_error() (thread-local). No C++ exception or abort crosses the ABI;
  *     where the reference panics on a shape/dtype violation (matmul.rs:851-857, :909-918,
  *     :1023-1033) this library returns BB_ERR_ARG / BB_ERR_SHAPE / BB_ERR_DTYPE instead.
- *   - Dtype codes are ggml's (tensor.rs:41-63): F32=0, F16=1, Q4_K=12, Q6_K=14.
+ *   - Dtype codes are ggml's (tensor.rs:41-63): F32=0, F16=1, Q4_K=12, Q6_K=14, BF16=30.
  *   - Weights are uploaded once (bb_tensor_upload) in their native GGUF block layout (Q4_K:
  *     144-byte blocks, Q6_K: 210-byte blocks) and are immutable afterwards; a tensor may be
  *     shared by any number of layers.
@@ -23,7 +23,7 @@
  *     must not overlap. Use one context per calling thread.
  *   - Results are bit-identical to the reference CPU path on the same inputs (integer dots
  *     exact, f32 epilogues in the reference's order), except rmsnorm's f64 sum order (see
- *     bb_rmsnorm).
+ *     bb_rmsnorm) and the paged-cache operators, which the reference does not have.
  */
 #ifndef BEBELM_MOE_H
 #define BEBELM_MOE_H
@@ -47,7 +47,8 @@ enum bb_status {
   BB_ERR_MISSING = 9 /* metadata key or tensor absent, or of another value type        */
 };
 
-enum bb_dtype { BB_F32 = 0, BB_F16 = 1, BB_Q4_K = 12, BB_Q6_K = 14 };
+/* BB_BF16 (ggml's code too) is a type of the paged-cache operators only. */
+enum bb_dtype { BB_F32 = 0, BB_F16 = 1, BB_Q4_K = 12, BB_Q6_K = 14, BB_BF16 = 30 };
 enum bb_loc { BB_LOC_HOST = 0, BB_LOC_DEVICE = 1 };
 
 typedef struct bb_ctx bb_ctx;
@@ -61,6 +62,8 @@ typedef struct bb_kv_cache bb_kv_cache;
 typedef struct bb_model bb_model;
 typedef struct bb_cache bb_cache;
 typedef struct bb_gguf bb_gguf;
+typedef struct bb_rope_plan bb_rope_plan;
+typedef struct bb_paged_kv bb_paged_kv;
 
 /* Message for the last failed call on this thread ("" if none). */
 const char* bb_last_error(void);
@@ -318,6 +321,132 @@ int bb_model_forward_step(bb_ctx* ctx, bb_model* m, uint32_t token, bb_cache* ca
  * token, sliding the KV window down to max_context after each (Agent::trim_context,
  * agent.rs:471-476). Token ids are checked before anything runs. */
 int bb_model_absorb(bb_ctx* ctx, bb_model* m, bb_cache* cache, const uint32_t* tokens, size_t n, size_t max_context);
+
+/* ---- paged cache: many conversations on one pool --------------------------------------------- */
+/* No counterpart in the reference, which keeps one growing f32 history per conversation
+ * (cache.rs:10-17). A pool holds pages of page_size positions; a page table says which pages a
+ * sequence has, in order. These operators take and give F32, F16 or BF16, compute in f32 (angles in
+ * f64) and round once, to the nearest, where they store. The pool is device memory in both `loc`s;
+ * `loc` says where the other arrays are. With BB_LOC_DEVICE the calls read the page table, lengths
+ * and positions on the device only (the host never waits for them), so a captured call follows what
+ * these arrays hold at each replay; with BB_LOC_HOST they are checked first (BB_ERR_RANGE) and the
+ * call may not be captured. Arrays of 16-byte aligned device memory, as everywhere; strides are in
+ * elements. n_tokens or n_seqs of 0: nothing is done. */
+
+/* Rotary positions. Pair i < rot_dim/2 of a head vector turns by the angle pos·f_i:
+ *   (a, b) -> magnitude·(a·cos - b·sin, a·sin + b·cos),
+ * (a, b) = (x[i], x[i + rot_dim/2]), or with `interleaved` (x[2i], x[2i+1]); elements from rot_dim
+ * on stay as they are. With f_i = freq_base^(-2i/rot_dim) for BB_ROPE_NONE:
+ *   BB_ROPE_LINEAR  f_i / factor
+ *   BB_ROPE_BASE    freq_base·factor^(rot_dim/(rot_dim-2)) in freq_base's place (rot_dim >= 4)
+ *   BB_ROPE_PARTS   f_i·(g + (1-g)/factor), g = (r - low_rotations)/(high_rotations - low_rotations)
+ *                   clamped to 0..1, r = original_positions·f_i/2pi (the turns of the pair over the
+ *                   context that the model was trained on)
+ * BB_ROPE_NONE reads rot_dim, interleaved, freq_base and magnitude only. rot_dim is even, 2..256.
+ * (bb_rope_neox gives the reference's own f32 angle sequence instead, bit for bit.) */
+enum bb_rope_scaling { BB_ROPE_NONE = 0, BB_ROPE_LINEAR = 1, BB_ROPE_BASE = 2, BB_ROPE_PARTS = 3 };
+typedef struct {
+  size_t rot_dim;
+  int interleaved;
+  int scaling;
+  double freq_base;          /* > 0 */
+  double factor;             /* > 0 */
+  double original_positions; /* > 0 (PARTS) */
+  double low_rotations;      /* < high_rotations (PARTS) */
+  double high_rotations;
+  float magnitude;           /* finite; 1 for plain rotations */
+} bb_rope_desc;
+/* The frequencies in the context's GPU: made once, used by any number of calls there. */
+int bb_rope_plan_create(bb_ctx* ctx, const bb_rope_desc* desc, bb_rope_plan** out);
+int bb_rope_plan_destroy(bb_rope_plan* plan);
+/* out[t][h] = x[t][h] turned by pos[t] (any int32) for n_heads vectors of head_dim <= 256 (>= rot_dim)
+ * per token; element (t, h, d) at t·token_stride + h·head_stride + d. out may be x (with x's
+ * strides); otherwise the two may not overlap. */
+int bb_rope(bb_ctx* ctx, const bb_rope_plan* plan, uint32_t dtype, const void* x, size_t token_stride,
+            size_t head_stride, size_t n_tokens, size_t n_heads, size_t head_dim, const int32_t* pos, void* out,
+            size_t out_token_stride, size_t out_head_stride, int loc);
+
+/* A pool of n_pages pages of page_size positions of n_kv_heads keys and values of head_dim (a
+ * multiple of 8, at most 256) in F32, F16 or BF16. bb_paged_kv_create allocates it (zeroed, position
+ * after position, heads side by side); bb_paged_kv_view takes the caller's device memory, element
+ * (page, position, head, d) at page·page_stride + position·pos_stride + head·head_stride + d for both
+ * keys and values: any order of the three, strides whole 16-byte pieces, no two elements in one
+ * place. The view's memory must outlive it. bb_paged_kv_pages gives the two device pointers. */
+int bb_paged_kv_create(bb_ctx* ctx, uint32_t dtype, size_t n_pages, size_t page_size, size_t n_kv_heads,
+                       size_t head_dim, bb_paged_kv** out);
+int bb_paged_kv_view(bb_ctx* ctx, uint32_t dtype, void* k, void* v, size_t n_pages, size_t page_size,
+                     size_t n_kv_heads, size_t head_dim, size_t page_stride, size_t pos_stride, size_t head_stride,
+                     bb_paged_kv** out);
+int bb_paged_kv_destroy(bb_paged_kv* kv);
+int bb_paged_kv_pages(const bb_paged_kv* kv, void** k, void** v);
+
+/* The sequences of a batch: sequence s has lens[s] positions cached (those of the call's own tokens
+ * included; 0: an empty place of the batch), position j in page page_table[s·table_stride +
+ * j/page_size] (max_pages entries per sequence; those past its pages and before the positions that a
+ * call stores or attends to are not read). On the device, a length is taken as at most
+ * max_pages·page_size, and a page number outside the pool as a page whose positions are not there:
+ * nothing is stored in it, nothing read. */
+typedef struct {
+  size_t n_seqs; /* at most 65536 */
+  size_t max_pages;
+  size_t table_stride; /* >= max_pages */
+  const int32_t* page_table;
+  const int32_t* lens;
+} bb_paged_seqs;
+
+/* The tokens of a call: k and v [n_tokens][n_kv_heads][head_dim] (heads side by side, tokens k_stride
+ * and v_stride apart) are stored at the end of their sequences. seq_start NULL: token t is sequence
+ * t's last position (n_tokens = n_seqs). Otherwise i32[n_seqs + 1], ascending from 0: sequence s brings
+ * tokens seq_start[s]..seq_start[s+1]-1, its last ones; tokens from seq_start[n_seqs] on are padding.
+ * On the way k is normed per head (k_norm set: rmsnorm with that gain f32[head_dim] and eps) and turned
+ * (plan given) by pos[t], or with pos NULL by its index in its sequence. q set: its n_heads vectors per
+ * token are normed (q_norm) and turned the same and go to q_out (q itself with the same stride, or
+ * memory that does not overlap it). Nothing is stored, to q_out neither, for padding and for tokens of
+ * sequences whose length leaves them no place. Two tokens of a call may not fall on one position
+ * (pages shared by sequences are whole pages that no token of the call falls in): which of them is
+ * kept is not defined. */
+typedef struct {
+  size_t n_tokens;
+  uint32_t dtype; /* of q, k, v, q_out */
+  const void* k;
+  const void* v;
+  size_t k_stride, v_stride;
+  const void* q;
+  void* q_out;
+  size_t n_heads, q_stride, q_out_stride;
+  const float* q_norm;
+  const float* k_norm;
+  float eps;
+  const int32_t* pos;
+  const int32_t* seq_start;
+} bb_paged_tokens;
+int bb_paged_append(bb_ctx* ctx, bb_paged_kv* kv, const bb_rope_plan* plan, const bb_paged_seqs* seqs,
+                    const bb_paged_tokens* tokens, int loc);
+
+/* One query token per sequence over its cached positions (attention_decode for every sequence):
+ *   out[s][h] = sum_j softmax_j(scale·q[s][h]·k[j][h / (n_heads/n_kv_heads)])·v[j][...]
+ * for max(0, lens[s] - window) <= j < lens[s] (window 0: all). q and out [n_seqs][n_heads][head_dim]
+ * (heads side by side, sequences q_stride and out_stride apart, not overlapping); scale 0 means
+ * 1/sqrt(head_dim). lse (f32[n_seqs][n_heads], or NULL) gets the natural logarithm of the softmax sums. A
+ * sequence with no position to attend to, and a head all of whose scores are -inf, gets zeros and
+ * -inf. workspace: device memory of workspace_bytes >= bb_paged_attention_workspace's answer, for this
+ * call alone while it runs; NULL takes the context's, which a captured call may not (a graph keeps the
+ * address, the context's workspace grows: BB_ERR_ARG). The sums are taken in an order that the batch's
+ * lengths fix, so equal calls give equal bits. */
+typedef struct {
+  uint32_t dtype; /* of q and out */
+  const void* q;
+  void* out;
+  size_t n_heads, q_stride, out_stride;
+  float scale;
+  size_t window;
+  float* lse;
+  void* workspace;
+  size_t workspace_bytes;
+} bb_paged_query;
+int bb_paged_attention_workspace(bb_ctx* ctx, const bb_paged_kv* kv, size_t n_heads, size_t n_seqs, size_t* bytes);
+int bb_paged_attention(bb_ctx* ctx, const bb_paged_kv* kv, const bb_paged_seqs* seqs, const bb_paged_query* query,
+                       int loc);
 
 /* ---- GGUF files (gguf.rs, config.rs:51-89, model.rs:36-50, :572-584, :619-660) ---------------- */
 /* GgufFile::open (gguf.rs:171-177): maps the file read-only and parses the header, the metadata
