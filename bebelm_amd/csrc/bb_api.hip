@@ -2965,6 +2965,8 @@ int bb_paged_attention(bb_ctx* c, const bb_paged_kv* kv, const bb_paged_seqs* sq
     });
     need(std::isfinite(pq->scale), BB_ERR_ARG, "scale must be finite");
     if (B == 0) return;
+    need(bb::paged_attn_fits((int)B, (int)nh, kv->view.n_kv, sq->max_pages * (size_t)kv->view.page_size), BB_ERR_RANGE,
+         "sequences times heads times positions beyond what one call counts");
     need(pq->q && pq->out, BB_ERR_ARG, "null query or output");
     need(B == 1 || (pq->q_stride >= row && pq->out_stride >= row), BB_ERR_ARG, "q_stride or out_stride below a sequence's row");
     need(pq->q_stride < STRIDE_MAX && pq->out_stride < STRIDE_MAX, BB_ERR_RANGE, "stride beyond 2^40 elements");
@@ -2994,13 +2996,14 @@ int bb_paged_attention(bb_ctx* c, const bb_paged_kv* kv, const bb_paged_seqs* sq
               q.out = d[3];
               q.q_stride = pq->q_stride;
               q.out_stride = pq->out_stride;
+              q.dt = (int)pq->dtype;
               q.n_heads = (int)nh;
               q.window = pq->window < ((size_t)1 << 31) ? (int)pq->window : 0;  // (lengths are below 2^31)
               q.scale = pq->scale != 0.0f ? pq->scale : 1.0f / std::sqrt((float)hd);
               q.lse = nl ? static_cast<float*>(d[4]) : nullptr;
               q.ws = pq->workspace ? pq->workspace : ensure_ws(c, want);
               launch_paged(c, cap, bb::K_PAGED_ATTN, [&] {
-                return bb::launch_paged_attn(c->stream, c->n_cu, (int)pq->dtype, (int)kv->dtype, q, kv->view,
+                return bb::launch_paged_attn(c->stream, c->n_cu, (int)kv->dtype, q, kv->view,
                                              seqs_of(sq, d[0], d[1]));
               });
             });

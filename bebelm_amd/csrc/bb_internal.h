@@ -402,13 +402,15 @@ struct PagedQuery {
   const void* q;
   void* out;
   size_t q_stride, out_stride;
-  int n_heads, window;
+  int dt, n_heads, window;  // dt: the type of q and out
   float scale;
   float* lse;
   void* ws;
 };
 size_t paged_attn_ws(int n_cu, int n_seqs, int n_heads, int n_kv, int hd);
-hipError_t launch_paged_attn(hipStream_t s, int n_cu, int dtype, int cache, const PagedQuery& q, const PagedView& kv,
+// Whether a batch's units of work can be counted in 30 bits (cap: positions of a sequence at most).
+bool paged_attn_fits(int n_seqs, int n_heads, int n_kv, size_t cap);
+hipError_t launch_paged_attn(hipStream_t s, int n_cu, int cache, const PagedQuery& q, const PagedView& kv,
                              const PagedSeqs& seqs);
 
 }  // namespace bb

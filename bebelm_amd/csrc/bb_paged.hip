@@ -3,6 +3,7 @@
 // counterpart: values are computed in f32 from the formulas and rounded once where they are stored.
 #include "bb_device.h"
 #include <algorithm>
+#include <type_traits>
 #include "bb_internal.h"
 
 namespace bb {
@@ -276,74 +277,664 @@ hipError_t launch_rope_rows(hipStream_t s, int dtype, int cache, const RopeRows&
 }
 
 // ---- attention of one token per sequence ---------------------------------------------------------
+//
+// out[s][h] = sum_j softmax_j(scale·q·k_j)·v_j in one pass over the keys and values, with the running
+// maximum and sum of the softmax. Bound by the cache's bytes: one kv head's keys and values are read
+// once for the (up to 16) query heads of a group, and nothing but sums leaves the registers.
+//
+// Work. A sequence's positions (from its window's first, rounded down to 32) are cut into units of 128,
+// and the units of all (sequence, head group) pairs, in that order, into equal runs, one a block: every
+// block reads about the same number of bytes however ragged the batch, with no host knowing a
+// length. A block's 4 waves take tiles of KT = 32 positions in turn and are joined in LDS at the end of
+// a pair; a pair that lies in several blocks leaves one partial sum each, which k_paged_join adds.
+//
+// Tiles on the matrix cores, with nothing moved between lanes. Lane l has column (head) n = l%16 and group
+// g = l/16. Scores are D[position][head] = K·q^T: A holds 16 positions' rows (lane: row l%16, the group's
+// 16-byte pieces), D leaves lane (n, g) the scores of positions 4g..4g+3. Output sums are
+// O[element][head] = V^T·p: for B, a lane's own weights (positions 4g..4g+3 of each 16) are already
+// where the instruction wants group g's part of the sum, when A's group g holds the values of the
+// same positions. So values are loaded row by row, lane m = l%16 an adjacent piece of the row of
+// each of its group's positions, and the row index m of instruction i stands for element i of lane
+// m's piece; 16-bit pieces are transposed in registers (one byte permute per two values).
+//
+// Exactness. Scores, weights, maxima and sums are f32. An f32 cache takes f32 matrix instructions. A 16-bit
+// cache takes 16-bit ones (an eighth of the time) on its values as they are, with q and the weights
+// split into NP 16-bit parts whose products with a cached value are exact in f32: bf16 by truncation (3
+// parts are all of an f32; 2 parts, 16 bits and rounded, where q and out are 16-bit themselves), f16
+// by rounding (2 parts, 22 bits) after scaling the row of q by the power of two that puts its largest
+// in 2^13..2^14 and the weights by 2^14, so that f16's range costs at most 2^-38 of the largest. A part
+// that is 0 meets an infinite key as NaN: such scores are taken from the first parts alone.
 namespace {
 
-constexpr int PA_THREADS = 256;
+constexpr int PA_WAVES = 4, PA_THREADS = 64 * PA_WAVES;
+constexpr int PA_UNIT = 128;      // positions of a unit: a tile for each wave
+constexpr int PA_HEADS = 16;      // heads of a group at most
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr float NEG_INF = -__builtin_inff();
 
-// One block per (sequence, head): chunks of 256 positions, a thread a position's score, then a thread
-// an element of the value sum; running maximum and sum over the chunks.
-template <class A, class C>
-__global__ void __launch_bounds__(PA_THREADS) k_paged_attn_rows(PagedQuery pq, PagedView kv, PagedSeqs sq) {
-  __shared__ float q[OPS_HD_MAX], p[PA_THREADS], red[PA_THREADS / 64];
-  __shared__ int64_t at[PA_THREADS];
-  const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, hd = kv.hd;
-  const int g = h / (pq.n_heads / kv.n_kv);
-  const A* qr = static_cast<const A*>(pq.q) + (size_t)s * pq.q_stride + (size_t)h * hd;
-  if (tid < hd) q[tid] = (float)qr[tid] * pq.scale;
-  const int64_t cap = (int64_t)sq.max_pages * kv.page_size;
-  const int len = (int)min((int64_t)max(sq.lens[s], 0), cap);
-  const int first = pq.window > 0 ? max(0, len - pq.window) : 0;
-  float m = -__builtin_inff(), l = 0.0f, o = 0.0f;
-  for (int j0 = first; j0 < len; j0 += PA_THREADS) {
-    const int j = j0 + tid;
-    int64_t e = -1;
-    if (j < len) {
-      const int page = j / kv.page_size;
-      e = page_base(kv, sq, s, page);
-      if (e >= 0) e += (int64_t)((size_t)(j - page * kv.page_size) * kv.pos_stride + (size_t)g * kv.head_stride);
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
+// Heads of a kv head's query heads: `split` groups of `hg` (the last may have fewer).
+struct PagedPlan {
+  int split, hg, n_groups, join;
+  int* chunk;     // [1 + n_seqs + 1]: units of a block's run, units before each sequence
+  float* sums;    // [2·blocks][hg][hd]
+  float2* ml;     // [2·blocks][hg]: maximum (base 2), sum of weights
+};
+
+struct SeqSpan {
+  int base, first, len, units;  // positions first..len-1, counted from base; units >= 1
+};
+__device__ __forceinline__ SeqSpan seq_span(int raw_len, int cap, int window) {
+  SeqSpan r;
+  r.len = min(max(raw_len, 0), cap);
+  r.first = window > 0 ? max(0, r.len - window) : 0;
+  r.base = r.first & ~31;
+  r.units = max(1, (r.len - r.base + PA_UNIT - 1) / PA_UNIT);
+  return r;
+}
+
+__device__ __forceinline__ float load_act(const void* p, size_t i, int dt) {
+  if (dt == BB_F32) return static_cast<const float*>(p)[i];
+  if (dt == BB_F16) return (float)static_cast<const _Float16*>(p)[i];
+  return (float)static_cast<const __bf16*>(p)[i];
+}
+__device__ __forceinline__ void store_act(void* p, size_t i, int dt, float x) {
+  if (dt == BB_F32) static_cast<float*>(p)[i] = x;
+  else if (dt == BB_F16) static_cast<_Float16*>(p)[i] = (_Float16)x;
+  else static_cast<__bf16*>(p)[i] = (__bf16)x;
+}
+
+// (by value: a bit cast of a vector's element itself reads the vector's first)
+__device__ __forceinline__ float as_float(uint32_t a) { return __builtin_bit_cast(float, a); }
+__device__ __forceinline__ uint32_t hi_halves(float a, float b) {  // the upper 16 bits of a (low) and b
+  return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
+}
+__device__ __forceinline__ float trunc_bf16(float a) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, a) & 0xffff0000u);
+}
+// Two values as NP packed 16-bit parts whose sums they are.
+template <int CT, int NP>
+__device__ __forceinline__ void split2(float a, float b, uint32_t (&w)[NP]) {
+  if constexpr (CT == BB_BF16) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      if (i + 1 == NP && NP < 3) {
+        typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+        const v2b r = {(__bf16)a, (__bf16)b};
+        w[i] = __builtin_bit_cast(uint32_t, r);
+      } else {
+        w[i] = hi_halves(a, b);
+        a = a - trunc_bf16(a);
+        b = b - trunc_bf16(b);
+      }
     }
-    __syncthreads();  // q is there; the chunk before is done with p and at
-    float sc = -__builtin_inff();
-    if (e >= 0) {
-      const C* k = static_cast<const C*>(kv.k) + e;
-      sc = 0.0f;
-      for (int d = 0; d < hd; ++d) sc += q[d] * (float)k[d];
-    }
-    float mx = wave_max(sc);
-    if ((tid & 63) == 0) red[tid >> 6] = mx;
-    at[tid] = e;
-    __syncthreads();
-    const float m1 = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-    const float ms = m1 == -__builtin_inff() ? 0.0f : m1;
-    p[tid] = e >= 0 ? expf(sc - ms) : 0.0f;
-    const float f = expf(m - ms);
-    m = m1;
-    __syncthreads();
-    l *= f;
-    o *= f;
-    for (int i = 0; i < min(PA_THREADS, len - j0); ++i) {
-      if (at[i] < 0) continue;
-      l += p[i];
-      if (tid < hd) o += p[i] * (float)(static_cast<const C*>(kv.v) + at[i])[tid];
+  } else {
+    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const v2h r = {(_Float16)a, (_Float16)b};
+      w[i] = __builtin_bit_cast(uint32_t, r);
+      a = a - (float)r[0];
+      b = b - (float)r[1];
     }
   }
-  const bool none = m == -__builtin_inff() && l == 0.0f;
-  if (tid < hd) (static_cast<A*>(pq.out) + (size_t)s * pq.out_stride + (size_t)h * hd)[tid] = (A)(none ? 0.0f : o / l);
-  if (tid == 0 && pq.lse) pq.lse[(size_t)s * pq.n_heads + h] = none ? m : m + logf(l);
+}
+
+template <int CT>
+__device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
+  if constexpr (CT == BB_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float group_max(float x) {  // over the four lanes of a column
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float group_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// Waves of a SIMD at a time for head sizes up to hdp: 128, 256, 512 registers each.
+constexpr int pa_waves(int hdp) { return hdp == 64 ? 4 : hdp == 128 ? 2 : 1; }
+
+// A tile's shape: CT the cache's type, HDP the head size (or the next of 64, 128, 256).
+template <int CT, int HDP>
+struct PaShape {
+  static constexpr int SZ = CT == BB_F32 ? 4 : 2;
+  static constexpr int KE = 16 / SZ;                     // elements of a 16-byte piece
+  static constexpr int NC = HDP / (4 * KE);              // pieces of a key row per lane
+  static constexpr int VE = HDP / 16;                    // elements of a value row per lane
+  static constexpr int PE = VE < KE ? VE : KE;           // in pieces of PE
+  static constexpr int NV = VE / PE;
+  static constexpr int KT = CT == BB_F32 && HDP == 256 ? 16 : 32;  // positions of a tile (registers)
+  static constexpr int NT = KT / 16;
+};
+
+// One wave's part of a (sequence, head group) pair: running maximum m (base 2), sum l and o[i][r] for element
+// (16p + 4g + r)·PE + e, i = p·PE + e, of head n.
+template <int CT, int NP, int HDP, bool UNI>
+struct PaWave {
+  typedef PaShape<CT, HDP> S;
+  static constexpr int NT = S::NT, NC = S::NC, NV = S::NV, VE = S::VE, PE = S::PE, KE = S::KE, SZ = S::SZ;
+  typedef typename std::conditional<S::PE * S::SZ == 16, v4u, v2u>::type VP;  // a piece of a value row
+  const PagedView& kv;
+  const PagedSeqs& sq;
+  const int n, g;
+  int s, head0, heads;  // head0: the first head of the group; heads: how many
+  size_t kv_off;        // the kv head's offset in the pool (elements)
+  SeqSpan sp;
+  v4u q[NP][NC];
+  int q_exp;   // f16: the row of q was scaled by 2^q_exp
+  float c;     // scale·log2(e)
+  float m, l;
+  v4f o[VE];
+  v4u k[NT][NC];
+  VP v[4 * NT][NV];
+  uint32_t valid;  // bit 4t + r: position 16t + 4g + r of the tile whose values are loaded is attended to
+
+  __device__ __forceinline__ PaWave(const PagedView& kv_, const PagedSeqs& sq_, int lane)
+      : kv(kv_), sq(sq_), n(lane & 15), g(lane >> 4) {}
+
+  __device__ void start(const PagedQuery& pq) {
+    const size_t row = (size_t)s * pq.q_stride + (size_t)(head0 + n) * kv.hd;
+    c = pq.scale * LOG2E;
+    m = NEG_INF;
+    l = 0.0f;
+    q_exp = 0;
+#pragma unroll
+    for (int i = 0; i < VE; ++i) o[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    float x[NC][KE];
+    float top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const int d = (4 * j + g) * KE;
+#pragma unroll
+      for (int e = 0; e < KE; ++e) x[j][e] = n < heads && d < kv.hd ? load_act(pq.q, row + d + e, pq.dt) : 0.0f;
+#pragma unroll
+      for (int e = 0; e < KE; ++e) top = fmaxf(top, fabsf(x[j][e]));
+    }
+    if constexpr (CT == BB_F16) {
+      // (0 and what is not finite keep their scale)
+      top = group_max(top);
+      if (top > 0.0f && top < __builtin_inff()) q_exp = 14 - ilogbf(top) - 1;
+#pragma unroll
+      for (int j = 0; j < NC; ++j)
+#pragma unroll
+        for (int e = 0; e < KE; ++e) x[j][e] = ldexpf(x[j][e], q_exp);
+    }
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      if constexpr (CT == BB_F32) {
+#pragma unroll
+        for (int e = 0; e < KE; ++e) q[0][j][e] = __float_as_uint(x[j][e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < KE; e += 2) {
+          uint32_t w[NP];
+          split2<CT, NP>(x[j][e], x[j][e + 1], w);
+#pragma unroll
+          for (int i = 0; i < NP; ++i) q[i][j][e / 2] = w[i];
+        }
+      }
+    }
+  }
+
+  // The places of a tile's positions. UNI (pages of whole 16 positions): off[t] is where the 16 positions t start,
+  // the same for the wave. Otherwise off[0] is lane i%32's: where position i of the tile is. -1: not there.
+  struct Places {
+    int64_t off[UNI ? NT : 1];
+    int key0;
+  };
+  __device__ __forceinline__ Places places(int key0) const {
+    Places p;
+    p.key0 = key0;
+    if constexpr (UNI) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int key = key0 + 16 * t;
+        int64_t b = -1;
+        if (key < sp.len) {
+          const int page = key / kv.page_size;
+          b = page_base(kv, sq, s, page);
+          if (b >= 0) b += (int64_t)((size_t)(key - page * kv.page_size) * kv.pos_stride + kv_off);
+        }
+        p.off[t] = b;
+      }
+    } else {
+      const int key = key0 + ((n + 16 * g) & (S::KT - 1));
+      int64_t b = -1;
+      if (key < sp.len && key >= sp.first) {
+        const int page = key / kv.page_size;
+        b = page_base(kv, sq, s, page);
+        if (b >= 0) b += (int64_t)((size_t)(key - page * kv.page_size) * kv.pos_stride + kv_off);
+      }
+      p.off[0] = b;
+    }
+    return p;
+  }
+
+  __device__ __forceinline__ void load_k(const Places& p) {
+    const char* base = static_cast<const char*>(kv.k);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      int64_t at;
+      if constexpr (UNI) at = p.off[t] < 0 ? -1 : p.off[t] + (int64_t)((size_t)n * kv.pos_stride);
+      else at = __shfl(p.off[0], n + 16 * t);
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        const int d = (4 * j + g) * KE;
+        k[t][j] = v4u{0, 0, 0, 0};
+        if (at >= 0 && d < kv.hd) k[t][j] = *reinterpret_cast<const v4u*>(base + (size_t)(at + d) * SZ);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void load_v(const Places& p) {
+    const char* base = static_cast<const char*>(kv.v);
+    valid = 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = 16 * t + 4 * g + r;
+        int64_t at;
+        if constexpr (UNI) {
+          const int key = p.key0 + i;
+          at = p.off[t] < 0 || key < sp.first || key >= sp.len
+                   ? -1
+                   : p.off[t] + (int64_t)((size_t)(4 * g + r) * kv.pos_stride);
+        } else {
+          at = __shfl(p.off[0], i);
+        }
+        valid |= (at >= 0 ? 1u : 0u) << (4 * t + r);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int d = (16 * j + n) * PE;
+          VP z{};
+          if (at >= 0 && d < kv.hd) z = *reinterpret_cast<const VP*>(base + (size_t)(at + d) * SZ);
+          v[4 * t + r][j] = z;
+        }
+      }
+  }
+
+  template <int PARTS>
+  __device__ __forceinline__ void scores(v4f (&x)[NT]) const {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) x[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if constexpr (CT == BB_F32) {
+#pragma unroll
+          for (int e = 0; e < KE; ++e)
+            x[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(as_float(k[t][j][e]), as_float(q[0][j][e]), x[t], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int i = PARTS - 1; i >= 0; --i) x[t] = mfma16<CT>(k[t][j], q[i][j], x[t]);
+        }
+      }
+  }
+
+  // Scores of the loaded keys (base-2 exponents, masked), from which the keys' registers are free again.
+  __device__ __forceinline__ void score(v4f (&x)[NT]) const {
+    scores<NP>(x);
+    if constexpr (NP > 1) {
+      bool odd = false;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) odd |= x[t][r] != x[t][r];
+      if (__any(odd)) {
+        v4f y[NT];
+        scores<1>(y);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (x[t][r] != x[t][r]) x[t][r] = y[t][r];
+      }
+    }
+  }
+
+  // Adds a tile: its scores x and the loaded values.
+  __device__ __forceinline__ void add(v4f (&x)[NT]) {
+    float mx = NEG_INF;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float y = x[t][r];
+        if constexpr (CT == BB_F16) y = ldexpf(y, -q_exp);
+        y = valid >> (4 * t + r) & 1 ? y * c : NEG_INF;
+        x[t][r] = y;
+        mx = fmaxf(mx, y);
+      }
+    mx = fmaxf(m, group_max(mx));
+    const float ref = mx == NEG_INF ? 0.0f : mx;
+    if (__any(mx > m)) {
+      const float f = __builtin_amdgcn_exp2f(m - ref);
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < VE; ++i) o[i] *= f;
+    }
+    m = mx;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[t][r] = __builtin_amdgcn_exp2f(x[t][r] - ref);
+        if constexpr (CT == BB_F16) x[t][r] *= 16384.0f;
+        l += x[t][r];
+      }
+    if constexpr (CT == BB_F32) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < VE; ++i)
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(as_float(v[4 * t + r][i / PE][i % PE]), x[t][r], o[i], 0, 0, 0);
+    } else {
+      v4u p[NP];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+          uint32_t w[NP];
+          split2<CT, NP>(x[t][r], x[t][r + 1], w);
+#pragma unroll
+          for (int i = 0; i < NP; ++i) p[i][2 * t + r / 2] = w[i];
+        }
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        v4u a;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          a[w] = __builtin_amdgcn_perm(v[2 * w + 1][i / PE][i % PE / 2], v[2 * w][i / PE][i % PE / 2],
+                                       i % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int j = NP - 1; j >= 0; --j) o[i] = mfma16<CT>(a, p[j], o[i]);
+      }
+    }
+  }
+
+  // Positions key, key + step, ... below end.
+  __device__ void run(int key, int end, int step) {
+    if (key >= end) return;
+    Places p = places(key);
+    load_k(p);
+    load_v(p);
+    for (;;) {
+      v4f x[NT];
+      const int next = key + step;
+      const bool more = next < end;
+      if (more) p = places(next);
+      score(x);
+      if (more) load_k(p);
+      add(x);
+      if (!more) return;
+      load_v(p);
+      key = next;
+    }
+  }
+};
+
+template <int CT, int NP, int HDP, bool UNI>
+__global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQuery pq, PagedView kv, PagedSeqs sq,
+                                                                        PagedPlan pl) {
+  typedef PaShape<CT, HDP> S;
+  constexpr int LD = HDP + 4;
+  extern __shared__ float so[];  // [waves][hg][LD]
+  __shared__ float s_m[PA_WAVES][PA_HEADS], s_l[PA_WAVES][PA_HEADS];
+  __shared__ int s_scan[PA_WAVES], s_at[3];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int cap = sq.max_pages * kv.page_size;
+
+  // units of 256 sequences from c0, their running sum within the 256 (inclusive) and their total
+  int c0 = 0, carry = 0, mine = 0, incl = 0, part = 0;
+  const auto scan = [&]() {
+    const int i = c0 + tid;
+    mine = i < sq.n_seqs ? seq_span(sq.lens[i], cap, pq.window).units : 0;
+    incl = mine;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(incl, o);
+      if (lane >= o) incl += y;
+    }
+    __syncthreads();
+    if (lane == 63) s_scan[wv] = incl;
+    __syncthreads();
+    part = 0;
+#pragma unroll
+    for (int w = 0; w < PA_WAVES; ++w) {
+      if (w < wv) incl += s_scan[w];
+      part += s_scan[w];
+    }
+  };
+  int total = 0;
+  for (c0 = 0; c0 < sq.n_seqs; c0 += PA_THREADS) {
+    scan();
+    if (pl.join && blockIdx.x == 0 && c0 + tid < sq.n_seqs) pl.chunk[2 + c0 + tid] = total + incl;
+    total += part;
+  }
+  const int chunk = (total * pl.n_groups + (int)gridDim.x - 1) / (int)gridDim.x;
+  if (pl.join && blockIdx.x == 0 && tid == 0) {
+    pl.chunk[0] = chunk;
+    pl.chunk[1] = 0;
+  }
+  int64_t u64 = (int64_t)blockIdx.x * chunk;
+  if (u64 >= (int64_t)total * pl.n_groups) return;
+  int u = (int)u64;
+  const int end = min(u + chunk, total * pl.n_groups);
+  c0 = 0;
+  if (sq.n_seqs > PA_THREADS) scan();
+
+  PaWave<CT, NP, HDP, UNI> w(kv, sq, lane);
+  const float up = CT == BB_F16 ? 14.0f : 0.0f;
+  for (bool first_pair = true; u < end; first_pair = false) {
+    // the sequence of unit u
+    while (u >= (carry + part) * pl.n_groups) {
+      carry += part;
+      c0 += PA_THREADS;
+      scan();
+    }
+    __syncthreads();  // (s_at, and the sums of the pair before)
+    const int lo = (carry + incl - mine) * pl.n_groups;
+    if (mine > 0 && u >= lo && u < lo + mine * pl.n_groups) {
+      s_at[0] = c0 + tid;
+      s_at[1] = lo;
+      s_at[2] = mine;
+    }
+    __syncthreads();
+    const int s = __builtin_amdgcn_readfirstlane(s_at[0]);
+    const int seq_lo = __builtin_amdgcn_readfirstlane(s_at[1]), nu = __builtin_amdgcn_readfirstlane(s_at[2]);
+    const int grp = (u - seq_lo) / nu, u0 = (u - seq_lo) - grp * nu, take = min(nu - u0, end - u);
+    const int kvh = grp / pl.split, sub = grp - kvh * pl.split;
+    w.s = s;
+    w.head0 = kvh * (pq.n_heads / kv.n_kv) + sub * pl.hg;
+    w.heads = min(pl.hg, pq.n_heads / kv.n_kv - sub * pl.hg);
+    w.kv_off = (size_t)kvh * kv.head_stride;
+    w.sp = seq_span(sq.lens[s], cap, pq.window);
+    w.start(pq);
+    const int k0 = w.sp.base + u0 * PA_UNIT;
+    w.run(k0 + wv * S::KT, min(k0 + take * PA_UNIT, w.sp.len), PA_WAVES * S::KT);
+
+    // the waves' sums together
+    const float l_all = group_sum(w.l);
+    if (w.g == 0) {
+      s_m[wv][w.n] = w.m;
+      s_l[wv][w.n] = l_all;
+    }
+    __syncthreads();
+    float top = NEG_INF;
+#pragma unroll
+    for (int i = 0; i < PA_WAVES; ++i) top = fmaxf(top, s_m[i][w.n]);
+    const float f = __builtin_amdgcn_exp2f(w.m - (top == NEG_INF ? 0.0f : top));
+    if (w.n < w.heads) {
+      float* to = so + ((size_t)wv * pl.hg + w.n) * LD;
+#pragma unroll
+      for (int p = 0; p < S::NV; ++p)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int e = 0; e < S::PE; ++e) to[(16 * p + 4 * w.g + r) * S::PE + e] = w.o[p * S::PE + e][r] * f;
+    }
+    __syncthreads();
+    const bool whole = take == nu;
+    const size_t slot = 2 * (size_t)blockIdx.x + (first_pair ? 0 : 1);
+    for (int i = tid; i < w.heads * kv.hd; i += PA_THREADS) {
+      const int h = i / kv.hd, d = i - h * kv.hd;
+      float mm = NEG_INF, ll = 0.0f, x = 0.0f;
+#pragma unroll
+      for (int j = 0; j < PA_WAVES; ++j) mm = fmaxf(mm, s_m[j][h]);
+#pragma unroll
+      for (int j = 0; j < PA_WAVES; ++j) {
+        ll += s_l[j][h] * __builtin_amdgcn_exp2f(s_m[j][h] - (mm == NEG_INF ? 0.0f : mm));
+        x += so[((size_t)j * pl.hg + h) * LD + d];
+      }
+      if (whole) {
+        const bool none = mm == NEG_INF && ll == 0.0f;
+        store_act(pq.out, (size_t)s * pq.out_stride + (size_t)(w.head0 + h) * kv.hd + d, pq.dt, none ? 0.0f : x / ll);
+        if (d == 0 && pq.lse) pq.lse[(size_t)s * pq.n_heads + w.head0 + h] = none ? NEG_INF : (mm + log2f(ll) - up) * LN2;
+      } else {
+        pl.sums[(slot * pl.hg + h) * kv.hd + d] = x;
+        if (d == 0) pl.ml[slot * pl.hg + h] = make_float2(mm, ll);
+      }
+    }
+    u += take;
+  }
+}
+
+// Adds the partial sums of a (sequence, head): those of the blocks whose runs hold units of it.
+constexpr int PJ_THREADS = 256;
+__global__ void __launch_bounds__(PJ_THREADS) k_paged_join(PagedQuery pq, int n_kv, int hd, PagedPlan pl, float up) {
+  __shared__ float red[PJ_THREADS / 64];
+  __shared__ __align__(16) float acc[PJ_THREADS * 4];
+  const int h = blockIdx.y, s = blockIdx.x, tid = threadIdx.x;
+  const int G = pq.n_heads / n_kv, kvh = h / G, sub = (h - kvh * G) / pl.hg, hh = h - kvh * G - sub * pl.hg;
+  const int chunk = pl.chunk[0], before = pl.chunk[1 + s], nu = pl.chunk[2 + s] - before;
+  const int lo = before * pl.n_groups + (kvh * pl.split + sub) * nu, hi = lo + nu;
+  const int b0 = lo / chunk, b1 = (hi - 1) / chunk;
+  if (b0 == b1) return;  // whole in one block
+  const int parts = b1 - b0 + 1;
+  // the first block's run may start before the pair, which is its second one then
+  const auto slot = [&](int i) { return (2 * (size_t)(b0 + i) + (i == 0 && b0 * chunk != lo ? 1 : 0)) * pl.hg + hh; };
+  float top = NEG_INF;
+  for (int i = tid; i < parts; i += PJ_THREADS) top = fmaxf(top, pl.ml[slot(i)].x);
+  top = wave_max(top);
+  if ((tid & 63) == 0) red[tid >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float ref = top == NEG_INF ? 0.0f : top;
+  // lanes: hd/4 (rounded up to a power of two) pieces of 4 elements, the rest of the block over the parts
+  int np = 1;
+  while (4 * np < hd) np *= 2;
+  const int piece = tid & (np - 1), rows = PJ_THREADS / np;
+  float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float l = 0.0f;
+  for (int i = tid / np; i < parts; i += rows) {
+    const size_t at = slot(i);
+    const float2 ml = pl.ml[at];
+    const float f = __builtin_amdgcn_exp2f(ml.x - ref);
+    l += ml.y * f;
+    if (4 * piece < hd) {
+      const float4 y = *reinterpret_cast<const float4*>(pl.sums + at * hd + 4 * piece);
+      x.x += y.x * f;
+      x.y += y.y * f;
+      x.z += y.z * f;
+      x.w += y.w * f;
+    }
+  }
+  __syncthreads();  // (red is read)
+  reinterpret_cast<float4*>(acc)[tid] = x;
+  __shared__ float lsum[PJ_THREADS];
+  if (piece == 0) lsum[tid / np] = l;
+  __syncthreads();
+  if (tid < hd) {
+    float y = 0.0f, ll = 0.0f;
+    for (int i = 0; i < rows; ++i) {
+      y += acc[4 * (i * np + tid / 4) + tid % 4];
+      ll += lsum[i];
+    }
+    const bool none = top == NEG_INF && ll == 0.0f;
+    store_act(pq.out, (size_t)s * pq.out_stride + (size_t)h * hd + tid, pq.dt, none ? 0.0f : y / ll);
+    if (tid == 0 && pq.lse) pq.lse[(size_t)s * pq.n_heads + h] = none ? NEG_INF : (top + log2f(ll) - up) * LN2;
+  }
+}
+
+int pa_class(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
+
+// Blocks that fit the device at once.
+int pa_blocks(int n_cu, int hd) { return n_cu * pa_waves(pa_class(hd)); }
+
+PagedPlan pa_plan(int n_seqs, int n_heads, int n_kv) {
+  PagedPlan p{};
+  const int G = n_heads / n_kv;
+  p.split = (G + PA_HEADS - 1) / PA_HEADS;
+  p.hg = (G + p.split - 1) / p.split;
+  p.n_groups = n_kv * p.split;
+  return p;
 }
 
 }  // namespace
 
-size_t paged_attn_ws(int, int, int, int, int) { return 0; }
+bool paged_attn_fits(int n_seqs, int n_heads, int n_kv, size_t cap) {
+  const PagedPlan p = pa_plan(n_seqs, n_heads, n_kv);
+  return (size_t)n_seqs * (size_t)p.n_groups * ((cap + PA_UNIT - 1) / PA_UNIT) < ((size_t)1 << 30);
+}
 
-hipError_t launch_paged_attn(hipStream_t s, int, int dtype, int cache, const PagedQuery& q, const PagedView& kv,
-                             const PagedSeqs& seqs) {
-  if (seqs.n_seqs == 0) return hipSuccess;
-  return by_dtypes(dtype, cache, [&](auto a, auto c) {
-    BB_LAUNCH((k_paged_attn_rows<typename decltype(a)::T, typename decltype(c)::T>), dim3(q.n_heads, seqs.n_seqs),
-              dim3(PA_THREADS), 0, s, q, kv, seqs);
-    return hipGetLastError();
-  });
+size_t paged_attn_ws(int n_cu, int n_seqs, int n_heads, int n_kv, int hd) {
+  const PagedPlan p = pa_plan(n_seqs, n_heads, n_kv);
+  const size_t slots = 2 * (size_t)pa_blocks(n_cu, hd) * p.hg;
+  return slots * ((size_t)hd * 4 + sizeof(float2)) + ((size_t)n_seqs + 2) * 4;
+}
+
+hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQuery& q, const PagedView& kv,
+                             const PagedSeqs& sq) {
+  if (sq.n_seqs == 0) return hipSuccess;
+  PagedPlan pl = pa_plan(sq.n_seqs, q.n_heads, kv.n_kv);
+  const size_t cap = (size_t)sq.max_pages * kv.page_size;
+  const int blocks_max = pa_blocks(n_cu, kv.hd);
+  const size_t slots = 2 * (size_t)blocks_max * pl.hg;
+  pl.sums = static_cast<float*>(q.ws);
+  pl.ml = reinterpret_cast<float2*>(pl.sums + slots * kv.hd);
+  pl.chunk = reinterpret_cast<int*>(pl.ml + slots);
+  const size_t units = (size_t)sq.n_seqs * pl.n_groups * ((cap + PA_UNIT - 1) / PA_UNIT);
+  const unsigned blocks = (unsigned)std::min<size_t>(blocks_max, units);
+  pl.join = cap > (size_t)PA_UNIT;  // else every pair is one unit
+  const bool uni = kv.page_size % 16 == 0;
+  const int cls = pa_class(kv.hd);
+  const size_t lds = (size_t)PA_WAVES * pl.hg * (cls + 4) * 4;
+#define BB_PA(ct, np, hdp)                                                                                     \
+  do {                                                                                                         \
+    if (uni) BB_LAUNCH((k_paged_attn<ct, np, hdp, true>), dim3(blocks), dim3(PA_THREADS), lds, st, q, kv, sq, pl); \
+    else BB_LAUNCH((k_paged_attn<ct, np, hdp, false>), dim3(blocks), dim3(PA_THREADS), lds, st, q, kv, sq, pl);    \
+  } while (0)
+#define BB_PA_HD(ct, np)             \
+  do {                               \
+    if (cls == 64) BB_PA(ct, np, 64); \
+    else if (cls == 128) BB_PA(ct, np, 128); \
+    else BB_PA(ct, np, 256);         \
+  } while (0)
+  if (cache == BB_F32) BB_PA_HD(BB_F32, 1);
+  else if (cache == BB_F16) BB_PA_HD(BB_F16, 2);
+  else if (q.dt == BB_F32) BB_PA_HD(BB_BF16, 3);
+  else BB_PA_HD(BB_BF16, 2);
+#undef BB_PA_HD
+#undef BB_PA
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !pl.join) return e;
+  BB_LAUNCH(k_paged_join, dim3(sq.n_seqs, q.n_heads), dim3(PJ_THREADS), 0, st, q, kv.n_kv, kv.hd, pl,
+            cache == BB_F16 ? 14.0f : 0.0f);
+  return hipGetLastError();
 }
 
 }  // namespace bb
