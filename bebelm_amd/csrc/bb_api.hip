@@ -2647,6 +2647,7 @@ bb_paged_kv* new_pool(bb_ctx* c, uint32_t dtype, void* k, void* v, size_t n_page
   p->device = c->device;
   p->dtype = dtype;
   p->view = {k, v, page_stride, pos_stride, head_stride, (int)n_pages, (int)page_size, (int)n_kv, (int)hd};
+  bb::paged_divisor(p->view);
   p->own = own;
   return p;
 }

@@ -58,11 +58,10 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
   }
 }
 
-// Where page `page` of sequence s starts in the pool, -1 for a page that is not there.
-__device__ __forceinline__ int64_t page_base(const PagedView& kv, const PagedSeqs& sq, int s, int page) {
-  if (page < 0 || page >= sq.max_pages) return -1;
-  const int p = sq.table[(size_t)s * sq.table_stride + page];
-  return p < 0 || p >= kv.n_pages ? -1 : (int64_t)((size_t)p * kv.page_stride);
+// i / page_size for 0 <= i < 2^31 (PagedView::page_mul = ceil(2^(31 + page_shift) / page_size), page_shift
+// = ceil(log2(page_size)): the product is off by less than i / 2^(31 + page_shift) < 1 / page_size).
+__device__ __forceinline__ int page_of(const PagedView& kv, int i) {
+  return (int)(((uint64_t)(uint32_t)i * kv.page_mul) >> (31 + kv.page_shift));
 }
 
 // ---- rotary positions, and the rows of an append ------------------------------------------------
@@ -116,12 +115,13 @@ __device__ __forceinline__ RowPlace row_place(const RopeRows& r, const PagedView
     index = (int64_t)sq.lens[s] - 1;
   }
   if (index < 0 || index >= (int64_t)sq.max_pages * kv.page_size) return w;
-  const int ix = (int)index, page = ix / kv.page_size;
+  const int ix = (int)index, page = page_of(kv, ix);
   w.live = 1;
   w.pos = r.pos ? r.pos[t] : ix;
   if (r.n_kv) {
-    const int64_t pb = page_base(kv, sq, s, page);
-    if (pb >= 0) w.base = pb + (int64_t)((size_t)(ix - page * kv.page_size) * kv.pos_stride);
+    const int pg = sq.table[(size_t)s * sq.table_stride + page];
+    if (pg >= 0 && pg < kv.n_pages)
+      w.base = (int64_t)((size_t)pg * kv.page_stride + (size_t)(ix - page * kv.page_size) * kv.pos_stride);
   }
   return w;
 }
@@ -338,15 +338,16 @@ __device__ __forceinline__ SeqSpan seq_span(int raw_len, int cap, int window) {
   return r;
 }
 
-__device__ __forceinline__ float load_act(const void* p, size_t i, int dt) {
-  if (dt == BB_F32) return static_cast<const float*>(p)[i];
-  if (dt == BB_F16) return (float)static_cast<const _Float16*>(p)[i];
-  return (float)static_cast<const __bf16*>(p)[i];
+// Four adjacent elements of a row of type dt, at any element's alignment.
+template <class T>
+__device__ __forceinline__ void store_row(void* p, size_t i, const v4f& x) {
+  const T y[4] = {(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+  __builtin_memcpy(static_cast<T*>(p) + i, y, sizeof(y));
 }
-__device__ __forceinline__ void store_act(void* p, size_t i, int dt, float x) {
-  if (dt == BB_F32) static_cast<float*>(p)[i] = x;
-  else if (dt == BB_F16) static_cast<_Float16*>(p)[i] = (_Float16)x;
-  else static_cast<__bf16*>(p)[i] = (__bf16)x;
+__device__ __forceinline__ void store_act(void* p, size_t i, int dt, const v4f& x) {
+  if (dt == BB_F32) store_row<float>(p, i, x);
+  else if (dt == BB_F16) store_row<_Float16>(p, i, x);
+  else store_row<__bf16>(p, i, x);
 }
 
 // (by value: a bit cast of a vector's element itself reads the vector's first)
@@ -418,18 +419,32 @@ struct PaShape {
   static constexpr int NT = KT / 16;
 };
 
+// N elements (16 bytes or 8) of a row of type dt at any element's alignment, as f32.
+template <class T, int N>
+__device__ __forceinline__ void load_row(const void* p, size_t i, float (&x)[N]) {
+  T v[N];
+  __builtin_memcpy(v, static_cast<const T*>(p) + i, sizeof(v));
+#pragma unroll
+  for (int j = 0; j < N; ++j) x[j] = (float)v[j];
+}
+
 // One wave's part of a (sequence, head group) pair: running maximum m (base 2), sum l and o[i][r] for element
 // (16p + 4g + r)·PE + e, i = p·PE + e, of head n.
+// UNI: pages of whole 16 positions, whose rows are within 2^31 bytes of the first: 16 positions have one
+// address the same for the wave. Otherwise every lane finds the page of one position and the lanes
+// exchange them (16-bit cache, 8 kv heads of 64, 64 sequences of 4096: UNI_FIGURES).
+// What is not there or not attended to is loaded as 0 (a weight of 0 times what lies there need not be 0).
 template <int CT, int NP, int HDP, bool UNI>
 struct PaWave {
   typedef PaShape<CT, HDP> S;
   static constexpr int NT = S::NT, NC = S::NC, NV = S::NV, VE = S::VE, PE = S::PE, KE = S::KE, SZ = S::SZ;
   typedef typename std::conditional<S::PE * S::SZ == 16, v4u, v2u>::type VP;  // a piece of a value row
   const PagedView& kv;
-  const PagedSeqs& sq;
   const int n, g;
-  int s, head0, heads;  // head0: the first head of the group; heads: how many
-  size_t kv_off;        // the kv head's offset in the pool (elements)
+  const int* __restrict__ row;  // the sequence's page table
+  int max_pages;
+  int head0, heads;  // head0: the first head of the group; heads: how many
+  size_t kv_off;     // the kv head's offset in the pool (elements)
   SeqSpan sp;
   v4u q[NP][NC];
   int q_exp;   // f16: the row of q was scaled by 2^q_exp
@@ -440,11 +455,16 @@ struct PaWave {
   VP v[4 * NT][NV];
   uint32_t valid;  // bit 4t + r: position 16t + 4g + r of the tile whose values are loaded is attended to
 
-  __device__ __forceinline__ PaWave(const PagedView& kv_, const PagedSeqs& sq_, int lane)
-      : kv(kv_), sq(sq_), n(lane & 15), g(lane >> 4) {}
+  __device__ __forceinline__ PaWave(const PagedView& kv_, int lane) : kv(kv_), n(lane & 15), g(lane >> 4) {}
 
-  __device__ void start(const PagedQuery& pq) {
-    const size_t row = (size_t)s * pq.q_stride + (size_t)(head0 + n) * kv.hd;
+  template <class A>
+  __device__ __forceinline__ void load_q(const PagedQuery& pq, int s, float (&x)[NC][KE]) const {
+    const size_t at = (size_t)s * pq.q_stride + (size_t)(head0 + min(n, heads - 1)) * kv.hd;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) load_row<A, KE>(pq.q, at + min((4 * j + g) * KE, kv.hd - KE), x[j]);
+  }
+
+  __device__ __forceinline__ void start(const PagedQuery& pq, int s) {
     c = pq.scale * LOG2E;
     m = NEG_INF;
     l = 0.0f;
@@ -452,19 +472,21 @@ struct PaWave {
 #pragma unroll
     for (int i = 0; i < VE; ++i) o[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     float x[NC][KE];
+    if (pq.dt == BB_F32) load_q<float>(pq, s, x);
+    else if (pq.dt == BB_F16) load_q<_Float16>(pq, s, x);
+    else load_q<__bf16>(pq, s, x);
     float top = 0.0f;
 #pragma unroll
-    for (int j = 0; j < NC; ++j) {
-      const int d = (4 * j + g) * KE;
+    for (int j = 0; j < NC; ++j)
 #pragma unroll
-      for (int e = 0; e < KE; ++e) x[j][e] = n < heads && d < kv.hd ? load_act(pq.q, row + d + e, pq.dt) : 0.0f;
-#pragma unroll
-      for (int e = 0; e < KE; ++e) top = fmaxf(top, fabsf(x[j][e]));
-    }
+      for (int e = 0; e < KE; ++e) {
+        x[j][e] = n < heads && (4 * j + g) * KE < kv.hd ? x[j][e] : 0.0f;
+        top = fmaxf(top, fabsf(x[j][e]));
+      }
     if constexpr (CT == BB_F16) {
       // (0 and what is not finite keep their scale)
       top = group_max(top);
-      if (top > 0.0f && top < __builtin_inff()) q_exp = 14 - ilogbf(top) - 1;
+      if (top > 0.0f && top < __builtin_inff()) q_exp = 13 - ilogbf(top);
 #pragma unroll
       for (int j = 0; j < NC; ++j)
 #pragma unroll
@@ -487,82 +509,121 @@ struct PaWave {
     }
   }
 
-  // The places of a tile's positions. UNI (pages of whole 16 positions): off[t] is where the 16 positions t start,
-  // the same for the wave. Otherwise off[0] is lane i%32's: where position i of the tile is. -1: not there.
-  struct Places {
-    int64_t off[UNI ? NT : 1];
+  // The pages of a tile's positions: UNI, of each 16 (the same for the wave); otherwise lane l's is that of position
+  // l % KT of the tile. -1: not there, or not attended to.
+  struct Pages {
     int key0;
+    int page[UNI ? NT : 1];
   };
-  __device__ __forceinline__ Places places(int key0) const {
-    Places p;
+  __device__ __forceinline__ int page_at(int key, int end) const {
+    int pg = row[page_of(kv, min(key, sp.len - 1))];
+    if constexpr (UNI) pg = __builtin_amdgcn_readfirstlane(pg);
+    return key < end && (uint32_t)pg < (uint32_t)kv.n_pages ? pg : -1;
+  }
+  __device__ __forceinline__ Pages pages(int key0, int end) const {
+    Pages p;
     p.key0 = key0;
     if constexpr (UNI) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int key = key0 + 16 * t;
-        int64_t b = -1;
-        if (key < sp.len) {
-          const int page = key / kv.page_size;
-          b = page_base(kv, sq, s, page);
-          if (b >= 0) b += (int64_t)((size_t)(key - page * kv.page_size) * kv.pos_stride + kv_off);
-        }
-        p.off[t] = b;
-      }
+      for (int t = 0; t < NT; ++t) p.page[t] = page_at(key0 + 16 * t, end);
     } else {
       const int key = key0 + ((n + 16 * g) & (S::KT - 1));
-      int64_t b = -1;
-      if (key < sp.len && key >= sp.first) {
-        const int page = key / kv.page_size;
-        b = page_base(kv, sq, s, page);
-        if (b >= 0) b += (int64_t)((size_t)(key - page * kv.page_size) * kv.pos_stride + kv_off);
-      }
-      p.off[0] = b;
+      p.page[0] = key >= sp.first ? page_at(key, end) : -1;
     }
     return p;
   }
+  // Where position `key` of a page starts in the pool (elements).
+  __device__ __forceinline__ size_t place(int page, int key) const {
+    return (size_t)page * kv.page_stride + (size_t)(key - page_of(kv, key) * kv.page_size) * kv.pos_stride + kv_off;
+  }
+  // Otherwise: the places of all the tile's positions, one a lane (-1: not there).
+  __device__ __forceinline__ int64_t lane_place(const Pages& p) const {
+    return p.page[0] < 0 ? -1 : (int64_t)place(p.page[0], p.key0 + ((n + 16 * g) & (S::KT - 1)));
+  }
 
-  __device__ __forceinline__ void load_k(const Places& p) {
-    const char* base = static_cast<const char*>(kv.k);
+  // UNI: the rows of 16 positions as a buffer that ends with row `rows` - 1 (0 rows: all of it reads as 0).
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* pool, const Pages& p, int t, int rows) const {
+    const bool there = p.page[t] >= 0 && rows > 0;
+    const char* base = static_cast<const char*>(pool) + (there ? place(p.page[t], p.key0 + 16 * t) * SZ : 0);
+    const uint32_t bytes = there ? (uint32_t)(rows - 1) * stride() + (uint32_t)(kv.hd * SZ) : 0;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, bytes, 0x00027000);
+  }
+  __device__ __forceinline__ uint32_t stride() const { return (uint32_t)kv.pos_stride * SZ; }
+
+  __device__ __forceinline__ void load_k(const Pages& p) {
+    if constexpr (UNI) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      int64_t at;
-      if constexpr (UNI) at = p.off[t] < 0 ? -1 : p.off[t] + (int64_t)((size_t)n * kv.pos_stride);
-      else at = __shfl(p.off[0], n + 16 * t);
+      for (int t = 0; t < NT; ++t) {
+        const auto rows = rows_of(kv.k, p, t, 16);
 #pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        const int d = (4 * j + g) * KE;
-        k[t][j] = v4u{0, 0, 0, 0};
-        if (at >= 0 && d < kv.hd) k[t][j] = *reinterpret_cast<const v4u*>(base + (size_t)(at + d) * SZ);
+        for (int j = 0; j < NC; ++j) {
+          // (pieces past the head: 0, which 0 times what lies there need not be)
+          const int d = (4 * j + g) * KE;
+          const uint32_t at = d < kv.hd ? (uint32_t)n * stride() + (uint32_t)(d * SZ) : 0x80000000u;
+          k[t][j] = __builtin_amdgcn_raw_buffer_load_b128(rows, at, 0, 0);
+        }
+      }
+    } else {
+      const int64_t mine = lane_place(p);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int64_t at = __shfl(mine, n + 16 * t);
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          const int d = (4 * j + g) * KE;
+          k[t][j] = v4u{0, 0, 0, 0};
+          if (at >= 0 && d < kv.hd) k[t][j] = *reinterpret_cast<const v4u*>(static_cast<const char*>(kv.k) + (size_t)(at + d) * SZ);
+        }
       }
     }
   }
 
-  __device__ __forceinline__ void load_v(const Places& p) {
-    const char* base = static_cast<const char*>(kv.v);
+  __device__ __forceinline__ void load_v(const Pages& p) {
     valid = 0;
+    if constexpr (UNI) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t) {
+        const int k0 = p.key0 + 16 * t, skip = max(0, sp.first - k0);
+        const auto rows = rows_of(kv.v, p, t, min(16, sp.len - k0));
+        if (p.page[t] >= 0) {
+          if (skip == 0 && k0 + 16 <= sp.len) {
+            valid |= 15u << 4 * t;
+          } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * t + 4 * g + r;
-        int64_t at;
-        if constexpr (UNI) {
-          const int key = p.key0 + i;
-          at = p.off[t] < 0 || key < sp.first || key >= sp.len
-                   ? -1
-                   : p.off[t] + (int64_t)((size_t)(4 * g + r) * kv.pos_stride);
-        } else {
-          at = __shfl(p.off[0], i);
+            for (int r = 0; r < 4; ++r)
+              valid |= (4 * g + r >= skip && 4 * g + r < sp.len - k0 ? 1u : 0u) << (4 * t + r);
+          }
         }
-        valid |= (at >= 0 ? 1u : 0u) << (4 * t + r);
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          const int d = (16 * j + n) * PE;
-          VP z{};
-          if (at >= 0 && d < kv.hd) z = *reinterpret_cast<const VP*>(base + (size_t)(at + d) * SZ);
-          v[4 * t + r][j] = z;
+        for (int r = 0; r < 4; ++r) {
+          // (pieces past the head end in elements of o that nobody reads)
+          const uint32_t at = 4 * g + r < skip ? 0x80000000u : (uint32_t)(4 * g + r) * stride() + (uint32_t)(n * PE * SZ);
+#pragma unroll
+          for (int j = 0; j < NV; ++j) {
+            if constexpr (PE * SZ == 16)
+              v[4 * t + r][j] = __builtin_amdgcn_raw_buffer_load_b128(rows, at + (uint32_t)(16 * j * PE * SZ), 0, 0);
+            else
+              v[4 * t + r][j] = __builtin_amdgcn_raw_buffer_load_b64(rows, at + (uint32_t)(16 * j * PE * SZ), 0, 0);
+          }
         }
       }
+    } else {
+      const int64_t mine = lane_place(p);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int64_t at = __shfl(mine, 16 * t + 4 * g + r);
+          valid |= (at >= 0 ? 1u : 0u) << (4 * t + r);
+#pragma unroll
+          for (int j = 0; j < NV; ++j) {
+            const int d = (16 * j + n) * PE;
+            v[4 * t + r][j] = VP{};
+            if (at >= 0 && d < kv.hd)
+              v[4 * t + r][j] = *reinterpret_cast<const VP*>(static_cast<const char*>(kv.v) + (size_t)(at + d) * SZ);
+          }
+        }
+    }
   }
 
   template <int PARTS>
@@ -584,7 +645,7 @@ struct PaWave {
       }
   }
 
-  // Scores of the loaded keys (base-2 exponents, masked), from which the keys' registers are free again.
+  // Scores of the loaded keys, from which the keys' registers are free again.
   __device__ __forceinline__ void score(v4f (&x)[NT]) const {
     scores<NP>(x);
     if constexpr (NP > 1) {
@@ -668,106 +729,135 @@ struct PaWave {
   }
 
   // Positions key, key + step, ... below end.
-  __device__ void run(int key, int end, int step) {
+  __device__ __forceinline__ void run(int key, int end, int step) {
     if (key >= end) return;
-    Places p = places(key);
+    Pages p = pages(key, end);
     load_k(p);
     load_v(p);
-    for (;;) {
+    // (The scheduler is held to this order: a load that moved up would need a second set of registers. The
+    // last turn's loads are of no pages and touch no memory.)
+    for (; key < end; key += step) {
       v4f x[NT];
-      const int next = key + step;
-      const bool more = next < end;
-      if (more) p = places(next);
+      p = pages(key + step, end);
+      __builtin_amdgcn_sched_barrier(0);
       score(x);
-      if (more) load_k(p);
+      __builtin_amdgcn_sched_barrier(0);
+      load_k(p);
+      __builtin_amdgcn_sched_barrier(0);
       add(x);
-      if (!more) return;
+      __builtin_amdgcn_sched_barrier(0);
       load_v(p);
-      key = next;
     }
   }
 };
 
-template <int CT, int NP, int HDP, bool UNI>
-__global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQuery pq, PagedView kv, PagedSeqs sq,
-                                                                        PagedPlan pl) {
-  typedef PaShape<CT, HDP> S;
-  constexpr int LD = HDP + 4;
-  extern __shared__ float so[];  // [waves][hg][LD]
-  __shared__ float s_m[PA_WAVES][PA_HEADS], s_l[PA_WAVES][PA_HEADS];
-  __shared__ int s_scan[PA_WAVES], s_at[3];
-  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int cap = sq.max_pages * kv.page_size;
-
-  // units of 256 sequences from c0, their running sum within the 256 (inclusive) and their total
-  int c0 = 0, carry = 0, mine = 0, incl = 0, part = 0;
-  const auto scan = [&]() {
-    const int i = c0 + tid;
-    mine = i < sq.n_seqs ? seq_span(sq.lens[i], cap, pq.window).units : 0;
-    incl = mine;
-    for (int o = 1; o < 64; o <<= 1) {
+// The sequences' units as a wave holds them: lane l has sequences 4l..4l+3 of the 256 from c0.
+struct SeqScan {
+  int c0, before;  // units of the sequences before c0
+  int len[4], units[4], incl;
+  int all;         // of the 256
+  __device__ __forceinline__ void load(const int* __restrict__ lens, int n_seqs, int cap, int window, int lane) {
+    const int left = n_seqs - c0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) len[i] = lens[c0 + min(4 * lane + i, left - 1)];
+    incl = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      units[i] = 4 * lane + i < left ? seq_span(len[i], cap, window).units : 0;
+      incl += units[i];
+    }
+    const int lanes = min(64, (left + 3) / 4);
+    for (int o = 1; o < lanes; o <<= 1) {
       const int y = __shfl_up(incl, o);
       if (lane >= o) incl += y;
     }
-    __syncthreads();
-    if (lane == 63) s_scan[wv] = incl;
-    __syncthreads();
-    part = 0;
-#pragma unroll
-    for (int w = 0; w < PA_WAVES; ++w) {
-      if (w < wv) incl += s_scan[w];
-      part += s_scan[w];
-    }
-  };
-  int total = 0;
-  for (c0 = 0; c0 < sq.n_seqs; c0 += PA_THREADS) {
-    scan();
-    if (pl.join && blockIdx.x == 0 && c0 + tid < sq.n_seqs) pl.chunk[2 + c0 + tid] = total + incl;
-    total += part;
+    all = __builtin_amdgcn_readlane(incl, lanes - 1);
   }
-  const int chunk = (total * pl.n_groups + (int)gridDim.x - 1) / (int)gridDim.x;
+};
+
+template <int CT, int NP, int HDP, bool UNI>
+__global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQuery pq, PagedView kv,
+                                                                        const int* __restrict__ table,
+                                                                        const int* __restrict__ lens, size_t table_stride,
+                                                                        int n_seqs, int max_pages, PagedPlan pl) {
+  typedef PaShape<CT, HDP> S;
+  constexpr int LD = HDP + 4, ROW4 = HDP / 4;
+  extern __shared__ __align__(16) float so[];  // [waves][hg][LD]
+  __shared__ float s_m[PA_WAVES][PA_HEADS], s_l[PA_WAVES][PA_HEADS];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int cap = max_pages * kv.page_size;
+
+  // every wave finds the block's run by itself
+  SeqScan sc;
+  int total = 0;
+  for (sc.c0 = 0;; sc.c0 += 256) {
+    sc.load(lens, n_seqs, cap, pq.window, lane);
+    if (pl.join && blockIdx.x == 0 && wv == 0) {
+      int sum = total + sc.incl - sc.units[0] - sc.units[1] - sc.units[2] - sc.units[3];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sum += sc.units[i];
+        if (sc.c0 + 4 * lane + i < n_seqs) pl.chunk[2 + sc.c0 + 4 * lane + i] = sum;
+      }
+    }
+    total += sc.all;
+    if (sc.c0 + 256 >= n_seqs) break;
+  }
+  total *= pl.n_groups;
+  const int chunk = (total + (int)gridDim.x - 1) / (int)gridDim.x;
   if (pl.join && blockIdx.x == 0 && tid == 0) {
     pl.chunk[0] = chunk;
     pl.chunk[1] = 0;
   }
-  int64_t u64 = (int64_t)blockIdx.x * chunk;
-  if (u64 >= (int64_t)total * pl.n_groups) return;
-  int u = (int)u64;
-  const int end = min(u + chunk, total * pl.n_groups);
-  c0 = 0;
-  if (sq.n_seqs > PA_THREADS) scan();
+  if ((int64_t)blockIdx.x * chunk >= total) return;
+  int u = (int)blockIdx.x * chunk;
+  const int end = min(u + chunk, total);
+  if (sc.c0 > 0) {
+    sc.c0 = 0;
+    sc.load(lens, n_seqs, cap, pq.window, lane);
+  }
+  sc.before = 0;
 
-  PaWave<CT, NP, HDP, UNI> w(kv, sq, lane);
+  PaWave<CT, NP, HDP, UNI> w(kv, lane);
+  w.max_pages = max_pages;
   const float up = CT == BB_F16 ? 14.0f : 0.0f;
   for (bool first_pair = true; u < end; first_pair = false) {
-    // the sequence of unit u
-    while (u >= (carry + part) * pl.n_groups) {
-      carry += part;
-      c0 += PA_THREADS;
-      scan();
+    // the sequence of unit u: the first lane whose units reach past it, the first of its four
+    while (u >= (sc.before + sc.all) * pl.n_groups) {
+      sc.before += sc.all;
+      sc.c0 += 256;
+      sc.load(lens, n_seqs, cap, pq.window, lane);
     }
-    __syncthreads();  // (s_at, and the sums of the pair before)
-    const int lo = (carry + incl - mine) * pl.n_groups;
-    if (mine > 0 && u >= lo && u < lo + mine * pl.n_groups) {
-      s_at[0] = c0 + tid;
-      s_at[1] = lo;
-      s_at[2] = mine;
+    const int at = __builtin_ctzll(__ballot((sc.before + sc.incl) * pl.n_groups > u));
+    int s = sc.c0 + 4 * at, nu = 0, len = 0;
+    int seq_lo = sc.before + __builtin_amdgcn_readlane(sc.incl - sc.units[0] - sc.units[1] - sc.units[2] - sc.units[3], at);
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int x = __builtin_amdgcn_readlane(sc.units[i], at), y = __builtin_amdgcn_readlane(sc.len[i], at);
+      if (!found) {
+        nu = x;
+        len = y;
+        found = (seq_lo + x) * pl.n_groups > u;
+        if (!found) {
+          seq_lo += x;
+          ++s;
+        }
+      }
     }
-    __syncthreads();
-    const int s = __builtin_amdgcn_readfirstlane(s_at[0]);
-    const int seq_lo = __builtin_amdgcn_readfirstlane(s_at[1]), nu = __builtin_amdgcn_readfirstlane(s_at[2]);
-    const int grp = (u - seq_lo) / nu, u0 = (u - seq_lo) - grp * nu, take = min(nu - u0, end - u);
+    const int in = u - seq_lo * pl.n_groups, grp = in / nu, u0 = in - grp * nu, take = min(nu - u0, end - u);
     const int kvh = grp / pl.split, sub = grp - kvh * pl.split;
-    w.s = s;
+    w.row = table + (size_t)s * table_stride;
     w.head0 = kvh * (pq.n_heads / kv.n_kv) + sub * pl.hg;
     w.heads = min(pl.hg, pq.n_heads / kv.n_kv - sub * pl.hg);
     w.kv_off = (size_t)kvh * kv.head_stride;
-    w.sp = seq_span(sq.lens[s], cap, pq.window);
-    w.start(pq);
+    w.sp = seq_span(len, cap, pq.window);
+    w.start(pq, s);
     const int k0 = w.sp.base + u0 * PA_UNIT;
     w.run(k0 + wv * S::KT, min(k0 + take * PA_UNIT, w.sp.len), PA_WAVES * S::KT);
 
     // the waves' sums together
+    if (!first_pair) __syncthreads();  // (the pair before is done with LDS)
     const float l_all = group_sum(w.l);
     if (w.g == 0) {
       s_m[wv][w.n] = w.m;
@@ -779,33 +869,39 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
     for (int i = 0; i < PA_WAVES; ++i) top = fmaxf(top, s_m[i][w.n]);
     const float f = __builtin_amdgcn_exp2f(w.m - (top == NEG_INF ? 0.0f : top));
     if (w.n < w.heads) {
-      float* to = so + ((size_t)wv * pl.hg + w.n) * LD;
+      float* to = so + (wv * pl.hg + w.n) * LD;
 #pragma unroll
       for (int p = 0; p < S::NV; ++p)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-          for (int e = 0; e < S::PE; ++e) to[(16 * p + 4 * w.g + r) * S::PE + e] = w.o[p * S::PE + e][r] * f;
+          for (int e = 0; e < S::PE; e += 4)
+            *reinterpret_cast<v4f*>(to + (16 * p + 4 * w.g + r) * S::PE + e) =
+                v4f{w.o[p * S::PE + e][r], w.o[p * S::PE + e + 1][r], w.o[p * S::PE + e + 2][r],
+                    w.o[p * S::PE + e + 3][r]} * f;
     }
     __syncthreads();
     const bool whole = take == nu;
     const size_t slot = 2 * (size_t)blockIdx.x + (first_pair ? 0 : 1);
-    for (int i = tid; i < w.heads * kv.hd; i += PA_THREADS) {
-      const int h = i / kv.hd, d = i - h * kv.hd;
-      float mm = NEG_INF, ll = 0.0f, x = 0.0f;
+    for (int i = tid; i < w.heads * ROW4; i += PA_THREADS) {
+      const int h = i / ROW4, d = 4 * (i % ROW4);
+      if (d >= kv.hd) continue;
+      float mm = NEG_INF, ll = 0.0f;
+      v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int j = 0; j < PA_WAVES; ++j) mm = fmaxf(mm, s_m[j][h]);
 #pragma unroll
       for (int j = 0; j < PA_WAVES; ++j) {
         ll += s_l[j][h] * __builtin_amdgcn_exp2f(s_m[j][h] - (mm == NEG_INF ? 0.0f : mm));
-        x += so[((size_t)j * pl.hg + h) * LD + d];
+        x += *reinterpret_cast<const v4f*>(so + (j * pl.hg + h) * LD + d);
       }
       if (whole) {
         const bool none = mm == NEG_INF && ll == 0.0f;
-        store_act(pq.out, (size_t)s * pq.out_stride + (size_t)(w.head0 + h) * kv.hd + d, pq.dt, none ? 0.0f : x / ll);
+        store_act(pq.out, (size_t)s * pq.out_stride + (size_t)(w.head0 + h) * kv.hd + d, pq.dt,
+                  none ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : x / ll);
         if (d == 0 && pq.lse) pq.lse[(size_t)s * pq.n_heads + w.head0 + h] = none ? NEG_INF : (mm + log2f(ll) - up) * LN2;
       } else {
-        pl.sums[(slot * pl.hg + h) * kv.hd + d] = x;
+        *reinterpret_cast<v4f*>(pl.sums + (slot * pl.hg + h) * kv.hd + d) = x;
         if (d == 0) pl.ml[slot * pl.hg + h] = make_float2(mm, ll);
       }
     }
@@ -840,6 +936,7 @@ __global__ void __launch_bounds__(PJ_THREADS) k_paged_join(PagedQuery pq, int n_
   const int piece = tid & (np - 1), rows = PJ_THREADS / np;
   float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float l = 0.0f;
+#pragma unroll 4
   for (int i = tid / np; i < parts; i += rows) {
     const size_t at = slot(i);
     const float2 ml = pl.ml[at];
@@ -858,14 +955,16 @@ __global__ void __launch_bounds__(PJ_THREADS) k_paged_join(PagedQuery pq, int n_
   __shared__ float lsum[PJ_THREADS];
   if (piece == 0) lsum[tid / np] = l;
   __syncthreads();
-  if (tid < hd) {
-    float y = 0.0f, ll = 0.0f;
+  if (4 * tid < hd) {
+    v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
+    float ll = 0.0f;
     for (int i = 0; i < rows; ++i) {
-      y += acc[4 * (i * np + tid / 4) + tid % 4];
+      y += reinterpret_cast<const v4f*>(acc)[i * np + tid];
       ll += lsum[i];
     }
     const bool none = top == NEG_INF && ll == 0.0f;
-    store_act(pq.out, (size_t)s * pq.out_stride + (size_t)h * hd + tid, pq.dt, none ? 0.0f : y / ll);
+    store_act(pq.out, (size_t)s * pq.out_stride + (size_t)h * hd + 4 * tid, pq.dt,
+              none ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : y / ll);
     if (tid == 0 && pq.lse) pq.lse[(size_t)s * pq.n_heads + h] = none ? NEG_INF : (top + log2f(ll) - up) * LN2;
   }
 }
@@ -891,6 +990,13 @@ bool paged_attn_fits(int n_seqs, int n_heads, int n_kv, size_t cap) {
   return (size_t)n_seqs * (size_t)p.n_groups * ((cap + PA_UNIT - 1) / PA_UNIT) < ((size_t)1 << 30);
 }
 
+void paged_divisor(PagedView& v) {
+  v.page_shift = 0;
+  while ((1 << v.page_shift) < v.page_size) ++v.page_shift;
+  const uint64_t two = (uint64_t)1 << (31 + v.page_shift);
+  v.page_mul = (uint32_t)((two + v.page_size - 1) / v.page_size);
+}
+
 size_t paged_attn_ws(int n_cu, int n_seqs, int n_heads, int n_kv, int hd) {
   const PagedPlan p = pa_plan(n_seqs, n_heads, n_kv);
   const size_t slots = 2 * (size_t)pa_blocks(n_cu, hd) * p.hg;
@@ -910,13 +1016,17 @@ hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQue
   const size_t units = (size_t)sq.n_seqs * pl.n_groups * ((cap + PA_UNIT - 1) / PA_UNIT);
   const unsigned blocks = (unsigned)std::min<size_t>(blocks_max, units);
   pl.join = cap > (size_t)PA_UNIT;  // else every pair is one unit
-  const bool uni = kv.page_size % 16 == 0;
+  const bool uni = kv.page_size % 16 == 0 && 16 * kv.pos_stride < ((size_t)1 << 29);
   const int cls = pa_class(kv.hd);
   const size_t lds = (size_t)PA_WAVES * pl.hg * (cls + 4) * 4;
 #define BB_PA(ct, np, hdp)                                                                                     \
   do {                                                                                                         \
-    if (uni) BB_LAUNCH((k_paged_attn<ct, np, hdp, true>), dim3(blocks), dim3(PA_THREADS), lds, st, q, kv, sq, pl); \
-    else BB_LAUNCH((k_paged_attn<ct, np, hdp, false>), dim3(blocks), dim3(PA_THREADS), lds, st, q, kv, sq, pl);    \
+    if (uni)                                                                                                   \
+      BB_LAUNCH((k_paged_attn<ct, np, hdp, true>), dim3(blocks), dim3(PA_THREADS), lds, st, q, kv, sq.table,   \
+                sq.lens, sq.table_stride, sq.n_seqs, sq.max_pages, pl);                                        \
+    else                                                                                                       \
+      BB_LAUNCH((k_paged_attn<ct, np, hdp, false>), dim3(blocks), dim3(PA_THREADS), lds, st, q, kv, sq.table,  \
+                sq.lens, sq.table_stride, sq.n_seqs, sq.max_pages, pl);                                        \
   } while (0)
 #define BB_PA_HD(ct, np)             \
   do {                               \
