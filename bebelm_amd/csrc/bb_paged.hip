@@ -285,8 +285,9 @@ hipError_t launch_rope_rows(hipStream_t s, int dtype, int cache, const RopeRows&
 // Work. A sequence's positions (from its window's first, rounded down to 32) are cut into units of 128,
 // and the units of all (sequence, head group) pairs, in that order, into equal runs, one a block: every
 // block reads about the same number of bytes however ragged the batch, with no host knowing a
-// length. A block's 4 waves take tiles of KT = 32 positions in turn and are joined in LDS at the end of
-// a pair; a pair that lies in several blocks leaves one partial sum each, which k_paged_join adds.
+// length. A pair counts PA_PAIR units more than it has, before its first, for what it costs to begin
+// and end it. A block's 4 waves take tiles of KT = 32 positions in turn and are joined in LDS at the end
+// of a pair; a pair that lies in several blocks leaves one partial sum each, which k_paged_join adds.
 //
 // Tiles on the matrix cores, with nothing moved between lanes. Lane l has column (head) n = l%16 and group
 // g = l/16. Scores are D[position][head] = K·q^T: A holds 16 positions' rows (lane: row l%16, the group's
@@ -308,6 +309,7 @@ namespace {
 
 constexpr int PA_WAVES = 4, PA_THREADS = 64 * PA_WAVES;
 constexpr int PA_UNIT = 128;      // positions of a unit: a tile for each wave
+constexpr int PA_PAIR = 2;        // what a pair costs besides its units
 constexpr int PA_HEADS = 16;      // heads of a group at most
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr float NEG_INF = -__builtin_inff();
@@ -318,11 +320,11 @@ typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
-// Heads of a kv head's query heads: `split` groups of `hg` (the last may have fewer).
+// A kv head's G query heads: `split` groups of `hg` (the last may have fewer).
 struct PagedPlan {
-  int split, hg, n_groups, join;
-  int* chunk;     // [1 + n_seqs + 1]: units of a block's run, units before each sequence
-  float* sums;    // [2·blocks][hg][hd]
+  int G, split, hg, n_groups, join;
+  int* chunk;     // [1 + n_seqs + 1]: cost of a block's run, cost of a group in the sequences before each
+  float* sums;    // [2·blocks][hg][hd]: of a pair that began in a block before (slot 0), that goes on in the next (1)
   float2* ml;     // [2·blocks][hg]: maximum (base 2), sum of weights
 };
 
@@ -394,13 +396,37 @@ __device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-__device__ __forceinline__ float group_max(float x) {  // over the four lanes of a column
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+// The four lanes of a column (l, l^16, l^32, l^48): (x, y) -> (lower rows of x and y, upper rows of both).
+__device__ __forceinline__ float group_max(float x) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(as_float(a[0]), as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(as_float(b[0]), as_float(b[1]));
 }
 __device__ __forceinline__ float group_sum(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = as_float(a[0]) + as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return as_float(b[0]) + as_float(b[1]);
+}
+
+// Inclusive sums over the wave's lanes.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the row before's last lane, to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row 1's last lane, to rows 2 and 3
+  return x;
+}
+
+// a / b for 0 <= a < 2^30, b >= 1 and a quotient below 2^20, the same for the wave: the f32 quotient is off by less than 1.
+__device__ __forceinline__ int small_div(int a, int b) {
+  int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
+  q -= q * b > a ? 1 : 0;
+  q += (q + 1) * b <= a ? 1 : 0;
+  return __builtin_amdgcn_readfirstlane(q);
 }
 
 // Waves of a SIMD at a time for head sizes up to hdp: 128, 256, 512 registers each.
@@ -442,18 +468,17 @@ struct PaWave {
   const PagedView& kv;
   const int n, g;
   const int* __restrict__ row;  // the sequence's page table
-  int max_pages;
   int head0, heads;  // head0: the first head of the group; heads: how many
   size_t kv_off;     // the kv head's offset in the pool (elements)
   SeqSpan sp;
   v4u q[NP][NC];
-  int q_exp;   // f16: the row of q was scaled by 2^q_exp
-  float c;     // scale·log2(e)
+  float c;        // what scores are multiplied by where NP is 2
   float m, l;
   v4f o[VE];
   v4u k[NT][NC];
   VP v[4 * NT][NV];
   uint32_t valid;  // bit 4t + r: position 16t + 4g + r of the tile whose values are loaded is attended to
+  static constexpr uint32_t ALL = (1u << 4 * NT) - 1;
 
   __device__ __forceinline__ PaWave(const PagedView& kv_, int lane) : kv(kv_), n(lane & 15), g(lane >> 4) {}
 
@@ -465,32 +490,35 @@ struct PaWave {
   }
 
   __device__ __forceinline__ void start(const PagedQuery& pq, int s) {
-    c = pq.scale * LOG2E;
     m = NEG_INF;
     l = 0.0f;
-    q_exp = 0;
 #pragma unroll
     for (int i = 0; i < VE; ++i) o[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     float x[NC][KE];
     if (pq.dt == BB_F32) load_q<float>(pq, s, x);
     else if (pq.dt == BB_F16) load_q<_Float16>(pq, s, x);
     else load_q<__bf16>(pq, s, x);
-    float top = 0.0f;
+    // scores are exponents of 2; parts that are all of an f32 take the factor in, two parts only hold q itself
+    c = pq.scale * LOG2E;
+    const float cq = NP == 2 ? 1.0f : c;
 #pragma unroll
     for (int j = 0; j < NC; ++j)
 #pragma unroll
-      for (int e = 0; e < KE; ++e) {
-        x[j][e] = n < heads && (4 * j + g) * KE < kv.hd ? x[j][e] : 0.0f;
-        top = fmaxf(top, fabsf(x[j][e]));
-      }
+      for (int e = 0; e < KE; ++e) x[j][e] = n < heads && (4 * j + g) * KE < kv.hd ? x[j][e] * cq : 0.0f;
     if constexpr (CT == BB_F16) {
-      // (0 and what is not finite keep their scale)
-      top = group_max(top);
-      if (top > 0.0f && top < __builtin_inff()) q_exp = 13 - ilogbf(top);
+      float top = 0.0f;
 #pragma unroll
       for (int j = 0; j < NC; ++j)
 #pragma unroll
-        for (int e = 0; e < KE; ++e) x[j][e] = ldexpf(x[j][e], q_exp);
+        for (int e = 0; e < KE; ++e) top = fmaxf(top, fabsf(x[j][e]));
+      // (0 and what is not finite keep their scale)
+      top = group_max(top);
+      const int e2 = top > 0.0f && top < __builtin_inff() ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
+      c = ldexpf(c, -e2);
+#pragma unroll
+      for (int j = 0; j < NC; ++j)
+#pragma unroll
+        for (int e = 0; e < KE; ++e) x[j][e] = ldexpf(x[j][e], e2);
     }
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
@@ -509,52 +537,48 @@ struct PaWave {
     }
   }
 
-  // The pages of a tile's positions: UNI, of each 16 (the same for the wave); otherwise lane l's is that of position
-  // l % KT of the tile. -1: not there, or not attended to.
-  struct Pages {
+  // Where a tile's positions are in the pool (elements; -1: not there, or not attended to): UNI, each 16, the same for
+  // the wave; otherwise lane l's is position l % KT's.
+  struct Places {
     int key0;
-    int page[UNI ? NT : 1];
+    int64_t at[UNI ? NT : 1];
   };
-  __device__ __forceinline__ int page_at(int key, int end) const {
-    int pg = row[page_of(kv, min(key, sp.len - 1))];
+  __device__ __forceinline__ int64_t place(int key, int end) const {
+    const int i = min(key, sp.len - 1), entry = page_of(kv, i);
+    int pg = row[entry];
     if constexpr (UNI) pg = __builtin_amdgcn_readfirstlane(pg);
-    return key < end && (uint32_t)pg < (uint32_t)kv.n_pages ? pg : -1;
+    const bool there = key < end && (uint32_t)pg < (uint32_t)kv.n_pages;
+    const int64_t at = (int64_t)((size_t)(uint32_t)pg * kv.page_stride +
+                                 (size_t)(uint32_t)(i - entry * kv.page_size) * kv.pos_stride + kv_off);
+    return there ? at : -1;
   }
-  __device__ __forceinline__ Pages pages(int key0, int end) const {
-    Pages p;
+  __device__ __forceinline__ Places places(int key0, int end) const {
+    Places p;
     p.key0 = key0;
     if constexpr (UNI) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) p.page[t] = page_at(key0 + 16 * t, end);
+      for (int t = 0; t < NT; ++t) p.at[t] = place(key0 + 16 * t, end);
     } else {
       const int key = key0 + ((n + 16 * g) & (S::KT - 1));
-      p.page[0] = key >= sp.first ? page_at(key, end) : -1;
+      p.at[0] = place(key, key >= sp.first ? end : 0);
     }
     return p;
   }
-  // Where position `key` of a page starts in the pool (elements).
-  __device__ __forceinline__ size_t place(int page, int key) const {
-    return (size_t)page * kv.page_stride + (size_t)(key - page_of(kv, key) * kv.page_size) * kv.pos_stride + kv_off;
-  }
-  // Otherwise: the places of all the tile's positions, one a lane (-1: not there).
-  __device__ __forceinline__ int64_t lane_place(const Pages& p) const {
-    return p.page[0] < 0 ? -1 : (int64_t)place(p.page[0], p.key0 + ((n + 16 * g) & (S::KT - 1)));
-  }
 
   // UNI: the rows of 16 positions as a buffer that ends with row `rows` - 1 (0 rows: all of it reads as 0).
-  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* pool, const Pages& p, int t, int rows) const {
-    const bool there = p.page[t] >= 0 && rows > 0;
-    const char* base = static_cast<const char*>(pool) + (there ? place(p.page[t], p.key0 + 16 * t) * SZ : 0);
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* pool, int64_t at, int rows) const {
+    const bool there = at >= 0 && rows > 0;
+    const char* base = static_cast<const char*>(pool) + (there ? (size_t)at * SZ : 0);
     const uint32_t bytes = there ? (uint32_t)(rows - 1) * stride() + (uint32_t)(kv.hd * SZ) : 0;
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, bytes, 0x00027000);
   }
   __device__ __forceinline__ uint32_t stride() const { return (uint32_t)kv.pos_stride * SZ; }
 
-  __device__ __forceinline__ void load_k(const Pages& p) {
+  __device__ __forceinline__ void load_k(const Places& p) {
     if constexpr (UNI) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const auto rows = rows_of(kv.k, p, t, 16);
+        const auto rows = rows_of(kv.k, p.at[t], 16);
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
           // (pieces past the head: 0, which 0 times what lies there need not be)
@@ -564,10 +588,9 @@ struct PaWave {
         }
       }
     } else {
-      const int64_t mine = lane_place(p);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const int64_t at = __shfl(mine, n + 16 * t);
+        const int64_t at = __shfl(p.at[0], n + 16 * t);
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
           const int d = (4 * j + g) * KE;
@@ -578,14 +601,14 @@ struct PaWave {
     }
   }
 
-  __device__ __forceinline__ void load_v(const Pages& p) {
+  __device__ __forceinline__ void load_v(const Places& p) {
     valid = 0;
     if constexpr (UNI) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const int k0 = p.key0 + 16 * t, skip = max(0, sp.first - k0);
-        const auto rows = rows_of(kv.v, p, t, min(16, sp.len - k0));
-        if (p.page[t] >= 0) {
+        const auto rows = rows_of(kv.v, p.at[t], min(16, sp.len - k0));
+        if (p.at[t] >= 0) {
           if (skip == 0 && k0 + 16 <= sp.len) {
             valid |= 15u << 4 * t;
           } else {
@@ -608,12 +631,11 @@ struct PaWave {
         }
       }
     } else {
-      const int64_t mine = lane_place(p);
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int64_t at = __shfl(mine, 16 * t + 4 * g + r);
+          const int64_t at = __shfl(p.at[0], 16 * t + 4 * g + r);
           valid |= (at >= 0 ? 1u : 0u) << (4 * t + r);
 #pragma unroll
           for (int j = 0; j < NV; ++j) {
@@ -668,17 +690,21 @@ struct PaWave {
 
   // Adds a tile: its scores x and the loaded values.
   __device__ __forceinline__ void add(v4f (&x)[NT]) {
+    if constexpr (NP == 2) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) x[t] *= c;
+    }
+    if (__any(valid != ALL)) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[t][r] = valid >> (4 * t + r) & 1 ? x[t][r] : NEG_INF;
+    }
     float mx = NEG_INF;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float y = x[t][r];
-        if constexpr (CT == BB_F16) y = ldexpf(y, -q_exp);
-        y = valid >> (4 * t + r) & 1 ? y * c : NEG_INF;
-        x[t][r] = y;
-        mx = fmaxf(mx, y);
-      }
+      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, x[t][r]);
     mx = fmaxf(m, group_max(mx));
     const float ref = mx == NEG_INF ? 0.0f : mx;
     if (__any(mx > m)) {
@@ -731,14 +757,14 @@ struct PaWave {
   // Positions key, key + step, ... below end.
   __device__ __forceinline__ void run(int key, int end, int step) {
     if (key >= end) return;
-    Pages p = pages(key, end);
+    Places p = places(key, end);
     load_k(p);
     load_v(p);
     // (The scheduler is held to this order: a load that moved up would need a second set of registers. The
     // last turn's loads are of no pages and touch no memory.)
     for (; key < end; key += step) {
       v4f x[NT];
-      p = pages(key + step, end);
+      p = places(key + step, end);
       __builtin_amdgcn_sched_barrier(0);
       score(x);
       __builtin_amdgcn_sched_barrier(0);
@@ -751,27 +777,25 @@ struct PaWave {
   }
 };
 
-// The sequences' units as a wave holds them: lane l has sequences 4l..4l+3 of the 256 from c0.
+// The sequences' costs (units + PA_PAIR) as a wave holds them: lane l has sequences c0 + 64i + l of 256, incl[i] the
+// costs from c0 up to and with its own.
 struct SeqScan {
-  int c0, before;  // units of the sequences before c0
-  int len[4], units[4], incl;
+  int c0, before;  // cost of the sequences before c0
+  int len[4], cost[4], incl[4];
   int all;         // of the 256
   __device__ __forceinline__ void load(const int* __restrict__ lens, int n_seqs, int cap, int window, int lane) {
-    const int left = n_seqs - c0;
+    all = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) len[i] = lens[c0 + min(4 * lane + i, left - 1)];
-    incl = 0;
+    for (int i = 0; i < 4; ++i) len[i] = c0 + 64 * i < n_seqs ? lens[min(c0 + 64 * i + lane, n_seqs - 1)] : 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      units[i] = 4 * lane + i < left ? seq_span(len[i], cap, window).units : 0;
-      incl += units[i];
+      cost[i] = incl[i] = 0;
+      if (c0 + 64 * i < n_seqs) {
+        cost[i] = c0 + 64 * i + lane < n_seqs ? seq_span(len[i], cap, window).units + PA_PAIR : 0;
+        incl[i] = all + wave_scan(cost[i]);
+        all = __builtin_amdgcn_readlane(incl[i], 63);
+      }
     }
-    const int lanes = min(64, (left + 3) / 4);
-    for (int o = 1; o < lanes; o <<= 1) {
-      const int y = __shfl_up(incl, o);
-      if (lane >= o) incl += y;
-    }
-    all = __builtin_amdgcn_readlane(incl, lanes - 1);
   }
 };
 
@@ -793,18 +817,15 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
   for (sc.c0 = 0;; sc.c0 += 256) {
     sc.load(lens, n_seqs, cap, pq.window, lane);
     if (pl.join && blockIdx.x == 0 && wv == 0) {
-      int sum = total + sc.incl - sc.units[0] - sc.units[1] - sc.units[2] - sc.units[3];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sum += sc.units[i];
-        if (sc.c0 + 4 * lane + i < n_seqs) pl.chunk[2 + sc.c0 + 4 * lane + i] = sum;
-      }
+      for (int i = 0; i < 4; ++i)
+        if (sc.c0 + 64 * i + lane < n_seqs) pl.chunk[2 + sc.c0 + 64 * i + lane] = total + sc.incl[i];
     }
     total += sc.all;
     if (sc.c0 + 256 >= n_seqs) break;
   }
   total *= pl.n_groups;
-  const int chunk = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+  const int chunk = total <= (int)gridDim.x ? 1 : (int)((uint32_t)(total + (int)gridDim.x - 1) / gridDim.x);
   if (pl.join && blockIdx.x == 0 && tid == 0) {
     pl.chunk[0] = chunk;
     pl.chunk[1] = 0;
@@ -819,37 +840,39 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
   sc.before = 0;
 
   PaWave<CT, NP, HDP, UNI> w(kv, lane);
-  w.max_pages = max_pages;
   const float up = CT == BB_F16 ? 14.0f : 0.0f;
-  for (bool first_pair = true; u < end; first_pair = false) {
-    // the sequence of unit u: the first lane whose units reach past it, the first of its four
+  bool lds_read = false;
+  while (u < end) {
+    // the sequence whose cost reaches past u
     while (u >= (sc.before + sc.all) * pl.n_groups) {
       sc.before += sc.all;
       sc.c0 += 256;
       sc.load(lens, n_seqs, cap, pq.window, lane);
     }
-    const int at = __builtin_ctzll(__ballot((sc.before + sc.incl) * pl.n_groups > u));
-    int s = sc.c0 + 4 * at, nu = 0, len = 0;
-    int seq_lo = sc.before + __builtin_amdgcn_readlane(sc.incl - sc.units[0] - sc.units[1] - sc.units[2] - sc.units[3], at);
+    int s = 0, cost = 0, len = 0, lo = 0;
     bool found = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int x = __builtin_amdgcn_readlane(sc.units[i], at), y = __builtin_amdgcn_readlane(sc.len[i], at);
-      if (!found) {
-        nu = x;
-        len = y;
-        found = (seq_lo + x) * pl.n_groups > u;
-        if (!found) {
-          seq_lo += x;
-          ++s;
-        }
+      if (found || sc.c0 + 64 * i >= n_seqs) continue;
+      const uint64_t past = __ballot((sc.before + sc.incl[i]) * pl.n_groups > u);
+      if (past) {
+        const int at = __builtin_ctzll(past);
+        found = true;
+        s = sc.c0 + 64 * i + at;
+        cost = __builtin_amdgcn_readlane(sc.cost[i], at);
+        len = __builtin_amdgcn_readlane(sc.len[i], at);
+        lo = (sc.before + __builtin_amdgcn_readlane(sc.incl[i], at) - cost) * pl.n_groups;
       }
     }
-    const int in = u - seq_lo * pl.n_groups, grp = in / nu, u0 = in - grp * nu, take = min(nu - u0, end - u);
-    const int kvh = grp / pl.split, sub = grp - kvh * pl.split;
+    const int grp = small_div(u - lo, cost), nu = cost - PA_PAIR;
+    lo += grp * cost + PA_PAIR;  // the pair's first unit
+    const int u0 = max(u - lo, 0), take = min(nu, end - lo) - u0;
+    u = min(lo + nu, end);
+    if (take <= 0) continue;  // (the run ends before the pair's units)
+    const int kvh = pl.split == 1 ? grp : small_div(grp, pl.split), sub = grp - kvh * pl.split;
     w.row = table + (size_t)s * table_stride;
-    w.head0 = kvh * (pq.n_heads / kv.n_kv) + sub * pl.hg;
-    w.heads = min(pl.hg, pq.n_heads / kv.n_kv - sub * pl.hg);
+    w.head0 = kvh * pl.G + sub * pl.hg;
+    w.heads = min(pl.hg, pl.G - sub * pl.hg);
     w.kv_off = (size_t)kvh * kv.head_stride;
     w.sp = seq_span(len, cap, pq.window);
     w.start(pq, s);
@@ -857,7 +880,8 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
     w.run(k0 + wv * S::KT, min(k0 + take * PA_UNIT, w.sp.len), PA_WAVES * S::KT);
 
     // the waves' sums together
-    if (!first_pair) __syncthreads();  // (the pair before is done with LDS)
+    if (lds_read) __syncthreads();  // (the pair before is done with LDS)
+    lds_read = true;
     const float l_all = group_sum(w.l);
     if (w.g == 0) {
       s_m[wv][w.n] = w.m;
@@ -882,7 +906,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
     }
     __syncthreads();
     const bool whole = take == nu;
-    const size_t slot = 2 * (size_t)blockIdx.x + (first_pair ? 0 : 1);
+    const size_t slot = 2 * (size_t)blockIdx.x + (u0 > 0 ? 0 : 1);
     for (int i = tid; i < w.heads * ROW4; i += PA_THREADS) {
       const int h = i / ROW4, d = 4 * (i % ROW4);
       if (d >= kv.hd) continue;
@@ -897,76 +921,65 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
       }
       if (whole) {
         const bool none = mm == NEG_INF && ll == 0.0f;
-        store_act(pq.out, (size_t)s * pq.out_stride + (size_t)(w.head0 + h) * kv.hd + d, pq.dt,
-                  none ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : x / ll);
-        if (d == 0 && pq.lse) pq.lse[(size_t)s * pq.n_heads + w.head0 + h] = none ? NEG_INF : (mm + log2f(ll) - up) * LN2;
+        store_act(pq.out, (size_t)s * pq.out_stride + (size_t)(w.head0 + h) * kv.hd + d, pq.dt, x * (none ? 0.0f : 1.0f / ll));
+        if (d == 0 && pq.lse)
+          pq.lse[(size_t)s * pq.n_heads + w.head0 + h] = none ? NEG_INF : (mm + (__builtin_amdgcn_logf(ll) - up)) * LN2;
       } else {
         *reinterpret_cast<v4f*>(pl.sums + (slot * pl.hg + h) * kv.hd + d) = x;
         if (d == 0) pl.ml[slot * pl.hg + h] = make_float2(mm, ll);
       }
     }
-    u += take;
   }
 }
 
-// Adds the partial sums of a (sequence, head): those of the blocks whose runs hold units of it.
-constexpr int PJ_THREADS = 256;
-__global__ void __launch_bounds__(PJ_THREADS) k_paged_join(PagedQuery pq, int n_kv, int hd, PagedPlan pl, float up) {
-  __shared__ float red[PJ_THREADS / 64];
-  __shared__ __align__(16) float acc[PJ_THREADS * 4];
-  const int h = blockIdx.y, s = blockIdx.x, tid = threadIdx.x;
-  const int G = pq.n_heads / n_kv, kvh = h / G, sub = (h - kvh * G) / pl.hg, hh = h - kvh * G - sub * pl.hg;
-  const int chunk = pl.chunk[0], before = pl.chunk[1 + s], nu = pl.chunk[2 + s] - before;
-  const int lo = before * pl.n_groups + (kvh * pl.split + sub) * nu, hi = lo + nu;
+// Adds the partial sums of a (sequence, head), PJ_PIECES pieces of 4 elements a block: those of the blocks whose
+// runs hold units of it. Threads: a row of PJ_PIECES for every PJ_ROWS-th part, joined in LDS.
+constexpr int PJ_THREADS = 256, PJ_PIECES = 8, PJ_ROWS = PJ_THREADS / PJ_PIECES;
+__global__ void __launch_bounds__(PJ_THREADS) k_paged_join(PagedQuery pq, int hd, PagedPlan pl, float up) {
+  __shared__ float s_m[PJ_ROWS], s_l[PJ_ROWS];
+  __shared__ v4f s_x[PJ_ROWS][PJ_PIECES];
+  const int s = blockIdx.x, h = blockIdx.y, piece = blockIdx.z * PJ_PIECES + threadIdx.x % PJ_PIECES;
+  const int row = threadIdx.x / PJ_PIECES;
+  const int chunk = pl.chunk[0], before = pl.chunk[1 + s], cost = pl.chunk[2 + s] - before;
+  const int kvh = h / pl.G, sub = (h - kvh * pl.G) / pl.hg, hh = h - kvh * pl.G - sub * pl.hg;
+  const int lo = before * pl.n_groups + (kvh * pl.split + sub) * cost + PA_PAIR, hi = lo + cost - PA_PAIR;
   const int b0 = lo / chunk, b1 = (hi - 1) / chunk;
   if (b0 == b1) return;  // whole in one block
   const int parts = b1 - b0 + 1;
-  // the first block's run may start before the pair, which is its second one then
-  const auto slot = [&](int i) { return (2 * (size_t)(b0 + i) + (i == 0 && b0 * chunk != lo ? 1 : 0)) * pl.hg + hh; };
-  float top = NEG_INF;
-  for (int i = tid; i < parts; i += PJ_THREADS) top = fmaxf(top, pl.ml[slot(i)].x);
-  top = wave_max(top);
-  if ((tid & 63) == 0) red[tid >> 6] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float ref = top == NEG_INF ? 0.0f : top;
-  // lanes: hd/4 (rounded up to a power of two) pieces of 4 elements, the rest of the block over the parts
-  int np = 1;
-  while (4 * np < hd) np *= 2;
-  const int piece = tid & (np - 1), rows = PJ_THREADS / np;
-  float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float l = 0.0f;
+  float m = NEG_INF, l = 0.0f;
+  v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-  for (int i = tid / np; i < parts; i += rows) {
-    const size_t at = slot(i);
+  for (int i = row; i < parts; i += PJ_ROWS) {
+    const size_t at = (2 * (size_t)(b0 + i) + (i == 0 ? 1 : 0)) * pl.hg + hh;
     const float2 ml = pl.ml[at];
-    const float f = __builtin_amdgcn_exp2f(ml.x - ref);
-    l += ml.y * f;
-    if (4 * piece < hd) {
-      const float4 y = *reinterpret_cast<const float4*>(pl.sums + at * hd + 4 * piece);
-      x.x += y.x * f;
-      x.y += y.y * f;
-      x.z += y.z * f;
-      x.w += y.w * f;
-    }
+    const v4f y = *reinterpret_cast<const v4f*>(pl.sums + at * hd + min(4 * piece, hd - 4));
+    const float top = fmaxf(m, ml.x), ref = top == NEG_INF ? 0.0f : top;
+    const float f0 = __builtin_amdgcn_exp2f(m - ref), f1 = __builtin_amdgcn_exp2f(ml.x - ref);
+    m = top;
+    l = l * f0 + ml.y * f1;
+    x = x * f0 + y * f1;
   }
-  __syncthreads();  // (red is read)
-  reinterpret_cast<float4*>(acc)[tid] = x;
-  __shared__ float lsum[PJ_THREADS];
-  if (piece == 0) lsum[tid / np] = l;
+  if (threadIdx.x % PJ_PIECES == 0) {
+    s_m[row] = m;
+    s_l[row] = l;
+  }
+  s_x[row][threadIdx.x % PJ_PIECES] = x;
   __syncthreads();
-  if (4 * tid < hd) {
-    v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
-    float ll = 0.0f;
-    for (int i = 0; i < rows; ++i) {
-      y += reinterpret_cast<const v4f*>(acc)[i * np + tid];
-      ll += lsum[i];
-    }
-    const bool none = top == NEG_INF && ll == 0.0f;
-    store_act(pq.out, (size_t)s * pq.out_stride + (size_t)h * hd + 4 * tid, pq.dt,
-              none ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : y / ll);
-    if (tid == 0 && pq.lse) pq.lse[(size_t)s * pq.n_heads + h] = none ? NEG_INF : (top + log2f(ll) - up) * LN2;
+  if (threadIdx.x >= PJ_PIECES || 4 * piece >= hd) return;
+  m = NEG_INF;
+  for (int i = 0; i < PJ_ROWS; ++i) m = fmaxf(m, s_m[i]);
+  const float ref = m == NEG_INF ? 0.0f : m;
+  l = 0.0f;
+  x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i = 0; i < PJ_ROWS; ++i) {
+    const float f = __builtin_amdgcn_exp2f(s_m[i] - ref);
+    l += s_l[i] * f;
+    x += s_x[i][threadIdx.x] * f;
   }
+  const bool none = m == NEG_INF && l == 0.0f;
+  store_act(pq.out, (size_t)s * pq.out_stride + (size_t)h * hd + 4 * piece, pq.dt, x * (none ? 0.0f : 1.0f / l));
+  if (piece == 0 && pq.lse)
+    pq.lse[(size_t)s * pq.n_heads + h] = none ? NEG_INF : (m + (__builtin_amdgcn_logf(l) - up)) * LN2;
 }
 
 int pa_class(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
@@ -976,9 +989,9 @@ int pa_blocks(int n_cu, int hd) { return n_cu * pa_waves(pa_class(hd)); }
 
 PagedPlan pa_plan(int n_seqs, int n_heads, int n_kv) {
   PagedPlan p{};
-  const int G = n_heads / n_kv;
-  p.split = (G + PA_HEADS - 1) / PA_HEADS;
-  p.hg = (G + p.split - 1) / p.split;
+  p.G = n_heads / n_kv;
+  p.split = (p.G + PA_HEADS - 1) / PA_HEADS;
+  p.hg = (p.G + p.split - 1) / p.split;
   p.n_groups = n_kv * p.split;
   return p;
 }
@@ -987,7 +1000,7 @@ PagedPlan pa_plan(int n_seqs, int n_heads, int n_kv) {
 
 bool paged_attn_fits(int n_seqs, int n_heads, int n_kv, size_t cap) {
   const PagedPlan p = pa_plan(n_seqs, n_heads, n_kv);
-  return (size_t)n_seqs * (size_t)p.n_groups * ((cap + PA_UNIT - 1) / PA_UNIT) < ((size_t)1 << 30);
+  return (size_t)n_seqs * (size_t)p.n_groups * ((cap + PA_UNIT - 1) / PA_UNIT + PA_PAIR) < ((size_t)1 << 29);
 }
 
 void paged_divisor(PagedView& v) {
@@ -1013,8 +1026,9 @@ hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQue
   pl.sums = static_cast<float*>(q.ws);
   pl.ml = reinterpret_cast<float2*>(pl.sums + slots * kv.hd);
   pl.chunk = reinterpret_cast<int*>(pl.ml + slots);
-  const size_t units = (size_t)sq.n_seqs * pl.n_groups * ((cap + PA_UNIT - 1) / PA_UNIT);
-  const unsigned blocks = (unsigned)std::min<size_t>(blocks_max, units);
+  // (pairs of one unit take a block each at most, longer ones a block for each unit)
+  const size_t units = (cap + PA_UNIT - 1) / PA_UNIT, pairs = (size_t)sq.n_seqs * pl.n_groups;
+  const unsigned blocks = (unsigned)std::min<size_t>(blocks_max, pairs * (units == 1 ? 1 : units + PA_PAIR));
   pl.join = cap > (size_t)PA_UNIT;  // else every pair is one unit
   const bool uni = kv.page_size % 16 == 0 && 16 * kv.pos_stride < ((size_t)1 << 29);
   const int cls = pa_class(kv.hd);
@@ -1042,8 +1056,8 @@ hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQue
 #undef BB_PA
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !pl.join) return e;
-  BB_LAUNCH(k_paged_join, dim3(sq.n_seqs, q.n_heads), dim3(PJ_THREADS), 0, st, q, kv.n_kv, kv.hd, pl,
-            cache == BB_F16 ? 14.0f : 0.0f);
+  BB_LAUNCH(k_paged_join, dim3(sq.n_seqs, q.n_heads, (kv.hd + 4 * PJ_PIECES - 1) / (4 * PJ_PIECES)), dim3(PJ_THREADS), 0,
+            st, q, kv.hd, pl, cache == BB_F16 ? 14.0f : 0.0f);
   return hipGetLastError();
 }
 
