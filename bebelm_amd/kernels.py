@@ -25,7 +25,7 @@ import numpy as np
 
 from . import _lib
 from ._lib import check, lib
-from .model import _dtype, _on, _ptr, _same_loc
+from .model import F32, INT32, _dtype, _ptr, _same_loc
 
 
 @dataclass
@@ -157,62 +157,66 @@ def rope_neox(ctx, x, head_dim, pos, freq_base):
     return x
 
 
-def _strides(a):
-    """Strides in elements."""
-    return tuple(a.stride()) if hasattr(a, "data_ptr") else tuple(n // a.itemsize for n in a.strides)
+# ---- arrays of the paged-cache operators (checked with few calls each: a step makes these for every
+# layer, and a decode step's kernels take a few microseconds)
+def _place(ctx, *arrays):
+    """Where the arrays are: all in host memory, or all on the context's GPU."""
+    where = None
+    for a in arrays:
+        if a is None:
+            continue
+        d = -1 if isinstance(a, np.ndarray) else a.get_device()
+        if where is None:
+            where = d
+        elif d != where:
+            raise ValueError("all arrays of one call must be host or all device")
+    if where >= 0 and where != ctx.device:
+        raise ValueError(f"tensors on GPU {where}, context on GPU {ctx.device}")
+    return _lib.LOC_HOST if where < 0 else _lib.LOC_DEVICE
 
 
 def _data(a):
-    return a.data_ptr() if hasattr(a, "data_ptr") else a.ctypes.data
+    return a.ctypes.data if isinstance(a, np.ndarray) else a.data_ptr()
 
 
-def _loc_of(ctx, *arrays):
-    """Where the arrays are (those of any strides among them), all in one place."""
-    _on(ctx, *arrays)
-    locs = {bool(getattr(a, "is_cuda", False)) for a in arrays if a is not None}
-    if len(locs) != 1:
-        raise ValueError("all arrays of one call must be host or all device")
-    return _lib.LOC_DEVICE if locs.pop() else _lib.LOC_HOST
-
-
-def _heads(a, what, n=None, heads=None, hd=None, packed=True):
-    """Strides (token, head) of [tokens, heads, head_dim], checked."""
-    if len(a.shape) != 3 or any(w is not None and w != g for w, g in zip((n, heads, hd), a.shape)):
-        raise ValueError(f"{what} must be [tokens, heads, head_dim], is {tuple(a.shape)}")
-    st, (t, h, d) = _strides(a), a.shape
-    if d > 1 and st[2] != 1:
+def _heads(a, what, n, heads, hd, packed=True):
+    """Strides (token, head) in elements of [n, heads, head_dim], checked."""
+    if a.shape != (n, heads, hd):
+        raise ValueError(f"{what} must be {[n, heads, hd]}, is {list(a.shape)}")
+    if a.flags["C_CONTIGUOUS"] if isinstance(a, np.ndarray) else a.is_contiguous():
+        return heads * hd, hd
+    st = [i // a.itemsize for i in a.strides] if isinstance(a, np.ndarray) else a.stride()
+    if hd > 1 and st[2] != 1:
         raise ValueError(f"{what}: the elements of a head must be adjacent")
-    if packed and h > 1 and st[1] != d:
+    if packed and heads > 1 and st[1] != hd:
         raise ValueError(f"{what}: the heads of a token must be adjacent")
-    if any(s < 0 for s in st):
+    if min(st) < 0:
         raise ValueError(f"{what}: negative strides")
-    return (st[0] if t > 1 else h * d), (st[1] if h > 1 else d)
+    return (st[0] if n > 1 else heads * hd), (st[1] if heads > 1 else hd)
 
 
-def _ints(a, what, shape):
+def _whole(a, what, code, *shape):
+    """Address of a contiguous array of the given type and shape (None: none)."""
     if a is None:
         return None
-    if str(a.dtype).replace("torch.", "") != "int32" or tuple(a.shape) != shape:
-        raise ValueError(f"{what} must be int32 {list(shape)}, is {a.dtype} {list(a.shape)}")
-    return _ptr(a)[0]
+    if _dtype(a) != code or a.shape != shape:
+        raise ValueError(f"{what} must be {'int32' if code == INT32 else 'float32'} {list(shape)}, is {a.dtype} {list(a.shape)}")
+    if not (a.flags["C_CONTIGUOUS"] if isinstance(a, np.ndarray) else a.is_contiguous()):
+        raise ValueError(f"{what} must be contiguous")
+    return _data(a)
 
 
-def _floats(a, what, shape):
-    if a is None:
-        return None
-    if str(a.dtype).replace("torch.", "") != "float32" or tuple(a.shape) != shape:
-        raise ValueError(f"{what} must be float32 {list(shape)}, is {a.dtype} {list(a.shape)}")
-    return _ptr(a)[0]
-
-
-def _seqs(kv, page_table, lens):
-    if len(page_table.shape) != 2 or str(page_table.dtype).replace("torch.", "") != "int32":
+def _seqs(page_table, lens):
+    if len(page_table.shape) != 2 or _dtype(page_table) != INT32:
         raise ValueError("page_table must be int32 [sequences, pages]")
     n, pages = page_table.shape
-    st = _strides(page_table)
-    if (pages > 1 and st[1] != 1) or st[0] < 0:
-        raise ValueError("page_table: the entries of a sequence must be adjacent")
-    return _lib.PagedSeqs(n, pages, st[0] if n > 1 else pages, _data(page_table), _ints(lens, "lens", (n,)))
+    row = pages
+    if not (page_table.flags["C_CONTIGUOUS"] if isinstance(page_table, np.ndarray) else page_table.is_contiguous()):
+        st = [i // 4 for i in page_table.strides] if isinstance(page_table, np.ndarray) else page_table.stride()
+        if (pages > 1 and st[1] != 1) or st[0] < 0:
+            raise ValueError("page_table: the entries of a sequence must be adjacent")
+        row = st[0] if n > 1 else pages
+    return n, _lib.PagedSeqs(n, pages, row, _data(page_table), _whole(lens, "lens", INT32, n))
 
 
 def rope(ctx, plan, x, pos, out=None):
@@ -220,12 +224,13 @@ def rope(ctx, plan, x, pos, out=None):
     RopePlan says, into out (x itself by default)."""
     out = x if out is None else out
     t, h, hd = x.shape
-    xs, os = _heads(x, "x", packed=False), _heads(out, "out", t, h, hd, packed=False)
-    if _dtype(x) != _dtype(out):
-        raise ValueError("x and out must be of one type")
-    loc = _loc_of(ctx, x, pos, out)
-    check(lib().bb_rope(ctx.handle, plan.handle, _dtype(x), _data(x), *xs, t, h, hd, _ints(pos, "pos", (t,)),
-                        _data(out), *os, loc))
+    xs = _heads(x, "x", t, h, hd, False)
+    os = xs if out is x else _heads(out, "out", t, h, hd, False)
+    code = _dtype(x)
+    if code == INT32 or _dtype(out) != code:
+        raise ValueError("x and out must be of one floating-point type")
+    check(lib().bb_rope(ctx.handle, plan.handle, code, _data(x), xs[0], xs[1], t, h, hd, _whole(pos, "pos", INT32, t),
+                        _data(out), os[0], os[1], _place(ctx, x, pos, out)))
     return out
 
 
@@ -237,27 +242,36 @@ def paged_append(ctx, kv, page_table, lens, k, v, rope=None, pos=None, seq_start
     index in its sequence. page_table int32 [sequences, pages] and lens int32 [sequences] count the
     call's tokens; seq_start int32 [sequences + 1] says which tokens each sequence brings (None: one
     each). Returns q_out."""
-    t = k.shape[0]
-    seqs = _seqs(kv, page_table, lens)
-    ks = _heads(k, "k", t, kv.n_kv_heads, kv.head_dim)
-    vs = _heads(v, "v", t, kv.n_kv_heads, kv.head_dim)
-    if q is not None and q_out is None:
-        q_out = q
-    if len({_dtype(a) for a in (k, v, q, q_out) if a is not None}) != 1:
-        raise ValueError("k, v, q and q_out must be of one type")
+    t, hd, nkv, code = len(k), kv.head_dim, kv.n_kv_heads, _dtype(k)
+    n, seqs = _seqs(page_table, lens)
+    ks, vs = _heads(k, "k", t, nkv, hd), _heads(v, "v", t, nkv, hd)
     if rope is not None and not rope.handle:
         raise ValueError("the RopePlan is closed")
-    heads, qs, qos = 0, (0, 0), (0, 0)
+    tok = _lib.PagedTokens(t, code, _data(k), _data(v), ks[0], vs[0])
+    ok = code != INT32 and _dtype(v) == code
     if q is not None:
+        q_out = q if q_out is None else q_out
         heads = q.shape[1]
-        qs, qos = _heads(q, "q", t, None, kv.head_dim), _heads(q_out, "q_out", t, heads, kv.head_dim)
-    loc = _loc_of(ctx, page_table, lens, k, v, pos, seq_start, q, q_out, q_norm, k_norm)
-    tok = _lib.PagedTokens(t, _dtype(k), _data(k), _data(v), ks[0], vs[0], _data(q) if q is not None else None,
-                           _data(q_out) if q_out is not None else None, heads, qs[0], qos[0],
-                           _floats(q_norm, "q_norm", (kv.head_dim,)), _floats(k_norm, "k_norm", (kv.head_dim,)), eps,
-                           _ints(pos, "pos", (t,)), _ints(seq_start, "seq_start", (seqs.n_seqs + 1,)))
+        ok = ok and _dtype(q) == code and _dtype(q_out) == code
+        tok.q, tok.q_out, tok.n_heads = _data(q), _data(q_out), heads
+        tok.q_stride = _heads(q, "q", t, heads, hd)[0]
+        tok.q_out_stride = _heads(q_out, "q_out", t, heads, hd)[0]
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    if not ok:
+        raise ValueError("k, v, q and q_out must be of one floating-point type")
+    tok.eps = eps
+    if q_norm is not None:
+        tok.q_norm = _whole(q_norm, "q_norm", F32, hd)
+    if k_norm is not None:
+        tok.k_norm = _whole(k_norm, "k_norm", F32, hd)
+    if pos is not None:
+        tok.pos = _whole(pos, "pos", INT32, t)
+    if seq_start is not None:
+        tok.seq_start = _whole(seq_start, "seq_start", INT32, n + 1)
     check(lib().bb_paged_append(ctx.handle, kv.handle, rope.handle if rope is not None else None, ctypes.byref(seqs),
-                                ctypes.byref(tok), loc))
+                                ctypes.byref(tok),
+                                _place(ctx, k, v, page_table, lens, pos, seq_start, q, q_out, q_norm, k_norm)))
     return q_out
 
 
@@ -267,24 +281,28 @@ def paged_attention(ctx, kv, page_table, lens, q, out, scale=None, window=0, lse
     n_heads] gets the softmax's log sums. scale None: 1/sqrt(head_dim). workspace: a device tensor of
     kv.attention_workspace(n_heads, sequences) bytes for this call alone (None: the context's; a call
     captured into a graph needs one)."""
-    seqs = _seqs(kv, page_table, lens)
-    n, heads = seqs.n_seqs, q.shape[1]
-    qs = _heads(q, "q", n, None, kv.head_dim)
-    os = _heads(out, "out", n, heads, kv.head_dim)
-    if _dtype(q) != _dtype(out):
-        raise ValueError("q and out must be of one type")
-    loc = _loc_of(ctx, page_table, lens, q, out, lse)
+    n, seqs = _seqs(page_table, lens)
+    heads, hd, code = q.shape[1], kv.head_dim, _dtype(q)
+    pq = _lib.PagedQuery(code, _data(q), _data(out), heads, _heads(q, "q", n, heads, hd)[0],
+                         _heads(out, "out", n, heads, hd)[0])
+    if code == INT32 or _dtype(out) != code:
+        raise ValueError("q and out must be of one floating-point type")
+    if scale is not None:
+        if scale == 0:
+            raise ValueError("scale must not be 0")
+        pq.scale = scale
+    if window:
+        if window < 0:
+            raise ValueError("window must not be negative")
+        pq.window = window
+    if lse is not None:
+        pq.lse = _whole(lse, "lse", F32, n, heads)
     if workspace is not None:
-        if not (getattr(workspace, "is_cuda", False) and workspace.is_contiguous()):
-            raise ValueError("the workspace must be a contiguous device tensor")
-        _on(ctx, workspace)
-    if scale is not None and scale == 0:
-        raise ValueError("scale must not be 0")
-    pq = _lib.PagedQuery(_dtype(q), _data(q), _data(out), heads, qs[0], os[0], 0.0 if scale is None else scale,
-                         int(window), _floats(lse, "lse", (n, heads)),
-                         workspace.data_ptr() if workspace is not None else None,
-                         workspace.numel() * workspace.element_size() if workspace is not None else 0)
-    check(lib().bb_paged_attention(ctx.handle, kv.handle, ctypes.byref(seqs), ctypes.byref(pq), loc))
+        if isinstance(workspace, np.ndarray) or workspace.get_device() != ctx.device or not workspace.is_contiguous():
+            raise ValueError("the workspace must be a contiguous tensor on the context's GPU")
+        pq.workspace, pq.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    check(lib().bb_paged_attention(ctx.handle, kv.handle, ctypes.byref(seqs), ctypes.byref(pq),
+                                   _place(ctx, q, out, page_table, lens, lse)))
     return out
 
 

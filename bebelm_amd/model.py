@@ -317,22 +317,20 @@ class KvCache:
 
 
 F32, F16, BF16 = 0, 1, 30  # element types of the paged-cache operators
-_DTYPES = {"float32": F32, "float16": F16, "bfloat16": BF16}
+INT32 = -1
+_CODES = {"float32": F32, "float16": F16, "bfloat16": BF16, "int32": INT32}
+_codes = {}  # the same by dtype object
 
 
 def _dtype(a):
     """The type code of an array's elements."""
-    code = _DTYPES.get(str(a.dtype).replace("torch.", ""))
+    code = _codes.get(a.dtype)
     if code is None:
-        raise ValueError(f"elements must be float32, float16 or bfloat16, not {a.dtype}")
+        code = _CODES.get(str(a.dtype).replace("torch.", ""))
+        if code is None:
+            raise ValueError(f"elements must be float32, float16, bfloat16 or (indexes) int32, not {a.dtype}")
+        _codes[a.dtype] = code
     return code
-
-
-def _on(ctx, *arrays):
-    """The torch tensors among the arrays are in host memory or on the context's GPU."""
-    for a in arrays:
-        if a is not None and getattr(a, "is_cuda", False) and a.device.index != ctx.device:
-            raise ValueError(f"tensor on {a.device}, context on GPU {ctx.device}")
 
 
 class RopePlan:
@@ -370,13 +368,12 @@ class PagedKv:
     view of another order will do). The tensors are kept; whoever holds them sees what is stored."""
 
     def __init__(self, ctx, k, v):
-        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
+        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or _dtype(k) == INT32:
             raise ValueError("keys and values must be of one type, shape [pages, positions, heads, head_dim] and strides")
-        if not (k.is_cuda and v.is_cuda):
-            raise ValueError("the pool must be in device memory")
+        if k.get_device() != ctx.device or v.get_device() != ctx.device:
+            raise ValueError(f"the pool must be in the memory of the context's GPU ({ctx.device})")
         if k.stride(3) != 1 and k.shape[3] > 1:
             raise ValueError("the elements of a head must be adjacent")
-        _on(ctx, k, v)
         self.ctx, self.k, self.v, self.handle = ctx, k, v, None
         self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = k.shape
         h = ctypes.c_void_p()
