@@ -441,7 +441,7 @@ struct PaShape {
   static constexpr int VE = HDP / 16;                    // elements of a value row per lane
   static constexpr int PE = VE < KE ? VE : KE;           // in pieces of PE
   static constexpr int NV = VE / PE;
-  static constexpr int KT = CT == BB_F32 && HDP == 256 ? 16 : 32;  // positions of a tile (registers)
+  static constexpr int KT = CT == BB_F32 ? 16 : 32;      // positions of a tile: 128 bytes of each element column
   static constexpr int NT = KT / 16;
 };
 
@@ -777,10 +777,10 @@ struct PaWave {
   }
 };
 
-// The sequences' costs (units + PA_PAIR) as a wave holds them: lane l has sequences c0 + 64i + l of 256, incl[i] the
-// costs from c0 up to and with its own.
+// The sequences' costs (units + PA_PAIR), 256 at a time: lane l has sequences c0 + 64i + l, incl[i] the costs from c0
+// up to and with its own.
 struct SeqScan {
-  int c0, before;  // cost of the sequences before c0
+  int c0;
   int len[4], cost[4], incl[4];
   int all;         // of the 256
   __device__ __forceinline__ void load(const int* __restrict__ lens, int n_seqs, int cap, int window, int lane) {
@@ -811,63 +811,72 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int cap = max_pages * kv.page_size;
 
-  // every wave finds the block's run by itself
-  SeqScan sc;
-  int total = 0;
-  for (sc.c0 = 0;; sc.c0 += 256) {
-    sc.load(lens, n_seqs, cap, pq.window, lane);
-    if (pl.join && blockIdx.x == 0 && wv == 0) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (sc.c0 + 64 * i + lane < n_seqs) pl.chunk[2 + sc.c0 + 64 * i + lane] = total + sc.incl[i];
-    }
-    total += sc.all;
-    if (sc.c0 + 256 >= n_seqs) break;
-  }
-  total *= pl.n_groups;
-  const int chunk = total <= (int)gridDim.x ? 1 : (int)((uint32_t)(total + (int)gridDim.x - 1) / gridDim.x);
-  if (pl.join && blockIdx.x == 0 && tid == 0) {
-    pl.chunk[0] = chunk;
-    pl.chunk[1] = 0;
-  }
-  if ((int64_t)blockIdx.x * chunk >= total) return;
-  int u = (int)blockIdx.x * chunk;
-  const int end = min(u + chunk, total);
-  if (sc.c0 > 0) {
-    sc.c0 = 0;
-    sc.load(lens, n_seqs, cap, pq.window, lane);
-  }
-  sc.before = 0;
-
-  PaWave<CT, NP, HDP, UNI> w(kv, lane);
-  const float up = CT == BB_F16 ? 14.0f : 0.0f;
-  bool lds_read = false;
-  while (u < end) {
-    // the sequence whose cost reaches past u
-    while (u >= (sc.before + sc.all) * pl.n_groups) {
-      sc.before += sc.all;
-      sc.c0 += 256;
+  // every wave finds the block's run by itself: the total cost, then the sequence in whose cost the run begins
+  int u = 0, end = 0, s = 0, cost = 0, len = 0, lo = 0;
+  {
+    SeqScan sc;
+    int total = 0;
+    for (sc.c0 = 0;; sc.c0 += 256) {
       sc.load(lens, n_seqs, cap, pq.window, lane);
+      if (pl.join && blockIdx.x == 0 && wv == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (sc.c0 + 64 * i + lane < n_seqs) pl.chunk[2 + sc.c0 + 64 * i + lane] = total + sc.incl[i];
+      }
+      total += sc.all;
+      if (sc.c0 + 256 >= n_seqs) break;
     }
-    int s = 0, cost = 0, len = 0, lo = 0;
+    total *= pl.n_groups;
+    const int grid = (int)gridDim.x, up_to = total + grid - 1;
+    const int chunk = total <= grid ? 1 : total < (1 << 20) ? small_div(up_to, grid) : (int)((uint32_t)up_to / grid);
+    if (pl.join && blockIdx.x == 0 && tid == 0) {
+      pl.chunk[0] = chunk;
+      pl.chunk[1] = 0;
+    }
+    if ((int64_t)blockIdx.x * chunk >= total) return;
+    u = (int)blockIdx.x * chunk;
+    end = min(u + chunk, total);
+    int before = 0;
+    if (sc.c0 > 0) {
+      sc.c0 = 0;
+      sc.load(lens, n_seqs, cap, pq.window, lane);
+      while (u >= (before + sc.all) * pl.n_groups) {
+        before += sc.all;
+        sc.c0 += 256;
+        sc.load(lens, n_seqs, cap, pq.window, lane);
+      }
+    }
     bool found = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (found || sc.c0 + 64 * i >= n_seqs) continue;
-      const uint64_t past = __ballot((sc.before + sc.incl[i]) * pl.n_groups > u);
+      const uint64_t past = __ballot((before + sc.incl[i]) * pl.n_groups > u);
       if (past) {
         const int at = __builtin_ctzll(past);
         found = true;
         s = sc.c0 + 64 * i + at;
         cost = __builtin_amdgcn_readlane(sc.cost[i], at);
         len = __builtin_amdgcn_readlane(sc.len[i], at);
-        lo = (sc.before + __builtin_amdgcn_readlane(sc.incl[i], at) - cost) * pl.n_groups;
+        lo = (before + __builtin_amdgcn_readlane(sc.incl[i], at) - cost) * pl.n_groups;
       }
     }
-    const int grp = small_div(u - lo, cost), nu = cost - PA_PAIR;
-    lo += grp * cost + PA_PAIR;  // the pair's first unit
-    const int u0 = max(u - lo, 0), take = min(nu, end - lo) - u0;
-    u = min(lo + nu, end);
+  }
+  int grp = small_div(u - lo, cost);
+  lo += grp * cost;
+
+  PaWave<CT, NP, HDP, UNI> w(kv, lane);
+  const float up = CT == BB_F16 ? 14.0f : 0.0f;
+  bool lds_read = false;
+  // the run's pairs: group grp of sequence s, whose cost begins at lo
+  for (; lo < end; lo += cost, ++grp) {
+    if (grp == pl.n_groups) {
+      grp = 0;
+      ++s;
+      len = __builtin_amdgcn_readfirstlane(lens[s]);
+      cost = seq_span(len, cap, pq.window).units + PA_PAIR;
+    }
+    const int nu = cost - PA_PAIR, first_unit = lo + PA_PAIR;
+    const int u0 = max(u - first_unit, 0), take = min(nu, end - first_unit) - u0;
     if (take <= 0) continue;  // (the run ends before the pair's units)
     const int kvh = pl.split == 1 ? grp : small_div(grp, pl.split), sub = grp - kvh * pl.split;
     w.row = table + (size_t)s * table_stride;
