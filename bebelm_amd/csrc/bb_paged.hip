@@ -81,7 +81,7 @@ __device__ __forceinline__ float2 cos_sin_turns(int pos, double turns) {
 }
 
 constexpr int RR_THREADS = 256;
-constexpr int RR_TPB_MAX = 8;  // tokens of a block at most
+constexpr int RR_TPB_MAX = 2;  // tokens of a block at most: a (cos, sin) a thread
 
 struct RowPlace {
   int64_t base;  // where its keys and values start in the pool, -1: nowhere
@@ -126,106 +126,121 @@ __device__ __forceinline__ RowPlace row_place(const RopeRows& r, const PagedView
   return w;
 }
 
-// A block takes tpb tokens. Its waves find the tokens' places, its threads the (cos, sin) of every
-// (token, pair) once into LDS; then groups of gs lanes (a power of two) take the tokens' head rows, a
-// lane two runs of VE elements that turn together (or one run past the turned part). VE 8: whole
-// 16-byte pieces; VE 1: any size and stride.
+// A block takes tpb tokens and rows blockIdx.y·rpb.. (rpb of them) of each. Its waves find the tokens' places, its
+// threads the (cos, sin) of every (token, pair) once into LDS; then groups of gs lanes (a power of two)
+// take a head row each, a lane up to MU pairs of runs of VE elements that turn together (or runs past
+// the turned part). VE 8: whole 16-byte pieces; VE 1: any size and stride.
+// One token's call is latency: what needs neither place nor angle (the first rows, gains, frequencies) is
+// asked for before the place is known. A long batch is bound by its bytes: ROPE_FIGURES.
 template <class A, class C, int VE>
 __global__ void __launch_bounds__(RR_THREADS) k_rope_rows(RopeRows r, RopeTurns rt, PagedView kv, PagedSeqs sq, int tpb,
-                                                          int gs) {
-  extern __shared__ float2 cs[];  // [tpb][half]
+                                                          int rpb, int gs) {
+  constexpr int MU = VE == 1 ? 4 : 1;
+  __shared__ float2 cs[RR_THREADS];  // [tpb][half]
+  __shared__ float s_gain[2][OPS_HD_MAX];
   __shared__ RowPlace place[RR_TPB_MAX];
-  const int tid = threadIdx.x, half = rt.half;
+  const int tid = threadIdx.x, half = rt.half, n_all = r.n_q + 2 * r.n_kv;
   const size_t t0 = (size_t)blockIdx.x * tpb;
-  for (int i = tid >> 6; i < tpb; i += RR_THREADS / 64) {
-    const RowPlace w = row_place(r, kv, sq, t0 + i);
-    if ((tid & 63) == 0) place[i] = w;
-  }
-  __syncthreads();
-  for (int i = tid; i < tpb * half; i += RR_THREADS) {
-    const float2 v = cos_sin_turns(place[i / half].pos, rt.turns[i % half]);
-    cs[i] = make_float2(rt.magnitude * v.x, rt.magnitude * v.y);
-  }
-  __syncthreads();
-  const int n_rows = r.n_q + 2 * r.n_kv, nu = half / VE, units = nu + (r.hd - 2 * half) / VE;
-  const int lane = tid & (gs - 1);
-  for (int i = tid / gs; i < tpb * n_rows; i += RR_THREADS / gs) {
-    const int tk = i / n_rows, row = i - tk * n_rows;
-    const RowPlace w = place[tk];
+  const int row0 = blockIdx.y * rpb, n_rows = min(rpb, n_all - row0), n_tok = (int)min((size_t)tpb, r.T - t0);
+  const int nu = half / VE, units = nu + (r.hd - 2 * half) / VE, lane = tid & (gs - 1);
+
+  float a[MU][VE], b[MU][VE];
+  const auto first_of = [&](int u) { return u < nu ? (rt.interleaved ? 2 * u * VE : u * VE) : 2 * half + (u - nu) * VE; };
+  const auto load = [&](int i) {
+    const int tk = i / n_rows, row = row0 + i - tk * n_rows;
     const size_t t = t0 + tk;
-    if (!w.live) continue;
+    const A* x = row < r.n_q            ? static_cast<const A*>(r.q) + t * r.q_ts + (size_t)row * r.q_hs
+                 : row < r.n_q + r.n_kv ? static_cast<const A*>(r.k) + t * r.k_ts + (size_t)(row - r.n_q) * r.hd
+                                        : static_cast<const A*>(r.v) + t * r.v_ts + (size_t)(row - r.n_q - r.n_kv) * r.hd;
+#pragma unroll
+    for (int m = 0; m < MU; ++m) {
+      const int u = lane + m * gs, e0 = first_of(u);
+#pragma unroll
+      for (int j = 0; j < VE; ++j) a[m][j] = b[m][j] = 0.0f;
+      if (u < units) load_vec<A, VE>(x + e0, a[m]);
+      if (u < nu) load_vec<A, VE>(x + (rt.interleaved ? e0 + VE : e0 + half), b[m]);
+    }
+  };
+  int i = tid / gs;
+  if (i < n_tok * n_rows) load(i);
+  const double turns = tid < tpb * half ? rt.turns[tid % half] : 0.0;
+  if (r.q_norm && tid < r.hd) s_gain[0][tid] = r.q_norm[tid];
+  if (r.k_norm && tid < r.hd) s_gain[1][tid] = r.k_norm[tid];
+  if (tid >> 6 < tpb) {
+    const RowPlace w = row_place(r, kv, sq, t0 + (tid >> 6));
+    if ((tid & 63) == 0) place[tid >> 6] = w;
+  }
+  __syncthreads();
+  if (tid < tpb * half) {
+    const float2 v = cos_sin_turns(place[tid / half].pos, turns);
+    cs[tid] = make_float2(rt.magnitude * v.x, rt.magnitude * v.y);
+  }
+  __syncthreads();
+  while (i < n_tok * n_rows) {
+    const int tk = i / n_rows, row = row0 + i - tk * n_rows;
+    const RowPlace w = place[tk];
     const bool is_q = row < r.n_q, is_k = !is_q && row < r.n_q + r.n_kv;
-    if (!is_q && w.base < 0) continue;
-    const int head = is_q ? row : is_k ? row - r.n_q : row - r.n_q - r.n_kv;
-    const A* x = is_q   ? static_cast<const A*>(r.q) + t * r.q_ts + (size_t)head * r.q_hs
-                 : is_k ? static_cast<const A*>(r.k) + t * r.k_ts + (size_t)head * r.hd
-                        : static_cast<const A*>(r.v) + t * r.v_ts + (size_t)head * r.hd;
-    A* yq = static_cast<A*>(r.q_out) + t * r.qo_ts + (size_t)head * r.qo_hs;
-    C* yc = static_cast<C*>(is_k ? kv.k : kv.v) + w.base + (size_t)head * kv.head_stride;
-    const float* gain = is_q ? r.q_norm : is_k ? r.k_norm : nullptr;
-    float scale = 1.0f;
-    if (gain) {
-      // rmsnorm over the head: the lanes of the group hold parts of it
-      float ss = 0.0f;
-      for (int u = lane; u < units; u += gs) {
-        const int e0 = u < nu ? (rt.interleaved ? 2 * u * VE : u * VE) : 2 * half + (u - nu) * VE;
-        float a[VE];
-        load_vec<A, VE>(x + e0, a);
+    if (w.live && (is_q || w.base >= 0)) {
+      const int head = is_q ? row : is_k ? row - r.n_q : row - r.n_q - r.n_kv;
+      A* yq = static_cast<A*>(r.q_out) + (t0 + tk) * r.qo_ts + (size_t)head * r.qo_hs;
+      C* yc = static_cast<C*>(is_k ? kv.k : kv.v) + w.base + (size_t)head * kv.head_stride;
+      if (is_q ? r.q_norm != nullptr : is_k && r.k_norm != nullptr) {
+        // rmsnorm over the head: the lanes of the group hold parts of it
+        const float* gain = s_gain[is_q ? 0 : 1];
+        float ss = 0.0f;
 #pragma unroll
-        for (int j = 0; j < VE; ++j) ss += a[j] * a[j];
-        if (u < nu) {
-          load_vec<A, VE>(x + (rt.interleaved ? e0 + VE : e0 + half), a);
+        for (int m = 0; m < MU; ++m)
 #pragma unroll
-          for (int j = 0; j < VE; ++j) ss += a[j] * a[j];
+          for (int j = 0; j < VE; ++j) ss += a[m][j] * a[m][j] + b[m][j] * b[m][j];
+        for (int o = 1; o < gs; o <<= 1) ss += __shfl_xor(ss, o);
+        const float scale = 1.0f / sqrtf(ss / (float)r.hd + r.eps);
+#pragma unroll
+        for (int m = 0; m < MU; ++m) {
+          const int u = lane + m * gs, e0 = first_of(u), e1 = rt.interleaved ? e0 + VE : e0 + half;
+          if (u < units)
+#pragma unroll
+            for (int j = 0; j < VE; ++j) a[m][j] = a[m][j] * scale * gain[e0 + j];
+          if (u < nu)
+#pragma unroll
+            for (int j = 0; j < VE; ++j) b[m][j] = b[m][j] * scale * gain[e1 + j];
         }
       }
-      for (int o = 1; o < gs; o <<= 1) ss += __shfl_xor(ss, o);
-      scale = 1.0f / sqrtf(ss / (float)r.hd + r.eps);
-    }
-    for (int u = lane; u < units; u += gs) {
-      const bool turn = u < nu;
-      const int e0 = turn ? (rt.interleaved ? 2 * u * VE : u * VE) : 2 * half + (u - nu) * VE;
-      const int e1 = rt.interleaved ? e0 + VE : e0 + half;
-      float a[VE], b[VE];
-      load_vec<A, VE>(x + e0, a);
-      if (turn) load_vec<A, VE>(x + e1, b);
-      if (gain) {
 #pragma unroll
-        for (int j = 0; j < VE; ++j) a[j] = a[j] * scale * gain[e0 + j];
-        if (turn)
+      for (int m = 0; m < MU; ++m) {
+        const int u = lane + m * gs, e0 = first_of(u), e1 = rt.interleaved ? e0 + VE : e0 + half;
+        if (u < nu && (is_q || is_k)) {
+          const float2* c = cs + tk * half + u * VE;
+          if (rt.interleaved && VE > 1) {
+            // pairs (0,1), (2,3), ... of the 2·VE elements a, b
 #pragma unroll
-          for (int j = 0; j < VE; ++j) b[j] = b[j] * scale * gain[e1 + j];
-      }
-      if (turn && (is_q || is_k)) {
-        const float2* c = cs + tk * half + u * VE;
-        if (rt.interleaved && VE > 1) {
-          // pairs (0,1), (2,3), ... of the 2·VE elements a, b
+            for (int j = 0; j < VE; j += 2) {
+              const float2 ca = c[j / 2], cb = c[VE / 2 + j / 2];
+              const float a0 = a[m][j], a1 = a[m][j + 1], b0 = b[m][j], b1 = b[m][j + 1];
+              a[m][j] = a0 * ca.x - a1 * ca.y;
+              a[m][j + 1] = a0 * ca.y + a1 * ca.x;
+              b[m][j] = b0 * cb.x - b1 * cb.y;
+              b[m][j + 1] = b0 * cb.y + b1 * cb.x;
+            }
+          } else {
 #pragma unroll
-          for (int j = 0; j < VE; j += 2) {
-            const float2 ca = c[j / 2], cb = c[VE / 2 + j / 2];
-            const float a0 = a[j], a1 = a[j + 1], b0 = b[j], b1 = b[j + 1];
-            a[j] = a0 * ca.x - a1 * ca.y;
-            a[j + 1] = a0 * ca.y + a1 * ca.x;
-            b[j] = b0 * cb.x - b1 * cb.y;
-            b[j + 1] = b0 * cb.y + b1 * cb.x;
+            for (int j = 0; j < VE; ++j) {
+              const float a0 = a[m][j], b0 = b[m][j];
+              a[m][j] = a0 * c[j].x - b0 * c[j].y;
+              b[m][j] = a0 * c[j].y + b0 * c[j].x;
+            }
           }
+        }
+        if (is_q) {
+          if (u < units) store_vec<A, VE>(yq + e0, a[m]);
+          if (u < nu) store_vec<A, VE>(yq + e1, b[m]);
         } else {
-#pragma unroll
-          for (int j = 0; j < VE; ++j) {
-            const float a0 = a[j], b0 = b[j];
-            a[j] = a0 * c[j].x - b0 * c[j].y;
-            b[j] = a0 * c[j].y + b0 * c[j].x;
-          }
+          if (u < units) store_vec<C, VE>(yc + e0, a[m]);
+          if (u < nu) store_vec<C, VE>(yc + e1, b[m]);
         }
       }
-      if (is_q) {
-        store_vec<A, VE>(yq + e0, a);
-        if (turn) store_vec<A, VE>(yq + e1, b);
-      } else {
-        store_vec<C, VE>(yc + e0, a);
-        if (turn) store_vec<C, VE>(yc + e1, b);
-      }
     }
+    i += RR_THREADS / gs;
+    if (i < n_tok * n_rows) load(i);
   }
 }
 
@@ -235,14 +250,18 @@ hipError_t rope_rows_of(hipStream_t s, const RopeRows& r, const RopeTurns& t, co
   // (arrays start 16-byte aligned, the pool's strides are whole 16-byte pieces)
   const bool wide = t.half % 8 == 0 && r.hd % 8 == 0 &&
                     (r.q_ts % per | r.q_hs % per | r.qo_ts % per | r.qo_hs % per | r.k_ts % per | r.v_ts % per) == 0;
-  const int ve = wide ? 8 : 1, units = t.half / ve + (r.hd - 2 * t.half) / ve;
+  const int ve = wide ? 8 : 1, units = t.half / ve + (r.hd - 2 * t.half) / ve, n_rows = r.n_q + 2 * r.n_kv;
   int gs = 1;
   while (gs < units && gs < 64) gs *= 2;
+  const int at_once = RR_THREADS / gs;
   const int tpb = r.T >= 4096 ? 2 : 1;
-  const dim3 grid((unsigned)((r.T + tpb - 1) / tpb));
-  const size_t lds = (size_t)tpb * t.half * sizeof(float2);
-  if (wide) BB_LAUNCH((k_rope_rows<A, C, 8>), grid, dim3(RR_THREADS), lds, s, r, t, kv, sq, tpb, gs);
-  else BB_LAUNCH((k_rope_rows<A, C, 1>), grid, dim3(RR_THREADS), lds, s, r, t, kv, sq, tpb, gs);
+  // a token's rows go to several blocks while that leaves the device's blocks few: one turn of the rows each
+  const size_t tok_blocks = (r.T + tpb - 1) / tpb;
+  const size_t want = std::max<size_t>(1, std::min<size_t>((n_rows + at_once - 1) / at_once, 2048 / tok_blocks));
+  const int rpb = (int)((n_rows + want - 1) / want);
+  const dim3 grid((unsigned)tok_blocks, (unsigned)((n_rows + rpb - 1) / rpb));
+  if (wide) BB_LAUNCH((k_rope_rows<A, C, 8>), grid, dim3(RR_THREADS), 0, s, r, t, kv, sq, tpb, rpb, gs);
+  else BB_LAUNCH((k_rope_rows<A, C, 1>), grid, dim3(RR_THREADS), 0, s, r, t, kv, sq, tpb, rpb, gs);
   return hipGetLastError();
 }
 
@@ -308,8 +327,13 @@ hipError_t launch_rope_rows(hipStream_t s, int dtype, int cache, const RopeRows&
 namespace {
 
 constexpr int PA_WAVES = 4, PA_THREADS = 64 * PA_WAVES;
-constexpr int PA_UNIT = 128;      // positions of a unit: a tile for each wave
-constexpr int PA_PAIR = 2;        // what a pair costs besides its units
+constexpr int PA_UNIT = 7;        // positions of a unit (their logarithm): a tile for each wave
+// The same where no sequence reaches past one: no pair is split and nothing is to be joined, which costs 4 to 5 us. By
+// the bytes of a head's row (one sequence, 8 kv heads; whole and split): bf16, 64 elements: 512
+// positions 8.1 and 10.1 us, 1000 11.7 and 11.0; f32, 64: 512 10.4 and 10.9; f32, 256 elements (4
+// sequences): 256 17.9 and 19.1, 512 27.0 and 19.1.
+__host__ __device__ constexpr int pa_unit_short(int row_bytes) { return row_bytes <= 256 ? 9 : 8; }
+constexpr int PA_PAIR = 1;        // what a pair costs besides its units
 constexpr int PA_HEADS = 16;      // heads of a group at most
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr float NEG_INF = -__builtin_inff();
@@ -322,7 +346,7 @@ typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 // A kv head's G query heads: `split` groups of `hg` (the last may have fewer).
 struct PagedPlan {
-  int G, split, hg, n_groups, join;
+  int G, split, hg, n_groups, join, unit;  // unit: the logarithm of a unit's positions
   int* chunk;     // [1 + n_seqs + 1]: cost of a block's run, cost of a group in the sequences before each
   float* sums;    // [2·blocks][hg][hd]: of a pair that began in a block before (slot 0), that goes on in the next (1)
   float2* ml;     // [2·blocks][hg]: maximum (base 2), sum of weights
@@ -331,12 +355,12 @@ struct PagedPlan {
 struct SeqSpan {
   int base, first, len, units;  // positions first..len-1, counted from base; units >= 1
 };
-__device__ __forceinline__ SeqSpan seq_span(int raw_len, int cap, int window) {
+__device__ __forceinline__ SeqSpan seq_span(int raw_len, int cap, int window, int unit) {
   SeqSpan r;
   r.len = min(max(raw_len, 0), cap);
   r.first = window > 0 ? max(0, r.len - window) : 0;
   r.base = r.first & ~31;
-  r.units = max(1, (r.len - r.base + PA_UNIT - 1) / PA_UNIT);
+  r.units = max(1, (r.len - r.base + (1 << unit) - 1) >> unit);
   return r;
 }
 
@@ -421,7 +445,7 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
-// a / b for 0 <= a < 2^30, b >= 1 and a quotient below 2^20, the same for the wave: the f32 quotient is off by less than 1.
+// a / b for 0 <= a < 2^30, b >= 1 and a quotient below 2^20 (the same for the wave): the f32 quotient is off by less than 1.
 __device__ __forceinline__ int small_div(int a, int b) {
   int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
   q -= q * b > a ? 1 : 0;
@@ -783,7 +807,7 @@ struct SeqScan {
   int c0;
   int len[4], cost[4], incl[4];
   int all;         // of the 256
-  __device__ __forceinline__ void load(const int* __restrict__ lens, int n_seqs, int cap, int window, int lane) {
+  __device__ __forceinline__ void load(const int* __restrict__ lens, int n_seqs, int cap, int window, int unit, int lane) {
     all = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) len[i] = c0 + 64 * i < n_seqs ? lens[min(c0 + 64 * i + lane, n_seqs - 1)] : 0;
@@ -791,7 +815,7 @@ struct SeqScan {
     for (int i = 0; i < 4; ++i) {
       cost[i] = incl[i] = 0;
       if (c0 + 64 * i < n_seqs) {
-        cost[i] = c0 + 64 * i + lane < n_seqs ? seq_span(len[i], cap, window).units + PA_PAIR : 0;
+        cost[i] = c0 + 64 * i + lane < n_seqs ? seq_span(len[i], cap, window, unit).units + PA_PAIR : 0;
         incl[i] = all + wave_scan(cost[i]);
         all = __builtin_amdgcn_readlane(incl[i], 63);
       }
@@ -817,7 +841,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
     SeqScan sc;
     int total = 0;
     for (sc.c0 = 0;; sc.c0 += 256) {
-      sc.load(lens, n_seqs, cap, pq.window, lane);
+      sc.load(lens, n_seqs, cap, pq.window, pl.unit, lane);
       if (pl.join && blockIdx.x == 0 && wv == 0) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -839,11 +863,11 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
     int before = 0;
     if (sc.c0 > 0) {
       sc.c0 = 0;
-      sc.load(lens, n_seqs, cap, pq.window, lane);
+      sc.load(lens, n_seqs, cap, pq.window, pl.unit, lane);
       while (u >= (before + sc.all) * pl.n_groups) {
         before += sc.all;
         sc.c0 += 256;
-        sc.load(lens, n_seqs, cap, pq.window, lane);
+        sc.load(lens, n_seqs, cap, pq.window, pl.unit, lane);
       }
     }
     bool found = false;
@@ -873,7 +897,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
       grp = 0;
       ++s;
       len = __builtin_amdgcn_readfirstlane(lens[s]);
-      cost = seq_span(len, cap, pq.window).units + PA_PAIR;
+      cost = seq_span(len, cap, pq.window, pl.unit).units + PA_PAIR;
     }
     const int nu = cost - PA_PAIR, first_unit = lo + PA_PAIR;
     const int u0 = max(u - first_unit, 0), take = min(nu, end - first_unit) - u0;
@@ -883,10 +907,10 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
     w.head0 = kvh * pl.G + sub * pl.hg;
     w.heads = min(pl.hg, pl.G - sub * pl.hg);
     w.kv_off = (size_t)kvh * kv.head_stride;
-    w.sp = seq_span(len, cap, pq.window);
+    w.sp = seq_span(len, cap, pq.window, pl.unit);
     w.start(pq, s);
-    const int k0 = w.sp.base + u0 * PA_UNIT;
-    w.run(k0 + wv * S::KT, min(k0 + take * PA_UNIT, w.sp.len), PA_WAVES * S::KT);
+    const int k0 = w.sp.base + (u0 << pl.unit);
+    w.run(k0 + wv * S::KT, min(k0 + (take << pl.unit), w.sp.len), PA_WAVES * S::KT);
 
     // the waves' sums together
     if (lds_read) __syncthreads();  // (the pair before is done with LDS)
@@ -944,16 +968,18 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
 // Adds the partial sums of a (sequence, head), PJ_PIECES pieces of 4 elements a block: those of the blocks whose
 // runs hold units of it. Threads: a row of PJ_PIECES for every PJ_ROWS-th part, joined in LDS.
 constexpr int PJ_THREADS = 256, PJ_PIECES = 8, PJ_ROWS = PJ_THREADS / PJ_PIECES;
-__global__ void __launch_bounds__(PJ_THREADS) k_paged_join(PagedQuery pq, int hd, PagedPlan pl, float up) {
+__global__ void __launch_bounds__(PJ_THREADS) k_paged_join(PagedQuery pq, int hd, int blocks_of_row, PagedPlan pl, float up) {
   __shared__ float s_m[PJ_ROWS], s_l[PJ_ROWS];
   __shared__ v4f s_x[PJ_ROWS][PJ_PIECES];
-  const int s = blockIdx.x, h = blockIdx.y, piece = blockIdx.z * PJ_PIECES + threadIdx.x % PJ_PIECES;
+  const int s = blockIdx.x, grp = blockIdx.y, hh = blockIdx.z / blocks_of_row;
+  const int piece = (blockIdx.z - hh * blocks_of_row) * PJ_PIECES + threadIdx.x % PJ_PIECES;
   const int row = threadIdx.x / PJ_PIECES;
   const int chunk = pl.chunk[0], before = pl.chunk[1 + s], cost = pl.chunk[2 + s] - before;
-  const int kvh = h / pl.G, sub = (h - kvh * pl.G) / pl.hg, hh = h - kvh * pl.G - sub * pl.hg;
-  const int lo = before * pl.n_groups + (kvh * pl.split + sub) * cost + PA_PAIR, hi = lo + cost - PA_PAIR;
-  const int b0 = lo / chunk, b1 = (hi - 1) / chunk;
+  const int lo = before * pl.n_groups + grp * cost + PA_PAIR, hi = lo + cost - PA_PAIR;
+  const int b0 = small_div(lo, chunk), b1 = small_div(hi - 1, chunk);
   if (b0 == b1) return;  // whole in one block
+  const int kvh = pl.split == 1 ? grp : grp / pl.split, in = (grp - kvh * pl.split) * pl.hg + hh, h = kvh * pl.G + in;
+  if (in >= pl.G) return;  // (the last group of a kv head may have fewer heads)
   const int parts = b1 - b0 + 1;
   float m = NEG_INF, l = 0.0f;
   v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -1009,7 +1035,7 @@ PagedPlan pa_plan(int n_seqs, int n_heads, int n_kv) {
 
 bool paged_attn_fits(int n_seqs, int n_heads, int n_kv, size_t cap) {
   const PagedPlan p = pa_plan(n_seqs, n_heads, n_kv);
-  return (size_t)n_seqs * (size_t)p.n_groups * ((cap + PA_UNIT - 1) / PA_UNIT + PA_PAIR) < ((size_t)1 << 29);
+  return (size_t)n_seqs * (size_t)p.n_groups * ((cap >> PA_UNIT) + 1 + PA_PAIR) < ((size_t)1 << 29);
 }
 
 void paged_divisor(PagedView& v) {
@@ -1029,16 +1055,20 @@ hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQue
                              const PagedSeqs& sq) {
   if (sq.n_seqs == 0) return hipSuccess;
   PagedPlan pl = pa_plan(sq.n_seqs, q.n_heads, kv.n_kv);
-  const size_t cap = (size_t)sq.max_pages * kv.page_size;
+  // positions of a sequence that count, at most (a window begins anywhere in 32)
+  size_t cap = (size_t)sq.max_pages * kv.page_size;
+  if (q.window > 0) cap = std::min(cap, (size_t)q.window + 31);
   const int blocks_max = pa_blocks(n_cu, kv.hd);
   const size_t slots = 2 * (size_t)blocks_max * pl.hg;
   pl.sums = static_cast<float*>(q.ws);
   pl.ml = reinterpret_cast<float2*>(pl.sums + slots * kv.hd);
   pl.chunk = reinterpret_cast<int*>(pl.ml + slots);
   // (pairs of one unit take a block each at most, longer ones a block for each unit)
-  const size_t units = (cap + PA_UNIT - 1) / PA_UNIT, pairs = (size_t)sq.n_seqs * pl.n_groups;
+  const int unit_short = pa_unit_short(kv.hd * (cache == BB_F32 ? 4 : 2));
+  pl.unit = cap <= (size_t)1 << unit_short ? unit_short : PA_UNIT;
+  const size_t units = ((cap - 1) >> pl.unit) + 1, pairs = (size_t)sq.n_seqs * pl.n_groups;
   const unsigned blocks = (unsigned)std::min<size_t>(blocks_max, pairs * (units == 1 ? 1 : units + PA_PAIR));
-  pl.join = cap > (size_t)PA_UNIT;  // else every pair is one unit
+  pl.join = units > 1;
   const bool uni = kv.page_size % 16 == 0 && 16 * kv.pos_stride < ((size_t)1 << 29);
   const int cls = pa_class(kv.hd);
   const size_t lds = (size_t)PA_WAVES * pl.hg * (cls + 4) * 4;
@@ -1065,8 +1095,9 @@ hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQue
 #undef BB_PA
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !pl.join) return e;
-  BB_LAUNCH(k_paged_join, dim3(sq.n_seqs, q.n_heads, (kv.hd + 4 * PJ_PIECES - 1) / (4 * PJ_PIECES)), dim3(PJ_THREADS), 0,
-            st, q, kv.hd, pl, cache == BB_F16 ? 14.0f : 0.0f);
+  const int blocks_of_row = (kv.hd + 4 * PJ_PIECES - 1) / (4 * PJ_PIECES);
+  BB_LAUNCH(k_paged_join, dim3(sq.n_seqs, pl.n_groups, pl.hg * blocks_of_row), dim3(PJ_THREADS), 0, st, q, kv.hd,
+            blocks_of_row, pl, cache == BB_F16 ? 14.0f : 0.0f);
   return hipGetLastError();
 }
 
