@@ -81,7 +81,6 @@ __device__ __forceinline__ float2 cos_sin_turns(int pos, double turns) {
 }
 
 constexpr int RR_THREADS = 256;
-constexpr int RR_TPB_MAX = 2;  // tokens of a block at most: a (cos, sin) a thread
 
 struct RowPlace {
   int64_t base;  // where its keys and values start in the pool, -1: nowhere
@@ -126,121 +125,114 @@ __device__ __forceinline__ RowPlace row_place(const RopeRows& r, const PagedView
   return w;
 }
 
-// A block takes tpb tokens and rows blockIdx.y·rpb.. (rpb of them) of each. Its waves find the tokens' places, its
-// threads the (cos, sin) of every (token, pair) once into LDS; then groups of gs lanes (a power of two)
-// take a head row each, a lane up to MU pairs of runs of VE elements that turn together (or runs past
-// the turned part). VE 8: whole 16-byte pieces; VE 1: any size and stride.
-// One token's call is latency: what needs neither place nor angle (the first rows, gains, frequencies) is
-// asked for before the place is known. A long batch is bound by its bytes: ROPE_FIGURES.
+// A block takes rpb of a token's head rows. Its first wave finds the token's place, its threads the (cos, sin) of the
+// pairs once into LDS; then groups of gs lanes (a power of two) take a head row each, a lane up to MU
+// pairs of runs of VE elements that turn together (or runs past the turned part). VE 8: whole 16-byte
+// pieces; VE 1: any size and stride.
+// One token's call is latency, a long batch is bound by its bytes: ROPE_FIGURES.
 template <class A, class C, int VE>
-__global__ void __launch_bounds__(RR_THREADS) k_rope_rows(RopeRows r, RopeTurns rt, PagedView kv, PagedSeqs sq, int tpb,
-                                                          int rpb, int gs) {
+__global__ void __launch_bounds__(RR_THREADS) k_rope_rows(RopeRows r, RopeTurns rt, PagedView kv, PagedSeqs sq, int rpb,
+                                                          int gs) {
   constexpr int MU = VE == 1 ? 4 : 1;
-  __shared__ float2 cs[RR_THREADS];  // [tpb][half]
+  __shared__ float2 cs[OPS_HD_MAX / 2];
   __shared__ float s_gain[2][OPS_HD_MAX];
-  __shared__ RowPlace place[RR_TPB_MAX];
-  const int tid = threadIdx.x, half = rt.half, n_all = r.n_q + 2 * r.n_kv;
-  const size_t t0 = (size_t)blockIdx.x * tpb;
-  const int row0 = blockIdx.y * rpb, n_rows = min(rpb, n_all - row0), n_tok = (int)min((size_t)tpb, r.T - t0);
+  __shared__ RowPlace place;
+  const int tid = threadIdx.x, half = rt.half;
+  const size_t t = blockIdx.x;
+  const int row0 = blockIdx.y * rpb, row1 = min(row0 + rpb, r.n_q + 2 * r.n_kv);
   const int nu = half / VE, units = nu + (r.hd - 2 * half) / VE, lane = tid & (gs - 1);
 
-  float a[MU][VE], b[MU][VE];
+  const double turns = tid < half ? rt.turns[tid] : 0.0;
+  if (r.q_norm && tid < r.hd) s_gain[0][tid] = r.q_norm[tid];
+  if (r.k_norm && tid < r.hd) s_gain[1][tid] = r.k_norm[tid];
+  if (tid < 64) {
+    const RowPlace w = row_place(r, kv, sq, t);
+    if (tid == 0) place = w;
+  }
+  __syncthreads();
+  const RowPlace w = place;
+  if (!w.live) return;  // the whole block
+  if (tid < half) {
+    const float2 v = cos_sin_turns(w.pos, turns);
+    cs[tid] = make_float2(rt.magnitude * v.x, rt.magnitude * v.y);
+  }
+  __syncthreads();
   const auto first_of = [&](int u) { return u < nu ? (rt.interleaved ? 2 * u * VE : u * VE) : 2 * half + (u - nu) * VE; };
-  const auto load = [&](int i) {
-    const int tk = i / n_rows, row = row0 + i - tk * n_rows;
-    const size_t t = t0 + tk;
-    const A* x = row < r.n_q            ? static_cast<const A*>(r.q) + t * r.q_ts + (size_t)row * r.q_hs
-                 : row < r.n_q + r.n_kv ? static_cast<const A*>(r.k) + t * r.k_ts + (size_t)(row - r.n_q) * r.hd
-                                        : static_cast<const A*>(r.v) + t * r.v_ts + (size_t)(row - r.n_q - r.n_kv) * r.hd;
+  for (int row = row0 + tid / gs; row < row1; row += RR_THREADS / gs) {
+    const bool is_q = row < r.n_q, is_k = !is_q && row < r.n_q + r.n_kv;
+    if (!is_q && w.base < 0) continue;
+    const int head = is_q ? row : is_k ? row - r.n_q : row - r.n_q - r.n_kv;
+    const A* x = is_q   ? static_cast<const A*>(r.q) + t * r.q_ts + (size_t)head * r.q_hs
+                 : is_k ? static_cast<const A*>(r.k) + t * r.k_ts + (size_t)head * r.hd
+                        : static_cast<const A*>(r.v) + t * r.v_ts + (size_t)head * r.hd;
+    float a[MU][VE], b[MU][VE];
 #pragma unroll
     for (int m = 0; m < MU; ++m) {
       const int u = lane + m * gs, e0 = first_of(u);
 #pragma unroll
       for (int j = 0; j < VE; ++j) a[m][j] = b[m][j] = 0.0f;
+      if (m * gs >= units) continue;
       if (u < units) load_vec<A, VE>(x + e0, a[m]);
       if (u < nu) load_vec<A, VE>(x + (rt.interleaved ? e0 + VE : e0 + half), b[m]);
     }
-  };
-  int i = tid / gs;
-  if (i < n_tok * n_rows) load(i);
-  const double turns = tid < tpb * half ? rt.turns[tid % half] : 0.0;
-  if (r.q_norm && tid < r.hd) s_gain[0][tid] = r.q_norm[tid];
-  if (r.k_norm && tid < r.hd) s_gain[1][tid] = r.k_norm[tid];
-  if (tid >> 6 < tpb) {
-    const RowPlace w = row_place(r, kv, sq, t0 + (tid >> 6));
-    if ((tid & 63) == 0) place[tid >> 6] = w;
-  }
-  __syncthreads();
-  if (tid < tpb * half) {
-    const float2 v = cos_sin_turns(place[tid / half].pos, turns);
-    cs[tid] = make_float2(rt.magnitude * v.x, rt.magnitude * v.y);
-  }
-  __syncthreads();
-  while (i < n_tok * n_rows) {
-    const int tk = i / n_rows, row = row0 + i - tk * n_rows;
-    const RowPlace w = place[tk];
-    const bool is_q = row < r.n_q, is_k = !is_q && row < r.n_q + r.n_kv;
-    if (w.live && (is_q || w.base >= 0)) {
-      const int head = is_q ? row : is_k ? row - r.n_q : row - r.n_q - r.n_kv;
-      A* yq = static_cast<A*>(r.q_out) + (t0 + tk) * r.qo_ts + (size_t)head * r.qo_hs;
-      C* yc = static_cast<C*>(is_k ? kv.k : kv.v) + w.base + (size_t)head * kv.head_stride;
-      if (is_q ? r.q_norm != nullptr : is_k && r.k_norm != nullptr) {
-        // rmsnorm over the head: the lanes of the group hold parts of it
-        const float* gain = s_gain[is_q ? 0 : 1];
-        float ss = 0.0f;
+    A* yq = static_cast<A*>(r.q_out) + t * r.qo_ts + (size_t)head * r.qo_hs;
+    C* yc = static_cast<C*>(is_k ? kv.k : kv.v) + w.base + (size_t)head * kv.head_stride;
+    if (is_q ? r.q_norm != nullptr : is_k && r.k_norm != nullptr) {
+      // rmsnorm over the head: the lanes of the group hold parts of it
+      const float* gain = s_gain[is_q ? 0 : 1];
+      float ss = 0.0f;
 #pragma unroll
-        for (int m = 0; m < MU; ++m)
+      for (int m = 0; m < MU; ++m)
 #pragma unroll
-          for (int j = 0; j < VE; ++j) ss += a[m][j] * a[m][j] + b[m][j] * b[m][j];
-        for (int o = 1; o < gs; o <<= 1) ss += __shfl_xor(ss, o);
-        const float scale = 1.0f / sqrtf(ss / (float)r.hd + r.eps);
-#pragma unroll
-        for (int m = 0; m < MU; ++m) {
-          const int u = lane + m * gs, e0 = first_of(u), e1 = rt.interleaved ? e0 + VE : e0 + half;
-          if (u < units)
-#pragma unroll
-            for (int j = 0; j < VE; ++j) a[m][j] = a[m][j] * scale * gain[e0 + j];
-          if (u < nu)
-#pragma unroll
-            for (int j = 0; j < VE; ++j) b[m][j] = b[m][j] * scale * gain[e1 + j];
-        }
-      }
+        for (int j = 0; j < VE; ++j) ss += a[m][j] * a[m][j] + b[m][j] * b[m][j];
+      for (int o = 1; o < gs; o <<= 1) ss += __shfl_xor(ss, o);
+      const float scale = 1.0f / sqrtf(ss / (float)r.hd + r.eps);
 #pragma unroll
       for (int m = 0; m < MU; ++m) {
         const int u = lane + m * gs, e0 = first_of(u), e1 = rt.interleaved ? e0 + VE : e0 + half;
-        if (u < nu && (is_q || is_k)) {
-          const float2* c = cs + tk * half + u * VE;
-          if (rt.interleaved && VE > 1) {
-            // pairs (0,1), (2,3), ... of the 2·VE elements a, b
+        if (m * gs >= units) break;
+        if (u < units)
 #pragma unroll
-            for (int j = 0; j < VE; j += 2) {
-              const float2 ca = c[j / 2], cb = c[VE / 2 + j / 2];
-              const float a0 = a[m][j], a1 = a[m][j + 1], b0 = b[m][j], b1 = b[m][j + 1];
-              a[m][j] = a0 * ca.x - a1 * ca.y;
-              a[m][j + 1] = a0 * ca.y + a1 * ca.x;
-              b[m][j] = b0 * cb.x - b1 * cb.y;
-              b[m][j + 1] = b0 * cb.y + b1 * cb.x;
-            }
-          } else {
+          for (int j = 0; j < VE; ++j) a[m][j] = a[m][j] * scale * gain[e0 + j];
+        if (u < nu)
 #pragma unroll
-            for (int j = 0; j < VE; ++j) {
-              const float a0 = a[m][j], b0 = b[m][j];
-              a[m][j] = a0 * c[j].x - b0 * c[j].y;
-              b[m][j] = a0 * c[j].y + b0 * c[j].x;
-            }
-          }
-        }
-        if (is_q) {
-          if (u < units) store_vec<A, VE>(yq + e0, a[m]);
-          if (u < nu) store_vec<A, VE>(yq + e1, b[m]);
-        } else {
-          if (u < units) store_vec<C, VE>(yc + e0, a[m]);
-          if (u < nu) store_vec<C, VE>(yc + e1, b[m]);
-        }
+          for (int j = 0; j < VE; ++j) b[m][j] = b[m][j] * scale * gain[e1 + j];
       }
     }
-    i += RR_THREADS / gs;
-    if (i < n_tok * n_rows) load(i);
+#pragma unroll
+    for (int m = 0; m < MU; ++m) {
+      const int u = lane + m * gs, e0 = first_of(u), e1 = rt.interleaved ? e0 + VE : e0 + half;
+      if (m * gs >= units) break;
+      if (u < nu && (is_q || is_k)) {
+        const float2* c = cs + u * VE;
+        if (rt.interleaved && VE > 1) {
+          // pairs (0,1), (2,3), ... of the 2·VE elements a, b
+#pragma unroll
+          for (int j = 0; j < VE; j += 2) {
+            const float2 ca = c[j / 2], cb = c[VE / 2 + j / 2];
+            const float a0 = a[m][j], a1 = a[m][j + 1], b0 = b[m][j], b1 = b[m][j + 1];
+            a[m][j] = a0 * ca.x - a1 * ca.y;
+            a[m][j + 1] = a0 * ca.y + a1 * ca.x;
+            b[m][j] = b0 * cb.x - b1 * cb.y;
+            b[m][j + 1] = b0 * cb.y + b1 * cb.x;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < VE; ++j) {
+            const float a0 = a[m][j], b0 = b[m][j];
+            a[m][j] = a0 * c[j].x - b0 * c[j].y;
+            b[m][j] = a0 * c[j].y + b0 * c[j].x;
+          }
+        }
+      }
+      if (is_q) {
+        if (u < units) store_vec<A, VE>(yq + e0, a[m]);
+        if (u < nu) store_vec<A, VE>(yq + e1, b[m]);
+      } else {
+        if (u < units) store_vec<C, VE>(yc + e0, a[m]);
+        if (u < nu) store_vec<C, VE>(yc + e1, b[m]);
+      }
+    }
   }
 }
 
@@ -254,14 +246,12 @@ hipError_t rope_rows_of(hipStream_t s, const RopeRows& r, const RopeTurns& t, co
   int gs = 1;
   while (gs < units && gs < 64) gs *= 2;
   const int at_once = RR_THREADS / gs;
-  const int tpb = r.T >= 4096 ? 2 : 1;
-  // a token's rows go to several blocks while that leaves the device's blocks few: one turn of the rows each
-  const size_t tok_blocks = (r.T + tpb - 1) / tpb;
-  const size_t want = std::max<size_t>(1, std::min<size_t>((n_rows + at_once - 1) / at_once, 2048 / tok_blocks));
+  // a token's rows go to several blocks, one turn of the rows each, while all the blocks fit the device at once
+  const size_t want = std::max<size_t>(1, std::min<size_t>((n_rows + at_once - 1) / at_once, 2048 / r.T));
   const int rpb = (int)((n_rows + want - 1) / want);
-  const dim3 grid((unsigned)tok_blocks, (unsigned)((n_rows + rpb - 1) / rpb));
-  if (wide) BB_LAUNCH((k_rope_rows<A, C, 8>), grid, dim3(RR_THREADS), 0, s, r, t, kv, sq, tpb, rpb, gs);
-  else BB_LAUNCH((k_rope_rows<A, C, 1>), grid, dim3(RR_THREADS), 0, s, r, t, kv, sq, tpb, rpb, gs);
+  const dim3 grid((unsigned)r.T, (unsigned)((n_rows + rpb - 1) / rpb));
+  if (wide) BB_LAUNCH((k_rope_rows<A, C, 8>), grid, dim3(RR_THREADS), 0, s, r, t, kv, sq, rpb, gs);
+  else BB_LAUNCH((k_rope_rows<A, C, 1>), grid, dim3(RR_THREADS), 0, s, r, t, kv, sq, rpb, gs);
   return hipGetLastError();
 }
 
