@@ -435,9 +435,12 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
-// a / b for 0 <= a < 2^30, b >= 1 and a quotient below 2^20 (the same for the wave): the f32 quotient is off by less than 1.
-__device__ __forceinline__ int small_div(int a, int b) {
-  int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
+// a / b for 0 <= a < 2^30, b >= 1 (the same for the wave): two steps of an f32 quotient, each off by less than
+// 2^-22 of itself and 1, then at most 1 off.
+__device__ __forceinline__ int uniform_div(int a, int b) {
+  const float inv = __builtin_amdgcn_rcpf((float)b);
+  int q = (int)((float)a * inv);
+  q += (int)((float)(a - q * b) * inv);
   q -= q * b > a ? 1 : 0;
   q += (q + 1) * b <= a ? 1 : 0;
   return __builtin_amdgcn_readfirstlane(q);
@@ -826,39 +829,43 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
   const int cap = max_pages * kv.page_size;
 
   // every wave finds the block's run by itself: the total cost, then the sequence in whose cost the run begins
+  // (more than 256 sequences are gone through twice)
   int u = 0, end = 0, s = 0, cost = 0, len = 0, lo = 0;
   {
     SeqScan sc;
-    int total = 0;
-    for (sc.c0 = 0;; sc.c0 += 256) {
-      sc.load(lens, n_seqs, cap, pq.window, pl.unit, lane);
-      if (pl.join && blockIdx.x == 0 && wv == 0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (sc.c0 + 64 * i + lane < n_seqs) pl.chunk[2 + sc.c0 + 64 * i + lane] = total + sc.incl[i];
-      }
-      total += sc.all;
-      if (sc.c0 + 256 >= n_seqs) break;
-    }
-    total *= pl.n_groups;
-    const int grid = (int)gridDim.x, up_to = total + grid - 1;
-    const int chunk = total <= grid ? 1 : total < (1 << 20) ? small_div(up_to, grid) : (int)((uint32_t)up_to / grid);
-    if (pl.join && blockIdx.x == 0 && tid == 0) {
-      pl.chunk[0] = chunk;
-      pl.chunk[1] = 0;
-    }
-    if ((int64_t)blockIdx.x * chunk >= total) return;
-    u = (int)blockIdx.x * chunk;
-    end = min(u + chunk, total);
+    sc.c0 = 0;
     int before = 0;
-    if (sc.c0 > 0) {
-      sc.c0 = 0;
+    for (;;) {
       sc.load(lens, n_seqs, cap, pq.window, pl.unit, lane);
-      while (u >= (before + sc.all) * pl.n_groups) {
-        before += sc.all;
-        sc.c0 += 256;
-        sc.load(lens, n_seqs, cap, pq.window, pl.unit, lane);
+      if (end == 0) {
+        if (pl.join && blockIdx.x == 0 && wv == 0) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (sc.c0 + 64 * i + lane < n_seqs) pl.chunk[2 + sc.c0 + 64 * i + lane] = before + sc.incl[i];
+        }
+        if (sc.c0 + 256 < n_seqs) {
+          before += sc.all;
+          sc.c0 += 256;
+          continue;
+        }
+        const int total = (before + sc.all) * pl.n_groups, grid = (int)gridDim.x;
+        const int chunk = total <= grid ? 1 : uniform_div(total + grid - 1, grid);
+        if (pl.join && blockIdx.x == 0 && tid == 0) {
+          pl.chunk[0] = chunk;
+          pl.chunk[1] = 0;
+        }
+        if ((int64_t)blockIdx.x * chunk >= total) return;
+        u = (int)blockIdx.x * chunk;
+        end = min(u + chunk, total);
+        before = 0;
+        if (sc.c0 > 0) {
+          sc.c0 = 0;
+          continue;
+        }
       }
+      if (u < (before + sc.all) * pl.n_groups) break;
+      before += sc.all;
+      sc.c0 += 256;
     }
     bool found = false;
 #pragma unroll
@@ -875,7 +882,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
       }
     }
   }
-  int grp = small_div(u - lo, cost);
+  int grp = uniform_div(u - lo, cost);
   lo += grp * cost;
 
   PaWave<CT, NP, HDP, UNI> w(kv, lane);
@@ -892,7 +899,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
     const int nu = cost - PA_PAIR, first_unit = lo + PA_PAIR;
     const int u0 = max(u - first_unit, 0), take = min(nu, end - first_unit) - u0;
     if (take <= 0) continue;  // (the run ends before the pair's units)
-    const int kvh = pl.split == 1 ? grp : small_div(grp, pl.split), sub = grp - kvh * pl.split;
+    const int kvh = pl.split == 1 ? grp : uniform_div(grp, pl.split), sub = grp - kvh * pl.split;
     w.row = table + (size_t)s * table_stride;
     w.head0 = kvh * pl.G + sub * pl.hg;
     w.heads = min(pl.hg, pl.G - sub * pl.hg);
@@ -966,7 +973,7 @@ __global__ void __launch_bounds__(PJ_THREADS) k_paged_join(PagedQuery pq, int hd
   const int row = threadIdx.x / PJ_PIECES;
   const int chunk = pl.chunk[0], before = pl.chunk[1 + s], cost = pl.chunk[2 + s] - before;
   const int lo = before * pl.n_groups + grp * cost + PA_PAIR, hi = lo + cost - PA_PAIR;
-  const int b0 = small_div(lo, chunk), b1 = small_div(hi - 1, chunk);
+  const int b0 = uniform_div(lo, chunk), b1 = uniform_div(hi - 1, chunk);
   if (b0 == b1) return;  // whole in one block
   const int kvh = pl.split == 1 ? grp : grp / pl.split, in = (grp - kvh * pl.split) * pl.hg + hh, h = kvh * pl.G + in;
   if (in >= pl.G) return;  // (the last group of a kv head may have fewer heads)
