@@ -7,9 +7,11 @@
 #include <cstdio>
 #include <cstring>
 #include <exception>
+#include <initializer_list>
 #include <mutex>
 #include <new>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/bebelm_moe.h"
@@ -930,6 +932,7 @@ struct bb_paged_kv {
   int device;
   uint32_t dtype;
   bb::PagedView view;
+  size_t span;             // bytes from the keys' (and the values') first element to past the last
   uint8_t* own = nullptr;  // the pool, when the library allocated it
 };
 
@@ -2579,7 +2582,8 @@ bool capturing(bb_ctx* c) {
   return st != hipStreamCaptureStatusNone;
 }
 
-// The launch wrapper for calls that may be captured: a captured launch is not timed.
+// The launch wrapper for calls that may be captured: a captured launch is not timed (`captured` is asked for
+// where it makes a difference).
 template <class F>
 void launch_paged(bb_ctx* c, bool captured, int id, F&& f) {
   if (captured) check_hip(f(), bb::kernel_name(id));
@@ -2648,8 +2652,18 @@ bb_paged_kv* new_pool(bb_ctx* c, uint32_t dtype, void* k, void* v, size_t n_page
   p->dtype = dtype;
   p->view = {k, v, page_stride, pos_stride, head_stride, (int)n_pages, (int)page_size, (int)n_kv, (int)hd};
   bb::paged_divisor(p->view);
+  p->span = ((n_pages - 1) * page_stride + (page_size - 1) * pos_stride + (n_kv - 1) * head_stride + hd) *
+            (dtype == BB_F32 ? 4 : 2);
   p->own = own;
   return p;
+}
+
+// Arrays on the device lie outside the pool.
+void need_off_pool(const bb_paged_kv* kv, int loc, std::initializer_list<std::pair<const void*, size_t>> arrays) {
+  if (loc != BB_LOC_DEVICE) return;
+  for (const auto& a : arrays)
+    need(!a.first || (!overlap(a.first, a.second, kv->view.k, kv->span) && !overlap(a.first, a.second, kv->view.v, kv->span)),
+         BB_ERR_ARG, "an array lies in the pool");
 }
 
 void need_pool_sizes(size_t n_pages, size_t page_size, size_t n_kv, size_t hd) {
@@ -2703,6 +2717,7 @@ int bb_rope_plan_create(bb_ctx* c, const bb_rope_desc* d, bb_rope_plan** out) {
       need(std::isfinite(turns[i]) && turns[i] < 1e18, BB_ERR_RANGE, "a frequency is out of range");
     }
     set_device(c);
+    need(!capturing(c), BB_ERR_ARG, "a plan cannot be made while a graph is captured");
     auto* dev = static_cast<double*>(dev_alloc(turns.size() * sizeof(double)));
     try {
       copy_to_dev(c, dev, turns.data(), turns.size() * sizeof(double), "rotary frequencies upload");
@@ -2761,7 +2776,7 @@ int bb_rope(bb_ctx* c, const bb_rope_plan* plan, uint32_t dtype, const void* x, 
                    (n_tokens == 1 || token_stride == out_token_stride) && (n_heads == 1 || head_stride == out_head_stride),
                    "out");
     set_device(c);
-    const bool cap = capturing(c);
+    const bool cap = (loc == BB_LOC_HOST || c->profile) && capturing(c);
     need(!(cap && loc == BB_LOC_HOST), BB_ERR_ARG, "a call on host memory cannot be captured");
     // (host memory: out's span goes in too, what lies between its rows stays as it is)
     with_io(c, loc, {{x, nx, true, false}, {pos, n_tokens * 4, true, false}, {out, no, true, true}},
@@ -2795,6 +2810,7 @@ int bb_paged_kv_create(bb_ctx* c, uint32_t dtype, size_t n_pages, size_t page_si
     need(n_pages * (page >> 10) < ((size_t)1 << 40), BB_ERR_RANGE, "pool too large");  // (below 2^61)
     const size_t half = round_up(n_pages * page * eb, 256);
     set_device(c);
+    need(!capturing(c), BB_ERR_ARG, "a pool cannot be made while a graph is captured");
     auto* dev = static_cast<uint8_t*>(dev_alloc(2 * half));
     try {
       clear_dev(c, dev, 2 * half);
@@ -2816,14 +2832,18 @@ int bb_paged_kv_view(bb_ctx* c, uint32_t dtype, void* k, void* v, size_t n_pages
     need_pool_sizes(n_pages, page_size, n_kv_heads, head_dim);
     need_aligned(k, "keys");
     need_aligned(v, "values");
-    need(k != v, BB_ERR_ARG, "keys and values must not be the same memory");
-    std::pair<size_t, size_t> dims[3] = {{page_stride, n_pages}, {pos_stride, page_size}, {head_stride, n_kv_heads}};
-    for (auto& d : dims) {
+    // (the values are a fourth step of two from the keys)
+    const uintptr_t ka = reinterpret_cast<uintptr_t>(k), va = reinterpret_cast<uintptr_t>(v);
+    const size_t apart = (ka < va ? va - ka : ka - va) / eb;
+    std::pair<size_t, size_t> dims[4] = {
+        {page_stride, n_pages}, {pos_stride, page_size}, {head_stride, n_kv_heads}, {apart, 2}};
+    for (int i = 0; i < 3; ++i) {
+      auto& d = dims[i];
       if (d.second == 1) d.first = 0;  // never stepped
       need(d.first < STRIDE_MAX, BB_ERR_RANGE, "stride beyond 2^40 elements");
       need(d.first * eb % 16 == 0, BB_ERR_ARG, "strides must be whole 16-byte pieces");
     }
-    std::sort(dims, dims + 3);
+    std::sort(dims, dims + 4);
     size_t span = head_dim;
     for (const auto& d : dims) {
       if (d.second == 1) continue;
@@ -2899,9 +2919,10 @@ int bb_paged_append(bb_ctx* c, bb_paged_kv* kv, const bb_rope_plan* plan, const 
     } else {
       need(!tk->q_norm && !tk->q_out, BB_ERR_ARG, "q_norm or q_out without q");
     }
+    need_off_pool(kv, loc, {{tk->k, nk}, {tk->v, nv}, {tk->q, nq}, {tk->q_out, nqo}});
     if (tk->q_norm || tk->k_norm) need(tk->eps >= 0.0f && std::isfinite(tk->eps), BB_ERR_ARG, "eps must not be negative");
     set_device(c);
-    const bool cap = capturing(c);
+    const bool cap = (loc == BB_LOC_HOST || c->profile) && capturing(c);
     need(!(cap && loc == BB_LOC_HOST), BB_ERR_ARG, "a call on host memory cannot be captured");
     const size_t nt = span_bytes(B, sq->table_stride, sq->max_pages, 4);
     with_io(c, loc,
@@ -2976,11 +2997,16 @@ int bb_paged_attention(bb_ctx* c, const bb_paged_kv* kv, const bb_paged_seqs* sq
     const size_t nl = pq->lse ? B * nh * 4 : 0;
     need(!overlap(pq->lse, nl, pq->out, no) && !overlap(pq->lse, nl, pq->q, nq), BB_ERR_ARG, "lse overlaps the query or out");
     set_device(c);
-    const bool cap = capturing(c);
+    const bool cap = (loc == BB_LOC_HOST || c->profile || !pq->workspace) && capturing(c);
+    need_off_pool(kv, loc, {{pq->out, no}, {pq->lse, nl}});
     need(!(cap && loc == BB_LOC_HOST), BB_ERR_ARG, "a call on host memory cannot be captured");
     if (pq->workspace) {
       need_aligned(pq->workspace, "workspace");
       need(pq->workspace_bytes >= want, BB_ERR_RANGE, "workspace smaller than bb_paged_attention_workspace's answer");
+      need(!overlap(pq->workspace, want, kv->view.k, kv->span) && !overlap(pq->workspace, want, kv->view.v, kv->span) &&
+               (loc == BB_LOC_HOST || (!overlap(pq->workspace, want, pq->q, nq) && !overlap(pq->workspace, want, pq->out, no) &&
+                                       !overlap(pq->workspace, want, pq->lse, nl))),
+           BB_ERR_ARG, "the workspace overlaps another array");
     } else {
       need(!cap, BB_ERR_ARG, "a captured call needs a workspace of its own");
     }

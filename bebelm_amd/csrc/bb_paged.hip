@@ -446,7 +446,7 @@ __device__ __forceinline__ int uniform_div(int a, int b) {
   return __builtin_amdgcn_readfirstlane(q);
 }
 
-// Waves of a SIMD at a time for head sizes up to hdp: 128, 256, 512 registers each.
+// Waves of a SIMD that fit: 128, 256, 512 registers each.
 constexpr int pa_waves(int hdp) { return hdp == 64 ? 4 : hdp == 128 ? 2 : 1; }
 
 // A tile's shape: CT the cache's type, HDP the head size (or the next of 64, 128, 256).
@@ -1017,7 +1017,13 @@ __global__ void __launch_bounds__(PJ_THREADS) k_paged_join(PagedQuery pq, int hd
 int pa_class(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 
 // Blocks that fit the device at once.
-int pa_blocks(int n_cu, int hd) { return n_cu * pa_waves(pa_class(hd)); }
+// Blocks of a launch: as many as fit the device where many pairs are begun and ended, or pages are found by lanes (more
+// waves hide more of that), else one a CU, whose loads fill the memory's queues as well and disturb
+// each other less. WAVES_FIGURES
+constexpr int PA_MANY_PAIRS = 3;  // a CU
+int pa_blocks(int n_cu, int hd, size_t pairs, bool uni) {
+  return n_cu * (uni && pairs < (size_t)PA_MANY_PAIRS * n_cu ? 1 : pa_waves(pa_class(hd)));
+}
 
 PagedPlan pa_plan(int n_seqs, int n_heads, int n_kv) {
   PagedPlan p{};
@@ -1044,7 +1050,7 @@ void paged_divisor(PagedView& v) {
 
 size_t paged_attn_ws(int n_cu, int n_seqs, int n_heads, int n_kv, int hd) {
   const PagedPlan p = pa_plan(n_seqs, n_heads, n_kv);
-  const size_t slots = 2 * (size_t)pa_blocks(n_cu, hd) * p.hg;
+  const size_t slots = 2 * (size_t)n_cu * pa_waves(pa_class(hd)) * p.hg;
   return slots * ((size_t)hd * 4 + sizeof(float2)) + ((size_t)n_seqs + 2) * 4;
 }
 
@@ -1055,7 +1061,9 @@ hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQue
   // positions of a sequence that count, at most (a window begins anywhere in 32)
   size_t cap = (size_t)sq.max_pages * kv.page_size;
   if (q.window > 0) cap = std::min(cap, (size_t)q.window + 31);
-  const int blocks_max = pa_blocks(n_cu, kv.hd);
+  const bool uni = kv.page_size % 16 == 0 && 16 * kv.pos_stride < ((size_t)1 << 29);
+  const size_t pairs = (size_t)sq.n_seqs * pl.n_groups;
+  const int blocks_max = pa_blocks(n_cu, kv.hd, pairs, uni);
   const size_t slots = 2 * (size_t)blocks_max * pl.hg;
   pl.sums = static_cast<float*>(q.ws);
   pl.ml = reinterpret_cast<float2*>(pl.sums + slots * kv.hd);
@@ -1063,10 +1071,9 @@ hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQue
   // (pairs of one unit take a block each at most, longer ones a block for each unit)
   const int unit_short = pa_unit_short(kv.hd * (cache == BB_F32 ? 4 : 2));
   pl.unit = cap <= (size_t)1 << unit_short ? unit_short : PA_UNIT;
-  const size_t units = ((cap - 1) >> pl.unit) + 1, pairs = (size_t)sq.n_seqs * pl.n_groups;
+  const size_t units = ((cap - 1) >> pl.unit) + 1;
   const unsigned blocks = (unsigned)std::min<size_t>(blocks_max, pairs * (units == 1 ? 1 : units + PA_PAIR));
   pl.join = units > 1;
-  const bool uni = kv.page_size % 16 == 0 && 16 * kv.pos_stride < ((size_t)1 << 29);
   const int cls = pa_class(kv.hd);
   const size_t lds = (size_t)PA_WAVES * pl.hg * (cls + 4) * 4;
 #define BB_PA(ct, np, hdp)                                                                                     \

@@ -525,6 +525,58 @@ def test_attention_wide_queries(gpu_ctx):
         check_attention(pool, q, out, lse, 0.125 * 2.0 ** -e, 0, F32, f"2^{e}")
 
 
+def test_attention_subnormal_keys_and_values(gpu_ctx):
+    """f16 values below 2^-14 count as what they are, bf16 ones over their whole range too."""
+    for ct, e in ((F16, -18), (BF16, -120), (F32, -120)):
+        pool = Pool(gpu_ctx, 126, [40, 300], ct, 16, 2, 64)
+        for x in (pool.k, pool.v):
+            x.copy_((torch.randn(x.shape, generator=gen(127)) * 2.0 ** e).to(TYPES[ct]))
+        q = randn(128, (2, 4, 64), F32) * 2.0 ** 10
+        scale = 2.0 ** (-10 - e - 3)
+        out, lse = attend(gpu_ctx, pool, q, scale=scale)
+        check_attention(pool, q, out, lse, scale, 0, F32, f"2^{e}")
+
+
+def test_attention_rows_at_odd_strides(gpu_ctx):
+    """Rows of q and out that start at any element."""
+    for dt in (F32, F16, BF16):
+        for ct, hd in ((F32, 64), (BF16, 64), (F16, 128), (BF16, 24)):
+            pool = Pool(gpu_ctx, 129, [40, 300, 5], ct, 16, 2, hd)
+            row = 4 * hd + 3
+            base = torch.randn(3 * row + 7, generator=gen(130)).to(TYPES[dt])
+            view = lambda a: a.as_strided((3, 4, hd), (row, hd, 1))
+            dev, out = base.cuda(), torch.full((3 * row + 7,), 7.0, dtype=TYPES[dt], device="cuda")
+            torch.cuda.synchronize()
+            kernels.paged_attention(gpu_ctx, pool.kv, pool.table.cuda(), pool.lens.cuda(), view(dev), view(out))
+            done(gpu_ctx)
+            check_attention(pool, view(base), view(out), None, 1 / math.sqrt(hd), 0, dt, f"{dt} {ct}")
+            view(out).fill_(7.0)
+            assert bool((out == 7.0).all())
+
+
+def test_one_pool_of_keys_and_values(gpu_ctx):
+    """Keys and values side by side in each page, and in each position."""
+    for shape, pick in (((9, 2, 16, 2, 64), lambda a, i: a[:, i]), ((9, 16, 2, 2, 64), lambda a, i: a[:, :, i]),
+                        ((9, 16, 2, 2, 64), lambda a, i: a[:, :, :, i])):
+        both = torch.zeros(shape, dtype=torch.bfloat16, device="cuda")
+        pool = PagedKv(gpu_ctx, pick(both, 0), pick(both, 1))
+        k, v, q = randn(153, (70, 2, 64), BF16), randn(154, (70, 2, 64), BF16), randn(155, (2, 4, 64), BF16)
+        table = torch.tensor([[8, 0, 3, 5], [1, 2, 7, 4]], dtype=torch.int32)
+        start = torch.tensor([0, 50, 70], dtype=torch.int32)
+        lens = torch.tensor([50, 20], dtype=torch.int32)
+        out = torch.empty(2, 4, 64, dtype=torch.bfloat16, device="cuda")
+        args = [x.cuda() for x in (table, lens, k, v, start, q)]
+        torch.cuda.synchronize()
+        kernels.paged_append(gpu_ctx, pool, args[0], args[1], args[2], args[3], seq_start=args[4])
+        kernels.paged_attention(gpu_ctx, pool, args[0], args[1], args[5], out)
+        done(gpu_ctx)
+        for s in range(2):
+            rows = slice(int(start[s]), int(start[s + 1]))
+            want, _, tol, _ = attention64(q[s], (k[rows], v[rows]), 0.125)
+            close(out[s], want, tol * (1 + half_step(BF16)) + half_step(BF16) * want.abs() + TINY[BF16], f"out {s}")
+        pool.close()
+
+
 def test_attention_ragged_batches(gpu_ctx):
     """Many sequences of all lengths: splits of every kind."""
     for seed, (n, longest, kv, g, hd, dt) in enumerate([(300, 60, 2, 4, 64, BF16), (70, 5000, 1, 2, 64, F16),
@@ -794,6 +846,8 @@ def test_refusals(gpu_ctx):
     k = torch.zeros(4, 16, 2, 64, device="cuda")
     v = torch.zeros_like(k)
     refused(ARG, lambda: PagedKv(c, k, k))
+    flat = torch.zeros(4 * 16 * 2 * 64 + 64, device="cuda")
+    refused(ARG, lambda: PagedKv(c, flat[:-64].view(4, 16, 2, 64), flat[64:].view(4, 16, 2, 64)))
     refused(SHAPE, lambda: PagedKv(c, k[..., :20], v[..., :20]))
     refused(SHAPE, lambda: PagedKv.create(c, F32, 4, 16, 2, 264))
     refused(ARG, lambda: PagedKv(c, k[:1].expand(4, 16, 2, 64), v[:1].expand(4, 16, 2, 64)))
@@ -823,6 +877,10 @@ def test_refusals(gpu_ctx):
     refused(ARG, lambda: kernels.paged_append(c, kv, table, lens, kk, kk, q=q[:, :2], q_out=kk))   # onto the keys
     many = torch.zeros(4, 4, 64, device="cuda")
     refused(ARG, lambda: kernels.paged_append(c, kv, table, lens, kk, kk, q=many[:3], q_out=many[1:]))
+    inside = k[0, :3]                                                              # rows of the pool itself
+    refused(ARG, lambda: kernels.paged_append(c, kv, table, lens, inside, kk))
+    refused(ARG, lambda: kernels.paged_append(c, kv, table, lens, kk, v[1, 2:5]))
+    refused(ARG, lambda: kernels.paged_append(c, kv, table, lens, kk, kk, q=inside))
     for bad in (lambda: kernels.paged_append(c, kv, table, lens, kk.half(), kk),
                 lambda: kernels.paged_append(c, kv, table, lens[:2], kk, kk),
                 lambda: kernels.paged_append(c, kv, table.long(), lens, kk, kk),
@@ -841,6 +899,10 @@ def test_refusals(gpu_ctx):
     need = kv.attention_workspace(4, 3)
     if need > 16:
         refused(RANGE, lambda: att(c, kv, table, lens, q, out, workspace=torch.zeros(need - 16, dtype=torch.uint8, device="cuda")))
+    refused(ARG, lambda: att(c, kv, table, lens, kk, inside))
+    ws = torch.zeros(need + 1024, dtype=torch.uint8, device="cuda")
+    refused(ARG, lambda: att(c, kv, table, lens, q, out, lse=ws[:48].view(torch.float32).view(3, 4), workspace=ws))
+    refused(ARG, lambda: att(c, kv, table, lens, q, out, workspace=ws[8:]))
     for bad in (lambda: att(c, kv, table, lens, q, out.half()), lambda: att(c, kv, table, lens, q, out[:2]),
                 lambda: att(c, kv, table, lens, q, out, lse=out), lambda: att(c, kv, table, lens, q, out, scale=0.0),
                 lambda: att(c, kv, table, lens, q, out, workspace=torch.zeros(1 << 20))):
