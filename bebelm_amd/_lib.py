@@ -6,6 +6,7 @@ missing library raises instead of falling back to anything else.
 import ctypes
 import os
 import re
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libbebelm_moe.so")
@@ -55,22 +56,14 @@ class RopeDesc(ctypes.Structure):
                 ("low_rotations", ctypes.c_double), ("high_rotations", ctypes.c_double), ("magnitude", c_float)]
 
 
-class PagedSeqs(ctypes.Structure):
-    _fields_ = [("n_seqs", c_size_t), ("max_pages", c_size_t), ("table_stride", c_size_t), ("page_table", c_void_p),
-                ("lens", c_void_p)]
-
-
-class PagedTokens(ctypes.Structure):
-    _fields_ = [("n_tokens", c_size_t), ("dtype", c_uint32), ("k", c_void_p), ("v", c_void_p), ("k_stride", c_size_t),
-                ("v_stride", c_size_t), ("q", c_void_p), ("q_out", c_void_p), ("n_heads", c_size_t),
-                ("q_stride", c_size_t), ("q_out_stride", c_size_t), ("q_norm", c_void_p), ("k_norm", c_void_p),
-                ("eps", c_float), ("pos", c_void_p), ("seq_start", c_void_p)]
-
-
-class PagedQuery(ctypes.Structure):
-    _fields_ = [("dtype", c_uint32), ("q", c_void_p), ("out", c_void_p), ("n_heads", c_size_t),
-                ("q_stride", c_size_t), ("out_stride", c_size_t), ("scale", c_float), ("window", c_size_t),
-                ("lse", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+# bb_paged_seqs, bb_paged_tokens and bb_paged_query, packed in one call each (a decode step fills them for every
+# layer): n_seqs, max_pages, table_stride, page_table, lens
+PAGED_SEQS = struct.Struct("@NNNPP")
+# n_tokens, dtype, k, v, k_stride, v_stride, q, q_out, n_heads, q_stride, q_out_stride, q_norm, k_norm, eps, pos,
+# seq_start
+PAGED_TOKENS = struct.Struct("@NIPPNNPPNNNPPfPP")
+# dtype, q, out, n_heads, q_stride, out_stride, scale, window, lse, workspace, workspace_bytes
+PAGED_QUERY = struct.Struct("@IPPNNNfNPPN")
 
 
 class GgufTensorInfo(ctypes.Structure):
@@ -157,9 +150,9 @@ _SIGS = {
                                  c_size_t, c_size_t, c_size_t, P(c_void_p)]),
     "bb_paged_kv_destroy": (c_int, [c_void_p]),
     "bb_paged_kv_pages": (c_int, [c_void_p, P(c_void_p), P(c_void_p)]),
-    "bb_paged_append": (c_int, [c_void_p, c_void_p, c_void_p, P(PagedSeqs), P(PagedTokens), c_int]),
+    "bb_paged_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int]),
     "bb_paged_attention_workspace": (c_int, [c_void_p, c_void_p, c_size_t, c_size_t, P(c_size_t)]),
-    "bb_paged_attention": (c_int, [c_void_p, c_void_p, P(PagedSeqs), P(PagedQuery), c_int]),
+    "bb_paged_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int]),
     "bb_gguf_open": (c_int, [ctypes.c_char_p, P(c_void_p)]),
     "bb_gguf_open_bytes": (c_int, [c_void_p, c_size_t, P(c_void_p)]),
     "bb_gguf_close": (c_int, [c_void_p]),

@@ -25,7 +25,7 @@ import numpy as np
 
 from . import _lib
 from ._lib import check, lib
-from .model import F32, INT32, _dtype, _ptr, _same_loc
+from .model import F32, INT32, _codes, _dtype, _ptr, _same_loc
 
 
 @dataclass
@@ -163,60 +163,80 @@ def _place(ctx, *arrays):
     """Where the arrays are: all in host memory, or all on the context's GPU."""
     where = None
     for a in arrays:
-        if a is None:
-            continue
-        d = -1 if isinstance(a, np.ndarray) else a.get_device()
-        if where is None:
-            where = d
-        elif d != where:
-            raise ValueError("all arrays of one call must be host or all device")
-    if where >= 0 and where != ctx.device:
+        if a is not None:
+            d = -1 if isinstance(a, np.ndarray) else a.get_device()
+            if d != where:
+                if where is not None:
+                    raise ValueError("all arrays of one call must be host or all device")
+                where = d
+    if where < 0:
+        return _lib.LOC_HOST
+    if where != ctx.device:
         raise ValueError(f"tensors on GPU {where}, context on GPU {ctx.device}")
-    return _lib.LOC_HOST if where < 0 else _lib.LOC_DEVICE
+    return _lib.LOC_DEVICE
 
 
 def _data(a):
     return a.ctypes.data if isinstance(a, np.ndarray) else a.data_ptr()
 
 
-def _heads(a, what, n, heads, hd, packed=True):
-    """Strides (token, head) in elements of [n, heads, head_dim], checked."""
+def _whole(a):
+    return a.flags["C_CONTIGUOUS"] if isinstance(a, np.ndarray) else a.is_contiguous()
+
+
+def _strides(a):
+    """In elements."""
+    return [i // a.itemsize for i in a.strides] if isinstance(a, np.ndarray) else a.stride()
+
+
+def _heads(a, what, code, n, heads, hd, packed=True):
+    """(address, token stride, head stride) of a [n, heads, head_dim] of the given type, checked."""
     if a.shape != (n, heads, hd):
         raise ValueError(f"{what} must be {[n, heads, hd]}, is {list(a.shape)}")
-    if a.flags["C_CONTIGUOUS"] if isinstance(a, np.ndarray) else a.is_contiguous():
-        return heads * hd, hd
-    st = [i // a.itemsize for i in a.strides] if isinstance(a, np.ndarray) else a.stride()
+    if _codes.get(a.dtype) != code and _dtype(a) != code:
+        raise ValueError(f"{what}: {a.dtype} is not the type of the other arrays")
+    if _whole(a):
+        return _data(a), heads * hd, hd
+    st = _strides(a)
     if hd > 1 and st[2] != 1:
         raise ValueError(f"{what}: the elements of a head must be adjacent")
     if packed and heads > 1 and st[1] != hd:
         raise ValueError(f"{what}: the heads of a token must be adjacent")
     if min(st) < 0:
         raise ValueError(f"{what}: negative strides")
-    return (st[0] if n > 1 else heads * hd), (st[1] if heads > 1 else hd)
+    return _data(a), (st[0] if n > 1 else heads * hd), (st[1] if heads > 1 else hd)
 
 
-def _whole(a, what, code, *shape):
-    """Address of a contiguous array of the given type and shape (None: none)."""
+def _flat(a, what, code, *shape):
+    """Address of a contiguous array of the given type and shape (None: 0)."""
     if a is None:
-        return None
-    if _dtype(a) != code or a.shape != shape:
+        return 0
+    if a.shape != shape or _dtype(a) != code:
         raise ValueError(f"{what} must be {'int32' if code == INT32 else 'float32'} {list(shape)}, is {a.dtype} {list(a.shape)}")
-    if not (a.flags["C_CONTIGUOUS"] if isinstance(a, np.ndarray) else a.is_contiguous()):
+    if not _whole(a):
         raise ValueError(f"{what} must be contiguous")
     return _data(a)
 
 
+def _floating(a, what):
+    code = _dtype(a)
+    if code == INT32:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16")
+    return code
+
+
 def _seqs(page_table, lens):
+    """(sequences, bb_paged_seqs)"""
     if len(page_table.shape) != 2 or _dtype(page_table) != INT32:
         raise ValueError("page_table must be int32 [sequences, pages]")
     n, pages = page_table.shape
     row = pages
-    if not (page_table.flags["C_CONTIGUOUS"] if isinstance(page_table, np.ndarray) else page_table.is_contiguous()):
-        st = [i // 4 for i in page_table.strides] if isinstance(page_table, np.ndarray) else page_table.stride()
+    if not _whole(page_table):
+        st = _strides(page_table)
         if (pages > 1 and st[1] != 1) or st[0] < 0:
             raise ValueError("page_table: the entries of a sequence must be adjacent")
         row = st[0] if n > 1 else pages
-    return n, _lib.PagedSeqs(n, pages, row, _data(page_table), _whole(lens, "lens", INT32, n))
+    return n, _lib.PAGED_SEQS.pack(n, pages, row, _data(page_table), _flat(lens, "lens", INT32, n))
 
 
 def rope(ctx, plan, x, pos, out=None):
@@ -224,13 +244,11 @@ def rope(ctx, plan, x, pos, out=None):
     RopePlan says, into out (x itself by default)."""
     out = x if out is None else out
     t, h, hd = x.shape
-    xs = _heads(x, "x", t, h, hd, False)
-    os = xs if out is x else _heads(out, "out", t, h, hd, False)
-    code = _dtype(x)
-    if code == INT32 or _dtype(out) != code:
-        raise ValueError("x and out must be of one floating-point type")
-    check(lib().bb_rope(ctx.handle, plan.handle, code, _data(x), xs[0], xs[1], t, h, hd, _whole(pos, "pos", INT32, t),
-                        _data(out), os[0], os[1], _place(ctx, x, pos, out)))
+    code = _floating(x, "x")
+    xa, xt, xh = _heads(x, "x", code, t, h, hd, False)
+    oa, ot, oh = _heads(out, "out", code, t, h, hd, False)
+    check(lib().bb_rope(ctx.handle, plan.handle, code, xa, xt, xh, t, h, hd, _flat(pos, "pos", INT32, t), oa, ot, oh,
+                        _place(ctx, x, pos, out)))
     return out
 
 
@@ -242,35 +260,27 @@ def paged_append(ctx, kv, page_table, lens, k, v, rope=None, pos=None, seq_start
     index in its sequence. page_table int32 [sequences, pages] and lens int32 [sequences] count the
     call's tokens; seq_start int32 [sequences + 1] says which tokens each sequence brings (None: one
     each). Returns q_out."""
-    t, hd, nkv, code = len(k), kv.head_dim, kv.n_kv_heads, _dtype(k)
+    t, hd, nkv, code = k.shape[0], kv.head_dim, kv.n_kv_heads, _floating(k, "k")
     n, seqs = _seqs(page_table, lens)
-    ks, vs = _heads(k, "k", t, nkv, hd), _heads(v, "v", t, nkv, hd)
-    if rope is not None and not rope.handle:
-        raise ValueError("the RopePlan is closed")
-    tok = _lib.PagedTokens(t, code, _data(k), _data(v), ks[0], vs[0])
-    ok = code != INT32 and _dtype(v) == code
+    ka, ks, _ = _heads(k, "k", code, t, nkv, hd)
+    va, vs, _ = _heads(v, "v", code, t, nkv, hd)
+    qa = qs = oa = os = heads = 0
     if q is not None:
         q_out = q if q_out is None else q_out
         heads = q.shape[1]
-        ok = ok and _dtype(q) == code and _dtype(q_out) == code
-        tok.q, tok.q_out, tok.n_heads = _data(q), _data(q_out), heads
-        tok.q_stride = _heads(q, "q", t, heads, hd)[0]
-        tok.q_out_stride = _heads(q_out, "q_out", t, heads, hd)[0]
+        qa, qs, _ = _heads(q, "q", code, t, heads, hd)
+        oa, os, _ = _heads(q_out, "q_out", code, t, heads, hd)
     elif q_out is not None:
         raise ValueError("q_out without q")
-    if not ok:
-        raise ValueError("k, v, q and q_out must be of one floating-point type")
-    tok.eps = eps
-    if q_norm is not None:
-        tok.q_norm = _whole(q_norm, "q_norm", F32, hd)
-    if k_norm is not None:
-        tok.k_norm = _whole(k_norm, "k_norm", F32, hd)
-    if pos is not None:
-        tok.pos = _whole(pos, "pos", INT32, t)
-    if seq_start is not None:
-        tok.seq_start = _whole(seq_start, "seq_start", INT32, n + 1)
-    check(lib().bb_paged_append(ctx.handle, kv.handle, rope.handle if rope is not None else None, ctypes.byref(seqs),
-                                ctypes.byref(tok),
+    plan = None
+    if rope is not None:
+        plan = rope.handle
+        if not plan:
+            raise ValueError("the RopePlan is closed")
+    tokens = _lib.PAGED_TOKENS.pack(t, code, ka, va, ks, vs, qa, oa, heads, qs, os, _flat(q_norm, "q_norm", F32, hd),
+                                    _flat(k_norm, "k_norm", F32, hd), eps, _flat(pos, "pos", INT32, t),
+                                    _flat(seq_start, "seq_start", INT32, n + 1))
+    check(lib().bb_paged_append(ctx.handle, kv.handle, plan, seqs, tokens,
                                 _place(ctx, k, v, page_table, lens, pos, seq_start, q, q_out, q_norm, k_norm)))
     return q_out
 
@@ -282,27 +292,23 @@ def paged_attention(ctx, kv, page_table, lens, q, out, scale=None, window=0, lse
     kv.attention_workspace(n_heads, sequences) bytes for this call alone (None: the context's; a call
     captured into a graph needs one)."""
     n, seqs = _seqs(page_table, lens)
-    heads, hd, code = q.shape[1], kv.head_dim, _dtype(q)
-    pq = _lib.PagedQuery(code, _data(q), _data(out), heads, _heads(q, "q", n, heads, hd)[0],
-                         _heads(out, "out", n, heads, hd)[0])
-    if code == INT32 or _dtype(out) != code:
-        raise ValueError("q and out must be of one floating-point type")
-    if scale is not None:
-        if scale == 0:
-            raise ValueError("scale must not be 0")
-        pq.scale = scale
-    if window:
-        if window < 0:
-            raise ValueError("window must not be negative")
-        pq.window = window
-    if lse is not None:
-        pq.lse = _whole(lse, "lse", F32, n, heads)
+    heads, hd, code = q.shape[1], kv.head_dim, _floating(q, "q")
+    qa, qs, _ = _heads(q, "q", code, n, heads, hd)
+    oa, os, _ = _heads(out, "out", code, n, heads, hd)
+    if scale is None:
+        scale = 0.0
+    elif scale == 0:
+        raise ValueError("scale must not be 0")
+    if window < 0:
+        raise ValueError("window must not be negative")
+    ws = ws_bytes = 0
     if workspace is not None:
         if isinstance(workspace, np.ndarray) or workspace.get_device() != ctx.device or not workspace.is_contiguous():
             raise ValueError("the workspace must be a contiguous tensor on the context's GPU")
-        pq.workspace, pq.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    check(lib().bb_paged_attention(ctx.handle, kv.handle, ctypes.byref(seqs), ctypes.byref(pq),
-                                   _place(ctx, q, out, page_table, lens, lse)))
+        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    query = _lib.PAGED_QUERY.pack(code, qa, oa, heads, qs, os, scale, window, _flat(lse, "lse", F32, n, heads), ws,
+                                  ws_bytes)
+    check(lib().bb_paged_attention(ctx.handle, kv.handle, seqs, query, _place(ctx, q, out, page_table, lens, lse)))
     return out
 
 
