@@ -2651,7 +2651,7 @@ bb_paged_kv* new_pool(bb_ctx* c, uint32_t dtype, void* k, void* v, size_t n_page
   p->device = c->device;
   p->dtype = dtype;
   p->view = {k, v, page_stride, pos_stride, head_stride, (int)n_pages, (int)page_size, (int)n_kv, (int)hd};
-  bb::paged_divisor(p->view);
+  p->view.set_slots((int)page_size);
   p->span = ((n_pages - 1) * page_stride + (page_size - 1) * pos_stride + (n_kv - 1) * head_stride + hd) *
             (dtype == BB_F32 ? 4 : 2);
   p->own = own;

@@ -370,10 +370,12 @@ struct PagedView {
   void *k, *v;
   size_t page_stride, pos_stride, head_stride;
   int n_pages, page_size, n_kv, hd;
-  uint32_t page_mul = 0;  // division by page_size (paged_divisor)
+  // pages counted as page_slots positions: page_size, or more where attention leaves places of a page empty
+  int page_slots = 0;
+  uint32_t page_mul = 0;  // division by page_slots
   int page_shift = 0;
+  void set_slots(int n);
 };
-void paged_divisor(PagedView& v);
 // The sequences of a batch (lens null: none, rows are only turned).
 struct PagedSeqs {
   const int32_t *table, *lens;

@@ -58,8 +58,8 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
   }
 }
 
-// i / page_size for 0 <= i < 2^31 (PagedView::page_mul = ceil(2^(31 + page_shift) / page_size), page_shift
-// = ceil(log2(page_size)): the product is off by less than i / 2^(31 + page_shift) < 1 / page_size).
+// i / page_slots for 0 <= i < 2^31 (PagedView::page_mul = ceil(2^(31 + page_shift) / page_slots), page_shift
+// = ceil(log2(page_slots)): the product is off by less than i / 2^(31 + page_shift) < 1 / page_slots).
 __device__ __forceinline__ int page_of(const PagedView& kv, int i) {
   return (int)(((uint64_t)(uint32_t)i * kv.page_mul) >> (31 + kv.page_shift));
 }
@@ -345,10 +345,16 @@ struct PagedPlan {
 struct SeqSpan {
   int base, first, len, units;  // positions first..len-1, counted from base; units >= 1
 };
-__device__ __forceinline__ SeqSpan seq_span(int raw_len, int cap, int window, int unit) {
+// (Positions as slots, see PaWave.)
+__device__ __forceinline__ SeqSpan seq_span(int raw_len, const PagedView& kv, int max_pages, int window, int unit) {
   SeqSpan r;
-  r.len = min(max(raw_len, 0), cap);
+  r.len = min(max(raw_len, 0), max_pages * kv.page_size);
   r.first = window > 0 ? max(0, r.len - window) : 0;
+  const int empty = kv.page_slots - kv.page_size;
+  if (empty > 0) {
+    r.first += (int)((uint32_t)r.first / (uint32_t)kv.page_size) * empty;
+    r.len += r.len > 0 ? (int)((uint32_t)(r.len - 1) / (uint32_t)kv.page_size) * empty : 0;
+  }
   r.base = r.first & ~31;
   r.units = max(1, (r.len - r.base + (1 << unit) - 1) >> unit);
   return r;
@@ -473,9 +479,9 @@ __device__ __forceinline__ void load_row(const void* p, size_t i, float (&x)[N])
 
 // One wave's part of a (sequence, head group) pair: running maximum m (base 2), sum l and o[i][r] for element
 // (16p + 4g + r)·PE + e, i = p·PE + e, of head n.
-// UNI: pages of whole 16 positions, whose rows are within 2^31 bytes of the first: 16 positions have one
-// address the same for the wave. Otherwise every lane finds the page of one position and the lanes
-// exchange them (16-bit cache, 8 kv heads of 64, 64 sequences of 4096: UNI_FIGURES).
+// UNI: a page counts as whole 16 positions (slots; the last few may be empty), whose rows are within 2^31 bytes of
+// the first, so that 16 slots have one address the same for the wave. Otherwise (pages below 8, rows
+// far apart) every lane finds the page of one position and the lanes exchange them. UNI_FIGURES
 // What is not there or not attended to is loaded as 0 (a weight of 0 times what lies there need not be 0).
 template <int CT, int NP, int HDP, bool UNI>
 struct PaWave {
@@ -555,29 +561,30 @@ struct PaWave {
   }
 
   // Where a tile's positions are in the pool (elements; -1: not there, or not attended to): UNI, each 16, the same for
-  // the wave; otherwise lane l's is position l % KT's.
+  // the wave, and how many of them from there on the page has; otherwise lane l's is position l % KT's.
   struct Places {
     int key0;
     int64_t at[UNI ? NT : 1];
+    int rows[UNI ? NT : 1];
   };
-  __device__ __forceinline__ int64_t place(int key, int end) const {
-    const int i = min(key, sp.len - 1), entry = page_of(kv, i);
+  __device__ __forceinline__ void place(Places& p, int t, int key, int end) const {
+    const int i = min(key, sp.len - 1), entry = page_of(kv, i), in = i - entry * kv.page_slots;
     int pg = row[entry];
     if constexpr (UNI) pg = __builtin_amdgcn_readfirstlane(pg);
     const bool there = key < end && (uint32_t)pg < (uint32_t)kv.n_pages;
-    const int64_t at = (int64_t)((size_t)(uint32_t)pg * kv.page_stride +
-                                 (size_t)(uint32_t)(i - entry * kv.page_size) * kv.pos_stride + kv_off);
-    return there ? at : -1;
+    const int64_t at = (int64_t)((size_t)(uint32_t)pg * kv.page_stride + (size_t)(uint32_t)in * kv.pos_stride + kv_off);
+    p.at[t] = there ? at : -1;
+    p.rows[t] = min(16, kv.page_size - in);
   }
   __device__ __forceinline__ Places places(int key0, int end) const {
     Places p;
     p.key0 = key0;
     if constexpr (UNI) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) p.at[t] = place(key0 + 16 * t, end);
+      for (int t = 0; t < NT; ++t) place(p, t, key0 + 16 * t, end);
     } else {
       const int key = key0 + ((n + 16 * g) & (S::KT - 1));
-      p.at[0] = place(key, key >= sp.first ? end : 0);
+      place(p, 0, key, key >= sp.first ? end : 0);
     }
     return p;
   }
@@ -595,7 +602,7 @@ struct PaWave {
     if constexpr (UNI) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const auto rows = rows_of(kv.k, p.at[t], 16);
+        const auto rows = rows_of(kv.k, p.at[t], p.rows[t]);
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
           // (pieces past the head: 0, which 0 times what lies there need not be)
@@ -624,14 +631,14 @@ struct PaWave {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const int k0 = p.key0 + 16 * t, skip = max(0, sp.first - k0);
-        const auto rows = rows_of(kv.v, p.at[t], min(16, sp.len - k0));
+        const int n_rows = min(p.rows[t], sp.len - k0);
+        const auto rows = rows_of(kv.v, p.at[t], n_rows);
         if (p.at[t] >= 0) {
-          if (skip == 0 && k0 + 16 <= sp.len) {
+          if (skip == 0 && n_rows == 16) {
             valid |= 15u << 4 * t;
           } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              valid |= (4 * g + r >= skip && 4 * g + r < sp.len - k0 ? 1u : 0u) << (4 * t + r);
+            for (int r = 0; r < 4; ++r) valid |= (4 * g + r >= skip && 4 * g + r < n_rows ? 1u : 0u) << (4 * t + r);
           }
         }
 #pragma unroll
@@ -800,7 +807,8 @@ struct SeqScan {
   int c0;
   int len[4], cost[4], incl[4];
   int all;         // of the 256
-  __device__ __forceinline__ void load(const int* __restrict__ lens, int n_seqs, int cap, int window, int unit, int lane) {
+  __device__ __forceinline__ void load(const int* __restrict__ lens, int n_seqs, const PagedView& kv, int max_pages,
+                                       int window, int unit, int lane) {
     all = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) len[i] = c0 + 64 * i < n_seqs ? lens[min(c0 + 64 * i + lane, n_seqs - 1)] : 0;
@@ -808,7 +816,7 @@ struct SeqScan {
     for (int i = 0; i < 4; ++i) {
       cost[i] = incl[i] = 0;
       if (c0 + 64 * i < n_seqs) {
-        cost[i] = c0 + 64 * i + lane < n_seqs ? seq_span(len[i], cap, window, unit).units + PA_PAIR : 0;
+        cost[i] = c0 + 64 * i + lane < n_seqs ? seq_span(len[i], kv, max_pages, window, unit).units + PA_PAIR : 0;
         incl[i] = all + wave_scan(cost[i]);
         all = __builtin_amdgcn_readlane(incl[i], 63);
       }
@@ -826,7 +834,6 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
   extern __shared__ __align__(16) float so[];  // [waves][hg][LD]
   __shared__ float s_m[PA_WAVES][PA_HEADS], s_l[PA_WAVES][PA_HEADS];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int cap = max_pages * kv.page_size;
 
   // every wave finds the block's run by itself: the total cost, then the sequence in whose cost the run begins
   // (more than 256 sequences are gone through twice)
@@ -836,7 +843,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
     sc.c0 = 0;
     int before = 0;
     for (;;) {
-      sc.load(lens, n_seqs, cap, pq.window, pl.unit, lane);
+      sc.load(lens, n_seqs, kv, max_pages, pq.window, pl.unit, lane);
       if (end == 0) {
         if (pl.join && blockIdx.x == 0 && wv == 0) {
 #pragma unroll
@@ -894,7 +901,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
       grp = 0;
       ++s;
       len = __builtin_amdgcn_readfirstlane(lens[s]);
-      cost = seq_span(len, cap, pq.window, pl.unit).units + PA_PAIR;
+      cost = seq_span(len, kv, max_pages, pq.window, pl.unit).units + PA_PAIR;
     }
     const int nu = cost - PA_PAIR, first_unit = lo + PA_PAIR;
     const int u0 = max(u - first_unit, 0), take = min(nu, end - first_unit) - u0;
@@ -904,7 +911,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
     w.head0 = kvh * pl.G + sub * pl.hg;
     w.heads = min(pl.hg, pl.G - sub * pl.hg);
     w.kv_off = (size_t)kvh * kv.head_stride;
-    w.sp = seq_span(len, cap, pq.window, pl.unit);
+    w.sp = seq_span(len, kv, max_pages, pq.window, pl.unit);
     w.start(pq, s);
     const int k0 = w.sp.base + (u0 << pl.unit);
     w.run(k0 + wv * S::KT, min(k0 + (take << pl.unit), w.sp.len), PA_WAVES * S::KT);
@@ -1038,14 +1045,14 @@ PagedPlan pa_plan(int n_seqs, int n_heads, int n_kv) {
 
 bool paged_attn_fits(int n_seqs, int n_heads, int n_kv, size_t cap) {
   const PagedPlan p = pa_plan(n_seqs, n_heads, n_kv);
-  return (size_t)n_seqs * (size_t)p.n_groups * ((cap >> PA_UNIT) + 1 + PA_PAIR) < ((size_t)1 << 29);
+  return (size_t)n_seqs * (size_t)p.n_groups * ((2 * cap >> PA_UNIT) + 1 + PA_PAIR) < ((size_t)1 << 29);  // (up to 2 slots a position)
 }
 
-void paged_divisor(PagedView& v) {
-  v.page_shift = 0;
-  while ((1 << v.page_shift) < v.page_size) ++v.page_shift;
-  const uint64_t two = (uint64_t)1 << (31 + v.page_shift);
-  v.page_mul = (uint32_t)((two + v.page_size - 1) / v.page_size);
+void PagedView::set_slots(int n) {
+  page_slots = n;
+  page_shift = 0;
+  while ((1 << page_shift) < n) ++page_shift;
+  page_mul = (uint32_t)((((uint64_t)1 << (31 + page_shift)) + n - 1) / n);
 }
 
 size_t paged_attn_ws(int n_cu, int n_seqs, int n_heads, int n_kv, int hd) {
@@ -1054,14 +1061,20 @@ size_t paged_attn_ws(int n_cu, int n_seqs, int n_heads, int n_kv, int hd) {
   return slots * ((size_t)hd * 4 + sizeof(float2)) + ((size_t)n_seqs + 2) * 4;
 }
 
-hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQuery& q, const PagedView& kv,
+hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQuery& q, const PagedView& pool,
                              const PagedSeqs& sq) {
   if (sq.n_seqs == 0) return hipSuccess;
-  PagedPlan pl = pa_plan(sq.n_seqs, q.n_heads, kv.n_kv);
-  // positions of a sequence that count, at most (a window begins anywhere in 32)
-  size_t cap = (size_t)sq.max_pages * kv.page_size;
-  if (q.window > 0) cap = std::min(cap, (size_t)q.window + 31);
-  const bool uni = kv.page_size % 16 == 0 && 16 * kv.pos_stride < ((size_t)1 << 29);
+  PagedPlan pl = pa_plan(sq.n_seqs, q.n_heads, pool.n_kv);
+  PagedView kv = pool;
+  const size_t slots16 = ((size_t)kv.page_size + 15) / 16 * 16;
+  const bool uni = kv.page_size >= 8 && 16 * kv.pos_stride < ((size_t)1 << 29) && sq.max_pages * slots16 < ((size_t)1 << 31);
+  if (uni) kv.set_slots((int)slots16);
+  // slots of a sequence that count, at most (a window begins anywhere in a page, and its slots anywhere in 32)
+  size_t cap = (size_t)sq.max_pages * kv.page_slots;
+  if (q.window > 0) {
+    const size_t pages = ((size_t)q.window + kv.page_size - 1) / kv.page_size + 1;
+    cap = std::min(cap, std::min((size_t)q.window + pages * (kv.page_slots - kv.page_size), pages * kv.page_slots) + 31);
+  }
   const size_t pairs = (size_t)sq.n_seqs * pl.n_groups;
   const int blocks_max = pa_blocks(n_cu, kv.hd, pairs, uni);
   const size_t slots = 2 * (size_t)blocks_max * pl.hg;
