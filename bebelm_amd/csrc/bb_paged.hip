@@ -325,6 +325,10 @@ constexpr int PA_UNIT = 7;        // positions of a unit (their logarithm): a ti
 __host__ __device__ constexpr int pa_unit_short(int row_bytes) { return row_bytes <= 256 ? 9 : 8; }
 constexpr int PA_PAIR = 1;        // what a pair costs besides its units
 constexpr int PA_HEADS = 16;      // heads of a group at most
+// From this average cost of a pair on, one block a CU works (the others end at once): its loads fill the memory's
+// queues as well as four blocks' and disturb each other less. Batches of shorter pairs keep all the
+// blocks that fit, which hide each other's beginnings and ends. FEW_FIGURES
+constexpr int PA_LONG = 16;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr float NEG_INF = -__builtin_inff();
 
@@ -337,6 +341,7 @@ typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 // A kv head's G query heads: `split` groups of `hg` (the last may have fewer).
 struct PagedPlan {
   int G, split, hg, n_groups, join, unit;  // unit: the logarithm of a unit's positions
+  int few;        // blocks that work where pairs are long
   int* chunk;     // [1 + n_seqs + 1]: cost of a block's run, cost of a group in the sequences before each
   float* sums;    // [2·blocks][hg][hd]: of a pair that began in a block before (slot 0), that goes on in the next (1)
   float2* ml;     // [2·blocks][hg]: maximum (base 2), sum of weights
@@ -479,9 +484,11 @@ __device__ __forceinline__ void load_row(const void* p, size_t i, float (&x)[N])
 
 // One wave's part of a (sequence, head group) pair: running maximum m (base 2), sum l and o[i][r] for element
 // (16p + 4g + r)·PE + e, i = p·PE + e, of head n.
-// UNI: a page counts as whole 16 positions (slots; the last few may be empty), whose rows are within 2^31 bytes of
-// the first, so that 16 slots have one address the same for the wave. Otherwise (pages below 8, rows
-// far apart) every lane finds the page of one position and the lanes exchange them. UNI_FIGURES
+// UNI: a page counts as whole 16 positions (slots; up to a third of them empty), whose rows are within 2^31 bytes of
+// the first, so that 16 slots have one address the same for the wave. Otherwise every lane finds the
+// page of one position and the lanes exchange them. Pages of 24, 64 sequences of 8192 (32 of 4000), UNI
+// and not: bf16, 8 kv heads of 64, 211 and 222 us; f16, of 128, 100 and 116 us. Pages of 8, half of
+// the slots empty: 300 and 223 us (bf16, 64).
 // What is not there or not attended to is loaded as 0 (a weight of 0 times what lies there need not be 0).
 template <int CT, int NP, int HDP, bool UNI>
 struct PaWave {
@@ -855,13 +862,14 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
           sc.c0 += 256;
           continue;
         }
-        const int total = (before + sc.all) * pl.n_groups, grid = (int)gridDim.x;
+        const int total = (before + sc.all) * pl.n_groups;
+        const int grid = before + sc.all >= PA_LONG * n_seqs ? min((int)gridDim.x, pl.few) : (int)gridDim.x;
         const int chunk = total <= grid ? 1 : uniform_div(total + grid - 1, grid);
         if (pl.join && blockIdx.x == 0 && tid == 0) {
           pl.chunk[0] = chunk;
           pl.chunk[1] = 0;
         }
-        if ((int64_t)blockIdx.x * chunk >= total) return;
+        if ((int64_t)blockIdx.x * chunk >= total) return;  // (all work is in the first `grid` blocks)
         u = (int)blockIdx.x * chunk;
         end = min(u + chunk, total);
         before = 0;
@@ -1024,13 +1032,6 @@ __global__ void __launch_bounds__(PJ_THREADS) k_paged_join(PagedQuery pq, int hd
 int pa_class(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 
 // Blocks that fit the device at once.
-// Blocks of a launch: as many as fit the device where many pairs are begun and ended, or pages are found by lanes (more
-// waves hide more of that), else one a CU, whose loads fill the memory's queues as well and disturb
-// each other less. WAVES_FIGURES
-constexpr int PA_MANY_PAIRS = 3;  // a CU
-int pa_blocks(int n_cu, int hd, size_t pairs, bool uni) {
-  return n_cu * (uni && pairs < (size_t)PA_MANY_PAIRS * n_cu ? 1 : pa_waves(pa_class(hd)));
-}
 
 PagedPlan pa_plan(int n_seqs, int n_heads, int n_kv) {
   PagedPlan p{};
@@ -1045,7 +1046,7 @@ PagedPlan pa_plan(int n_seqs, int n_heads, int n_kv) {
 
 bool paged_attn_fits(int n_seqs, int n_heads, int n_kv, size_t cap) {
   const PagedPlan p = pa_plan(n_seqs, n_heads, n_kv);
-  return (size_t)n_seqs * (size_t)p.n_groups * ((2 * cap >> PA_UNIT) + 1 + PA_PAIR) < ((size_t)1 << 29);  // (up to 2 slots a position)
+  return (size_t)n_seqs * (size_t)p.n_groups * ((3 * cap / 2 >> PA_UNIT) + 1 + PA_PAIR) < ((size_t)1 << 29);  // (up to 3 slots for 2 positions)
 }
 
 void PagedView::set_slots(int n) {
@@ -1067,7 +1068,7 @@ hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQue
   PagedPlan pl = pa_plan(sq.n_seqs, q.n_heads, pool.n_kv);
   PagedView kv = pool;
   const size_t slots16 = ((size_t)kv.page_size + 15) / 16 * 16;
-  const bool uni = kv.page_size >= 8 && 16 * kv.pos_stride < ((size_t)1 << 29) && sq.max_pages * slots16 < ((size_t)1 << 31);
+  const bool uni = 2 * slots16 <= 3 * (size_t)kv.page_size && 16 * kv.pos_stride < ((size_t)1 << 29) && sq.max_pages * slots16 < ((size_t)1 << 31);
   if (uni) kv.set_slots((int)slots16);
   // slots of a sequence that count, at most (a window begins anywhere in a page, and its slots anywhere in 32)
   size_t cap = (size_t)sq.max_pages * kv.page_slots;
@@ -1076,7 +1077,8 @@ hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQue
     cap = std::min(cap, std::min((size_t)q.window + pages * (kv.page_slots - kv.page_size), pages * kv.page_slots) + 31);
   }
   const size_t pairs = (size_t)sq.n_seqs * pl.n_groups;
-  const int blocks_max = pa_blocks(n_cu, kv.hd, pairs, uni);
+  const int blocks_max = n_cu * pa_waves(pa_class(kv.hd));
+  pl.few = uni ? n_cu : blocks_max;
   const size_t slots = 2 * (size_t)blocks_max * pl.hg;
   pl.sums = static_cast<float*>(q.ws);
   pl.ml = reinterpret_cast<float2*>(pl.sums + slots * kv.hd);
