@@ -325,6 +325,9 @@ constexpr int PA_UNIT = 7;        // positions of a unit (their logarithm): a ti
 __host__ __device__ constexpr int pa_unit_short(int row_bytes) { return row_bytes <= 256 ? 9 : 8; }
 constexpr int PA_PAIR = 1;        // what a pair costs besides its units
 constexpr int PA_HEADS = 16;      // heads of a group at most
+// A pair of one tile is a wave's alone, and a pair of one unit where the block's run has this many of them: nothing is
+// then joined, and a block is in four pairs at once. ALONE_FIGURES
+constexpr int PA_ALONE = 2;
 // From this average cost of a pair on, one block a CU works (the others end at once): its loads fill the memory's
 // queues as well as four blocks' and disturb each other less. Batches of shorter pairs keep all the
 // blocks that fit, which hide each other's beginnings and ends. FEW_FIGURES
@@ -785,6 +788,25 @@ struct PaWave {
     }
   }
 
+  // A whole pair's results from this wave's sums alone.
+  __device__ __forceinline__ void finish(const PagedQuery& pq, int s, float up) {
+    l = group_sum(l);
+    if (n >= heads) return;
+    const bool none = m == NEG_INF && l == 0.0f;
+    const float f = none ? 0.0f : 1.0f / l;
+    const size_t out = (size_t)s * pq.out_stride + (size_t)(head0 + n) * kv.hd;
+#pragma unroll
+    for (int p = 0; p < NV; ++p)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int e = 0; e < PE; e += 4) {
+          const int d = (16 * p + 4 * g + r) * PE + e, i = p * PE + e;
+          if (d < kv.hd) store_act(pq.out, out + d, pq.dt, v4f{o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]} * f);
+        }
+    if (g == 0 && pq.lse) pq.lse[(size_t)s * pq.n_heads + head0 + n] = none ? NEG_INF : (m + (__builtin_amdgcn_logf(l) - up)) * LN2;
+  }
+
   // Positions key, key + step, ... below end.
   __device__ __forceinline__ void run(int key, int end, int step) {
     if (key >= end) return;
@@ -903,6 +925,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
   PaWave<CT, NP, HDP, UNI> w(kv, lane);
   const float up = CT == BB_F16 ? 14.0f : 0.0f;
   bool lds_read = false;
+  int turn = 0;
   // the run's pairs: group grp of sequence s, whose cost begins at lo
   for (; lo < end; lo += cost, ++grp) {
     if (grp == pl.n_groups) {
@@ -914,15 +937,22 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
     const int nu = cost - PA_PAIR, first_unit = lo + PA_PAIR;
     const int u0 = max(u - first_unit, 0), take = min(nu, end - first_unit) - u0;
     if (take <= 0) continue;  // (the run ends before the pair's units)
+    const SeqSpan sp = seq_span(len, kv, max_pages, pq.window, pl.unit);
+    const bool alone = nu == 1 && (sp.len - sp.base <= S::KT || end - u >= PA_ALONE * (1 + PA_PAIR));
+    if (alone && (turn++ & (PA_WAVES - 1)) != wv) continue;
     const int kvh = pl.split == 1 ? grp : uniform_div(grp, pl.split), sub = grp - kvh * pl.split;
     w.row = table + (size_t)s * table_stride;
     w.head0 = kvh * pl.G + sub * pl.hg;
     w.heads = min(pl.hg, pl.G - sub * pl.hg);
     w.kv_off = (size_t)kvh * kv.head_stride;
-    w.sp = seq_span(len, kv, max_pages, pq.window, pl.unit);
+    w.sp = sp;
     w.start(pq, s);
     const int k0 = w.sp.base + (u0 << pl.unit);
-    w.run(k0 + wv * S::KT, min(k0 + (take << pl.unit), w.sp.len), PA_WAVES * S::KT);
+    w.run(alone ? k0 : k0 + wv * S::KT, min(k0 + (take << pl.unit), w.sp.len), alone ? S::KT : PA_WAVES * S::KT);
+    if (alone) {
+      w.finish(pq, s, up);
+      continue;
+    }
 
     // the waves' sums together
     if (lds_read) __syncthreads();  // (the pair before is done with LDS)
