@@ -25,17 +25,21 @@ struct ElemOf<BB_BF16> {
   typedef __bf16 T;
 };
 
-// N consecutive elements (whole 16-byte pieces, or one element) as f32, and back, rounded to nearest.
+// N consecutive elements at any element's alignment as f32, and back, rounded to nearest (16-byte accesses).
+template <class T, int N>
+struct RunOf {
+  static constexpr int M = N * sizeof(T) > 16 ? 16 / sizeof(T) : N;
+  typedef T V __attribute__((ext_vector_type(M), aligned(sizeof(T))));
+};
 template <class T, int N>
 __device__ __forceinline__ void load_vec(const T* p, float (&x)[N]) {
   if constexpr (N == 1) {
     x[0] = (float)p[0];
   } else {
-    constexpr int M = 16 / sizeof(T);
-    typedef T V __attribute__((ext_vector_type(M)));
+    constexpr int M = RunOf<T, N>::M;
 #pragma unroll
     for (int i = 0; i < N; i += M) {
-      const V v = *reinterpret_cast<const V*>(p + i);
+      const auto v = *reinterpret_cast<const typename RunOf<T, N>::V*>(p + i);
 #pragma unroll
       for (int j = 0; j < M; ++j) x[i + j] = (float)v[j];
     }
@@ -46,14 +50,13 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
   if constexpr (N == 1) {
     p[0] = (T)x[0];
   } else {
-    constexpr int M = 16 / sizeof(T);
-    typedef T V __attribute__((ext_vector_type(M)));
+    constexpr int M = RunOf<T, N>::M;
 #pragma unroll
     for (int i = 0; i < N; i += M) {
-      V v;
+      typename RunOf<T, N>::V v;
 #pragma unroll
       for (int j = 0; j < M; ++j) v[j] = (T)x[i + j];
-      *reinterpret_cast<V*>(p + i) = v;
+      *reinterpret_cast<typename RunOf<T, N>::V*>(p + i) = v;
     }
   }
 }
@@ -127,10 +130,12 @@ __device__ __forceinline__ RowPlace row_place(const RopeRows& r, const PagedView
 
 // A block takes rpb of a token's head rows. Its first wave finds the token's place, its threads the (cos, sin) of the
 // pairs once into LDS; then groups of gs lanes (a power of two) take a head row each, a lane up to MU
-// pairs of runs of VE elements that turn together (or runs past the turned part). VE 8: whole 16-byte
-// pieces; VE 1: any size and stride.
+// pairs of runs of VE elements that turn together (or runs past the turned part). VE 8: the last run of
+// a part that is no multiple of 8 begins where it still fits, its first elements being done twice,
+// with the same result (a group's lanes are in one wave, which loads a row before it stores it).
+// VE 1: parts shorter than 8.
 // One token's call is latency, a long batch is bound by its bytes: ROPE_FIGURES.
-template <class A, class C, int VE>
+template <class A, class C, int VE, bool EVEN>
 __global__ void __launch_bounds__(RR_THREADS) k_rope_rows(RopeRows r, RopeTurns rt, PagedView kv, PagedSeqs sq, int rpb,
                                                           int gs) {
   constexpr int MU = VE == 1 ? 4 : 1;
@@ -140,7 +145,7 @@ __global__ void __launch_bounds__(RR_THREADS) k_rope_rows(RopeRows r, RopeTurns 
   const int tid = threadIdx.x, half = rt.half;
   const size_t t = blockIdx.x;
   const int row0 = blockIdx.y * rpb, row1 = min(row0 + rpb, r.n_q + 2 * r.n_kv);
-  const int nu = half / VE, units = nu + (r.hd - 2 * half) / VE, lane = tid & (gs - 1);
+  const int rest = r.hd - 2 * half, nu = (half + VE - 1) / VE, units = nu + (rest + VE - 1) / VE, lane = tid & (gs - 1);
 
   const double turns = tid < half ? rt.turns[tid] : 0.0;
   if (r.q_norm && tid < r.hd) s_gain[0][tid] = r.q_norm[tid];
@@ -157,7 +162,13 @@ __global__ void __launch_bounds__(RR_THREADS) k_rope_rows(RopeRows r, RopeTurns 
     cs[tid] = make_float2(rt.magnitude * v.x, rt.magnitude * v.y);
   }
   __syncthreads();
-  const auto first_of = [&](int u) { return u < nu ? (rt.interleaved ? 2 * u * VE : u * VE) : 2 * half + (u - nu) * VE; };
+  // run u's first pair, its first element and how many of its pairs (elements past the turned part) another run has
+  const auto pair_of = [&](int u) { return EVEN ? u * VE : min(u * VE, half - VE); };
+  const auto rest_of = [&](int u) { return EVEN ? (u - nu) * VE : min((u - nu) * VE, rest - VE); };
+  const auto first_of = [&](int u) {
+    return u < nu ? (rt.interleaved ? 2 : 1) * pair_of(u) : 2 * half + rest_of(u);
+  };
+  const auto twice_of = [&](int u) { return EVEN ? 0 : u < nu ? u * VE - pair_of(u) : (u - nu) * VE - rest_of(u); };
   for (int row = row0 + tid / gs; row < row1; row += RR_THREADS / gs) {
     const bool is_q = row < r.n_q, is_k = !is_q && row < r.n_q + r.n_kv;
     if (!is_q && w.base < 0) continue;
@@ -182,9 +193,15 @@ __global__ void __launch_bounds__(RR_THREADS) k_rope_rows(RopeRows r, RopeTurns 
       const float* gain = s_gain[is_q ? 0 : 1];
       float ss = 0.0f;
 #pragma unroll
-      for (int m = 0; m < MU; ++m)
+      for (int m = 0; m < MU; ++m) {
+        const int u = lane + m * gs, twice = twice_of(u);
+        const bool flat = rt.interleaved && u < nu;  // a and b are one run of pairs
 #pragma unroll
-        for (int j = 0; j < VE; ++j) ss += a[m][j] * a[m][j] + b[m][j] * b[m][j];
+        for (int j = 0; j < VE; ++j) {
+          ss += EVEN || j >= (flat ? 2 * twice : twice) ? a[m][j] * a[m][j] : 0.0f;
+          ss += EVEN || j >= (flat ? 2 * twice - VE : twice) ? b[m][j] * b[m][j] : 0.0f;
+        }
+      }
       for (int o = 1; o < gs; o <<= 1) ss += __shfl_xor(ss, o);
       const float scale = 1.0f / sqrtf(ss / (float)r.hd + r.eps);
 #pragma unroll
@@ -204,7 +221,7 @@ __global__ void __launch_bounds__(RR_THREADS) k_rope_rows(RopeRows r, RopeTurns 
       const int u = lane + m * gs, e0 = first_of(u), e1 = rt.interleaved ? e0 + VE : e0 + half;
       if (m * gs >= units) break;
       if (u < nu && (is_q || is_k)) {
-        const float2* c = cs + u * VE;
+        const float2* c = cs + pair_of(u);
         if (rt.interleaved && VE > 1) {
           // pairs (0,1), (2,3), ... of the 2·VE elements a, b
 #pragma unroll
@@ -238,11 +255,9 @@ __global__ void __launch_bounds__(RR_THREADS) k_rope_rows(RopeRows r, RopeTurns 
 
 template <class A, class C>
 hipError_t rope_rows_of(hipStream_t s, const RopeRows& r, const RopeTurns& t, const PagedView& kv, const PagedSeqs& sq) {
-  const size_t per = 16 / sizeof(A);
-  // (arrays start 16-byte aligned, the pool's strides are whole 16-byte pieces)
-  const bool wide = t.half % 8 == 0 && r.hd % 8 == 0 &&
-                    (r.q_ts % per | r.q_hs % per | r.qo_ts % per | r.qo_hs % per | r.k_ts % per | r.v_ts % per) == 0;
-  const int ve = wide ? 8 : 1, units = t.half / ve + (r.hd - 2 * t.half) / ve, n_rows = r.n_q + 2 * r.n_kv;
+  const int rest = r.hd - 2 * t.half, n_rows = r.n_q + 2 * r.n_kv;
+  const bool wide = (t.half == 0 || t.half >= 8) && (rest == 0 || rest >= 8);
+  const int ve = wide ? 8 : 1, units = (t.half + ve - 1) / ve + (rest + ve - 1) / ve;
   int gs = 1;
   while (gs < units && gs < 64) gs *= 2;
   const int at_once = RR_THREADS / gs;
@@ -250,8 +265,9 @@ hipError_t rope_rows_of(hipStream_t s, const RopeRows& r, const RopeTurns& t, co
   const size_t want = std::max<size_t>(1, std::min<size_t>((n_rows + at_once - 1) / at_once, 2048 / r.T));
   const int rpb = (int)((n_rows + want - 1) / want);
   const dim3 grid((unsigned)r.T, (unsigned)((n_rows + rpb - 1) / rpb));
-  if (wide) BB_LAUNCH((k_rope_rows<A, C, 8>), grid, dim3(RR_THREADS), 0, s, r, t, kv, sq, rpb, gs);
-  else BB_LAUNCH((k_rope_rows<A, C, 1>), grid, dim3(RR_THREADS), 0, s, r, t, kv, sq, rpb, gs);
+  if (!wide) BB_LAUNCH((k_rope_rows<A, C, 1, true>), grid, dim3(RR_THREADS), 0, s, r, t, kv, sq, rpb, gs);
+  else if (t.half % 8 || rest % 8) BB_LAUNCH((k_rope_rows<A, C, 8, false>), grid, dim3(RR_THREADS), 0, s, r, t, kv, sq, rpb, gs);
+  else BB_LAUNCH((k_rope_rows<A, C, 8, true>), grid, dim3(RR_THREADS), 0, s, r, t, kv, sq, rpb, gs);
   return hipGetLastError();
 }
 
@@ -371,8 +387,8 @@ __device__ __forceinline__ SeqSpan seq_span(int raw_len, const PagedView& kv, in
 // Four adjacent elements of a row of type dt, at any element's alignment.
 template <class T>
 __device__ __forceinline__ void store_row(void* p, size_t i, const v4f& x) {
-  const T y[4] = {(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
-  __builtin_memcpy(static_cast<T*>(p) + i, y, sizeof(y));
+  const float y[4] = {x[0], x[1], x[2], x[3]};
+  store_vec<T, 4>(static_cast<T*>(p) + i, y);
 }
 __device__ __forceinline__ void store_act(void* p, size_t i, int dt, const v4f& x) {
   if (dt == BB_F32) store_row<float>(p, i, x);
@@ -476,15 +492,6 @@ struct PaShape {
   static constexpr int NT = KT / 16;
 };
 
-// N elements (16 bytes or 8) of a row of type dt at any element's alignment, as f32.
-template <class T, int N>
-__device__ __forceinline__ void load_row(const void* p, size_t i, float (&x)[N]) {
-  T v[N];
-  __builtin_memcpy(v, static_cast<const T*>(p) + i, sizeof(v));
-#pragma unroll
-  for (int j = 0; j < N; ++j) x[j] = (float)v[j];
-}
-
 // One wave's part of a (sequence, head group) pair: running maximum m (base 2), sum l and o[i][r] for element
 // (16p + 4g + r)·PE + e, i = p·PE + e, of head n.
 // UNI: a page counts as whole 16 positions (slots; up to a third of them empty), whose rows are within 2^31 bytes of
@@ -519,7 +526,7 @@ struct PaWave {
   __device__ __forceinline__ void load_q(const PagedQuery& pq, int s, float (&x)[NC][KE]) const {
     const size_t at = (size_t)s * pq.q_stride + (size_t)(head0 + min(n, heads - 1)) * kv.hd;
 #pragma unroll
-    for (int j = 0; j < NC; ++j) load_row<A, KE>(pq.q, at + min((4 * j + g) * KE, kv.hd - KE), x[j]);
+    for (int j = 0; j < NC; ++j) load_vec<A, KE>(static_cast<const A*>(pq.q) + at + min((4 * j + g) * KE, kv.hd - KE), x[j]);
   }
 
   __device__ __forceinline__ void start(const PagedQuery& pq, int s) {

@@ -182,7 +182,7 @@ def attend(ctx, pool, q, window=0, scale=None, workspace=None, kv=None):
 
 # ---- rotary positions -----------------------------------------------------------------------------
 ROPE_SIZES = [(1, 1, 2, 2), (1, 40, 64, 64), (3, 5, 64, 32), (7, 2, 80, 26), (2, 3, 10, 6), (5, 1, 256, 256),
-              (4500, 2, 48, 16), (33, 9, 96, 96), (2, 2, 255, 254)]
+              (4500, 2, 48, 16), (33, 9, 96, 96), (2, 2, 255, 254), (3, 4, 64, 46), (5, 3, 100, 36), (2, 3, 33, 18)]
 
 
 @pytest.mark.parametrize("dt", [F32, F16, BF16])
@@ -329,6 +329,8 @@ APPEND_SHAPES = [
     (16, 1, 256, 256, True, 128, [200], [129]),
     (24, 2, 40, 26, False, 16, [0] * 70, [i % 3 for i in range(70)]),
     (2, 2, 64, 0, False, 16, [17, 0], [3, 3]),
+    (6, 2, 64, 46, True, 16, [5, 9], [3, 20]),
+    (6, 2, 72, 54, False, 16, [5, 9], [3, 20]),
 ]
 
 
