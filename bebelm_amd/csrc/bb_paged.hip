@@ -134,7 +134,11 @@ __device__ __forceinline__ RowPlace row_place(const RopeRows& r, const PagedView
 // a part that is no multiple of 8 begins where it still fits, its first elements being done twice,
 // with the same result (a group's lanes are in one wave, which loads a row before it stores it).
 // VE 1: parts shorter than 8.
-// One token's call is latency, a long batch is bound by its bytes: ROPE_FIGURES.
+// One token's call is latency (40 heads of 64, f32: 2.7 us; with norm and append 3.5), a long batch is bound by its
+// bytes: 4097 tokens of 32 heads of 128, bf16, 14.2 us, 4.7 TB/s read and written; 5003 tokens of 32 query
+// and 8 kv heads appended 27.1 us, 4.5 TB/s (a plain copy of 4 GiB: 4.9). Two tokens a block: 14.4 and
+// 30 us; elements one at a time where a part is no multiple of 8 (1176 tokens, 118 of 128 turned,
+// 28.9 MB): 28 us, in runs 12.7.
 template <class A, class C, int VE, bool EVEN>
 __global__ void __launch_bounds__(RR_THREADS) k_rope_rows(RopeRows r, RopeTurns rt, PagedView kv, PagedSeqs sq, int rpb,
                                                           int gs) {
@@ -266,7 +270,8 @@ hipError_t rope_rows_of(hipStream_t s, const RopeRows& r, const RopeTurns& t, co
   const int rpb = (int)((n_rows + want - 1) / want);
   const dim3 grid((unsigned)r.T, (unsigned)((n_rows + rpb - 1) / rpb));
   if (!wide) BB_LAUNCH((k_rope_rows<A, C, 1, true>), grid, dim3(RR_THREADS), 0, s, r, t, kv, sq, rpb, gs);
-  else if (t.half % 8 || rest % 8) BB_LAUNCH((k_rope_rows<A, C, 8, false>), grid, dim3(RR_THREADS), 0, s, r, t, kv, sq, rpb, gs);
+  else if (t.half % 8 || rest % 8)
+    BB_LAUNCH((k_rope_rows<A, C, 8, false>), grid, dim3(RR_THREADS), 0, s, r, t, kv, sq, rpb, gs);
   else BB_LAUNCH((k_rope_rows<A, C, 8, true>), grid, dim3(RR_THREADS), 0, s, r, t, kv, sq, rpb, gs);
   return hipGetLastError();
 }
@@ -307,6 +312,9 @@ hipError_t launch_rope_rows(hipStream_t s, int dtype, int cache, const RopeRows&
 // maximum and sum of the softmax. Bound by the cache's bytes: one kv head's keys and values are read
 // once for the (up to 16) query heads of a group, and nothing but sums leaves the registers.
 //
+// 64 sequences of 8192, 32 query on 8 kv heads of 128, f16: 357 us, 6.0 TB/s; one sequence of 9001, of 64,
+// bf16: 13 us, of which 4 are the second launch and 3 pass until the first keys are asked for.
+//
 // Work. A sequence's positions (from its window's first, rounded down to 32) are cut into units of 128,
 // and the units of all (sequence, head group) pairs, in that order, into equal runs, one a block: every
 // block reads about the same number of bytes however ragged the batch, with no host knowing a
@@ -333,20 +341,27 @@ hipError_t launch_rope_rows(hipStream_t s, int dtype, int cache, const RopeRows&
 namespace {
 
 constexpr int PA_WAVES = 4, PA_THREADS = 64 * PA_WAVES;
-constexpr int PA_UNIT = 7;        // positions of a unit (their logarithm): a tile for each wave
-// The same where no sequence reaches past one: no pair is split and nothing is to be joined, which costs 4 to 5 us. By
-// the bytes of a head's row (one sequence, 8 kv heads; whole and split): bf16, 64 elements: 512
-// positions 8.1 and 10.1 us, 1000 11.7 and 11.0; f32, 64: 512 10.4 and 10.9; f32, 256 elements (4
-// sequences): 256 17.9 and 19.1, 512 27.0 and 19.1.
+// Positions of a unit (their logarithm): a tile for each wave. 64 and 256 are no faster (34 sequences of
+// up to 16384, 38.6 and 40.8 us where 128 gave 41.6; one of 9001, 15.1 and 14.2 for 14.5).
+constexpr int PA_UNIT = 7;
+// The same where no sequence reaches past one: no pair is split and nothing is to be joined, which costs
+// 4 to 5 us. By the bytes of a head's row (one sequence, 8 kv heads; whole and split): bf16, 64
+// elements: 512 positions 8.1 and 10.1 us, 1000 11.7 and 11.0; f32, 64: 512 10.4 and 10.9; f32, 256
+// elements (4 sequences): 256 17.9 and 19.1, 512 27.0 and 19.1.
 __host__ __device__ constexpr int pa_unit_short(int row_bytes) { return row_bytes <= 256 ? 9 : 8; }
 constexpr int PA_PAIR = 1;        // what a pair costs besides its units
 constexpr int PA_HEADS = 16;      // heads of a group at most
-// A pair of one tile is a wave's alone, and a pair of one unit where the block's run has this many of them: nothing is
-// then joined, and a block is in four pairs at once. ALONE_FIGURES
+// A pair of one tile is a wave's alone, and a pair of one unit where the block's run has this many of
+// them: nothing is then joined, and a block is in four pairs at once. 168 sequences of up to 62, 16 kv
+// heads of 256, 33 us (all waves on every pair: 58); 131 of up to 3, of 64, 8.4 and 13.6; 200 of up to
+// 500, 8 heads of 128, 28 and 36.
 constexpr int PA_ALONE = 2;
-// From this average cost of a pair on, one block a CU works (the others end at once): its loads fill the memory's
-// queues as well as four blocks' and disturb each other less. Batches of shorter pairs keep all the
-// blocks that fit, which hide each other's beginnings and ends. FEW_FIGURES
+// From this average cost of a pair on, one block a CU works (the others end at once): its loads fill the
+// memory's queues as well as four blocks' and disturb each other less. Batches of shorter pairs keep
+// all the blocks that fit, which hide each other's beginnings and ends. One a CU and all, 8 kv heads:
+// 64 sequences of 8192, 64 elements, bf16 191 and 199 us, f32 355 and 381; of 128, f16, 357 and 375; 100
+// sequences of 2000, of 64, f16, 85 and 92. Up to 2000, 128 sequences, 16 heads of 64: 59 and 44; up to
+// 700, 200 sequences, of 128: 50 and 41.
 constexpr int PA_LONG = 16;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr float NEG_INF = -__builtin_inff();
@@ -526,7 +541,8 @@ struct PaWave {
   __device__ __forceinline__ void load_q(const PagedQuery& pq, int s, float (&x)[NC][KE]) const {
     const size_t at = (size_t)s * pq.q_stride + (size_t)(head0 + min(n, heads - 1)) * kv.hd;
 #pragma unroll
-    for (int j = 0; j < NC; ++j) load_vec<A, KE>(static_cast<const A*>(pq.q) + at + min((4 * j + g) * KE, kv.hd - KE), x[j]);
+    for (int j = 0; j < NC; ++j)
+      load_vec<A, KE>(static_cast<const A*>(pq.q) + at + min((4 * j + g) * KE, kv.hd - KE), x[j]);
   }
 
   __device__ __forceinline__ void start(const PagedQuery& pq, int s) {
@@ -636,7 +652,8 @@ struct PaWave {
         for (int j = 0; j < NC; ++j) {
           const int d = (4 * j + g) * KE;
           k[t][j] = v4u{0, 0, 0, 0};
-          if (at >= 0 && d < kv.hd) k[t][j] = *reinterpret_cast<const v4u*>(static_cast<const char*>(kv.k) + (size_t)(at + d) * SZ);
+          if (at >= 0 && d < kv.hd)
+            k[t][j] = *reinterpret_cast<const v4u*>(static_cast<const char*>(kv.k) + (size_t)(at + d) * SZ);
         }
       }
     }
@@ -811,7 +828,8 @@ struct PaWave {
           const int d = (16 * p + 4 * g + r) * PE + e, i = p * PE + e;
           if (d < kv.hd) store_act(pq.out, out + d, pq.dt, v4f{o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]} * f);
         }
-    if (g == 0 && pq.lse) pq.lse[(size_t)s * pq.n_heads + head0 + n] = none ? NEG_INF : (m + (__builtin_amdgcn_logf(l) - up)) * LN2;
+    if (g == 0 && pq.lse)
+      pq.lse[(size_t)s * pq.n_heads + head0 + n] = none ? NEG_INF : (m + (__builtin_amdgcn_logf(l) - up)) * LN2;
   }
 
   // Positions key, key + step, ... below end.
@@ -1003,7 +1021,8 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
       }
       if (whole) {
         const bool none = mm == NEG_INF && ll == 0.0f;
-        store_act(pq.out, (size_t)s * pq.out_stride + (size_t)(w.head0 + h) * kv.hd + d, pq.dt, x * (none ? 0.0f : 1.0f / ll));
+        store_act(pq.out, (size_t)s * pq.out_stride + (size_t)(w.head0 + h) * kv.hd + d, pq.dt,
+                  x * (none ? 0.0f : 1.0f / ll));
         if (d == 0 && pq.lse)
           pq.lse[(size_t)s * pq.n_heads + w.head0 + h] = none ? NEG_INF : (mm + (__builtin_amdgcn_logf(ll) - up)) * LN2;
       } else {
@@ -1017,7 +1036,8 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
 // Adds the partial sums of a (sequence, head), PJ_PIECES pieces of 4 elements a block: those of the blocks whose
 // runs hold units of it. Threads: a row of PJ_PIECES for every PJ_ROWS-th part, joined in LDS.
 constexpr int PJ_THREADS = 256, PJ_PIECES = 8, PJ_ROWS = PJ_THREADS / PJ_PIECES;
-__global__ void __launch_bounds__(PJ_THREADS) k_paged_join(PagedQuery pq, int hd, int blocks_of_row, PagedPlan pl, float up) {
+__global__ void __launch_bounds__(PJ_THREADS) k_paged_join(PagedQuery pq, int hd, int blocks_of_row, PagedPlan pl,
+                                                           float up) {
   __shared__ float s_m[PJ_ROWS], s_l[PJ_ROWS];
   __shared__ v4f s_x[PJ_ROWS][PJ_PIECES];
   const int s = blockIdx.x, grp = blockIdx.y, hh = blockIdx.z / blocks_of_row;
@@ -1083,7 +1103,8 @@ PagedPlan pa_plan(int n_seqs, int n_heads, int n_kv) {
 
 bool paged_attn_fits(int n_seqs, int n_heads, int n_kv, size_t cap) {
   const PagedPlan p = pa_plan(n_seqs, n_heads, n_kv);
-  return (size_t)n_seqs * (size_t)p.n_groups * ((3 * cap / 2 >> PA_UNIT) + 1 + PA_PAIR) < ((size_t)1 << 29);  // (up to 3 slots for 2 positions)
+  // (up to 3 slots for 2 positions)
+  return (size_t)n_seqs * (size_t)p.n_groups * ((3 * cap / 2 >> PA_UNIT) + 1 + PA_PAIR) < ((size_t)1 << 29);
 }
 
 void PagedView::set_slots(int n) {
@@ -1105,7 +1126,8 @@ hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQue
   PagedPlan pl = pa_plan(sq.n_seqs, q.n_heads, pool.n_kv);
   PagedView kv = pool;
   const size_t slots16 = ((size_t)kv.page_size + 15) / 16 * 16;
-  const bool uni = 2 * slots16 <= 3 * (size_t)kv.page_size && 16 * kv.pos_stride < ((size_t)1 << 29) && sq.max_pages * slots16 < ((size_t)1 << 31);
+  const bool uni = 2 * slots16 <= 3 * (size_t)kv.page_size && 16 * kv.pos_stride < ((size_t)1 << 29) &&
+                   sq.max_pages * slots16 < ((size_t)1 << 31);
   if (uni) kv.set_slots((int)slots16);
   // slots of a sequence that count, at most (a window begins anywhere in a page, and its slots anywhere in 32)
   size_t cap = (size_t)sq.max_pages * kv.page_slots;

@@ -8,6 +8,8 @@ Names follow the reference so call sites read alike:
   Model::attn_step / attn_batch (model.rs:430, :222)    -> AttnOp.forward (KvCache: cache.rs)
   Model::run_layers(_batch) / forward_step, Agent::absorb -> Model (model.rs:97-181, agent.rs:454)
   Cache (cache.rs:10-49), Cache: Clone                  -> Cache (Model.new_cache, Cache.clone)
+RopePlan and PagedKv are the handles of the paged-cache operators (kernels.rope, paged_append,
+paged_attention), which the reference does not have.
 Arrays are numpy (host memory, BB_LOC_HOST) or torch CUDA tensors (device memory,
 BB_LOC_DEVICE). Everything runs on the GPU through libbebelm_moe.so; there is no other path.
 """

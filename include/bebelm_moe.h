@@ -431,7 +431,8 @@ int bb_paged_append(bb_ctx* ctx, bb_paged_kv* kv, const bb_rope_plan* plan, cons
  * sequence with no position to attend to, and a head all of whose scores are -inf, gets zeros and
  * -inf. workspace: device memory of workspace_bytes >= bb_paged_attention_workspace's answer, for this
  * call alone while it runs; NULL takes the context's, which a captured call may not (a graph keeps the
- * address, the context's workspace grows: BB_ERR_ARG). The sums are taken in an order that the batch's
+ * address, the context's workspace grows: BB_ERR_ARG). A value that is attended to and is not finite makes
+ * the elements of out that it reaches not finite (an infinite one may give NaN). The sums are taken in an order that the batch's
  * lengths fix, so equal calls give equal bits. */
 typedef struct {
   uint32_t dtype; /* of q and out */
