@@ -2615,8 +2615,10 @@ void need_plan(const bb_ctx* c, const bb_rope_plan* p, size_t head_dim) {
 template <class F>
 void need_seqs(const bb_paged_kv* kv, const bb_paged_seqs* q, int loc, F&& first) {
   need(q->n_seqs <= PAGED_SEQS_MAX, BB_ERR_RANGE, "more than 65536 sequences");
-  need(q->max_pages >= 1 && q->max_pages * (size_t)kv->view.page_size < ((size_t)1 << 31) && q->max_pages < ((size_t)1 << 31),
-       BB_ERR_RANGE, "max_pages * page_size must be below 2^31");
+  // (2^30: positions, their slots and a tile past them are 31-bit numbers on the device)
+  need(q->max_pages >= 1 && q->max_pages < ((size_t)1 << 30) &&
+           q->max_pages * (size_t)kv->view.page_size < ((size_t)1 << 30),
+       BB_ERR_RANGE, "max_pages * page_size must be below 2^30");
   need(q->table_stride >= q->max_pages && q->table_stride < STRIDE_MAX, BB_ERR_ARG, "table_stride below max_pages");
   if (q->n_seqs == 0) return;
   need(q->page_table && q->lens, BB_ERR_ARG, "null page table or lengths");

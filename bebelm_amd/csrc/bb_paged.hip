@@ -1126,8 +1126,7 @@ hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQue
   PagedPlan pl = pa_plan(sq.n_seqs, q.n_heads, pool.n_kv);
   PagedView kv = pool;
   const size_t slots16 = ((size_t)kv.page_size + 15) / 16 * 16;
-  const bool uni = 2 * slots16 <= 3 * (size_t)kv.page_size && 16 * kv.pos_stride < ((size_t)1 << 29) &&
-                   sq.max_pages * slots16 < ((size_t)1 << 31);
+  const bool uni = 2 * slots16 <= 3 * (size_t)kv.page_size && 16 * kv.pos_stride < ((size_t)1 << 29);
   if (uni) kv.set_slots((int)slots16);
   // slots of a sequence that count, at most (a window begins anywhere in a page, and its slots anywhere in 32)
   size_t cap = (size_t)sq.max_pages * kv.page_slots;

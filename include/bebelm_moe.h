@@ -331,7 +331,7 @@ int bb_model_absorb(bb_ctx* ctx, bb_model* m, bb_cache* cache, const uint32_t* t
  * and positions on the device only (the host never waits for them), so a captured call follows what
  * these arrays hold at each replay; with BB_LOC_HOST they are checked first (BB_ERR_RANGE) and the
  * call may not be captured. Arrays of 16-byte aligned device memory, as everywhere; strides are in
- * elements. n_tokens or n_seqs of 0: nothing is done. */
+ * elements. n_tokens (below 2^22) or n_seqs of 0: nothing is done. */
 
 /* Rotary positions. Pair i < rot_dim/2 of a head vector turns by the angle pos·f_i:
  *   (a, b) -> magnitude·(a·cos - b·sin, a·sin + b·cos),
@@ -387,8 +387,8 @@ int bb_paged_kv_pages(const bb_paged_kv* kv, void** k, void** v);
  * max_pages·page_size, and a page number outside the pool as a page whose positions are not there:
  * nothing is stored in it, nothing read. */
 typedef struct {
-  size_t n_seqs; /* at most 65536 */
-  size_t max_pages;
+  size_t n_seqs;       /* at most 65536 */
+  size_t max_pages;    /* max_pages * page_size below 2^30 */
   size_t table_stride; /* >= max_pages */
   const int32_t* page_table;
   const int32_t* lens;
