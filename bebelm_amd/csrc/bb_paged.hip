@@ -503,7 +503,7 @@ struct PaShape {
   static constexpr int VE = HDP / 16;                    // elements of a value row per lane
   static constexpr int PE = VE < KE ? VE : KE;           // in pieces of PE
   static constexpr int NV = VE / PE;
-  static constexpr int KT = CT == BB_F32 ? 16 : 32;      // positions of a tile: 128 bytes of each element column
+  static constexpr int KT = CT == BB_F32 ? 16 : 32;      // positions of a tile (registers)
   static constexpr int NT = KT / 16;
 };
 

@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from bebelm_amd import BBError, _lib, kernels, synth
-from bebelm_amd.model import BF16, F16, F32, AttnOp, PagedKv, RopePlan
+from bebelm_amd.model import BF16, F16, F32, AttnOp, Context, PagedKv, RopePlan
 
 pytestmark = pytest.mark.gpu
 
@@ -583,7 +583,9 @@ def test_attention_ragged_batches(gpu_ctx):
     """Many sequences of all lengths: splits of every kind."""
     for seed, (n, longest, kv, g, hd, dt) in enumerate([(300, 60, 2, 4, 64, BF16), (70, 5000, 1, 2, 64, F16),
                                                         (3, 40000, 2, 3, 128, BF16), (1000, 9, 1, 1, 64, F32),
-                                                        (40, 900, 8, 4, 64, F32)]):
+                                                        (40, 900, 8, 4, 64, F32), (270, 2500, 1, 2, 64, BF16),
+                                                        (5, 3000, 1, 24, 64, F16), (4, 2000, 2, 17, 128, F32),
+                                                        (600, 300, 2, 1, 256, F16)]):
         print("ragged", n, longest, flush=True)
         lens = [int(longest ** u) if u > 0.1 else 0 for u in torch.rand(n, generator=gen(seed)).tolist()]
         lens[-1] = longest
@@ -742,6 +744,30 @@ def test_captured_step(gpu_ctx):
         check_attention(pool, q_out.cpu(), out, lse, 0.125, 0, F32, "replay of the third")
     finally:
         gpu_ctx.set_stream(0)
+
+
+def test_two_contexts_at_once(gpu_ctx):
+    """Two contexts on two streams, many calls of each under way together, on one pool."""
+    pool = Pool(gpu_ctx, 181, [3000, 17, 900, 0, 2000], BF16, 16, 2, 64)
+    other = Context(0)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    try:
+        table, lens = pool.table.cuda(), pool.lens.cuda()
+        qs = [[randn(182 + 10 * c + i, (5, 8, 64), F32).cuda() for i in range(6)] for c in range(2)]
+        outs = [[torch.empty_like(q) for q in c] for c in qs]
+        torch.cuda.synchronize()
+        for ctx, st in zip((gpu_ctx, other), streams):
+            ctx.set_stream(st.cuda_stream)
+        for i in range(6):
+            for c, ctx in enumerate((gpu_ctx, other)):
+                kernels.paged_attention(ctx, pool.kv, table, lens, qs[c][i], outs[c][i])
+        torch.cuda.synchronize()
+        for c in range(2):
+            for i in range(6):
+                check_attention(pool, qs[c][i].cpu(), outs[c][i], None, 0.125, 0, F32, f"context {c} call {i}")
+    finally:
+        gpu_ctx.set_stream(0)
+        other.close()
 
 
 def test_decode_beside_the_attention_operator(gpu_ctx):
