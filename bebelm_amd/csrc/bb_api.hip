@@ -2567,7 +2567,10 @@ int bb_model_absorb(bb_ctx* c, bb_model* m, bb_cache* k, const uint32_t* tokens,
 namespace {
 
 constexpr size_t PAGED_SEQS_MAX = 65536;
-constexpr size_t STRIDE_MAX = (size_t)1 << 40;  // elements; with counts below 2^20 no product passes 64 bits
+// Elements. With counts below 2^22 an array's span stays below 2^61 bytes and the sum of a call's spans below 2^64,
+// so that none wraps and passes for a small one.
+constexpr size_t STRIDE_MAX = (size_t)1 << 36;
+constexpr size_t SPAN_MAX = (size_t)1 << 48;  // elements of a pool, past any address
 
 // Bytes of an element of the paged operators' types.
 size_t elem_bytes(uint32_t dt, const char* what) {
@@ -2619,7 +2622,8 @@ void need_seqs(const bb_paged_kv* kv, const bb_paged_seqs* q, int loc, F&& first
   need(q->max_pages >= 1 && q->max_pages < ((size_t)1 << 30) &&
            q->max_pages * (size_t)kv->view.page_size < ((size_t)1 << 30),
        BB_ERR_RANGE, "max_pages * page_size must be below 2^30");
-  need(q->table_stride >= q->max_pages && q->table_stride < STRIDE_MAX, BB_ERR_ARG, "table_stride below max_pages");
+  need(q->table_stride >= q->max_pages, BB_ERR_ARG, "table_stride below max_pages");
+  need(q->table_stride < STRIDE_MAX, BB_ERR_RANGE, "strides must be below 2^36 elements");
   if (q->n_seqs == 0) return;
   need(q->page_table && q->lens, BB_ERR_ARG, "null page table or lengths");
   if (loc != BB_LOC_HOST) return;
@@ -2764,7 +2768,7 @@ int bb_rope(bb_ctx* c, const bb_rope_plan* plan, uint32_t dtype, const void* x, 
     if (n_tokens == 0) return;
     need(x && pos && out, BB_ERR_ARG, "null argument");
     for (const size_t st : {token_stride, head_stride, out_token_stride, out_head_stride})
-      need(st < STRIDE_MAX, BB_ERR_RANGE, "stride beyond 2^40 elements");
+      need(st < STRIDE_MAX, BB_ERR_RANGE, "strides must be below 2^36 elements");
     // every element of out has a place of its own: the smaller stride holds a head vector, the larger one all of
     // the smaller's
     const bool tok_major = out_token_stride >= out_head_stride;
@@ -2842,7 +2846,7 @@ int bb_paged_kv_view(bb_ctx* c, uint32_t dtype, void* k, void* v, size_t n_pages
     for (int i = 0; i < 3; ++i) {
       auto& d = dims[i];
       if (d.second == 1) d.first = 0;  // never stepped
-      need(d.first < STRIDE_MAX, BB_ERR_RANGE, "stride beyond 2^40 elements");
+      need(d.first < STRIDE_MAX, BB_ERR_RANGE, "strides must be below 2^36 elements");
       need(d.first * eb % 16 == 0, BB_ERR_ARG, "strides must be whole 16-byte pieces");
     }
     std::sort(dims, dims + 4);
@@ -2850,7 +2854,7 @@ int bb_paged_kv_view(bb_ctx* c, uint32_t dtype, void* k, void* v, size_t n_pages
     for (const auto& d : dims) {
       if (d.second == 1) continue;
       need(d.first >= span, BB_ERR_ARG, "strides put two elements in one place");
-      need(d.second - 1 < ((size_t)1 << 62) / d.first, BB_ERR_RANGE, "pool too large");
+      need(d.second - 1 <= (SPAN_MAX - span) / d.first, BB_ERR_RANGE, "pool too large");
       span += (d.second - 1) * d.first;
     }
     *out = new_pool(c, dtype, k, v, n_pages, page_size, n_kv_heads, head_dim, page_stride, pos_stride, head_stride,
@@ -2904,7 +2908,7 @@ int bb_paged_append(bb_ctx* c, bb_paged_kv* kv, const bb_rope_plan* plan, const 
     if (T == 0 || B == 0) return;
     need(tk->k && tk->v, BB_ERR_ARG, "null keys or values");
     need(T == 1 || (tk->k_stride >= row && tk->v_stride >= row), BB_ERR_ARG, "k_stride or v_stride below a token's row");
-    need(tk->k_stride < STRIDE_MAX && tk->v_stride < STRIDE_MAX, BB_ERR_RANGE, "stride beyond 2^40 elements");
+    need(tk->k_stride < STRIDE_MAX && tk->v_stride < STRIDE_MAX, BB_ERR_RANGE, "strides must be below 2^36 elements");
     const size_t nk = span_bytes(T, tk->k_stride, row, eb), nv = span_bytes(T, tk->v_stride, row, eb);
     size_t nq = 0, nqo = 0;
     if (tk->q) {
@@ -2912,7 +2916,7 @@ int bb_paged_append(bb_ctx* c, bb_paged_kv* kv, const bb_rope_plan* plan, const 
       need(tk->n_heads >= 1 && tk->n_heads < ((size_t)1 << 16), BB_ERR_RANGE, "n_heads must be in 1..65535");
       const size_t qr = tk->n_heads * hd;
       need(T == 1 || (tk->q_stride >= qr && tk->q_out_stride >= qr), BB_ERR_ARG, "q_stride or q_out_stride below a token's row");
-      need(tk->q_stride < STRIDE_MAX && tk->q_out_stride < STRIDE_MAX, BB_ERR_RANGE, "stride beyond 2^40 elements");
+      need(tk->q_stride < STRIDE_MAX && tk->q_out_stride < STRIDE_MAX, BB_ERR_RANGE, "strides must be below 2^36 elements");
       nq = span_bytes(T, tk->q_stride, qr, eb);
       nqo = span_bytes(T, tk->q_out_stride, qr, eb);
       need_out_apart(tk->q, nq, tk->q_out, nqo, T == 1 || tk->q_stride == tk->q_out_stride, "q_out");
@@ -2993,7 +2997,7 @@ int bb_paged_attention(bb_ctx* c, const bb_paged_kv* kv, const bb_paged_seqs* sq
          "sequences times heads times positions beyond what one call counts");
     need(pq->q && pq->out, BB_ERR_ARG, "null query or output");
     need(B == 1 || (pq->q_stride >= row && pq->out_stride >= row), BB_ERR_ARG, "q_stride or out_stride below a sequence's row");
-    need(pq->q_stride < STRIDE_MAX && pq->out_stride < STRIDE_MAX, BB_ERR_RANGE, "stride beyond 2^40 elements");
+    need(pq->q_stride < STRIDE_MAX && pq->out_stride < STRIDE_MAX, BB_ERR_RANGE, "strides must be below 2^36 elements");
     const size_t nq = span_bytes(B, pq->q_stride, row, eb), no = span_bytes(B, pq->out_stride, row, eb);
     need(!overlap(pq->q, nq, pq->out, no), BB_ERR_ARG, "out overlaps the query");
     const size_t nl = pq->lse ? B * nh * 4 : 0;

@@ -6,6 +6,7 @@ Tolerances count roundings. u = 2^-24 is half a step of f32. A sum of n terms is
 n·u of the terms' absolute sum, and by independent roundings of about sqrt(n)·u of it: 8·sqrt(n)·u is
 allowed. A stored value of type t is off by finfo(t).eps / 2 of itself.
 """
+import ctypes
 import math
 
 import numpy as np
@@ -954,3 +955,25 @@ def test_refusals(gpu_ctx):
     refused(ARG, lambda: kernels.rope(c, closed, x, pos))
     done(c)
     assert bool((k == 0).all()) and bool((v == 0).all())
+
+
+def test_spans_past_any_memory_are_refused(gpu_ctx):
+    """Strides whose products with the counts could pass 64 bits, in the call's arrays and in a view."""
+    c, lib = gpu_ctx, _lib.lib()
+    plan = RopePlan(c, 32, 1e4)
+    pos = torch.zeros(1, dtype=torch.int32, device="cuda")
+    x = torch.ones(64, device="cuda")
+    for at in range(4):
+        st = [64] * 4
+        st[at] = 1 << 36
+        assert lib.bb_rope(c.handle, plan.handle, F32, x.data_ptr(), st[0], st[1], 1, 1, 64, pos.data_ptr(), x.data_ptr(),
+                           st[2], st[3], _lib.LOC_DEVICE) == _lib.BB_ERR_RANGE, at
+    done(c)
+    assert bool((x == 1).all())
+    k, v = torch.zeros(1024, device="cuda"), torch.zeros(1024, device="cuda")
+    for pages, size, heads, strides in ((1 << 20, 1, 1, (1 << 35, 0, 0)), (1 << 30, 1, 1, (1 << 25, 0, 0)),
+                                        (3, 1, 1, (1 << 36, 0, 0)), (1, 1 << 19, 2, (0, 64, 1 << 36))):
+        view = ctypes.c_void_p()
+        assert lib.bb_paged_kv_view(c.handle, F32, k.data_ptr(), v.data_ptr(), pages, size, heads, 64, *strides,
+                                    ctypes.byref(view)) == _lib.BB_ERR_RANGE, (pages, size, heads, strides)
+        assert not view.value
