@@ -16,6 +16,7 @@
 
 #include "../../include/bebelm_moe.h"
 #include "bb_internal.h"
+#include "bb_rows.h"
 
 namespace {
 
@@ -2603,9 +2604,12 @@ bool overlap(const void* a, size_t na, const void* b, size_t nb) {
   return na > 0 && nb > 0 && x < y + nb && y < x + na;
 }
 
-void need_out_apart(const void* x, size_t nx, const void* out, size_t nout, bool same_layout, const char* what) {
-  if (x == out && same_layout) return;
-  need(!overlap(x, nx, out, nout), BB_ERR_ARG, std::string(what) + " overlaps its input");
+using bb::Rows;
+using bb::rows_of;
+
+void need_out_apart(const Rows& x, const Rows& out, bool same_layout, const char* what) {
+  if (x.p == out.p && same_layout) return;
+  need(!rows_overlap(x, out), BB_ERR_ARG, std::string(what) + " overlaps its input");
 }
 
 void need_plan(const bb_ctx* c, const bb_rope_plan* p, size_t head_dim) {
@@ -2778,7 +2782,12 @@ int bb_rope(bb_ctx* c, const bb_rope_plan* plan, uint32_t dtype, const void* x, 
          "out's strides put two elements in one place");
     const size_t nx = ((n_tokens - 1) * token_stride + (n_heads - 1) * head_stride + head_dim) * eb;
     const size_t no = ((n_tokens - 1) * out_token_stride + (n_heads - 1) * out_head_stride + head_dim) * eb;
-    need_out_apart(x, nx, out, no,
+    // (groups by out's larger stride)
+    const auto rows = [&](const void* p, size_t ts, size_t hs) {
+      return tok_major ? Rows{p, {n_tokens, n_heads}, {ts * eb, hs * eb}, head_dim * eb}
+                       : Rows{p, {n_heads, n_tokens}, {hs * eb, ts * eb}, head_dim * eb};
+    };
+    need_out_apart(rows(x, token_stride, head_stride), rows(out, out_token_stride, out_head_stride),
                    (n_tokens == 1 || token_stride == out_token_stride) && (n_heads == 1 || head_stride == out_head_stride),
                    "out");
     set_device(c);
@@ -2919,9 +2928,11 @@ int bb_paged_append(bb_ctx* c, bb_paged_kv* kv, const bb_rope_plan* plan, const 
       need(tk->q_stride < STRIDE_MAX && tk->q_out_stride < STRIDE_MAX, BB_ERR_RANGE, "strides must be below 2^36 elements");
       nq = span_bytes(T, tk->q_stride, qr, eb);
       nqo = span_bytes(T, tk->q_out_stride, qr, eb);
-      need_out_apart(tk->q, nq, tk->q_out, nqo, T == 1 || tk->q_stride == tk->q_out_stride, "q_out");
-      need(!overlap(tk->k, nk, tk->q_out, nqo) && !overlap(tk->v, nv, tk->q_out, nqo), BB_ERR_ARG,
-           "q_out overlaps the keys or values");
+      const Rows q_out = rows_of(tk->q_out, T, tk->q_out_stride, qr, eb);
+      need_out_apart(rows_of(tk->q, T, tk->q_stride, qr, eb), q_out, T == 1 || tk->q_stride == tk->q_out_stride, "q_out");
+      need(!rows_overlap(rows_of(tk->k, T, tk->k_stride, row, eb), q_out) &&
+               !rows_overlap(rows_of(tk->v, T, tk->v_stride, row, eb), q_out),
+           BB_ERR_ARG, "q_out overlaps the keys or values");
     } else {
       need(!tk->q_norm && !tk->q_out, BB_ERR_ARG, "q_norm or q_out without q");
     }
@@ -2999,7 +3010,8 @@ int bb_paged_attention(bb_ctx* c, const bb_paged_kv* kv, const bb_paged_seqs* sq
     need(B == 1 || (pq->q_stride >= row && pq->out_stride >= row), BB_ERR_ARG, "q_stride or out_stride below a sequence's row");
     need(pq->q_stride < STRIDE_MAX && pq->out_stride < STRIDE_MAX, BB_ERR_RANGE, "strides must be below 2^36 elements");
     const size_t nq = span_bytes(B, pq->q_stride, row, eb), no = span_bytes(B, pq->out_stride, row, eb);
-    need(!overlap(pq->q, nq, pq->out, no), BB_ERR_ARG, "out overlaps the query");
+    need(!rows_overlap(rows_of(pq->q, B, pq->q_stride, row, eb), rows_of(pq->out, B, pq->out_stride, row, eb)),
+         BB_ERR_ARG, "out overlaps the query");
     const size_t nl = pq->lse ? B * nh * 4 : 0;
     need(!overlap(pq->lse, nl, pq->out, no) && !overlap(pq->lse, nl, pq->q, nq), BB_ERR_ARG, "lse overlaps the query or out");
     set_device(c);

@@ -331,7 +331,9 @@ int bb_model_absorb(bb_ctx* ctx, bb_model* m, bb_cache* cache, const uint32_t* t
  * and positions on the device only (the host never waits for them), so a captured call follows what
  * these arrays hold at each replay; with BB_LOC_HOST they are checked first (BB_ERR_RANGE) and the
  * call may not be captured. Arrays of 16-byte aligned device memory, as everywhere; strides are in
- * elements, below 2^36. n_tokens (below 2^22) or n_seqs of 0: nothing is done. */
+ * elements, below 2^36. Arrays overlap where they share an element: rows of one may lie between rows of
+ * another that are the same strides apart (q, k and v of one fused projection, q turned in place).
+ * n_tokens (below 2^22) or n_seqs of 0: nothing is done. */
 
 /* Rotary positions. Pair i < rot_dim/2 of a head vector turns by the angle pos·f_i:
  *   (a, b) -> magnitude·(a·cos - b·sin, a·sin + b·cos),

@@ -977,3 +977,109 @@ def test_spans_past_any_memory_are_refused(gpu_ctx):
         assert lib.bb_paged_kv_view(c.handle, F32, k.data_ptr(), v.data_ptr(), pages, size, heads, 64, *strides,
                                     ctypes.byref(view)) == _lib.BB_ERR_RANGE, (pages, size, heads, strides)
         assert not view.value
+
+
+# ---- rows of one buffer side by side -------------------------------------------------------------
+def fused_parts(buf, heads, kv, order):
+    """q, k and v as the columns of one projection's rows, in the given order ('-': a head of something else)."""
+    at, got = 0, {}
+    for c in order:
+        n = {"q": heads, "k": kv, "v": kv, "-": 1}[c]
+        got[c] = buf[:, at:at + n]
+        at += n
+    return got["q"], got["k"], got["v"]
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("order", ["qkv", "kvq", "k-q-v"])
+@pytest.mark.parametrize("norm", [False, True])
+def test_append_in_place_in_a_fused_projection(gpu_ctx, dt, order, norm):
+    """q turned where it lies, between k and v of the same rows: the bits of a call with a q_out of its own."""
+    heads, kv, hd = 6, 2, 64
+    plan = RopePlan(gpu_ctx, hd, 1e6)
+    gains = [(1 + 0.1 * torch.randn(hd, generator=gen(i))).cuda() if norm else None for i in (201, 202)]
+    for bring, lens in (([1, 1], [5, 30]), ([3, 0, 9], [3, 17, 40])):
+        t = sum(bring)
+        start = None if bring == [1, 1] else torch.tensor([0, 3, 3, 12], dtype=torch.int32)
+        base = randn(203, (t, heads + 2 * kv + order.count("-"), hd), dt)
+        results = []
+        for where in ("apart", "in place", "host"):
+            pool = Pool(gpu_ctx, 204, lens, BF16, 16, kv, hd)
+            index = [pool.table, pool.lens, start]
+            g = gains
+            if where == "host" and dt == F32:
+                buf = base.numpy().copy()
+                index = [i if i is None else i.numpy() for i in index]
+                g = [i if i is None else i.cpu().numpy() for i in gains]
+            else:
+                buf = base.cuda()
+                index = [i if i is None else i.cuda() for i in index]
+            q, k, v = fused_parts(buf, heads, kv, order)
+            out = torch.empty(t, heads, hd, dtype=TYPES[dt], device="cuda") if where == "apart" else None
+            torch.cuda.synchronize()
+            got = kernels.paged_append(gpu_ctx, pool.kv, index[0], index[1], k, v, rope=plan, seq_start=index[2], q=q,
+                                       q_out=out, q_norm=g[0], k_norm=g[1])
+            done(gpu_ctx)
+            _, k0, v0 = fused_parts(base, heads, kv, order)
+            assert torch.equal(torch.as_tensor(k).cpu(), k0) and torch.equal(torch.as_tensor(v).cpu(), v0)
+            results.append((torch.as_tensor(got).cpu().clone(), pool.k.cpu(), pool.v.cpu()))
+        for other in results[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(results[0], other))
+
+
+def test_attention_and_rope_between_rows_of_their_output(gpu_ctx):
+    """Queries and outputs as the halves of one buffer's rows; turned heads beside the ones they come from."""
+    pool = Pool(gpu_ctx, 211, [40, 300, 0, 5], BF16, 16, 2, 64)
+    both = torch.full((4, 9, 64), 7.0, device="cuda")
+    both[:, 1:5] = randn(212, (4, 4, 64), F32).cuda()
+    q = both[:, 1:5].clone()
+    want, _ = attend(gpu_ctx, pool, q)
+    kernels.paged_attention(gpu_ctx, pool.kv, pool.table.cuda(), pool.lens.cuda(), both[:, 1:5], both[:, 5:])
+    done(gpu_ctx)
+    assert torch.equal(both[:, 5:], want) and torch.equal(both[:, 1:5], q) and bool((both[:, 0] == 7.0).all())
+    host = both.cpu().numpy()
+    host[:, 5:] = 0.0
+    kernels.paged_attention(gpu_ctx, pool.kv, pool.table.numpy(), pool.lens.numpy(), host[:, 1:5], host[:, 5:])
+    assert np.array_equal(host, both.cpu().numpy())
+    plan = RopePlan(gpu_ctx, 64, 1e4)
+    pos = torch.arange(5, dtype=torch.int32, device="cuda")
+    for shape, pick in (((5, 6, 64), lambda a, i: a[:, 3 * i:3 * i + 3]), ((5, 6, 64), lambda a, i: a[:, i::2]),
+                        ((3, 10, 64), lambda a, i: a.permute(1, 0, 2)[5 * i:5 * i + 5]),
+                        ((3, 10, 64), lambda a, i: a.permute(1, 0, 2)[i::2])):
+        both = randn(213, shape, F32).cuda()
+        x = pick(both, 0).contiguous()
+        out = torch.empty_like(x)
+        torch.cuda.synchronize()
+        kernels.rope(gpu_ctx, plan, x, pos, out)
+        kernels.rope(gpu_ctx, plan, pick(both, 0), pos, pick(both, 1))
+        done(gpu_ctx)
+        assert torch.equal(pick(both, 1), out) and torch.equal(pick(both, 0), x)
+
+
+def test_rows_that_share_elements_are_refused(gpu_ctx):
+    c, ARG = gpu_ctx, _lib.BB_ERR_ARG
+    pool = Pool(c, 221, [20, 20, 20], F32, 16, 2, 64)
+    table, lens = pool.table.cuda(), pool.lens.cuda()
+    row = 8 * 64
+    buf = torch.zeros(4 * row, device="cuda")
+
+    def at(offset, heads, stride=row):
+        return buf.as_strided((3, heads, 64), (stride, 64, 1), offset)
+
+    q, k, v = at(0, 4), at(256, 2), at(384, 2)
+    append = lambda q_out, **kw: kernels.paged_append(c, pool.kv, table, lens, **{**dict(k=k, v=v, q=q), **kw}, q_out=q_out)
+    refused(ARG, lambda: append(at(64, 4)))                    # half on q, half on k
+    refused(ARG, lambda: append(at(192, 2), q=at(0, 2)))       # its second head is k's first
+    refused(ARG, lambda: append(at(row - 64, 2), q=at(128, 2)))  # v's last head
+    refused(ARG, lambda: append(at(row - 64, 2), k=at(0, 2), v=at(128, 2), q=at(256, 2)))   # the next row's k
+    refused(ARG, lambda: append(at(384, 2, row + 64), k=at(0, 2), v=at(128, 2), q=at(256, 2)))  # other strides
+    att = lambda a, b: kernels.paged_attention(c, pool.kv, table, lens, a, b)
+    refused(ARG, lambda: att(at(0, 4), at(192, 4)))
+    refused(ARG, lambda: att(at(64, 4), at(384, 4)))
+    refused(ARG, lambda: att(at(0, 4), at(row, 4)))            # the next sequence's rows
+    plan, pos = RopePlan(c, 64, 1e4), torch.zeros(3, dtype=torch.int32, device="cuda")
+    refused(ARG, lambda: kernels.rope(c, plan, at(0, 4), pos, at(192, 4)))
+    refused(ARG, lambda: kernels.rope(c, plan, at(0, 4)[:, ::2], pos, at(32, 4)[:, ::2]))
+    refused(ARG, lambda: kernels.rope(c, plan, at(0, 4), pos, at(row + 64, 4)))
+    done(c)
+    assert bool((buf == 0).all())
