@@ -2636,7 +2636,9 @@ void need_seqs(const bb_paged_kv* kv, const bb_paged_seqs* q, int loc, F&& first
     const int64_t n = q->lens[s];
     need(n >= 0 && (size_t)n <= q->max_pages * ps, BB_ERR_RANGE,
          "sequence " + std::to_string(s) + ": length " + std::to_string(n) + " is not in its pages");
-    for (size_t i = (size_t)first(s, n) / ps; i < ((size_t)n + ps - 1) / ps; ++i) {
+    const int64_t from = first(s, n);
+    if (from == n) continue;  // (no position, also where n is inside a page)
+    for (size_t i = (size_t)from / ps; i < ((size_t)n + ps - 1) / ps; ++i) {
       const int32_t pg = q->page_table[s * q->table_stride + i];
       need(pg >= 0 && pg < kv->view.n_pages, BB_ERR_RANGE,
            "sequence " + std::to_string(s) + ": page " + std::to_string(pg) + " is not in the pool");

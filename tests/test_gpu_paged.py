@@ -1083,3 +1083,31 @@ def test_rows_that_share_elements_are_refused(gpu_ctx):
     refused(ARG, lambda: kernels.rope(c, plan, at(0, 4), pos, at(row + 64, 4)))
     done(c)
     assert bool((buf == 0).all())
+
+
+# ---- what a call does not look at ------------------------------------------------------------------
+def test_host_append_needs_no_page_of_a_sequence_without_tokens(gpu_ctx):
+    """A sequence that brings nothing may have any entries: also the one of its partly filled last page."""
+    pool = Pool(gpu_ctx, 231, [20, 37, 3], F32, 16, 2, 64)
+    table = pool.table.numpy().copy()
+    table[1] = -1
+    k = randn(232, (5, 2, 64), F32)
+    start = np.array([0, 4, 4, 5], np.int32)
+    before = pool.k.cpu(), pool.v.cpu()
+    kernels.paged_append(gpu_ctx, pool.kv, table, pool.lens.numpy(), k.numpy(), 2 * k.numpy(), seq_start=start)
+    done(gpu_ctx)
+    got = pool.k.cpu(), pool.v.cpu()
+    for s in (0, 2):
+        p, r = (i[-(start[s + 1] - start[s]):] for i in pool.where(s))
+        for x, old, want in zip(got, before, (k, 2 * k)):
+            assert torch.equal(x[p, r], want[start[s]:start[s + 1]])
+            x[p, r] = old[p, r]
+    assert all(torch.equal(a, b) for a, b in zip(got, before))
+    # the entries that it stores through are looked at, and lengths that no table holds
+    table[0, 1] = -1
+    refused(_lib.BB_ERR_RANGE, lambda: kernels.paged_append(gpu_ctx, pool.kv, table, pool.lens.numpy(), k.numpy(),
+                                                            k.numpy(), seq_start=start))
+    table = pool.table.numpy()
+    for n in (-1, 16 * table.shape[1] + 1):
+        refused(_lib.BB_ERR_RANGE, lambda: kernels.paged_append(gpu_ctx, pool.kv, table, np.array([20, n, 3], np.int32),
+                                                                k.numpy(), k.numpy(), seq_start=start))
