@@ -2621,14 +2621,14 @@ void need_plan(const bb_ctx* c, const bb_rope_plan* p, size_t head_dim) {
 // the one of position first(s, length) on.
 template <class F>
 void need_seqs(const bb_paged_kv* kv, const bb_paged_seqs* q, int loc, F&& first) {
+  if (q->n_seqs == 0) return;  // (nothing is done, whatever the table's shape)
   need(q->n_seqs <= PAGED_SEQS_MAX, BB_ERR_RANGE, "more than 65536 sequences");
   // (2^30: positions, their slots and a tile past them are 31-bit numbers on the device)
   need(q->max_pages >= 1 && q->max_pages < ((size_t)1 << 30) &&
            q->max_pages * (size_t)kv->view.page_size < ((size_t)1 << 30),
-       BB_ERR_RANGE, "max_pages * page_size must be below 2^30");
+       BB_ERR_RANGE, "max_pages must be at least 1, max_pages * page_size below 2^30");
   need(q->table_stride >= q->max_pages, BB_ERR_ARG, "table_stride below max_pages");
   need(q->table_stride < STRIDE_MAX, BB_ERR_RANGE, "strides must be below 2^36 elements");
-  if (q->n_seqs == 0) return;
   need(q->page_table && q->lens, BB_ERR_ARG, "null page table or lengths");
   if (loc != BB_LOC_HOST) return;
   const size_t ps = (size_t)kv->view.page_size;

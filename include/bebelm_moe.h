@@ -390,7 +390,7 @@ int bb_paged_kv_pages(const bb_paged_kv* kv, void** k, void** v);
  * nothing is stored in it, nothing read. */
 typedef struct {
   size_t n_seqs;       /* at most 65536 */
-  size_t max_pages;    /* max_pages * page_size below 2^30 */
+  size_t max_pages;    /* at least 1; max_pages * page_size below 2^30 */
   size_t table_stride; /* >= max_pages */
   const int32_t* page_table;
   const int32_t* lens;

@@ -1111,3 +1111,21 @@ def test_host_append_needs_no_page_of_a_sequence_without_tokens(gpu_ctx):
     for n in (-1, 16 * table.shape[1] + 1):
         refused(_lib.BB_ERR_RANGE, lambda: kernels.paged_append(gpu_ctx, pool.kv, table, np.array([20, n, 3], np.int32),
                                                                 k.numpy(), k.numpy(), seq_start=start))
+
+
+@pytest.mark.parametrize("where", ["cpu", "cuda"])
+@pytest.mark.parametrize("pages", [0, 3])
+def test_a_batch_of_no_sequences(gpu_ctx, where, pages):
+    pool = Pool(gpu_ctx, 241, [20], F32, 16, 2, 64)
+    before = pool.k.clone()
+    new = lambda *shape, **kw: torch.zeros(*shape, device=where, **kw)
+    table, lens = new(0, pages, dtype=torch.int32), new(0, dtype=torch.int32)
+    q, k = new(0, 4, 64), new(0, 2, 64)
+    assert kernels.paged_append(gpu_ctx, pool.kv, table, lens, k, k, q=q) is q
+    assert kernels.paged_attention(gpu_ctx, pool.kv, table, lens, q, new(0, 4, 64)).numel() == 0
+    # tokens that are all padding
+    q = new(3, 4, 64) + 7.0
+    kernels.paged_append(gpu_ctx, pool.kv, table, lens, new(3, 2, 64), new(3, 2, 64), q=q,
+                         seq_start=new(1, dtype=torch.int32))
+    done(gpu_ctx)
+    assert torch.equal(pool.k, before) and bool((q == 7.0).all())
