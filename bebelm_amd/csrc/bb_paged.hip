@@ -190,6 +190,8 @@ __global__ void __launch_bounds__(RR_THREADS) k_rope_rows(RopeRows r, RopeTurns 
       if (u < units) load_vec<A, VE>(x + e0, a[m]);
       if (u < nu) load_vec<A, VE>(x + (rt.interleaved ? e0 + VE : e0 + half), b[m]);
     }
+    // (in place, a lane stores elements that its neighbour loads too: none may move up past the loads)
+    if constexpr (!EVEN) __builtin_amdgcn_wave_barrier();
     A* yq = static_cast<A*>(r.q_out) + t * r.qo_ts + (size_t)head * r.qo_hs;
     C* yc = static_cast<C*>(is_k ? kv.k : kv.v) + w.base + (size_t)head * kv.head_stride;
     if (is_q ? r.q_norm != nullptr : is_k && r.k_norm != nullptr) {
