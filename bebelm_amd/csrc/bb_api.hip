@@ -308,9 +308,10 @@ void need_ctx(bb_ctx* c) { need(c != nullptr, BB_ERR_ARG, "null context"); }
 
 void need_loc(int loc) { need(loc == BB_LOC_HOST || loc == BB_LOC_DEVICE, BB_ERR_ARG, "loc must be BB_LOC_HOST or BB_LOC_DEVICE"); }
 
-void need_aligned(const void* p, const char* what) {
+void need_aligned(const void* p, const char* what, size_t align = 16) {
   if (p == nullptr) fail(BB_ERR_ARG, std::string(what) + " is null");
-  if ((reinterpret_cast<uintptr_t>(p) & 15) != 0) fail(BB_ERR_ARG, std::string(what) + " must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(p) % align != 0)
+    fail(BB_ERR_ARG, std::string(what) + " must be " + std::to_string(align) + "-byte aligned");
 }
 
 size_t tensor_elems(const bb_tensor* t) {
@@ -652,6 +653,7 @@ struct Io {
   const void* host;
   size_t bytes;
   bool in, out;
+  size_t align = 16;  // of device memory
 };
 
 template <class F>
@@ -659,7 +661,7 @@ void with_io(bb_ctx* c, int loc, std::vector<Io> ios, F&& body) {
   std::vector<void*> dev(ios.size());
   if (loc == BB_LOC_DEVICE) {
     for (size_t i = 0; i < ios.size(); ++i) {
-      if (ios[i].bytes) need_aligned(ios[i].host, "device pointer");
+      if (ios[i].bytes) need_aligned(ios[i].host, "device pointer", ios[i].align);
       dev[i] = const_cast<void*>(ios[i].host);
     }
     body(dev);
@@ -2796,7 +2798,7 @@ int bb_rope(bb_ctx* c, const bb_rope_plan* plan, uint32_t dtype, const void* x, 
     const bool cap = (loc == BB_LOC_HOST || c->profile) && capturing(c);
     need(!(cap && loc == BB_LOC_HOST), BB_ERR_ARG, "a call on host memory cannot be captured");
     // (host memory: out's span goes in too, what lies between its rows stays as it is)
-    with_io(c, loc, {{x, nx, true, false}, {pos, n_tokens * 4, true, false}, {out, no, true, true}},
+    with_io(c, loc, {{x, nx, true, false}, {pos, n_tokens * 4, true, false, 4}, {out, no, true, true}},
             [&](std::vector<void*>& d) {
               bb::RopeRows r{};
               r.T = n_tokens;
@@ -2945,16 +2947,16 @@ int bb_paged_append(bb_ctx* c, bb_paged_kv* kv, const bb_rope_plan* plan, const 
     need(!(cap && loc == BB_LOC_HOST), BB_ERR_ARG, "a call on host memory cannot be captured");
     const size_t nt = span_bytes(B, sq->table_stride, sq->max_pages, 4);
     with_io(c, loc,
-            {{sq->page_table, nt, true, false},
-             {sq->lens, B * 4, true, false},
+            {{sq->page_table, nt, true, false, 4},
+             {sq->lens, B * 4, true, false, 4},
              {tk->k, nk, true, false},
              {tk->v, nv, true, false},
              {tk->q, nq, true, false},
              {tk->q_out, nqo, true, true},
-             {tk->q_norm, tk->q_norm ? hd * 4 : 0, true, false},
-             {tk->k_norm, tk->k_norm ? hd * 4 : 0, true, false},
-             {tk->pos, tk->pos ? T * 4 : 0, true, false},
-             {tk->seq_start, tk->seq_start ? (B + 1) * 4 : 0, true, false}},
+             {tk->q_norm, tk->q_norm ? hd * 4 : 0, true, false, 4},
+             {tk->k_norm, tk->k_norm ? hd * 4 : 0, true, false, 4},
+             {tk->pos, tk->pos ? T * 4 : 0, true, false, 4},
+             {tk->seq_start, tk->seq_start ? (B + 1) * 4 : 0, true, false, 4}},
             [&](std::vector<void*>& d) {
               bb::RopeRows r{};
               r.T = T;
@@ -3032,11 +3034,11 @@ int bb_paged_attention(bb_ctx* c, const bb_paged_kv* kv, const bb_paged_seqs* sq
     }
     const size_t nt = span_bytes(B, sq->table_stride, sq->max_pages, 4);
     with_io(c, loc,
-            {{sq->page_table, nt, true, false},
-             {sq->lens, B * 4, true, false},
+            {{sq->page_table, nt, true, false, 4},
+             {sq->lens, B * 4, true, false, 4},
              {pq->q, nq, true, false},
              {pq->out, no, true, true},
-             {pq->lse, nl, false, true}},
+             {pq->lse, nl, false, true, 4}},
             [&](std::vector<void*>& d) {
               bb::PagedQuery q{};
               q.q = d[2];

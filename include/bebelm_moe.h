@@ -330,7 +330,8 @@ int bb_model_absorb(bb_ctx* ctx, bb_model* m, bb_cache* cache, const uint32_t* t
  * `loc` says where the other arrays are. With BB_LOC_DEVICE the calls read the page table, lengths
  * and positions on the device only (the host never waits for them), so a captured call follows what
  * these arrays hold at each replay; with BB_LOC_HOST they are checked first (BB_ERR_RANGE) and the
- * call may not be captured. Arrays of 16-byte aligned device memory, as everywhere; strides are in
+ * call may not be captured. Device arrays are 16-byte aligned, as everywhere, but for those read word by
+ * word: page table, lengths, starts, positions, gains and lse begin at any word. Strides are in
  * elements, below 2^36. Arrays overlap where they share an element: rows of one may lie between rows of
  * another that are the same strides apart (q, k and v of one fused projection, q turned in place).
  * n_tokens (below 2^22) or n_seqs of 0: nothing is done. */

@@ -1129,3 +1129,37 @@ def test_a_batch_of_no_sequences(gpu_ctx, where, pages):
                          seq_start=new(1, dtype=torch.int32))
     done(gpu_ctx)
     assert torch.equal(pool.k, before) and bool((q == 7.0).all())
+
+
+def test_the_decode_part_of_a_mixed_batch(gpu_ctx):
+    """Index arrays, gains and sums as slices that begin at any word: three prompts' entries lie before those of the
+    sequences that take one step."""
+    pool = Pool(gpu_ctx, 251, [20, 37, 3, 40, 700, 18, 1], F32, 16, 1, 64, extra=2)
+    other = Pool(gpu_ctx, 251, [20, 37, 3, 40, 700, 18, 1], F32, 16, 1, 64, extra=2)
+    plan = RopePlan(gpu_ctx, 64, 1e6)
+    table = torch.zeros(7, pool.table.shape[1] + 1, dtype=torch.int32)
+    table[:, 1:] = pool.table
+    table, lens = table.cuda(), pool.lens.cuda()
+    pos = torch.arange(900, 907, dtype=torch.int32, device="cuda")
+    words = torch.arange(-1, 5, dtype=torch.int32, device="cuda")   # [1:]: 0, 1, 2, 3, 4
+    gains = (1 + 0.1 * torch.randn(129, generator=gen(252))).cuda()
+    q, k, v = (randn(253 + i, (4, n, 64), F32).cuda() for i, n in enumerate((3, 1, 1)))
+    lse = torch.full((7, 3), 7.0, device="cuda")
+    got = []
+    for p, own in ((pool, lambda x: x), (other, lambda x: x.clone())):
+        q_out, out = torch.empty_like(q), torch.empty_like(q)
+        sums = own(lse[3:])
+        assert own(lens[3:]).data_ptr() % 16 == (0 if p is other else 12)
+        torch.cuda.synchronize()
+        kernels.paged_append(gpu_ctx, p.kv, own(table[3:, 1:]), own(lens[3:]), k, v, rope=plan, pos=own(pos[3:]),
+                             seq_start=own(words[1:]), q=q, q_out=q_out, q_norm=own(gains[1:65]), k_norm=own(gains[65:]))
+        kernels.paged_attention(gpu_ctx, p.kv, own(table[3:, 1:]), own(lens[3:]), q_out, out, lse=sums)
+        x = kernels.rope(gpu_ctx, plan, q, own(pos[3:]), torch.empty_like(q))
+        done(gpu_ctx)
+        got.append((q_out, out, sums.clone(), x, p.k, p.v))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    assert bool((lse[:3] == 7.0).all()) and not bool((lse[3:] == 7.0).any())
+    # a word that begins inside another is refused
+    x = got[0][3]
+    assert _lib.lib().bb_rope(gpu_ctx.handle, plan.handle, F32, q.data_ptr(), 192, 64, 1, 3, 64, pos.data_ptr() + 2,
+                              x.data_ptr(), 192, 64, _lib.LOC_DEVICE) == _lib.BB_ERR_ARG
