@@ -385,10 +385,11 @@ int bb_paged_kv_pages(const bb_paged_kv* kv, void** k, void** v);
 
 /* The sequences of a batch: sequence s has lens[s] positions cached (those of the call's own tokens
  * included; 0: an empty place of the batch), position j in page page_table[s·table_stride +
- * j/page_size] (max_pages entries per sequence; those past its pages and before the positions that a
- * call stores or attends to are not read). On the device, a length is taken as at most
- * max_pages·page_size, and a page number outside the pool as a page whose positions are not there:
- * nothing is stored in it, nothing read. */
+ * j/page_size] (max_pages entries per sequence). Entries past a sequence's pages are not read, and those
+ * before the positions that a call stores or attends to make no difference, nor does what lies in the
+ * pages they name (attention may read a few of them before its window). On the device attention takes
+ * a length as at most max_pages·page_size, an append has no place for tokens past that, and a page
+ * number outside the pool is a page whose positions are not there: nothing is stored in it, nothing read. */
 typedef struct {
   size_t n_seqs;       /* at most 65536 */
   size_t max_pages;    /* at least 1; max_pages * page_size below 2^30 */
@@ -434,9 +435,10 @@ int bb_paged_append(bb_ctx* ctx, bb_paged_kv* kv, const bb_rope_plan* plan, cons
  * sequence with no position to attend to, and a head all of whose scores are -inf, gets zeros and
  * -inf. workspace: device memory of workspace_bytes >= bb_paged_attention_workspace's answer, for this
  * call alone while it runs; NULL takes the context's, which a captured call may not (a graph keeps the
- * address, the context's workspace grows: BB_ERR_ARG). A value that is attended to and is not finite makes
- * the elements of out that it reaches not finite (an infinite one may give NaN). The sums are taken in an order that the batch's
- * lengths fix, so equal calls give equal bits. */
+ * address, the context's workspace grows: BB_ERR_ARG); between calls that take it on two streams
+ * (bb_ctx_set_stream) the caller lets the first end. A value that is attended to and is not finite makes
+ * the elements of out that it reaches not finite (an infinite one may give NaN). The sums are taken in an
+ * order that the batch's lengths, max_pages and the window fix, so equal calls give equal bits. */
 typedef struct {
   uint32_t dtype; /* of q and out */
   const void* q;

@@ -1163,3 +1163,33 @@ def test_the_decode_part_of_a_mixed_batch(gpu_ctx):
     x = got[0][3]
     assert _lib.lib().bb_rope(gpu_ctx.handle, plan.handle, F32, q.data_ptr(), 192, 64, 1, 3, 64, pos.data_ptr() + 2,
                               x.data_ptr(), 192, 64, _lib.LOC_DEVICE) == _lib.BB_ERR_ARG
+
+
+# ---- windows over every form of page ---------------------------------------------------------------
+@pytest.mark.parametrize("page", [1, 5, 8, 13, 16, 24, 40])
+@pytest.mark.parametrize("ct,dt,hd", [(F32, F32, 64), (F16, F16, 80), (BF16, F32, 128), (BF16, BF16, 24)])
+def test_attention_window_over_other_pages(gpu_ctx, page, ct, dt, hd):
+    """Whole and odd pages, tiles of 16 and 32 positions: what lies before the window (and behind the last position)
+    makes no difference, be its pages in the pool and full of NaN, or gone."""
+    print("window", page, ct, dt, hd, flush=True)
+    lens = [700, 3, 0, 64, 17, 333, 130]
+    for window in (1, 31, 33, 100, 650):
+        pool = Pool(gpu_ctx, 261, lens, ct, page, 2, hd, fill=float("nan"))
+        hist = []
+        for s, n in enumerate(lens):
+            p, r = (i[max(0, n - window):] for i in pool.where(s))
+            kv = [randn(262 + 2 * s + i, (len(p), 2, hd), ct) for i in range(2)]
+            for x, h in zip((pool.k, pool.v), kv):
+                x[p.cuda(), r.cuda()] = h.cuda()
+            hist.append(kv)
+            if s % 2:
+                pool.table[s, :max(0, n - window) // page] = -1
+        q = randn(290, (len(lens), 6, hd), dt)
+        out, lse = attend(gpu_ctx, pool, q, window=window)
+        for s in range(len(lens)):
+            want, wl, tol, tl = attention64(q[s], hist[s], 1 / math.sqrt(hd))
+            close(out[s], want, tol * (1 + half_step(dt)) + half_step(dt) * want.abs() + TINY[dt], f"{window} out {s}")
+            if lens[s]:
+                close(lse[s], wl, tl + U * wl.abs(), f"{window} lse {s}")
+            else:
+                assert bool(torch.isneginf(lse[s]).all())
