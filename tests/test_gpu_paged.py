@@ -1193,3 +1193,67 @@ def test_attention_window_over_other_pages(gpu_ctx, page, ct, dt, hd):
                 close(lse[s], wl, tl + U * wl.abs(), f"{window} lse {s}")
             else:
                 assert bool(torch.isneginf(lse[s]).all())
+
+
+# ---- what the tests above leave out ----------------------------------------------------------------
+@pytest.mark.parametrize("low,high", [(1.0, 32.0), (0.25, 4.0), (0.0, 0.5), (8.0, 1000.0), (-3.0, 2.0), (1e5, 1e6)])
+def test_rope_parts_between_other_rotations(gpu_ctx, low, high):
+    more = {"factor": 16.0, "original_positions": 8192.0, "low_rotations": low, "high_rotations": high}
+    plan = RopePlan(gpu_ctx, 128, 1e4, scaling="parts", magnitude=1.5, **more)
+    f = frequencies(128, 1e4, "parts", **more)
+    x, pos = randn(301, (9, 2, 128), F32), torch.randint(0, 130_000, (9,), generator=gen(302), dtype=torch.int32)
+    out = torch.empty(9, 2, 128, device="cuda")
+    xd, pd = x.cuda(), pos.cuda()
+    torch.cuda.synchronize()
+    kernels.rope(gpu_ctx, plan, xd, pd, out)
+    done(gpu_ctx)
+    want, mag = turned(x, pos.numpy(), f, False, 1.5)
+    close(out, want, turn_tol(want, mag, pos.numpy(), f, F32), f"{low}..{high}")
+
+
+def test_append_with_starts_that_do_not_ascend(gpu_ctx):
+    """Device starts are not checked: a token's sequence is the number of sequences that end at or before it, its
+    place counts from that one's end, and nothing but such places is written."""
+    pool = Pool(gpu_ctx, 311, [20, 16, 33, 5], F32, 16, 2, 64)
+    start, lens, t = [0, 9, 2, 3, 4], [12, 2, 3, 4], 12
+    k, v = randn(312, (t, 2, 64), F32), randn(313, (t, 2, 64), F32)
+    want = [pool.k.cpu(), pool.v.cpu()]
+    for i in range(t):
+        s = sum(e <= i for e in start[1:])
+        at = lens[s] - start[s + 1] + i if s < 4 else -1
+        page = int(pool.table[s, at // 16]) if 0 <= at < 16 * pool.table.shape[1] else -1
+        if 0 <= page < pool.n_pages:
+            for w, x in zip(want, (k, v)):
+                w[page, at % 16] = x[i]
+    args = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in (lens, start)]
+    kd, vd, table = k.cuda(), v.cuda(), pool.table.cuda()
+    torch.cuda.synchronize()
+    kernels.paged_append(gpu_ctx, pool.kv, table, args[0], kd, vd, seq_start=args[1])
+    done(gpu_ctx)
+    assert torch.equal(pool.k.cpu(), want[0]) and torch.equal(pool.v.cpu(), want[1])
+
+
+def test_sums_past_32_bits(gpu_ctx):
+    """The log sums of pages past 2^32 elements, a long sequence split over many blocks among them."""
+    page, kv, hd = 64, 2, 64
+    n_pages = (1 << 32) // (page * kv * hd) + 200
+    pools = [torch.empty(n_pages, page, kv, hd, dtype=torch.float16, device="cuda") for _ in range(2)]
+    ids = torch.cat((torch.arange(n_pages - 150, n_pages), torch.tensor([0, 7, n_pages // 2])))
+    lens = [len(ids) * page - 11, 3 * page]
+    table = torch.full((2, len(ids)), -1, dtype=torch.int32)
+    table[0], table[1, :3] = ids, ids[-3:]
+    for i, x in enumerate(pools):
+        x[ids.cuda()] = randn(321 + i, (len(ids), page, kv, hd), F16).cuda()
+    pool = PagedKv(gpu_ctx, *pools)
+    q, out, lse = randn(323, (2, 8, hd), F16), torch.empty(2, 8, hd, dtype=torch.float16, device="cuda"), torch.empty(2, 8, device="cuda")
+    args = table.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"), q.cuda()
+    torch.cuda.synchronize()
+    kernels.paged_attention(gpu_ctx, pool, *args, out, lse=lse)
+    done(gpu_ctx)
+    for s, n in enumerate(lens):
+        pages = ids if s == 0 else ids[-3:]
+        hist = [x[pages.cuda()].cpu().flatten(0, 1)[:n] for x in pools]
+        want, wl, tol, tl = attention64(q[s], hist, 0.125)
+        close(out[s], want, tol * (1 + half_step(F16)) + half_step(F16) * want.abs() + TINY[F16], f"out {s}")
+        close(lse[s], wl, tl + U * wl.abs(), f"lse {s}")
+    pool.close()
