@@ -167,7 +167,8 @@ def _shuffled(seed, items):
 
 
 class _Program:
-    """What a process keeps: one context, its work on one torch stream."""
+    """What a process keeps: one context, and one torch stream that is the current one from its making on, so that
+    what fills the inputs, the calls and what reads their results are in order."""
     ctx = None
     stream = None
 
@@ -178,6 +179,8 @@ class _Program:
             cls.stream = torch.cuda.Stream()
             cls.ctx = Context(torch.cuda.current_device())
             cls.ctx.set_stream(cls.stream.cuda_stream)
+            cls.stream.wait_stream(torch.cuda.current_stream())
+            torch.cuda.set_stream(cls.stream)
         return cls.ctx
 
 
@@ -191,6 +194,8 @@ def _plan(case):
 def prepare(case, seed):
     kind, dtype, hd = case["kind"], case["dtype"], case["hd"]
     s = {"case": case}
+    if own:
+        _Program.context()   # (the inputs are made on its stream)
     if kind == "rope":
         t = case["tokens"]
         first = int(torch.randint(0, max(1, case["far"] - t), (1,), generator=_gen(seed, 14, "cpu")))
