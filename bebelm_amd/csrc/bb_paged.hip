@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <type_traits>
 #include "bb_internal.h"
+#include "bb_paged_plan.h"
 
 namespace bb {
 
@@ -61,10 +62,9 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
   }
 }
 
-// i / page_slots for 0 <= i < 2^31 (PagedView::page_mul = ceil(2^(31 + page_shift) / page_slots), page_shift
-// = ceil(log2(page_slots)): the product is off by less than i / 2^(31 + page_shift) < 1 / page_slots).
+// i / page_slots for 0 <= i < 2^31.
 __device__ __forceinline__ int page_of(const PagedView& kv, int i) {
-  return (int)(((uint64_t)(uint32_t)i * kv.page_mul) >> (31 + kv.page_shift));
+  return slot_quotient(i, kv.page_mul, kv.page_shift);
 }
 
 // ---- rotary positions, and the rows of an append ------------------------------------------------
@@ -343,28 +343,6 @@ hipError_t launch_rope_rows(hipStream_t s, int dtype, int cache, const RopeRows&
 namespace {
 
 constexpr int PA_WAVES = 4, PA_THREADS = 64 * PA_WAVES;
-// Positions of a unit (their logarithm): a tile for each wave. 64 and 256 are no faster (34 sequences of
-// up to 16384, 38.6 and 40.8 us where 128 gave 41.6; one of 9001, 15.1 and 14.2 for 14.5).
-constexpr int PA_UNIT = 7;
-// The same where no sequence reaches past one: no pair is split and nothing is to be joined, which costs
-// 4 to 5 us. By the bytes of a head's row (one sequence, 8 kv heads; whole and split): bf16, 64
-// elements: 512 positions 8.1 and 10.1 us, 1000 11.7 and 11.0; f32, 64: 512 10.4 and 10.9; f32, 256
-// elements (4 sequences): 256 17.9 and 19.1, 512 27.0 and 19.1.
-__host__ __device__ constexpr int pa_unit_short(int row_bytes) { return row_bytes <= 256 ? 9 : 8; }
-constexpr int PA_PAIR = 1;        // what a pair costs besides its units
-constexpr int PA_HEADS = 16;      // heads of a group at most
-// A pair of one tile is a wave's alone, and a pair of one unit where the block's run has this many of
-// them: nothing is then joined, and a block is in four pairs at once. 168 sequences of up to 62, 16 kv
-// heads of 256, 33 us (all waves on every pair: 58); 131 of up to 3, of 64, 8.4 and 13.6; 200 of up to
-// 500, 8 heads of 128, 28 and 36.
-constexpr int PA_ALONE = 2;
-// From this average cost of a pair on, one block a CU works (the others end at once): its loads fill the
-// memory's queues as well as four blocks' and disturb each other less. Batches of shorter pairs keep
-// all the blocks that fit, which hide each other's beginnings and ends. One a CU and all, 8 kv heads:
-// 64 sequences of 8192, 64 elements, bf16 191 and 199 us, f32 355 and 381; of 128, f16, 357 and 375; 100
-// sequences of 2000, of 64, f16, 85 and 92. Up to 2000, 128 sequences, 16 heads of 64: 59 and 44; up to
-// 700, 200 sequences, of 128: 50 and 41.
-constexpr int PA_LONG = 16;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr float NEG_INF = -__builtin_inff();
 
@@ -383,22 +361,8 @@ struct PagedPlan {
   float2* ml;     // [2·blocks][hg]: maximum (base 2), sum of weights
 };
 
-struct SeqSpan {
-  int base, first, len, units;  // positions first..len-1, counted from base; units >= 1
-};
-// (Positions as slots, see PaWave.)
 __device__ __forceinline__ SeqSpan seq_span(int raw_len, const PagedView& kv, int max_pages, int window, int unit) {
-  SeqSpan r;
-  r.len = min(max(raw_len, 0), max_pages * kv.page_size);
-  r.first = window > 0 ? max(0, r.len - window) : 0;
-  const int empty = kv.page_slots - kv.page_size;
-  if (empty > 0) {
-    r.first += (int)((uint32_t)r.first / (uint32_t)kv.page_size) * empty;
-    r.len += r.len > 0 ? (int)((uint32_t)(r.len - 1) / (uint32_t)kv.page_size) * empty : 0;
-  }
-  r.base = r.first & ~31;
-  r.units = max(1, (r.len - r.base + (1 << unit) - 1) >> unit);
-  return r;
+  return span_of(raw_len, kv.page_size, kv.page_slots, max_pages, window, unit);
 }
 
 // Four adjacent elements of a row of type dt, at any element's alignment.
@@ -481,20 +445,6 @@ __device__ __forceinline__ int wave_scan(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row 1's last lane, to rows 2 and 3
   return x;
 }
-
-// a / b for 0 <= a < 2^30, b >= 1 (the same for the wave): two steps of an f32 quotient, each off by less than
-// 2^-22 of itself and 1, then at most 1 off.
-__device__ __forceinline__ int uniform_div(int a, int b) {
-  const float inv = __builtin_amdgcn_rcpf((float)b);
-  int q = (int)((float)a * inv);
-  q += (int)((float)(a - q * b) * inv);
-  q -= q * b > a ? 1 : 0;
-  q += (q + 1) * b <= a ? 1 : 0;
-  return __builtin_amdgcn_readfirstlane(q);
-}
-
-// Waves of a SIMD that fit: 128, 256, 512 registers each.
-constexpr int pa_waves(int hdp) { return hdp == 64 ? 4 : hdp == 128 ? 2 : 1; }
 
 // A tile's shape: CT the cache's type, HDP the head size (or the next of 64, 128, 256).
 template <int CT, int HDP>
@@ -912,8 +862,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
           continue;
         }
         const int total = (before + sc.all) * pl.n_groups;
-        const int grid = before + sc.all >= PA_LONG * n_seqs ? min((int)gridDim.x, pl.few) : (int)gridDim.x;
-        const int chunk = total <= grid ? 1 : uniform_div(total + grid - 1, grid);
+        const int chunk = run_cost(before + sc.all, n_seqs, pl.n_groups, (int)gridDim.x, pl.few);
         if (pl.join && blockIdx.x == 0 && tid == 0) {
           pl.chunk[0] = chunk;
           pl.chunk[1] = 0;
@@ -961,11 +910,12 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
       len = __builtin_amdgcn_readfirstlane(lens[s]);
       cost = seq_span(len, kv, max_pages, pq.window, pl.unit).units + PA_PAIR;
     }
-    const int nu = cost - PA_PAIR, first_unit = lo + PA_PAIR;
-    const int u0 = max(u - first_unit, 0), take = min(nu, end - first_unit) - u0;
+    const int nu = cost - PA_PAIR;
+    const PairPart part = pair_part(u, end, lo, nu);
+    const int u0 = part.first, take = part.units;
     if (take <= 0) continue;  // (the run ends before the pair's units)
     const SeqSpan sp = seq_span(len, kv, max_pages, pq.window, pl.unit);
-    const bool alone = nu == 1 && (sp.len - sp.base <= S::KT || end - u >= PA_ALONE * (1 + PA_PAIR));
+    const bool alone = pair_alone(nu, sp, S::KT, end - u);
     if (alone && (turn++ & (PA_WAVES - 1)) != wv) continue;
     const int kvh = pl.split == 1 ? grp : uniform_div(grp, pl.split), sub = grp - kvh * pl.split;
     w.row = table + (size_t)s * table_stride;
@@ -1008,7 +958,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
     }
     __syncthreads();
     const bool whole = take == nu;
-    const size_t slot = 2 * (size_t)blockIdx.x + (u0 > 0 ? 0 : 1);
+    const size_t slot = partial_slot((int)blockIdx.x, u0 == 0);
     for (int i = tid; i < w.heads * ROW4; i += PA_THREADS) {
       const int h = i / ROW4, d = 4 * (i % ROW4);
       if (d >= kv.hd) continue;
@@ -1046,8 +996,8 @@ __global__ void __launch_bounds__(PJ_THREADS) k_paged_join(PagedQuery pq, int hd
   const int piece = (blockIdx.z - hh * blocks_of_row) * PJ_PIECES + threadIdx.x % PJ_PIECES;
   const int row = threadIdx.x / PJ_PIECES;
   const int chunk = pl.chunk[0], before = pl.chunk[1 + s], cost = pl.chunk[2 + s] - before;
-  const int lo = before * pl.n_groups + grp * cost + PA_PAIR, hi = lo + cost - PA_PAIR;
-  const int b0 = uniform_div(lo, chunk), b1 = uniform_div(hi - 1, chunk);
+  const PairBlocks blocks = pair_blocks(before * pl.n_groups + grp * cost, cost, chunk);
+  const int b0 = blocks.first, b1 = blocks.last;
   if (b0 == b1) return;  // whole in one block
   const int kvh = pl.split == 1 ? grp : grp / pl.split, in = (grp - kvh * pl.split) * pl.hg + hh, h = kvh * pl.G + in;
   if (in >= pl.G) return;  // (the last group of a kv head may have fewer heads)
@@ -1056,7 +1006,7 @@ __global__ void __launch_bounds__(PJ_THREADS) k_paged_join(PagedQuery pq, int hd
   v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
   for (int i = row; i < parts; i += PJ_ROWS) {
-    const size_t at = (2 * (size_t)(b0 + i) + (i == 0 ? 1 : 0)) * pl.hg + hh;
+    const size_t at = partial_slot(b0 + i, i == 0) * pl.hg + hh;
     const float2 ml = pl.ml[at];
     const v4f y = *reinterpret_cast<const v4f*>(pl.sums + at * hd + min(4 * piece, hd - 4));
     const float top = fmaxf(m, ml.x), ref = top == NEG_INF ? 0.0f : top;
@@ -1088,67 +1038,39 @@ __global__ void __launch_bounds__(PJ_THREADS) k_paged_join(PagedQuery pq, int hd
     pq.lse[(size_t)s * pq.n_heads + h] = none ? NEG_INF : (m + (__builtin_amdgcn_logf(l) - up)) * LN2;
 }
 
-int pa_class(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
-
-// Blocks that fit the device at once.
-
-PagedPlan pa_plan(int n_seqs, int n_heads, int n_kv) {
-  PagedPlan p{};
-  p.G = n_heads / n_kv;
-  p.split = (p.G + PA_HEADS - 1) / PA_HEADS;
-  p.hg = (p.G + p.split - 1) / p.split;
-  p.n_groups = n_kv * p.split;
-  return p;
-}
-
 }  // namespace
 
 bool paged_attn_fits(int n_seqs, int n_heads, int n_kv, size_t cap) {
-  const PagedPlan p = pa_plan(n_seqs, n_heads, n_kv);
-  // (up to 3 slots for 2 positions)
-  return (size_t)n_seqs * (size_t)p.n_groups * ((3 * cap / 2 >> PA_UNIT) + 1 + PA_PAIR) < ((size_t)1 << 29);
+  return head_groups(n_heads, n_kv).fits(n_seqs, cap);
 }
 
 void PagedView::set_slots(int n) {
+  const SlotDivision d = slot_division(n);
   page_slots = n;
-  page_shift = 0;
-  while ((1 << page_shift) < n) ++page_shift;
-  page_mul = (uint32_t)((((uint64_t)1 << (31 + page_shift)) + n - 1) / n);
+  page_mul = d.mul;
+  page_shift = d.shift;
 }
 
 size_t paged_attn_ws(int n_cu, int n_seqs, int n_heads, int n_kv, int hd) {
-  const PagedPlan p = pa_plan(n_seqs, n_heads, n_kv);
-  const size_t slots = 2 * (size_t)n_cu * pa_waves(pa_class(hd)) * p.hg;
+  const size_t slots = 2 * (size_t)blocks_at_once(n_cu, hd) * head_groups(n_heads, n_kv).hg;
   return slots * ((size_t)hd * 4 + sizeof(float2)) + ((size_t)n_seqs + 2) * 4;
 }
 
 hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQuery& q, const PagedView& pool,
                              const PagedSeqs& sq) {
   if (sq.n_seqs == 0) return hipSuccess;
-  PagedPlan pl = pa_plan(sq.n_seqs, q.n_heads, pool.n_kv);
+  const HeadGroups g = head_groups(q.n_heads, pool.n_kv);
+  const PagedCut cut = paged_cut(n_cu, sq.n_seqs, g.n_groups, pool.page_size, pool.pos_stride, sq.max_pages, q.window,
+                                 pool.hd, cache == BB_F32 ? 4 : 2);
+  const bool uni = cut.uni;
   PagedView kv = pool;
-  const size_t slots16 = ((size_t)kv.page_size + 15) / 16 * 16;
-  const bool uni = 2 * slots16 <= 3 * (size_t)kv.page_size && 16 * kv.pos_stride < ((size_t)1 << 29);
-  if (uni) kv.set_slots((int)slots16);
-  // slots of a sequence that count, at most (a window begins anywhere in a page, and its slots anywhere in 32)
-  size_t cap = (size_t)sq.max_pages * kv.page_slots;
-  if (q.window > 0) {
-    const size_t pages = ((size_t)q.window + kv.page_size - 1) / kv.page_size + 1;
-    cap = std::min(cap, std::min((size_t)q.window + pages * (kv.page_slots - kv.page_size), pages * kv.page_slots) + 31);
-  }
-  const size_t pairs = (size_t)sq.n_seqs * pl.n_groups;
-  const int blocks_max = n_cu * pa_waves(pa_class(kv.hd));
-  pl.few = uni ? n_cu : blocks_max;
-  const size_t slots = 2 * (size_t)blocks_max * pl.hg;
+  if (uni) kv.set_slots(cut.slots);
+  PagedPlan pl{g.G, g.split, g.hg, g.n_groups, cut.join, cut.unit, cut.few, nullptr, nullptr, nullptr};
+  const size_t slots = 2 * (size_t)blocks_at_once(n_cu, kv.hd) * pl.hg;
   pl.sums = static_cast<float*>(q.ws);
   pl.ml = reinterpret_cast<float2*>(pl.sums + slots * kv.hd);
   pl.chunk = reinterpret_cast<int*>(pl.ml + slots);
-  // (pairs of one unit take a block each at most, longer ones a block for each unit)
-  const int unit_short = pa_unit_short(kv.hd * (cache == BB_F32 ? 4 : 2));
-  pl.unit = cap <= (size_t)1 << unit_short ? unit_short : PA_UNIT;
-  const size_t units = ((cap - 1) >> pl.unit) + 1;
-  const unsigned blocks = (unsigned)std::min<size_t>(blocks_max, pairs * (units == 1 ? 1 : units + PA_PAIR));
-  pl.join = units > 1;
+  const unsigned blocks = (unsigned)cut.blocks;
   const int cls = pa_class(kv.hd);
   const size_t lds = (size_t)PA_WAVES * pl.hg * (cls + 4) * 4;
 #define BB_PA(ct, np, hdp)                                                                                     \
