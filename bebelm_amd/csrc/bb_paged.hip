@@ -314,7 +314,7 @@ hipError_t launch_rope_rows(hipStream_t s, int dtype, int cache, const RopeRows&
 // maximum and sum of the softmax. Bound by the cache's bytes: one kv head's keys and values are read
 // once for the (up to 16) query heads of a group, and nothing but sums leaves the registers.
 //
-// 64 sequences of 8192, 32 query on 8 kv heads of 128, f16: 357 us, 6.0 TB/s; one sequence of 9001, of 64,
+// 64 sequences of 8192, 32 query on 8 kv heads of 128, f16: 357 to 368 us, 5.8 to 6.0 TB/s; one sequence of 9001, of 64,
 // bf16: 13 us, of which 4 are the second launch and 3 pass until the first keys are asked for.
 //
 // Work. A sequence's positions (from its window's first, rounded down to 32) are cut into units of 128,
@@ -629,7 +629,8 @@ struct PaWave {
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          // (pieces past the head end in elements of o that nobody reads)
+          // (pieces past the head end in elements of o that nobody reads; what they fetch counts: 7 sequences with 16
+          // heads of 80 fetch 59.9 MB, their keys and values are 31.7)
           const uint32_t at = 4 * g + r < skip ? 0x80000000u : (uint32_t)(4 * g + r) * stride() + (uint32_t)(n * PE * SZ);
 #pragma unroll
           for (int j = 0; j < NV; ++j) {

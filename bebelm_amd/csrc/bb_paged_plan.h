@@ -52,13 +52,15 @@ BB_BOTH int uniform_div(int a, int b) {
 }
 
 // ---- pairs and units ------------------------------------------------------------------------------
-// Positions of a unit (their logarithm): a tile for each wave. 64 and 256 are no faster (34 sequences of
-// up to 16384, 38.6 and 40.8 us where 128 gave 41.6; one of 9001, 15.1 and 14.2 for 14.5).
+// Positions of a unit (their logarithm): a 16-bit tile for each wave, two f32 ones. Of 64, 128 and 256, calls: 34
+// sequences of up to 16384, bf16, 50.7, 41.2 and 42.0 us; one of 9001, 15.1, 13.7, 14.5; 7 of up to 3001, heads of
+// 80, f16, 23.7, 20.8, 21.4; 2 of the last 100000, one kv head, 27.1, 25.9, 26.4; 64 of 8192, 368 each. f32 alone is
+// a little faster with 64: 24 of up to 4096 with their append 26.4, 27.1, 28.3.
 constexpr int PA_UNIT = 7;
-// The same where no sequence reaches past one: no pair is split and nothing is to be joined, which costs
-// 4 to 5 us. By the bytes of a head's row (one sequence, 8 kv heads; whole and split): bf16, 64
-// elements: 512 positions 8.1 and 10.1 us, 1000 11.7 and 11.0; f32, 64: 512 10.4 and 10.9; f32, 256
-// elements (4 sequences): 256 17.9 and 19.1, 512 27.0 and 19.1.
+// The same where no sequence can reach past one, by the table's width and the window (the launch knows no length):
+// no pair is split and nothing is to be joined, which costs 4 to 5 us. By the bytes of a head's row (one sequence,
+// 8 kv heads; whole and split): bf16, 64 elements: 512 positions 8.1 and 10.1 us, 1000 11.7 and 11.0; f32,
+// 64: 512 10.4 and 10.9; f32, 256 elements (4 sequences): 256 17.9 and 19.1, 512 27.0 and 19.1.
 constexpr int pa_unit_short(int row_bytes) { return row_bytes <= 256 ? 9 : 8; }
 constexpr int PA_PAIR = 1;        // what a pair costs besides its units
 constexpr int PA_HEADS = 16;      // heads of a group at most
@@ -71,11 +73,15 @@ constexpr int PA_ALONE = 2;
 // memory's queues as well as four blocks' and disturb each other less. Batches of shorter pairs keep
 // all the blocks that fit, which hide each other's beginnings and ends. One a CU and all, 8 kv heads:
 // 64 sequences of 8192, 64 elements, bf16 191 and 199 us, f32 355 and 381; of 128, f16, 357 and 375; 100
-// sequences of 2000, of 64, f16, 85 and 92. Up to 2000, 128 sequences, 16 heads of 64: 59 and 44; up to
-// 700, 200 sequences, of 128: 50 and 41.
+// sequences of 2000, of 64, f16, 85 and 92; one of 9001, of 64, bf16, 13.7 and 15.8; 2 of 100000, one kv head of 128,
+// 25.9 and 28.4. Up to 2000, 128 sequences, 16 heads of 64: 59 and 44; up to 700, 200 sequences, of 128: 50 and 41;
+// 7 of up to 3001, 16 heads of 80, 22.4 and 20.8. Near the threshold the average (which knows neither how many pairs there
+// are nor how unlike) misses by 4%: 34 of up to 16384 (18) 41.0 and 39.9; 24 of up to 4096, f32 (7) 26.1 and 27.2.
 constexpr int PA_LONG = 16;
 
-// Waves of a SIMD that fit: 128, 256, 512 registers each.
+// Waves of a SIMD that fit: 128, 256, 512 registers each. (The forms with heads of up to 64 fill theirs: f32 queries on a
+// bf16 cache, and all 16-bit caches of odd pages, spill 12 to 24 of them, at a pair's beginning and end, none in the loop
+// over tiles.)
 constexpr int pa_waves(int hdp) { return hdp == 64 ? 4 : hdp == 128 ? 2 : 1; }
 constexpr int pa_class(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 inline int blocks_at_once(int n_cu, int hd) { return n_cu * pa_waves(pa_class(hd)); }

@@ -392,7 +392,8 @@ int bb_paged_kv_pages(const bb_paged_kv* kv, void** k, void** v);
  * number outside the pool is a page whose positions are not there: nothing is stored in it, nothing read. */
 typedef struct {
   size_t n_seqs;       /* at most 65536 */
-  size_t max_pages;    /* at least 1; max_pages * page_size below 2^30 */
+  size_t max_pages;    /* at least 1; max_pages * page_size below 2^30. Attention chooses its launches by it, not by the
+                        * lengths: a table of 256 positions and less takes one launch, a wider one two */
   size_t table_stride; /* >= max_pages */
   const int32_t* page_table;
   const int32_t* lens;
