@@ -257,7 +257,7 @@ def paged_append(ctx, kv, page_table, lens, k, v, rope=None, pos=None, seq_start
     """Stores k and v [tokens, n_kv_heads, head_dim] at the end of their sequences in the PagedKv's
     pages; on the way k (and q [tokens, n_heads, head_dim], into q_out, q itself by default) is normed
     with k_norm (q_norm) and turned as the RopePlan `rope` says, by pos int32 [tokens] or each token's
-    index in its sequence. page_table int32 [sequences, pages] and lens int32 [sequences] count the
+    index in its sequence. q, k and v may be slices of one projection's rows. page_table int32 [sequences, pages] and lens int32 [sequences] count the
     call's tokens; seq_start int32 [sequences + 1] says which tokens each sequence brings (None: one
     each). Returns q_out."""
     t, hd, nkv, code = k.shape[0], kv.head_dim, kv.n_kv_heads, _floating(k, "k")

@@ -439,7 +439,9 @@ int bb_paged_append(bb_ctx* ctx, bb_paged_kv* kv, const bb_rope_plan* plan, cons
  * address, the context's workspace grows: BB_ERR_ARG); between calls that take it on two streams
  * (bb_ctx_set_stream) the caller lets the first end. A value that is attended to and is not finite makes
  * the elements of out that it reaches not finite (an infinite one may give NaN). The sums are taken in an
- * order that the batch's lengths, max_pages and the window fix, so equal calls give equal bits. */
+ * order that the batch's lengths, max_pages and the window fix, so equal calls give equal bits. One call
+ * takes n_seqs·n_kv_heads·ceil(n_heads / n_kv_heads / 16)·(3·max_pages·page_size / 256 + 2) below 2^29
+ * (BB_ERR_RANGE: cut the batch). */
 typedef struct {
   uint32_t dtype; /* of q and out */
   const void* q;

@@ -1257,3 +1257,21 @@ def test_sums_past_32_bits(gpu_ctx):
         close(out[s], want, tol * (1 + half_step(F16)) + half_step(F16) * want.abs() + TINY[F16], f"out {s}")
         close(lse[s], wl, tl + U * wl.abs(), f"lse {s}")
     pool.close()
+
+
+def test_a_batch_too_large_to_count_is_refused(gpu_ctx):
+    """65536 sequences of 8 kv heads under a table of 2^17 positions; half of them are served."""
+    pool = torch.zeros(2, 16, 8, 8, device="cuda"), torch.zeros(2, 16, 8, 8, device="cuda")
+    kv = PagedKv(gpu_ctx, *pool)
+    n = 65536
+    table, lens = torch.zeros(n, 8192, dtype=torch.int32, device="cuda"), torch.zeros(n, dtype=torch.int32, device="cuda")
+    q, out = torch.ones(n, 8, 8, device="cuda"), torch.full((n, 8, 8), 7.0, device="cuda")
+    refused(_lib.BB_ERR_RANGE, lambda: kernels.paged_attention(gpu_ctx, kv, table, lens, q, out))
+    done(gpu_ctx)
+    assert bool((out == 7.0).all())
+    half = n // 2
+    lens[half - 1] = 16
+    torch.cuda.synchronize()
+    kernels.paged_attention(gpu_ctx, kv, table[:half], lens[:half], q[:half], out[:half])
+    done(gpu_ctx)
+    assert bool((out[:half] == 0.0).all()) and bool((out[half:] == 7.0).all())
