@@ -64,6 +64,11 @@ PAGED_SEQS = struct.Struct("@NNNPP")
 PAGED_TOKENS = struct.Struct("@NIPPNNPPNNNPPfPP")
 # dtype, q, out, n_heads, q_stride, out_stride, scale, window, lse, workspace, workspace_bytes
 PAGED_QUERY = struct.Struct("@IPPNNNfNPPN")
+# bb_paged_queries: n_tokens, dtype, q, out, n_heads, q_stride, out_stride, scale, cap, window, slopes, prefix, seq_start,
+# lse, workspace, workspace_bytes
+PAGED_QUERIES = struct.Struct("@NIPPNNNffNPPPPPN")
+# bb_paged_rows: n_tokens, dtype, k, v, k_stride, v_stride, seq_start
+PAGED_ROWS = struct.Struct("@NIPPNNP")
 
 
 class GgufTensorInfo(ctypes.Structure):
@@ -153,6 +158,12 @@ _SIGS = {
     "bb_paged_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int]),
     "bb_paged_attention_workspace": (c_int, [c_void_p, c_void_p, c_size_t, c_size_t, P(c_size_t)]),
     "bb_paged_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int]),
+    "bb_paged_kv4_bytes": (c_int, [c_size_t, c_size_t, P(c_size_t)]),
+    "bb_paged_kv_view4": (c_int, [c_void_p, c_void_p, c_void_p, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t,
+                                  c_size_t, P(c_void_p)]),
+    "bb_paged_read": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int]),
+    "bb_paged_prompt_attention_workspace": (c_int, [c_void_p, c_void_p, c_size_t, c_size_t, c_size_t, P(c_size_t)]),
+    "bb_paged_prompt_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int]),
     "bb_gguf_open": (c_int, [ctypes.c_char_p, P(c_void_p)]),
     "bb_gguf_open_bytes": (c_int, [c_void_p, c_size_t, P(c_void_p)]),
     "bb_gguf_close": (c_int, [c_void_p]),

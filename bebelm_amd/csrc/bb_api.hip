@@ -16,6 +16,7 @@
 
 #include "../../include/bebelm_moe.h"
 #include "bb_internal.h"
+#include "bb_paged4.h"
 #include "bb_rows.h"
 
 namespace {
@@ -2666,8 +2667,9 @@ bb_paged_kv* new_pool(bb_ctx* c, uint32_t dtype, void* k, void* v, size_t n_page
   p->dtype = dtype;
   p->view = {k, v, page_stride, pos_stride, head_stride, (int)n_pages, (int)page_size, (int)n_kv, (int)hd};
   p->view.set_slots((int)page_size);
-  p->span = ((n_pages - 1) * page_stride + (page_size - 1) * pos_stride + (n_kv - 1) * head_stride + hd) *
-            (dtype == BB_F32 ? 4 : 2);
+  p->span = dtype == BB_KV4 ? (n_pages - 1) * page_stride + (n_kv - 1) * head_stride + bb::kv4_chunk(page_size, hd)
+                            : ((n_pages - 1) * page_stride + (page_size - 1) * pos_stride + (n_kv - 1) * head_stride + hd) *
+                                  (dtype == BB_F32 ? 4 : 2);
   p->own = own;
   return p;
 }
@@ -2685,6 +2687,56 @@ void need_pool_sizes(size_t n_pages, size_t page_size, size_t n_kv, size_t hd) {
   need(hd % 8 == 0 && hd <= (size_t)bb::OPS_HD_MAX, BB_ERR_SHAPE, "head_dim must be a multiple of 8, at most 256");
   need(n_pages < ((size_t)1 << 31) && page_size < ((size_t)1 << 20) && n_kv <= 4096, BB_ERR_RANGE,
        "pool sizes beyond 2^31 pages, 2^20 positions a page or 4096 heads");
+}
+
+// A caller's pool: pieces of `piece` elements, the steps between them and how many there are of each.
+void need_view(void* k, void* v, size_t eb, size_t piece, std::vector<std::pair<size_t, size_t>> dims) {
+  need_aligned(k, "keys");
+  need_aligned(v, "values");
+  for (auto& d : dims) {
+    if (d.second == 1) d.first = 0;  // never stepped
+    need(d.first < STRIDE_MAX, BB_ERR_RANGE, "strides must be below 2^36 elements");
+    need(d.first * eb % 16 == 0, BB_ERR_ARG, "strides must be whole 16-byte pieces");
+  }
+  // (the values are one more step of two from the keys)
+  const uintptr_t ka = reinterpret_cast<uintptr_t>(k), va = reinterpret_cast<uintptr_t>(v);
+  dims.push_back({(ka < va ? va - ka : ka - va) / eb, 2});
+  std::sort(dims.begin(), dims.end());
+  size_t span = piece;
+  for (const auto& d : dims) {
+    if (d.second == 1) continue;
+    need(d.first >= span, BB_ERR_ARG, "strides put two elements in one place");
+    need(d.second - 1 <= (SPAN_MAX - span) / d.first, BB_ERR_RANGE, "pool too large");
+    span += (d.second - 1) * d.first;
+  }
+}
+
+void need_kv4(size_t hd) { need(hd % 32 == 0, BB_ERR_SHAPE, "a 4-bit pool's head_dim must be a multiple of 32"); }
+
+// What seq_start says where it is host memory: ascending from 0, up to the call's tokens.
+void need_starts(const int32_t* start, size_t n_seqs, size_t n_tokens) {
+  need(n_seqs <= PAGED_SEQS_MAX, BB_ERR_RANGE, "more than 65536 sequences");
+  need(start[0] == 0, BB_ERR_RANGE, "seq_start must start at 0");
+  for (size_t s = 0; s < n_seqs; ++s)
+    need(start[s + 1] >= start[s] && (size_t)start[s + 1] <= n_tokens, BB_ERR_RANGE, "seq_start must ascend, up to n_tokens");
+}
+// How many tokens sequence s of length n brings, no more than it has.
+int64_t tokens_of(const int32_t* start, size_t s, int64_t n) {
+  const int64_t bring = start ? start[s + 1] - start[s] : std::min<int64_t>(n, 1);
+  need(bring <= n, BB_ERR_RANGE, "a sequence is shorter than its tokens");
+  return bring;
+}
+
+size_t prompt_ws(bb_ctx* c, const bb_paged_kv* kv, size_t n_heads, size_t n_seqs, size_t n_tokens) {
+  const size_t n_kv = (size_t)kv->view.n_kv;
+  need(n_heads >= 1 && n_heads % n_kv == 0, BB_ERR_ARG, "n_heads must be a multiple of n_kv_heads");
+  need(n_heads < ((size_t)1 << 16), BB_ERR_RANGE, "n_heads must be below 65536");
+  need(n_seqs <= PAGED_SEQS_MAX, BB_ERR_RANGE, "more than 65536 sequences");
+  need(n_tokens < ((size_t)1 << 22), BB_ERR_RANGE, "n_tokens must be below 2^22");
+  // (rows of a kv head are 31-bit numbers, threads of a launch 32-bit ones)
+  need(n_tokens * n_heads / 32 + n_seqs * n_kv < ((size_t)1 << 24) && n_tokens * (n_heads / n_kv) < ((size_t)1 << 31),
+       BB_ERR_RANGE, "tokens times heads beyond what one call takes");
+  return bb::paged_prompt_ws(c->n_cu, (int)kv->dtype, n_tokens, n_seqs, (int)n_heads, (int)n_kv, kv->view.hd);
 }
 
 size_t paged_ws(bb_ctx* c, const bb_paged_kv* kv, size_t n_heads, size_t n_seqs) {
@@ -2823,9 +2875,12 @@ int bb_paged_kv_create(bb_ctx* c, uint32_t dtype, size_t n_pages, size_t page_si
   return guard([&] {
     need_ctx(c);
     need(out != nullptr, BB_ERR_ARG, "out is null");
-    const size_t eb = elem_bytes(dtype, "pool");
+    const bool four = dtype == BB_KV4;
+    const size_t eb = four ? 1 : elem_bytes(dtype, "pool");
     need_pool_sizes(n_pages, page_size, n_kv_heads, head_dim);
-    const size_t page = page_size * n_kv_heads * head_dim;
+    if (four) need_kv4(head_dim);
+    const size_t chunk = four ? bb::kv4_chunk(page_size, head_dim) : 0;
+    const size_t page = four ? n_kv_heads * chunk : page_size * n_kv_heads * head_dim;
     need(n_pages * (page >> 10) < ((size_t)1 << 40), BB_ERR_RANGE, "pool too large");  // (below 2^61)
     const size_t half = round_up(n_pages * page * eb, 256);
     set_device(c);
@@ -2833,8 +2888,8 @@ int bb_paged_kv_create(bb_ctx* c, uint32_t dtype, size_t n_pages, size_t page_si
     auto* dev = static_cast<uint8_t*>(dev_alloc(2 * half));
     try {
       clear_dev(c, dev, 2 * half);
-      *out = new_pool(c, dtype, dev, dev + half, n_pages, page_size, n_kv_heads, head_dim, page, n_kv_heads * head_dim,
-                      head_dim, dev);
+      *out = new_pool(c, dtype, dev, dev + half, n_pages, page_size, n_kv_heads, head_dim, page,
+                      four ? 0 : n_kv_heads * head_dim, four ? chunk : head_dim, dev);
     } catch (...) {
       (void)hipFree(dev);
       throw;
@@ -2849,29 +2904,30 @@ int bb_paged_kv_view(bb_ctx* c, uint32_t dtype, void* k, void* v, size_t n_pages
     need(out != nullptr, BB_ERR_ARG, "out is null");
     const size_t eb = elem_bytes(dtype, "pool");
     need_pool_sizes(n_pages, page_size, n_kv_heads, head_dim);
-    need_aligned(k, "keys");
-    need_aligned(v, "values");
-    // (the values are a fourth step of two from the keys)
-    const uintptr_t ka = reinterpret_cast<uintptr_t>(k), va = reinterpret_cast<uintptr_t>(v);
-    const size_t apart = (ka < va ? va - ka : ka - va) / eb;
-    std::pair<size_t, size_t> dims[4] = {
-        {page_stride, n_pages}, {pos_stride, page_size}, {head_stride, n_kv_heads}, {apart, 2}};
-    for (int i = 0; i < 3; ++i) {
-      auto& d = dims[i];
-      if (d.second == 1) d.first = 0;  // never stepped
-      need(d.first < STRIDE_MAX, BB_ERR_RANGE, "strides must be below 2^36 elements");
-      need(d.first * eb % 16 == 0, BB_ERR_ARG, "strides must be whole 16-byte pieces");
-    }
-    std::sort(dims, dims + 4);
-    size_t span = head_dim;
-    for (const auto& d : dims) {
-      if (d.second == 1) continue;
-      need(d.first >= span, BB_ERR_ARG, "strides put two elements in one place");
-      need(d.second - 1 <= (SPAN_MAX - span) / d.first, BB_ERR_RANGE, "pool too large");
-      span += (d.second - 1) * d.first;
-    }
+    need_view(k, v, eb, head_dim, {{page_stride, n_pages}, {pos_stride, page_size}, {head_stride, n_kv_heads}});
     *out = new_pool(c, dtype, k, v, n_pages, page_size, n_kv_heads, head_dim, page_stride, pos_stride, head_stride,
                     nullptr);
+  });
+}
+
+int bb_paged_kv4_bytes(size_t page_size, size_t head_dim, size_t* bytes) {
+  return guard([&] {
+    need(bytes != nullptr, BB_ERR_ARG, "bytes is null");
+    need_pool_sizes(1, page_size, 1, head_dim);
+    need_kv4(head_dim);
+    *bytes = bb::kv4_chunk(page_size, head_dim);
+  });
+}
+
+int bb_paged_kv_view4(bb_ctx* c, void* k, void* v, size_t n_pages, size_t page_size, size_t n_kv_heads, size_t head_dim,
+                      size_t page_stride, size_t head_stride, bb_paged_kv** out) {
+  return guard([&] {
+    need_ctx(c);
+    need(out != nullptr, BB_ERR_ARG, "out is null");
+    need_pool_sizes(n_pages, page_size, n_kv_heads, head_dim);
+    need_kv4(head_dim);
+    need_view(k, v, 1, bb::kv4_chunk(page_size, head_dim), {{page_stride, n_pages}, {head_stride, n_kv_heads}});
+    *out = new_pool(c, BB_KV4, k, v, n_pages, page_size, n_kv_heads, head_dim, page_stride, 0, head_stride, nullptr);
   });
 }
 
@@ -2904,18 +2960,8 @@ int bb_paged_append(bb_ctx* c, bb_paged_kv* kv, const bb_rope_plan* plan, const 
     const size_t T = tk->n_tokens, B = sq->n_seqs, hd = (size_t)kv->view.hd, row = (size_t)kv->view.n_kv * hd;
     const size_t eb = elem_bytes(tk->dtype, "tokens");
     need(T < ((size_t)1 << 22), BB_ERR_RANGE, "n_tokens must be below 2^22");
-    if (loc == BB_LOC_HOST && tk->seq_start && B > 0) {
-      need(B <= PAGED_SEQS_MAX, BB_ERR_RANGE, "more than 65536 sequences");
-      need(tk->seq_start[0] == 0, BB_ERR_RANGE, "seq_start must start at 0");
-      for (size_t s = 0; s < B; ++s)
-        need(tk->seq_start[s + 1] >= tk->seq_start[s] && (size_t)tk->seq_start[s + 1] <= T, BB_ERR_RANGE,
-             "seq_start must ascend, up to n_tokens");
-    }
-    need_seqs(kv, sq, loc, [&](size_t s, int64_t n) {
-      const int64_t bring = tk->seq_start ? tk->seq_start[s + 1] - tk->seq_start[s] : std::min<int64_t>(n, 1);
-      need(bring <= n, BB_ERR_RANGE, "a sequence is shorter than its tokens");
-      return n - bring;
-    });
+    if (loc == BB_LOC_HOST && tk->seq_start && B > 0) need_starts(tk->seq_start, B, T);
+    need_seqs(kv, sq, loc, [&](size_t s, int64_t n) { return n - tokens_of(tk->seq_start, s, n); });
     if (plan) need_plan(c, plan, hd);
     if (!tk->seq_start) need(T == B, BB_ERR_SHAPE, "without seq_start every sequence has one token");
     if (T == 0 || B == 0) return;
@@ -3003,6 +3049,7 @@ int bb_paged_attention(bb_ctx* c, const bb_paged_kv* kv, const bb_paged_seqs* sq
     const size_t B = sq->n_seqs, hd = (size_t)kv->view.hd, nh = pq->n_heads, row = nh * hd;
     const size_t eb = elem_bytes(pq->dtype, "query");
     const size_t want = paged_ws(c, kv, nh, B);
+    need(kv->dtype != BB_KV4, BB_ERR_DTYPE, "a 4-bit pool");
     need_seqs(kv, sq, loc, [&](size_t, int64_t n) {
       return pq->window > 0 && pq->window < (size_t)n ? n - (int64_t)pq->window : 0;
     });
@@ -3054,6 +3101,144 @@ int bb_paged_attention(bb_ctx* c, const bb_paged_kv* kv, const bb_paged_seqs* sq
               launch_paged(c, cap, bb::K_PAGED_ATTN, [&] {
                 return bb::launch_paged_attn(c->stream, c->n_cu, (int)kv->dtype, q, kv->view,
                                              seqs_of(sq, d[0], d[1]));
+              });
+            });
+  });
+}
+
+int bb_paged_read(bb_ctx* c, const bb_paged_kv* kv, const bb_paged_seqs* sq, const bb_paged_rows* rw, int loc) {
+  return guard([&] {
+    need_ctx(c);
+    need_loc(loc);
+    need_pool(c, kv);
+    need(sq && rw, BB_ERR_ARG, "null argument");
+    const size_t T = rw->n_tokens, B = sq->n_seqs, row = (size_t)kv->view.n_kv * (size_t)kv->view.hd;
+    const size_t eb = elem_bytes(rw->dtype, "rows");
+    need(T < ((size_t)1 << 22), BB_ERR_RANGE, "n_tokens must be below 2^22");
+    if (loc == BB_LOC_HOST && rw->seq_start && B > 0) need_starts(rw->seq_start, B, T);
+    need_seqs(kv, sq, loc, [&](size_t s, int64_t n) { return n - tokens_of(rw->seq_start, s, n); });
+    if (!rw->seq_start) need(T == B, BB_ERR_SHAPE, "without seq_start every sequence has one token");
+    if (T == 0 || B == 0 || (!rw->k && !rw->v)) return;
+    const size_t ks = rw->k ? rw->k_stride : row, vs = rw->v ? rw->v_stride : row;
+    need(T == 1 || (ks >= row && vs >= row), BB_ERR_ARG, "k_stride or v_stride below a token's row");
+    need(ks < STRIDE_MAX && vs < STRIDE_MAX, BB_ERR_RANGE, "strides must be below 2^36 elements");
+    const size_t nk = rw->k ? span_bytes(T, ks, row, eb) : 0, nv = rw->v ? span_bytes(T, vs, row, eb) : 0;
+    need(!rw->k || !rw->v || !rows_overlap(rows_of(rw->k, T, ks, row, eb), rows_of(rw->v, T, vs, row, eb)), BB_ERR_ARG,
+         "the keys overlap the values");
+    need_off_pool(kv, loc, {{rw->k, nk}, {rw->v, nv}});
+    set_device(c);
+    const bool cap = (loc == BB_LOC_HOST || c->profile) && capturing(c);
+    need(!(cap && loc == BB_LOC_HOST), BB_ERR_ARG, "a call on host memory cannot be captured");
+    // (host memory: the rows' spans go in too, what is not written stays as it is)
+    with_io(c, loc,
+            {{sq->page_table, span_bytes(B, sq->table_stride, sq->max_pages, 4), true, false, 4},
+             {sq->lens, B * 4, true, false, 4},
+             {rw->k, nk, true, true},
+             {rw->v, nv, true, true},
+             {rw->seq_start, rw->seq_start ? (B + 1) * 4 : 0, true, false, 4}},
+            [&](std::vector<void*>& d) {
+              bb::ReadRows r{};
+              r.T = T;
+              r.k = nk ? d[2] : nullptr;
+              r.v = nv ? d[3] : nullptr;
+              r.k_ts = ks;
+              r.v_ts = vs;
+              r.seq_start = rw->seq_start ? static_cast<const int32_t*>(d[4]) : nullptr;
+              launch_paged(c, cap, bb::K_PAGED_READ, [&] {
+                return bb::launch_paged_read(c->stream, (int)rw->dtype, (int)kv->dtype, r, kv->view, seqs_of(sq, d[0], d[1]));
+              });
+            });
+  });
+}
+
+int bb_paged_prompt_attention_workspace(bb_ctx* c, const bb_paged_kv* kv, size_t n_heads, size_t n_seqs, size_t n_tokens,
+                                        size_t* bytes) {
+  return guard([&] {
+    need_ctx(c);
+    need_pool(c, kv);
+    need(bytes != nullptr, BB_ERR_ARG, "bytes is null");
+    *bytes = prompt_ws(c, kv, n_heads, n_seqs, n_tokens);
+  });
+}
+
+int bb_paged_prompt_attention(bb_ctx* c, const bb_paged_kv* kv, const bb_paged_seqs* sq, const bb_paged_queries* pq,
+                              int loc) {
+  return guard([&] {
+    need_ctx(c);
+    need_loc(loc);
+    need_pool(c, kv);
+    need(sq && pq, BB_ERR_ARG, "null argument");
+    const size_t T = pq->n_tokens, B = sq->n_seqs, hd = (size_t)kv->view.hd, nh = pq->n_heads, row = nh * hd;
+    const size_t eb = elem_bytes(pq->dtype, "query"), ps = (size_t)kv->view.page_size;
+    const size_t want = prompt_ws(c, kv, nh, B, T);
+    if (loc == BB_LOC_HOST && pq->seq_start && B > 0) need_starts(pq->seq_start, B, T);
+    need_seqs(kv, sq, loc, [&](size_t s, int64_t n) {
+      // (pages of positions between a prefix and the first token's window may be missing)
+      const int64_t bring = tokens_of(pq->seq_start, s, n), prefix = pq->prefix ? std::min<int64_t>(pq->prefix[s], n) : 0;
+      need(prefix >= 0, BB_ERR_RANGE, "a prefix must not be negative");
+      for (size_t i = 0; i * ps < (size_t)prefix; ++i) {
+        const int32_t pg = sq->page_table[s * sq->table_stride + i];
+        need(pg >= 0 && pg < kv->view.n_pages, BB_ERR_RANGE,
+             "sequence " + std::to_string(s) + ": page " + std::to_string(pg) + " is not in the pool");
+      }
+      const size_t reach = (size_t)(n - bring) + 1;  // positions up to the first token's own
+      return bring == 0 ? n : pq->window > 0 && pq->window < reach ? (int64_t)(reach - pq->window) : 0;
+    });
+    if (!pq->seq_start) need(T == B, BB_ERR_SHAPE, "without seq_start every sequence has one token");
+    need(std::isfinite(pq->scale), BB_ERR_ARG, "scale must be finite");
+    need(std::isfinite(pq->cap) && pq->cap >= 0.0f, BB_ERR_ARG, "cap must be finite and not negative");
+    if (T == 0 || B == 0) return;
+    need(pq->q && pq->out, BB_ERR_ARG, "null query or output");
+    need(T == 1 || (pq->q_stride >= row && pq->out_stride >= row), BB_ERR_ARG, "q_stride or out_stride below a token's row");
+    need(pq->q_stride < STRIDE_MAX && pq->out_stride < STRIDE_MAX, BB_ERR_RANGE, "strides must be below 2^36 elements");
+    const size_t nq = span_bytes(T, pq->q_stride, row, eb), no = span_bytes(T, pq->out_stride, row, eb);
+    need(!rows_overlap(rows_of(pq->q, T, pq->q_stride, row, eb), rows_of(pq->out, T, pq->out_stride, row, eb)),
+         BB_ERR_ARG, "out overlaps the query");
+    const size_t nl = pq->lse ? T * nh * 4 : 0;
+    need(!overlap(pq->lse, nl, pq->out, no) && !overlap(pq->lse, nl, pq->q, nq), BB_ERR_ARG, "lse overlaps the query or out");
+    set_device(c);
+    const bool cap = (loc == BB_LOC_HOST || c->profile || (want > 0 && !pq->workspace)) && capturing(c);
+    need_off_pool(kv, loc, {{pq->out, no}, {pq->lse, nl}});
+    need(!(cap && loc == BB_LOC_HOST), BB_ERR_ARG, "a call on host memory cannot be captured");
+    if (pq->workspace) {
+      need_aligned(pq->workspace, "workspace");
+      need(pq->workspace_bytes >= want, BB_ERR_RANGE, "workspace smaller than bb_paged_prompt_attention_workspace's answer");
+      need(!overlap(pq->workspace, want, kv->view.k, kv->span) && !overlap(pq->workspace, want, kv->view.v, kv->span) &&
+               (loc == BB_LOC_HOST || (!overlap(pq->workspace, want, pq->q, nq) && !overlap(pq->workspace, want, pq->out, no) &&
+                                       !overlap(pq->workspace, want, pq->lse, nl))),
+           BB_ERR_ARG, "the workspace overlaps another array");
+    } else if (want > 0) {
+      need(!cap, BB_ERR_ARG, "a captured call needs a workspace of its own");
+    }
+    // (host memory: out's and lse's spans go in too, what is not written stays as it is)
+    with_io(c, loc,
+            {{sq->page_table, span_bytes(B, sq->table_stride, sq->max_pages, 4), true, false, 4},
+             {sq->lens, B * 4, true, false, 4},
+             {pq->q, nq, true, false},
+             {pq->out, no, true, true},
+             {pq->lse, nl, true, true, 4},
+             {pq->slopes, pq->slopes ? nh * 4 : 0, true, false, 4},
+             {pq->prefix, pq->prefix ? B * 4 : 0, true, false, 4},
+             {pq->seq_start, pq->seq_start ? (B + 1) * 4 : 0, true, false, 4}},
+            [&](std::vector<void*>& d) {
+              bb::PromptQuery q{};
+              q.q = d[2];
+              q.out = d[3];
+              q.q_stride = pq->q_stride;
+              q.out_stride = pq->out_stride;
+              q.dt = (int)pq->dtype;
+              q.n_heads = (int)nh;
+              q.n_tokens = (int)T;
+              q.window = pq->window < ((size_t)1 << 31) ? (int)pq->window : 0;  // (lengths are below 2^31)
+              q.scale = pq->scale != 0.0f ? pq->scale : 1.0f / std::sqrt((float)hd);
+              q.cap = pq->cap;
+              q.lse = nl ? static_cast<float*>(d[4]) : nullptr;
+              q.slopes = pq->slopes ? static_cast<const float*>(d[5]) : nullptr;
+              q.prefix = pq->prefix ? static_cast<const int32_t*>(d[6]) : nullptr;
+              q.seq_start = pq->seq_start ? static_cast<const int32_t*>(d[7]) : nullptr;
+              q.ws = want == 0 ? nullptr : pq->workspace ? pq->workspace : ensure_ws(c, want);
+              launch_paged(c, cap, bb::K_PAGED_PROMPT, [&] {
+                return bb::launch_paged_prompt(c->stream, c->n_cu, (int)kv->dtype, q, kv->view, seqs_of(sq, d[0], d[1]));
               });
             });
   });

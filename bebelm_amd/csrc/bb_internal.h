@@ -98,6 +98,8 @@ enum KernelId : int {
   K_ROPE,
   K_PAGED_APPEND,
   K_PAGED_ATTN,
+  K_PAGED_READ,
+  K_PAGED_PROMPT,
   K_COUNT
 };
 const char* kernel_name(int id);
@@ -365,7 +367,7 @@ hipError_t launch_embed(hipStream_t s, const uint8_t* te, int dtype, size_t row_
 
 // ---- paged cache (bb_paged.hip) ----
 // A pool: element (page, position, head, d) of keys and values at page·page_stride + position·pos_stride
-// + head·head_stride + d.
+// + head·head_stride + d. Of 4 bits: the piece of (page, head) at page·page_stride + head·head_stride bytes (pos_stride 0).
 struct PagedView {
   void *k, *v;
   size_t page_stride, pos_stride, head_stride;
@@ -400,6 +402,14 @@ struct RopeRows {
   float eps;
   const int32_t *pos, *seq_start;
 };
+// The rows of an append read back (k, v: one may be null).
+struct ReadRows {
+  size_t T, k_ts, v_ts;
+  void *k, *v;
+  const int32_t* seq_start;
+};
+hipError_t launch_paged_read(hipStream_t s, int dtype, int cache, const ReadRows& r, const PagedView& kv,
+                             const PagedSeqs& seqs);
 // dtype of q, k, v and q_out; cache: the pool's dtype (n_kv > 0).
 hipError_t launch_rope_rows(hipStream_t s, int dtype, int cache, const RopeRows& r, const RopeTurns& t,
                             const PagedView& kv, const PagedSeqs& seqs);
@@ -417,6 +427,21 @@ size_t paged_attn_ws(int n_cu, int n_seqs, int n_heads, int n_kv, int hd);
 bool paged_attn_fits(int n_seqs, int n_heads, int n_kv, size_t cap);
 hipError_t launch_paged_attn(hipStream_t s, int n_cu, int cache, const PagedQuery& q, const PagedView& kv,
                              const PagedSeqs& seqs);
+// Several tokens per sequence (bb_paged_prompt.hip). seq_start null: one each.
+struct PromptQuery {
+  const void* q;
+  void* out;
+  size_t q_stride, out_stride;
+  int dt, n_heads, n_tokens, window;
+  float scale, cap;
+  const float* slopes;
+  const int32_t *prefix, *seq_start;
+  float* lse;
+  void* ws;
+};
+size_t paged_prompt_ws(int n_cu, int cache, size_t n_tokens, size_t n_seqs, int n_heads, int n_kv, int hd);
+hipError_t launch_paged_prompt(hipStream_t s, int n_cu, int cache, const PromptQuery& q, const PagedView& kv,
+                               const PagedSeqs& seqs);
 
 }  // namespace bb
 #endif

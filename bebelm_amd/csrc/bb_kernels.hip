@@ -24,7 +24,7 @@ const char* kernel_name(int id) {
                                        "combine",      "residual_norm", "residual_route", "conv",
                                        "conv_state",   "norm_rope",     "attn_scores",  "attn_pv",
                                        "softmax",      "embed",        "rope",         "paged_append",
-                                       "paged_attn"};
+                                       "paged_attn",   "paged_read",   "paged_prompt"};
   return (id >= 0 && id < K_COUNT) ? names[id] : "?";
 }
 

@@ -1,71 +1,13 @@
 // bb_paged.hip — rotary positions, appending to a paged key/value cache, and attention of one new
 // token per sequence over it (include/bebelm_moe.h states the operators). The reference has no
 // counterpart: values are computed in f32 from the formulas and rounded once where they are stored.
-#include "bb_device.h"
 #include <algorithm>
-#include <type_traits>
-#include "bb_internal.h"
-#include "bb_paged_plan.h"
+#include "bb_paged4.h"
+#include "bb_paged_device.h"
 
 namespace bb {
 
 namespace {
-
-template <int DT>
-struct ElemOf;
-template <>
-struct ElemOf<BB_F32> {
-  typedef float T;
-};
-template <>
-struct ElemOf<BB_F16> {
-  typedef _Float16 T;
-};
-template <>
-struct ElemOf<BB_BF16> {
-  typedef __bf16 T;
-};
-
-// N consecutive elements at any element's alignment as f32, and back, rounded to nearest (16-byte accesses).
-template <class T, int N>
-struct RunOf {
-  static constexpr int M = N * sizeof(T) > 16 ? 16 / sizeof(T) : N;
-  typedef T V __attribute__((ext_vector_type(M), aligned(sizeof(T))));
-};
-template <class T, int N>
-__device__ __forceinline__ void load_vec(const T* p, float (&x)[N]) {
-  if constexpr (N == 1) {
-    x[0] = (float)p[0];
-  } else {
-    constexpr int M = RunOf<T, N>::M;
-#pragma unroll
-    for (int i = 0; i < N; i += M) {
-      const auto v = *reinterpret_cast<const typename RunOf<T, N>::V*>(p + i);
-#pragma unroll
-      for (int j = 0; j < M; ++j) x[i + j] = (float)v[j];
-    }
-  }
-}
-template <class T, int N>
-__device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
-  if constexpr (N == 1) {
-    p[0] = (T)x[0];
-  } else {
-    constexpr int M = RunOf<T, N>::M;
-#pragma unroll
-    for (int i = 0; i < N; i += M) {
-      typename RunOf<T, N>::V v;
-#pragma unroll
-      for (int j = 0; j < M; ++j) v[j] = (T)x[i + j];
-      *reinterpret_cast<typename RunOf<T, N>::V*>(p + i) = v;
-    }
-  }
-}
-
-// i / page_slots for 0 <= i < 2^31.
-__device__ __forceinline__ int page_of(const PagedView& kv, int i) {
-  return slot_quotient(i, kv.page_mul, kv.page_shift);
-}
 
 // ---- rotary positions, and the rows of an append ------------------------------------------------
 
@@ -87,18 +29,23 @@ constexpr int RR_THREADS = 256;
 
 struct RowPlace {
   int64_t base;  // where its keys and values start in the pool, -1: nowhere
+  int row;       // its position in the page
   int pos;
-  int live;
+  int live;      // 0: no place
+  int seq;       // its sequence (-1: none, padding)
 };
 
 // The place and position of token t. Called by a whole wave; every lane gets the answer.
-__device__ __forceinline__ RowPlace row_place(const RopeRows& r, const PagedView& kv, const PagedSeqs& sq, size_t t) {
-  RowPlace w{-1, 0, 0};
+template <class R>
+__device__ __forceinline__ RowPlace row_place(const R& r, const PagedView& kv, const PagedSeqs& sq, size_t t) {
+  RowPlace w{-1, 0, 0, 0, -1};
   if (t >= r.T) return w;
-  if (!sq.lens) {
-    w.pos = r.pos[t];
-    w.live = 1;
-    return w;
+  if constexpr (std::is_same<R, RopeRows>::value) {
+    if (!sq.lens) {
+      w.pos = r.pos[t];
+      w.live = 1;
+      return w;
+    }
   }
   int s = (int)t;
   int64_t index;
@@ -112,18 +59,26 @@ __device__ __forceinline__ RowPlace row_place(const RopeRows& r, const PagedView
       s += __popcll(__ballot(before));
     }
     if (s >= sq.n_seqs) return w;
+    w.seq = s;
     index = (int64_t)sq.lens[s] - r.seq_start[s + 1] + (int64_t)t;
   } else {
+    w.seq = s;
     index = (int64_t)sq.lens[s] - 1;
   }
   if (index < 0 || index >= (int64_t)sq.max_pages * kv.page_size) return w;
   const int ix = (int)index, page = page_of(kv, ix);
   w.live = 1;
-  w.pos = r.pos ? r.pos[t] : ix;
-  if (r.n_kv) {
+  w.pos = ix;
+  w.row = ix - page * kv.page_size;
+  bool pool = true;
+  if constexpr (std::is_same<R, RopeRows>::value) {
+    if (r.pos) w.pos = r.pos[t];
+    pool = r.n_kv > 0;
+  }
+  if (pool) {
     const int pg = sq.table[(size_t)s * sq.table_stride + page];
     if (pg >= 0 && pg < kv.n_pages)
-      w.base = (int64_t)((size_t)pg * kv.page_stride + (size_t)(ix - page * kv.page_size) * kv.pos_stride);
+      w.base = (int64_t)((size_t)pg * kv.page_stride + (size_t)w.row * kv.pos_stride);
   }
   return w;
 }
@@ -139,10 +94,15 @@ __device__ __forceinline__ RowPlace row_place(const RopeRows& r, const PagedView
 // and 8 kv heads appended 27.1 us, 4.5 TB/s (a plain copy of 4 GiB: 4.9). Two tokens a block: 14.4 and
 // 30 us; elements one at a time where a part is no multiple of 8 (1176 tokens, 118 of 128 turned,
 // 28.9 MB): 28 us, in runs 12.7.
+// C Kv4Pool: keys and values go to LDS first, from which four lanes take a block of 32 and quantise it.
+struct Kv4Pool {};
 template <class A, class C, int VE, bool EVEN>
 __global__ void __launch_bounds__(RR_THREADS) k_rope_rows(RopeRows r, RopeTurns rt, PagedView kv, PagedSeqs sq, int rpb,
                                                           int gs) {
   constexpr int MU = VE == 1 ? 4 : 1;
+  constexpr bool KV4 = std::is_same<C, Kv4Pool>::value;
+  // (a group has at least 4 lanes and a lane at most 16 of a row's elements: the rows at work are 4096 at most)
+  __shared__ float s_rows[KV4 ? 4096 : 1];
   __shared__ float2 cs[OPS_HD_MAX / 2];
   __shared__ float s_gain[2][OPS_HD_MAX];
   __shared__ RowPlace place;
@@ -193,7 +153,9 @@ __global__ void __launch_bounds__(RR_THREADS) k_rope_rows(RopeRows r, RopeTurns 
     // (in place, a lane stores elements that its neighbour loads too: none may move up past the loads)
     if constexpr (!EVEN) __builtin_amdgcn_wave_barrier();
     A* yq = static_cast<A*>(r.q_out) + t * r.qo_ts + (size_t)head * r.qo_hs;
-    C* yc = static_cast<C*>(is_k ? kv.k : kv.v) + w.base + (size_t)head * kv.head_stride;
+    typedef typename std::conditional<KV4, float, C>::type Y;
+    Y* yc = KV4 ? reinterpret_cast<Y*>(s_rows) + tid / gs * r.hd
+                : static_cast<Y*>(is_k ? kv.k : kv.v) + w.base + (size_t)head * kv.head_stride;
     if (is_q ? r.q_norm != nullptr : is_k && r.k_norm != nullptr) {
       // rmsnorm over the head: the lanes of the group hold parts of it
       const float* gain = s_gain[is_q ? 0 : 1];
@@ -252,9 +214,25 @@ __global__ void __launch_bounds__(RR_THREADS) k_rope_rows(RopeRows r, RopeTurns 
         if (u < units) store_vec<A, VE>(yq + e0, a[m]);
         if (u < nu) store_vec<A, VE>(yq + e1, b[m]);
       } else {
-        if (u < units) store_vec<C, VE>(yc + e0, a[m]);
-        if (u < nu) store_vec<C, VE>(yc + e1, b[m]);
+        if (u < units) store_vec<Y, VE>(yc + e0, a[m]);
+        if (u < nu) store_vec<Y, VE>(yc + e1, b[m]);
       }
+    }
+    if constexpr (KV4) {
+      if (is_q) continue;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (a row's lanes are in one wave)
+      __builtin_amdgcn_wave_barrier();
+      char* piece = static_cast<char*>(is_k ? kv.k : kv.v) + w.base + (size_t)head * kv.head_stride;
+      for (int u = lane; u < r.hd / 8; u += gs) {
+        float x[8];
+        load_vec<Y, 8>(yc + 8 * u, x);
+        uint32_t head16;
+        const uint32_t word = kv4_quantise(x, head16);
+        *reinterpret_cast<uint32_t*>(piece + (size_t)w.row * (r.hd / 2) + 4 * u) = word;
+        if (u % 4 == 0) *reinterpret_cast<uint16_t*>(piece + kv4_head_at(kv, w.row, u / 4)) = (uint16_t)head16;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
     }
   }
 }
@@ -266,6 +244,7 @@ hipError_t rope_rows_of(hipStream_t s, const RopeRows& r, const RopeTurns& t, co
   const int ve = wide ? 8 : 1, units = (t.half + ve - 1) / ve + (rest + ve - 1) / ve;
   int gs = 1;
   while (gs < units && gs < 64) gs *= 2;
+  if (std::is_same<C, Kv4Pool>::value) gs = std::max(gs, 4);
   const int at_once = RR_THREADS / gs;
   // a token's rows go to several blocks, one turn of the rows each, while all the blocks fit the device at once
   const size_t want = std::max<size_t>(1, std::min<size_t>((n_rows + at_once - 1) / at_once, 2048 / r.T));
@@ -278,7 +257,59 @@ hipError_t rope_rows_of(hipStream_t s, const RopeRows& r, const RopeTurns& t, co
   return hipGetLastError();
 }
 
-// f(type of DT a, type of DT b)
+// The keys and values of tokens' positions, as they are in the pool, one element's run of 8 a thread: a block per token
+// (few tokens: several). Bound by its bytes.
+template <class A, class C>
+__global__ void __launch_bounds__(RR_THREADS) k_paged_read(ReadRows r, PagedView kv, PagedSeqs sq, int per) {
+  __shared__ RowPlace place;
+  const int tid = threadIdx.x;
+  const size_t t = blockIdx.x;
+  if (tid < 64) {
+    const RowPlace w = row_place(r, kv, sq, t);
+    if (tid == 0) place = w;
+  }
+  __syncthreads();
+  const RowPlace w = place;
+  if (w.seq < 0) return;
+  const int runs = kv.n_kv * (kv.hd / 8), all = (r.k ? runs : 0) + (r.v ? runs : 0);
+  const int end = min(all, ((int)blockIdx.y + 1) * per);
+  for (int u = blockIdx.y * per + tid; u < end; u += RR_THREADS) {
+    const bool is_v = !r.k || u >= runs;
+    const int i = is_v && r.k ? u - runs : u, head = i / (kv.hd / 8), d = 8 * (i - head * (kv.hd / 8));
+    const char* pool = static_cast<const char*>(is_v ? kv.v : kv.k);
+    float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (w.live && w.base >= 0) {
+      const size_t at = (size_t)w.base + (size_t)head * kv.head_stride;
+      if constexpr (std::is_same<C, Kv4Pool>::value) {
+        const uint32_t word = *reinterpret_cast<const uint32_t*>(pool + at + (size_t)w.row * (kv.hd / 2) + d / 2);
+        const uint32_t h = *reinterpret_cast<const uint16_t*>(pool + at + kv4_head_at(kv, w.row, d / 32));
+        const v8h y = __builtin_bit_cast(v8h, Kv4Block(h).natural(word));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = (float)y[e];
+      } else {
+        load_vec<C, 8>(reinterpret_cast<const C*>(pool) + at + d, x);
+      }
+    }
+    A* to = static_cast<A*>(is_v ? r.v : r.k) + t * (is_v ? r.v_ts : r.k_ts) + (size_t)head * kv.hd + d;
+    store_vec<A, 8>(to, x);
+  }
+}
+
+template <class A, class C>
+hipError_t paged_read_of(hipStream_t s, const ReadRows& r, const PagedView& kv, const PagedSeqs& sq) {
+  const int all = kv.n_kv * (kv.hd / 8) * ((r.k != nullptr) + (r.v != nullptr));
+  // (as an append's rows: several blocks a token while all of them fit the device at once)
+  const size_t want = std::max<size_t>(1, std::min<size_t>((all + RR_THREADS - 1) / RR_THREADS, 2048 / r.T));
+  const int per = (int)((all + want - 1) / want);
+  BB_LAUNCH((k_paged_read<A, C>), dim3((unsigned)r.T, (unsigned)((all + per - 1) / per)), dim3(RR_THREADS), 0, s, r, kv, sq,
+            per);
+  return hipGetLastError();
+}
+
+// f(type of DT a, type of DT b, a type or BB_KV4)
+struct Kv4Elem {
+  typedef Kv4Pool T;
+};
 template <class F>
 hipError_t by_dtypes(int a, int b, F&& f) {
   const auto second = [&](auto x) {
@@ -286,6 +317,7 @@ hipError_t by_dtypes(int a, int b, F&& f) {
       case BB_F32: return f(x, ElemOf<BB_F32>());
       case BB_F16: return f(x, ElemOf<BB_F16>());
       case BB_BF16: return f(x, ElemOf<BB_BF16>());
+      case BB_KV4: return f(x, Kv4Elem());
       default: return hipErrorInvalidValue;
     }
   };
@@ -298,6 +330,14 @@ hipError_t by_dtypes(int a, int b, F&& f) {
 }
 
 }  // namespace
+
+hipError_t launch_paged_read(hipStream_t s, int dtype, int cache, const ReadRows& r, const PagedView& kv,
+                             const PagedSeqs& seqs) {
+  if (r.T == 0 || (!r.k && !r.v)) return hipSuccess;
+  return by_dtypes(dtype, cache, [&](auto a, auto c) {
+    return paged_read_of<typename decltype(a)::T, typename decltype(c)::T>(s, r, kv, seqs);
+  });
+}
 
 hipError_t launch_rope_rows(hipStream_t s, int dtype, int cache, const RopeRows& r, const RopeTurns& t,
                             const PagedView& kv, const PagedSeqs& seqs) {
@@ -343,14 +383,6 @@ hipError_t launch_rope_rows(hipStream_t s, int dtype, int cache, const RopeRows&
 namespace {
 
 constexpr int PA_WAVES = 4, PA_THREADS = 64 * PA_WAVES;
-constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
-constexpr float NEG_INF = -__builtin_inff();
-
-typedef float v4f __attribute__((ext_vector_type(4)));
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef __bf16 v8b __attribute__((ext_vector_type(8)));
-typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 // A kv head's G query heads: `split` groups of `hg` (the last may have fewer).
 struct PagedPlan {
@@ -363,54 +395,6 @@ struct PagedPlan {
 
 __device__ __forceinline__ SeqSpan seq_span(int raw_len, const PagedView& kv, int max_pages, int window, int unit) {
   return span_of(raw_len, kv.page_size, kv.page_slots, max_pages, window, unit);
-}
-
-// Four adjacent elements of a row of type dt, at any element's alignment.
-template <class T>
-__device__ __forceinline__ void store_row(void* p, size_t i, const v4f& x) {
-  const float y[4] = {x[0], x[1], x[2], x[3]};
-  store_vec<T, 4>(static_cast<T*>(p) + i, y);
-}
-__device__ __forceinline__ void store_act(void* p, size_t i, int dt, const v4f& x) {
-  if (dt == BB_F32) store_row<float>(p, i, x);
-  else if (dt == BB_F16) store_row<_Float16>(p, i, x);
-  else store_row<__bf16>(p, i, x);
-}
-
-// (by value: a bit cast of a vector's element itself reads the vector's first)
-__device__ __forceinline__ float as_float(uint32_t a) { return __builtin_bit_cast(float, a); }
-__device__ __forceinline__ uint32_t hi_halves(float a, float b) {  // the upper 16 bits of a (low) and b
-  return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
-}
-__device__ __forceinline__ float trunc_bf16(float a) {
-  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, a) & 0xffff0000u);
-}
-// Two values as NP packed 16-bit parts whose sums they are.
-template <int CT, int NP>
-__device__ __forceinline__ void split2(float a, float b, uint32_t (&w)[NP]) {
-  if constexpr (CT == BB_BF16) {
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      if (i + 1 == NP && NP < 3) {
-        typedef __bf16 v2b __attribute__((ext_vector_type(2)));
-        const v2b r = {(__bf16)a, (__bf16)b};
-        w[i] = __builtin_bit_cast(uint32_t, r);
-      } else {
-        w[i] = hi_halves(a, b);
-        a = a - trunc_bf16(a);
-        b = b - trunc_bf16(b);
-      }
-    }
-  } else {
-    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const v2h r = {(_Float16)a, (_Float16)b};
-      w[i] = __builtin_bit_cast(uint32_t, r);
-      a = a - (float)r[0];
-      b = b - (float)r[1];
-    }
-  }
 }
 
 template <int CT>
@@ -433,17 +417,6 @@ __device__ __forceinline__ float group_sum(float x) {
   x = as_float(a[0]) + as_float(a[1]);
   auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return as_float(b[0]) + as_float(b[1]);
-}
-
-// Inclusive sums over the wave's lanes.
-__device__ __forceinline__ int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr 1, 2, 4, 8
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the row before's last lane, to rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row 1's last lane, to rows 2 and 3
-  return x;
 }
 
 // A tile's shape: CT the cache's type, HDP the head size (or the next of 64, 128, 256).

@@ -1,0 +1,124 @@
+// bb_paged4.h — the blocks of a 4-bit paged cache: 32 elements of a head row, 16 bytes of codes (element 2i in the low
+// half of byte i) and a 16-bit head with the step d (bits 6 to 14: an f16 number of 5 significant bits) and the
+// offset z (bits 0 to 5, bit 15 for -64). An element stands for d·(code + z): with code + z in -47..63 that is 6 bits
+// times 5, exact in f16, so that the matrix cores' 16-bit instructions take it as it is; and so is
+// d·(z - 16), which makes the value one multiply-add of the f16 number 16 + code. A (page, head) of the pool is
+// one piece: the codes of its positions, then their heads of blocks (an even number a position).
+#ifndef BB_PAGED4_H
+#define BB_PAGED4_H
+#include <stddef.h>
+#include <stdint.h>
+
+namespace bb {
+
+// Blocks' heads that a position has, bytes of a (page, head).
+constexpr size_t kv4_heads(size_t hd) { return (hd / 32 + 1) / 2 * 2; }
+constexpr size_t kv4_chunk(size_t page_size, size_t hd) {
+  return (page_size * (hd / 2 + 2 * kv4_heads(hd)) + 15) / 16 * 16;
+}
+
+}  // namespace bb
+
+#ifdef __HIPCC__
+#include "bb_paged_device.h"
+namespace bb {
+namespace {
+
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+
+// Where the head of block b of a page's position lies in its (page, head).
+__device__ __forceinline__ int kv4_head_at(const PagedView& kv, int pos, int b) {
+  return kv.page_size * (kv.hd / 2) + 2 * (pos * ((kv.hd / 32 + 1) & ~1) + b);
+}
+
+template <int N>
+__device__ __forceinline__ void load_words(const char* p, uint32_t* w) {
+  typedef uint32_t V __attribute__((ext_vector_type(N), aligned(4 * N)));
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else {
+    const V v = *reinterpret_cast<const V*>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = v[i];
+  }
+}
+
+// A block's head as what its codes are multiplied by and what is added.
+struct Kv4Block {
+  v2h d, zd;
+  __device__ __forceinline__ explicit Kv4Block(uint32_t head) {
+    const _Float16 step = __builtin_bit_cast(_Float16, (uint16_t)(head & 0x7fc0u));
+    const int z = (int)(head & 63u) - (int)(head >> 9 & 64u) - 16;
+    const _Float16 add = (_Float16)(float)z * step;
+    d = v2h{step, step};
+    zd = v2h{add, add};
+  }
+  // Elements i and i + 4 of a word's 8 (i-th and (i + 4)-th half byte).
+  template <int I>
+  __device__ __forceinline__ uint32_t pair(uint32_t w) const {
+    const uint32_t at = I == 0 ? w << 6 : I == 1 ? w << 2 : I == 2 ? w >> 2 : w >> 6;  // to bits 6 to 9 of each half
+    const v2h x = __builtin_bit_cast(v2h, (at & 0x03c003c0u) | 0x4c004c00u);           // 16 + code
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x, d, zd));
+  }
+  // A word's 8 elements in their order, and in the order 0 4 1 5 2 6 3 7.
+  __device__ __forceinline__ v4u natural(uint32_t w) const {
+    const uint32_t a = pair<0>(w), b = pair<1>(w), c = pair<2>(w), e = pair<3>(w);
+    return v4u{__builtin_amdgcn_perm(b, a, 0x05040100u), __builtin_amdgcn_perm(e, c, 0x05040100u),
+               __builtin_amdgcn_perm(b, a, 0x07060302u), __builtin_amdgcn_perm(e, c, 0x07060302u)};
+  }
+  __device__ __forceinline__ v4u paired(uint32_t w) const { return v4u{pair<0>(w), pair<1>(w), pair<2>(w), pair<3>(w)}; }
+};
+
+// Whether step d (at least 0) reaches from lo to hi in 15 steps, and each of them by the offsets there are. (In f64: the
+// products are exact, and so is the difference but for values 2^28 times apart.)
+__device__ __forceinline__ bool kv4_step_holds(float d, float lo, float hi) {
+  return 15.0 * (double)d >= (double)hi - (double)lo && 63.0 * (double)d >= (double)hi && 47.0 * (double)d >= -(double)lo;
+}
+// The smallest step that holds: from the largest that the f32 quotients (off by 2^-22) reach, the next at most.
+__device__ __forceinline__ float kv4_step(float lo, float hi) {
+  constexpr float UNIT = 3.814697265625e-6f;  // 2^-18, of the steps below 2^-13
+  const float r = fmaxf((hi - lo) * (1.0f / 15.0f), fmaxf(hi * (1.0f / 63.0f), lo * (-1.0f / 47.0f)));
+  const float d = r < 6.103515625e-5f ? floorf(r * 262144.0f) * UNIT : as_float(__float_as_uint(r) & 0xfff80000u);
+  if (kv4_step_holds(d, lo, hi)) return d;
+  return d < 6.103515625e-5f ? d + UNIT : as_float(__float_as_uint(d) + 0x00080000u);
+}
+// Eight elements of a block, of which four adjacent lanes hold a quarter each, as a word of codes; `head` is the block's.
+// (x / d rounded to f32 and then to an integer is x / d rounded to an integer: the borders (n + 1/2)·d, n below 64, are f32
+// numbers, so that an x which is not on one is at least 2^-24 of itself away, and a quotient's rounding moves it less
+// than that towards one.)
+__device__ __forceinline__ uint32_t kv4_quantise(float (&x)[8], uint32_t& head) {
+  bool odd = false;
+  float lo = __builtin_inff(), hi = NEG_INF;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    odd |= !(fabsf(x[i]) < __builtin_inff());
+    x[i] = fminf(fmaxf(x[i], -16384.0f), 16384.0f);
+    lo = fminf(lo, x[i]);
+    hi = fmaxf(hi, x[i]);
+  }
+  int any = odd;
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    lo = fminf(lo, __shfl_xor(lo, o));
+    hi = fmaxf(hi, __shfl_xor(hi, o));
+    any |= __shfl_xor(any, o);
+  }
+  if (any) {
+    head = 0x7fc0u;
+    return 0;
+  }
+  const float d = kv4_step(lo, hi);
+  head = 0;
+  if (d == 0.0f) return 0;
+  const int z = (int)rintf(lo / d);
+  head = __builtin_bit_cast(uint16_t, (_Float16)d) | (uint32_t)(z & 63) | (z < 0 ? 0x8000u : 0u);
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w |= (uint32_t)min(max((int)rintf(x[i] / d) - z, 0), 15) << 4 * i;
+  return w;
+}
+
+}  // namespace
+}  // namespace bb
+#endif
+#endif

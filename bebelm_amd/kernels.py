@@ -15,6 +15,7 @@
 The paged-cache operators have no counterpart there:
   rope                                     rotary positions of any layout and frequency rule
   paged_append / paged_attention           a batch of conversations on one pool of cache pages
+  paged_prompt_attention / paged_read      several tokens of each attending over it, what it holds
 Each function takes the Context first; `w` is an uploaded Tensor (plus a byte offset where the
 reference passes a sub-slice of the weight bytes).
 """
@@ -301,15 +302,64 @@ def paged_attention(ctx, kv, page_table, lens, q, out, scale=None, window=0, lse
         raise ValueError("scale must not be 0")
     if window < 0:
         raise ValueError("window must not be negative")
-    ws = ws_bytes = 0
-    if workspace is not None:
-        if isinstance(workspace, np.ndarray) or workspace.get_device() != ctx.device or not workspace.is_contiguous():
-            raise ValueError("the workspace must be a contiguous tensor on the context's GPU")
-        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    ws, ws_bytes = _workspace(ctx, workspace)
     query = _lib.PAGED_QUERY.pack(code, qa, oa, heads, qs, os, scale, window, _flat(lse, "lse", F32, n, heads), ws,
                                   ws_bytes)
     check(lib().bb_paged_attention(ctx.handle, kv.handle, seqs, query, _place(ctx, q, out, page_table, lens, lse)))
     return out
+
+
+def _workspace(ctx, workspace):
+    """(address, bytes)"""
+    if workspace is None:
+        return 0, 0
+    if isinstance(workspace, np.ndarray) or workspace.get_device() != ctx.device or not workspace.is_contiguous():
+        raise ValueError("the workspace must be a contiguous tensor on the context's GPU")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def paged_prompt_attention(ctx, kv, page_table, lens, q, out, seq_start=None, scale=None, window=0, cap=0.0, slopes=None,
+                           prefix=None, lse=None, workspace=None):
+    """Several query tokens per sequence, q [tokens, n_heads, head_dim], each over its sequence's positions in the
+    PagedKv's pages up to its own (the last `window` of them; 0: all) and those below prefix int32 [sequences], into
+    out. seq_start int32 [sequences + 1] says which tokens each sequence has, its last ones (None: one each). Scores
+    are capped (cap > 0: cap·tanh(score / cap)) and get -slopes[head]·distance (slopes float32 [n_heads]); lse
+    float32 [tokens, n_heads] gets the softmax's log sums. scale None: 1/sqrt(head_dim). workspace: a device
+    tensor of kv.prompt_workspace(n_heads, sequences, tokens) bytes for this call alone (None: the context's; a call
+    captured into a graph needs one unless that is 0)."""
+    n, seqs = _seqs(page_table, lens)
+    t, heads, hd, code = q.shape[0], q.shape[1], kv.head_dim, _floating(q, "q")
+    qa, qs, _ = _heads(q, "q", code, t, heads, hd)
+    oa, os, _ = _heads(out, "out", code, t, heads, hd)
+    if scale is None:
+        scale = 0.0
+    elif scale == 0:
+        raise ValueError("scale must not be 0")
+    if window < 0:
+        raise ValueError("window must not be negative")
+    ws, ws_bytes = _workspace(ctx, workspace)
+    queries = _lib.PAGED_QUERIES.pack(t, code, qa, oa, heads, qs, os, scale, cap, window,
+                                      _flat(slopes, "slopes", F32, heads), _flat(prefix, "prefix", INT32, n),
+                                      _flat(seq_start, "seq_start", INT32, n + 1), _flat(lse, "lse", F32, t, heads), ws,
+                                      ws_bytes)
+    check(lib().bb_paged_prompt_attention(ctx.handle, kv.handle, seqs, queries,
+                                          _place(ctx, q, out, page_table, lens, seq_start, slopes, prefix, lse)))
+    return out
+
+
+def paged_read(ctx, kv, page_table, lens, k=None, v=None, seq_start=None):
+    """The keys and values that the PagedKv's pages hold at the tokens' positions (those that paged_append with the
+    same page_table, lens and seq_start stores to), into k and v [tokens, n_kv_heads, head_dim] (either may be None)."""
+    some = k if k is not None else v
+    if some is None:
+        raise ValueError("neither k nor v to read")
+    n, seqs = _seqs(page_table, lens)
+    t, hd, nkv, code = some.shape[0], kv.head_dim, kv.n_kv_heads, _floating(some, "k" if k is not None else "v")
+    ka, ks, _ = _heads(k, "k", code, t, nkv, hd) if k is not None else (0, 0, 0)
+    va, vs, _ = _heads(v, "v", code, t, nkv, hd) if v is not None else (0, 0, 0)
+    rows = _lib.PAGED_ROWS.pack(t, code, ka, va, ks, vs, _flat(seq_start, "seq_start", INT32, n + 1))
+    check(lib().bb_paged_read(ctx.handle, kv.handle, seqs, rows, _place(ctx, k, v, page_table, lens, seq_start)))
+    return k, v
 
 
 def _n(a):

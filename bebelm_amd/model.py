@@ -8,8 +8,8 @@ Names follow the reference so call sites read alike:
   Model::attn_step / attn_batch (model.rs:430, :222)    -> AttnOp.forward (KvCache: cache.rs)
   Model::run_layers(_batch) / forward_step, Agent::absorb -> Model (model.rs:97-181, agent.rs:454)
   Cache (cache.rs:10-49), Cache: Clone                  -> Cache (Model.new_cache, Cache.clone)
-RopePlan and PagedKv are the handles of the paged-cache operators (kernels.rope, paged_append,
-paged_attention), which the reference does not have.
+RopePlan and PagedKv are the handles of the paged-cache operators (kernels.rope, paged_append, paged_read,
+paged_attention, paged_prompt_attention), which the reference does not have.
 Arrays are numpy (host memory, BB_LOC_HOST) or torch CUDA tensors (device memory,
 BB_LOC_DEVICE). Everything runs on the GPU through libbebelm_moe.so; there is no other path.
 """
@@ -319,6 +319,7 @@ class KvCache:
 
 
 F32, F16, BF16 = 0, 1, 30  # element types of the paged-cache operators
+KV4 = 4096                 # and of a pool of 4-bit blocks
 INT32 = -1
 _CODES = {"float32": F32, "float16": F16, "bfloat16": BF16, "int32": INT32}
 _codes = {}  # the same by dtype object
@@ -364,6 +365,13 @@ class RopePlan:
             pass
 
 
+def kv4_bytes(page_size, head_dim):
+    """Bytes of a (page, head) of a 4-bit pool."""
+    n = ctypes.c_size_t()
+    check(lib().bb_paged_kv4_bytes(page_size, head_dim, ctypes.byref(n)))
+    return n.value
+
+
 class PagedKv:
     """A pool of pages of keys and values (bb_paged_kv) over two torch CUDA tensors of one shape and
     strides, [n_pages, page_size, n_kv_heads, head_dim] with adjacent elements of a head (a permuted
@@ -384,8 +392,30 @@ class PagedKv:
         self.handle = h
 
     @classmethod
+    def four_bit(cls, ctx, k, v, page_size, head_dim):
+        """A pool in 4 bits over two torch CUDA uint8 tensors [n_pages, n_kv_heads, kv4_bytes(page_size, head_dim)] of one
+        shape and strides, the bytes of a (page, head) adjacent (bebelm_moe.h states their layout; zeros are zeros)."""
+        if (k.dim() != 3 or k.shape != v.shape or k.stride() != v.stride() or k.element_size() != 1 or v.dtype != k.dtype or
+                k.shape[2] != kv4_bytes(page_size, head_dim)):
+            raise ValueError("keys and values must be bytes of one shape [pages, heads, kv4_bytes(page_size, head_dim)] "
+                             "and strides")
+        if k.get_device() != ctx.device or v.get_device() != ctx.device:
+            raise ValueError(f"the pool must be in the memory of the context's GPU ({ctx.device})")
+        if k.stride(2) != 1:
+            raise ValueError("the bytes of a (page, head) must be adjacent")
+        self = cls.__new__(cls)
+        self.ctx, self.k, self.v, self.handle = ctx, k, v, None
+        self.n_pages, self.n_kv_heads, _ = k.shape
+        self.page_size, self.head_dim = page_size, head_dim
+        h = ctypes.c_void_p()
+        check(lib().bb_paged_kv_view4(ctx.handle, k.data_ptr(), v.data_ptr(), self.n_pages, page_size, self.n_kv_heads,
+                                      head_dim, *k.stride()[:2], ctypes.byref(h)))
+        self.handle = h
+        return self
+
+    @classmethod
     def create(cls, ctx, dtype, n_pages, page_size, n_kv_heads, head_dim):
-        """A pool in device memory of the library's (dtype F32, F16 or BF16), zeroed; k and v are None."""
+        """A pool in device memory of the library's (dtype F32, F16, BF16 or KV4), zeroed; k and v are None."""
         self = cls.__new__(cls)
         self.ctx, self.k, self.v, self.handle = ctx, None, None, None
         self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = n_pages, page_size, n_kv_heads, head_dim
@@ -404,6 +434,13 @@ class PagedKv:
         """Bytes of device memory that kernels.paged_attention needs (its workspace argument)."""
         n = ctypes.c_size_t()
         check(lib().bb_paged_attention_workspace(self.ctx.handle, self.handle, n_heads, n_seqs, ctypes.byref(n)))
+        return n.value
+
+    def prompt_workspace(self, n_heads, n_seqs, n_tokens):
+        """Bytes of device memory that kernels.paged_prompt_attention needs (its workspace argument)."""
+        n = ctypes.c_size_t()
+        check(lib().bb_paged_prompt_attention_workspace(self.ctx.handle, self.handle, n_heads, n_seqs, n_tokens,
+                                                        ctypes.byref(n)))
         return n.value
 
     def close(self):

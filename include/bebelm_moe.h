@@ -47,8 +47,9 @@ enum bb_status {
   BB_ERR_MISSING = 9 /* metadata key or tensor absent, or of another value type        */
 };
 
-/* BB_BF16 (ggml's code too) is a type of the paged-cache operators only. */
-enum bb_dtype { BB_F32 = 0, BB_F16 = 1, BB_Q4_K = 12, BB_Q6_K = 14, BB_BF16 = 30 };
+/* BB_BF16 (ggml's code too) is a type of the paged-cache operators only, BB_KV4 (a code of this library's) one of
+ * their pools. */
+enum bb_dtype { BB_F32 = 0, BB_F16 = 1, BB_Q4_K = 12, BB_Q6_K = 14, BB_BF16 = 30, BB_KV4 = 4096 };
 enum bb_loc { BB_LOC_HOST = 0, BB_LOC_DEVICE = 1 };
 
 typedef struct bb_ctx bb_ctx;
@@ -382,6 +383,20 @@ int bb_paged_kv_view(bb_ctx* ctx, uint32_t dtype, void* k, void* v, size_t n_pag
                      bb_paged_kv** out);
 int bb_paged_kv_destroy(bb_paged_kv* kv);
 int bb_paged_kv_pages(const bb_paged_kv* kv, void** k, void** v);
+/* A pool in 4 bits (BB_KV4; head_dim a multiple of 32): bb_paged_kv_create allocates it, bb_paged_kv_view4 takes the
+ * caller's device memory, the piece of (page, head) at page·page_stride + head·head_stride bytes (whole 16-byte pieces,
+ * no two in one place). A piece has bb_paged_kv4_bytes' answer: the codes of its positions one after the other (head_dim / 2
+ * bytes each, element 2i in the low half of byte i), then their blocks' heads (16 bits for each 32 elements, an
+ * even number a position), and what fills it up to 16 bytes. A head holds a step d (bits 6 to 14: those of an F16
+ * number whose other bits are 0) and an offset z in two's complement (bits 0 to 5 and 15); an element stands for
+ * d·(code + z). Memory of zeros stands for zeros. Storing takes values past ±16384 as that, the smallest such d with
+ * 15d >= max - min, 63d >= max and 47d >= -min of the block (0 for a block of zeros), z = min / d and the codes x / d - z,
+ * both quotients rounded to the nearest integer (ties to even) and the codes held to 0..15: no element is off by more than
+ * d / 2. A block with an element that is not finite stands for NaN. (Heads that others made may have code + z
+ * past -47..63: what those stand for is rounded to F16.) */
+int bb_paged_kv4_bytes(size_t page_size, size_t head_dim, size_t* bytes);
+int bb_paged_kv_view4(bb_ctx* ctx, void* k, void* v, size_t n_pages, size_t page_size, size_t n_kv_heads,
+                      size_t head_dim, size_t page_stride, size_t head_stride, bb_paged_kv** out);
 
 /* The sequences of a batch: sequence s has lens[s] positions cached (those of the call's own tokens
  * included; 0: an empty place of the batch), position j in page page_table[s·table_stride +
@@ -428,6 +443,20 @@ typedef struct {
 int bb_paged_append(bb_ctx* ctx, bb_paged_kv* kv, const bb_rope_plan* plan, const bb_paged_seqs* seqs,
                     const bb_paged_tokens* tokens, int loc);
 
+/* The other way: the keys and values that the cache holds at the tokens' positions (those that bb_paged_append with
+ * the same sequences and seq_start stores to), as [n_tokens][n_kv_heads][head_dim] of F32, F16 or BF16 (heads side by
+ * side, tokens k_stride and v_stride apart, not overlapping; k or v may be NULL). Tokens without a place get zeros,
+ * padding is left as it is. With seq_start the running sums of the lengths that is all that the sequences hold. */
+typedef struct {
+  size_t n_tokens;
+  uint32_t dtype; /* of k and v */
+  void* k;
+  void* v;
+  size_t k_stride, v_stride;
+  const int32_t* seq_start;
+} bb_paged_rows;
+int bb_paged_read(bb_ctx* ctx, const bb_paged_kv* kv, const bb_paged_seqs* seqs, const bb_paged_rows* rows, int loc);
+
 /* One query token per sequence over its cached positions (attention_decode for every sequence):
  *   out[s][h] = sum_j softmax_j(scale·q[s][h]·k[j][h / (n_heads/n_kv_heads)])·v[j][...]
  * for max(0, lens[s] - window) <= j < lens[s] (window 0: all). q and out [n_seqs][n_heads][head_dim]
@@ -456,6 +485,42 @@ typedef struct {
 int bb_paged_attention_workspace(bb_ctx* ctx, const bb_paged_kv* kv, size_t n_heads, size_t n_seqs, size_t* bytes);
 int bb_paged_attention(bb_ctx* ctx, const bb_paged_kv* kv, const bb_paged_seqs* seqs, const bb_paged_query* query,
                        int loc);
+
+/* Several query tokens per sequence (a prompt, a chunk of one, drafts to verify), each over the positions up to its own
+ * and those of a prefix, with scores that may be capped and get a bias by distance:
+ *   out[t][h] = sum_j softmax_j(x[t][h][j])·v[j][...],  x = cap·tanh(scale·q[t][h]·k[j][...] / cap) - slopes[h]·|i - j|
+ * (cap 0: the scaled product itself; slopes NULL: no bias). Tokens are those of bb_paged_append: seq_start says which
+ * each sequence has, its last ones (NULL: one each, n_tokens = n_seqs); token t of sequence s has index
+ * i = lens[s] - seq_start[s+1] + t and sees the j below lens[s] with i - window < j <= i (window 0: j <= i), and those
+ * below prefix[s] (i32[n_seqs], or NULL) wherever they are: a prefix read in both directions, or with a window the first
+ * positions that stay in reach. Between a prefix and a window's first position nothing is read. q and out
+ * [n_tokens][n_heads][head_dim] (heads side by side, tokens q_stride and out_stride apart, not overlapping); scale 0 means
+ * 1/sqrt(head_dim); lse, as in bb_paged_attention, f32[n_tokens][n_heads] or NULL. A token that sees nothing gets zeros and
+ * -inf; of padding nothing is written. A value that is not finite makes not finite what it reaches, and nothing else: the
+ * rows that do not see it are as if it were not there. Weights are rounded to the cache's type (F16 for BB_KV4) where out is
+ * F16 on an F16 or BB_KV4 cache, or BF16; elsewhere they keep what out can hold. workspace: as in bb_paged_attention, of
+ * bb_paged_prompt_attention_workspace's answer (which may be 0: then a captured call needs none). Equal calls give equal
+ * bits. One call takes n_tokens·n_heads / 32 + n_seqs·n_kv_heads below 2^24 (BB_ERR_RANGE: cut the batch). */
+typedef struct {
+  size_t n_tokens;
+  uint32_t dtype; /* of q and out */
+  const void* q;
+  void* out;
+  size_t n_heads, q_stride, out_stride;
+  float scale;
+  float cap; /* >= 0 */
+  size_t window;
+  const float* slopes; /* f32[n_heads] */
+  const int32_t* prefix;
+  const int32_t* seq_start;
+  float* lse;
+  void* workspace;
+  size_t workspace_bytes;
+} bb_paged_queries;
+int bb_paged_prompt_attention_workspace(bb_ctx* ctx, const bb_paged_kv* kv, size_t n_heads, size_t n_seqs, size_t n_tokens,
+                                        size_t* bytes);
+int bb_paged_prompt_attention(bb_ctx* ctx, const bb_paged_kv* kv, const bb_paged_seqs* seqs,
+                              const bb_paged_queries* queries, int loc);
 
 /* ---- GGUF files (gguf.rs, config.rs:51-89, model.rs:36-50, :572-584, :619-660) ---------------- */
 /* GgufFile::open (gguf.rs:171-177): maps the file read-only and parses the header, the metadata
