@@ -10,6 +10,8 @@ namespace bb {
 namespace {
 
 constexpr int PP_THREADS = 256;
+// Weights go up to 2^SLACK, as f16 to 2^(SLACK + F16_UP) = 2^14, whose range then costs at most 2^-33 of the largest.
+constexpr float SLACK = 6.0f, F16_UP = 8.0f;
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 
@@ -21,20 +23,38 @@ struct PpShape {
   static constexpr int BN = WK > 1 || HDP * SZ >= 1024 ? 32 : 64;  // keys of a wave's tile
   static constexpr int KT = WK * BN;                               // keys of the block's
   static constexpr int NT = BN / 32;
-  // Rows in LDS (bytes): keys are read in 16-byte pieces of 16 rows at once, 16-bit values in 64-byte pieces of 4 rows,
-  // f32 values in 128-byte pieces of rows 4 apart, each spread over the banks.
-  static constexpr int KS = HDP * SZ + 16, VS = HDP * SZ + (SZ == 2 ? 64 : 32);
-  static constexpr int BUF = KT * (KS + VS);
+  // Rows in LDS: 16-byte pieces, of which row r has piece u at place u ^ k_swap(r) (keys) or u ^ v_swap(r) (values).
+  // Keys are read a piece of 16 rows at once, 16-bit values 4 pieces of 4 rows, f32 values 8 pieces of
+  // rows 4 apart: each time all banks.
+  static constexpr int ROW = HDP * SZ, PPR = ROW / 16;
+  __device__ static __forceinline__ int k_swap(int r) { return PPR == 8 ? r >> 1 & 7 : r & 15; }
+  __device__ static __forceinline__ int v_swap(int r) {
+    return SZ == 4 ? (r >> 2 & 1) << 3 : PPR == 8 ? (r >> 1 & 1) << 2 : (r & 3) << 2;
+  }
+  static constexpr int BUF = 2 * KT * ROW;
   static constexpr int NBUF = 2 * BUF <= 158 * 1024 ? 2 : 1;
+  static constexpr int LD = HDP + 4;                                        // a row of the waves' sums, in the same place
+  static constexpr int SUMS = WK > 1 ? 4 * 32 * (LD * 4 + 8) : 0;
+  static constexpr int LDS = NBUF * BUF > SUMS ? NBUF * BUF : SUMS;
   static constexpr int RPW = KT / 4;  // rows a wave brings
   // pieces of 16 bytes in LDS that a lane brings of keys (and of values); of a 4-bit cache, units of UE elements
-  static constexpr int PPR = HDP * SZ / 16, NPC = RPW * PPR / 64;
+  static constexpr int NPC = RPW * PPR / 64;
   static constexpr int UE = RPW * HDP / 64 < 32 ? RPW * HDP / 64 : 32, UPR = HDP / UE, NU = RPW * UPR / 64;
   static constexpr int QW = CT == BB_F32 ? HDP / 2 : NQ * HDP / 4;  // registers of the query rows
   static constexpr int REGS = HDP / 2 + QW + 16 * NT + (CT == BB_F32 ? 0 : 8 * NP * NT) +
-                              (KV4 ? 2 * NU * (UE / 8 + 1) : 8 * NPC);
-  static constexpr int WAVES = REGS <= 208 && NBUF * BUF <= 79 * 1024 ? 2 : 1;  // of a SIMD
+                              (KV4 ? 2 * NU * (UE / 8 + 1) : 0);
+  static constexpr int WAVES = REGS <= 208 && LDS <= 79 * 1024 ? 2 : 1;  // of a SIMD
 };
+
+__device__ __attribute__((aligned(16))) uint32_t g_zeros[4];
+// 16 bytes of every lane from its own address to lds + 16·lane.
+__device__ __forceinline__ void to_lds(const char* from, char* lds) {
+  typedef __attribute__((address_space(1))) const uint32_t* global_u32;
+  typedef __attribute__((address_space(3))) uint32_t* lds_u32;
+  __builtin_amdgcn_global_load_lds((global_u32)(from), (lds_u32)(lds), 16, 0, 0);
+}
+// All of a wave's loads into LDS are there, for the waves behind the barrier that follows.
+__device__ __forceinline__ void landed() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
 
 __device__ __forceinline__ float half_max(float x) {
   auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -69,8 +89,9 @@ __device__ __forceinline__ float tanh_of(float y) {
   const float a = fabsf(y), z = y * y;
   const float e = __builtin_amdgcn_exp2f((a > 15.0f ? 15.0f : a) * (2.0f * LOG2E));
   const bool small = a < 0.6f;
-  const float num = small ? a * (945.0f + z * (105.0f + z)) : e - 1.0f;
-  const float den = small ? 945.0f + z * (420.0f + 15.0f * z) : e + 1.0f;
+  float n0 = a * (fmaf(z, 105.0f + z, 945.0f)), d0 = fmaf(z, fmaf(z, 15.0f, 420.0f), 945.0f), n1 = e - 1.0f, d1 = e + 1.0f;
+  asm("" : "+v"(n0), "+v"(d0), "+v"(n1), "+v"(d1));  // (both in line: a branch each would cost more)
+  const float num = small ? n0 : n1, den = small ? d0 : d1;
   return copysignf(num * __builtin_amdgcn_rcpf(den), y);
 }
 
@@ -102,7 +123,6 @@ struct PpWave {
   v4u q[NQ][HDP / 16];
   v4f qf[CT == BB_F32 ? HDP / 8 : 1];
   v16f o[HDP / 32];
-  v4u sk[KV4 ? 1 : S::NPC], sv[KV4 ? 1 : S::NPC];
   uint32_t ck[KV4 ? S::NU * S::UE / 8 : 1], cv[KV4 ? S::NU * S::UE / 8 : 1], hk[KV4 ? S::NU : 1], hv[KV4 ? S::NU : 1];
   int page, in;               // of the row that the lane finds for its wave (page -1: not there)
 
@@ -168,10 +188,11 @@ struct PpWave {
     }
   }
 
-  // Asks for the rows found. Returns which of the wave's rows are there.
-  __device__ __forceinline__ uint32_t load() {
+  // Asks for the rows found: 4-bit ones into registers, others straight into the tiles at `lds`, 1024 bytes an
+  // instruction, each lane a piece (zeros where nothing is). Returns which of the wave's rows are there.
+  __device__ __forceinline__ uint32_t load(char* lds) {
     const bool there = (uint32_t)page < (uint32_t)kv.n_pages;
-    const uint32_t ok = (uint32_t)__ballot(there) & (S::RPW == 32 ? ~0u : (1u << S::RPW) - 1);
+    const uint32_t ok = (uint32_t)__ballot(there) & (~0u >> (32 - S::RPW));
     if constexpr (KV4) {
       const size_t at = there ? (size_t)(uint32_t)page * kv.page_stride + kv_off : 0;
       const uint32_t alo = (uint32_t)at, ahi = (uint32_t)(at >> 32);
@@ -198,42 +219,38 @@ struct PpWave {
                                            (size_t)(uint32_t)in * kv.pos_stride + kv_off)
                                : -1;
       const uint32_t alo = (uint32_t)at, ahi = (uint32_t)(at >> 32);
+      char* lk = lds + wv * S::RPW * S::ROW;
 #pragma unroll
       for (int p = 0; p < S::NPC; ++p) {
-        const int e = p * 64 + lane, r = e / S::PPR, d = e % S::PPR * (16 / SZ);
+        const int e = p * 64 + lane, r = e / S::PPR, u = e % S::PPR, rr = wv * S::RPW + r;
         const int64_t base = (int64_t)((uint64_t)(uint32_t)__shfl((int)ahi, r) << 32 | (uint32_t)__shfl((int)alo, r));
-        sk[p] = sv[p] = v4u{0, 0, 0, 0};
-        if (base >= 0 && d < kv.hd) {
-          sk[p] = *reinterpret_cast<const v4u*>(static_cast<const char*>(kv.k) + (size_t)(base + d) * SZ);
-          sv[p] = *reinterpret_cast<const v4u*>(static_cast<const char*>(kv.v) + (size_t)(base + d) * SZ);
-        }
+        const int dk = (u ^ S::k_swap(rr)) * (16 / SZ), dv = (u ^ S::v_swap(rr)) * (16 / SZ);
+        const auto from = [&](const void* pool, int d) {
+          uint64_t a = reinterpret_cast<uint64_t>(pool) + (uint64_t)(base + d) * SZ;
+          asm("" : "+v"(a));  // (a select, no branch)
+          return reinterpret_cast<const char*>(base >= 0 && d < kv.hd ? a : reinterpret_cast<uint64_t>(g_zeros));
+        };
+        to_lds(from(kv.k, dk), lk + p * 1024);
+        to_lds(from(kv.v, dv), lk + S::KT * S::ROW + p * 1024);
       }
     }
     return ok;
   }
 
-  // Puts the rows asked for into LDS.
+  // Puts 4-bit rows into the tiles, as the f16 values they stand for.
   __device__ __forceinline__ void put(char* lds) const {
-    char* lk = lds + wv * S::RPW * S::KS;
-    char* lv = lds + S::KT * S::KS + wv * S::RPW * S::VS;
     if constexpr (KV4) {
 #pragma unroll
       for (int p = 0; p < S::NU; ++p) {
-        const int e = p * 64 + lane, r = e / S::UPR, u = e % S::UPR;
+        const int e = p * 64 + lane, r = wv * S::RPW + e / S::UPR, u = e % S::UPR;
         const Kv4Block bk(hk[p]), bv(hv[p]);
+        char* lk = lds + r * S::ROW;
 #pragma unroll
         for (int w = 0; w < S::UE / 8; ++w) {
-          const int at = (u * S::UE + 8 * w) * 2;
-          *reinterpret_cast<v4u*>(lk + r * S::KS + at) = bk.natural(ck[p * S::UE / 8 + w]);
-          *reinterpret_cast<v4u*>(lv + r * S::VS + at) = bv.natural(cv[p * S::UE / 8 + w]);
+          const int piece = u * (S::UE / 8) + w;
+          *reinterpret_cast<v4u*>(lk + (piece ^ S::k_swap(r)) * 16) = bk.natural(ck[p * S::UE / 8 + w]);
+          *reinterpret_cast<v4u*>(lk + S::KT * S::ROW + (piece ^ S::v_swap(r)) * 16) = bv.natural(cv[p * S::UE / 8 + w]);
         }
-      }
-    } else {
-#pragma unroll
-      for (int p = 0; p < S::NPC; ++p) {
-        const int e = p * 64 + lane, r = e / S::PPR, at = e % S::PPR * 16;
-        *reinterpret_cast<v4u*>(lk + r * S::KS + at) = sk[p];
-        *reinterpret_cast<v4u*>(lv + r * S::VS + at) = sv[p];
       }
     }
   }
@@ -245,18 +262,20 @@ struct PpWave {
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[t][e] = 0.0f;
-      const char* at = lk + (wk * S::BN + 32 * t + col) * S::KS + 16 * half;
+      const int r = wk * S::BN + 32 * t + col;
+      const char* at = lk + r * S::ROW;
+      const int swap = S::k_swap(r);
       if constexpr (CT == BB_F32) {
 #pragma unroll
         for (int j = 0; j < HDP / 8; ++j) {
-          const v4f a = *reinterpret_cast<const v4f*>(at + 32 * j);
+          const v4f a = *reinterpret_cast<const v4f*>(at + ((2 * j + half) ^ swap) * 16);
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], qf[j][e], x[t], 0, 0, 0);
         }
       } else {
 #pragma unroll
         for (int j = 0; j < HDP / 16; ++j) {
-          const v4u a = *reinterpret_cast<const v4u*>(at + 32 * j);
+          const v4u a = *reinterpret_cast<const v4u*>(at + ((2 * j + half) ^ swap) * 16);
 #pragma unroll
           for (int k = PARTS - 1; k >= 0; --k) x[t] = mfma32<CT>(a, q[k][j], x[t]);
         }
@@ -266,21 +285,26 @@ struct PpWave {
 
   // Elements 32·dt + lane % 32 of the values at the keys whose weights are registers 8s..8s+7 of a tile (16-bit types).
   __device__ __forceinline__ v4u values(const char* lv, int t, int s, int dt) const {
-    const char* at = lv + (wk * S::BN + 32 * t + 16 * s + 4 * half + (lane & 15) / 4) * S::VS +
-                     (32 * dt + (lane & 16) + 4 * (lane & 3)) * 2;
+    const int r = wk * S::BN + 32 * t + 16 * s + 4 * half + (lane & 15) / 4;
+    const int piece = 4 * dt + (lane & 16) / 8 + (lane & 2) / 2;
+    const char* at = lv + r * S::ROW + (piece ^ S::v_swap(r)) * 16 + (lane & 1) * 8;
     typedef __attribute__((address_space(3))) v4s* lds_v4s;
     const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at));
-    const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at + 8 * S::VS));
+    const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at + 8 * S::ROW));
     const v2u x = __builtin_bit_cast(v2u, a), y = __builtin_bit_cast(v2u, b);
     return v4u{x[0], x[1], y[0], y[1]};
   }
   // (the same of an f32 cache: at the key of register e)
   __device__ __forceinline__ float value(const char* lv, int t, int e, int dt) const {
-    return *reinterpret_cast<const float*>(lv + (wk * S::BN + 32 * t + 8 * (e / 4) + 4 * half + e % 4) * S::VS +
-                                           (32 * dt + col) * 4);
+    const int r = wk * S::BN + 32 * t + 8 * (e / 4) + 4 * half + e % 4;
+    return *reinterpret_cast<const float*>(lv + r * S::ROW + ((8 * dt + col / 4) ^ S::v_swap(r)) * 16 + col % 4 * 4);
   }
 
-  __device__ __forceinline__ bool sees(int j) const { return (j <= i && j >= lo) || j < prefix; }
+  // Which of 32 keys from j0 on the row sees, of those in `ok`: the bits of the lane's registers e at 8(e / 4) + e % 4.
+  __device__ __forceinline__ uint32_t seen(int j0, uint32_t ok) const {
+    const auto below = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; };  // keys 0..n-1
+    return ((below(i + 1 - j0) & ~below(lo - j0)) | below(prefix - j0)) & ok;
+  }
 
   // One tile: keys from j0 on, `ok` those that are there. Values that are not finite reach the rows that see them and no
   // others: where a tile is not seen whole by all rows of the wave, its values are looked at first, and where one is
@@ -323,22 +347,20 @@ struct PpWave {
         for (int e = 0; e < 16; ++e) x[t][e] *= c;
     }
     if (pq.slopes) {
+      const float away = (float)(i - j0 - 4 * half);
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int j = j0 + 32 * t + 8 * (e / 4) + 4 * half + e % 4;
-          x[t][e] = fmaf(-slope, fabsf((float)(i - j)), x[t][e]);
-        }
+        for (int e = 0; e < 16; ++e)
+          x[t][e] = fmaf(-slope, fabsf(away - (float)(32 * t + 8 * (e / 4) + e % 4)), x[t][e]);
     }
     if (!whole) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t) {
+        const uint32_t see = seen(j0 + 32 * t, t ? ok1 : ok0) >> 4 * half;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int k = 8 * (e / 4) + 4 * half + e % 4;
-          x[t][e] = ((t ? ok1 : ok0) >> k & 1) && sees(j0 + 32 * t + k) ? x[t][e] : NEG_INF;
-        }
+        for (int e = 0; e < 16; ++e) x[t][e] = see >> (8 * (e / 4) + e % 4) & 1 ? x[t][e] : NEG_INF;
+      }
     }
     float mx = NEG_INF;
 #pragma unroll
@@ -346,9 +368,11 @@ struct PpWave {
 #pragma unroll
       for (int e = 0; e < 16; ++e) mx = fmaxf(mx, x[t][e]);
     mx = half_max(mx) * by;
-    mx = fmaxf(m, mx);
+    // (m stays until a score is SLACK past it: the sums are as exact, and seldom multiplied)
+    const bool past = mx > m + SLACK;
+    mx = past ? mx : m;
     const float ref = mx == NEG_INF ? 0.0f : mx;
-    if (__any(mx > m)) {
+    if (__any(past)) {
       const float f = __builtin_amdgcn_exp2f(m - ref);
       l *= f;
 #pragma unroll
@@ -357,8 +381,7 @@ struct PpWave {
         for (int e = 0; e < 16; ++e) o[d][e] *= f;
     }
     m = mx;
-    // (f16: weights up to 2^14, so that its range costs at most 2^-38 of the largest)
-    const float less = F16 ? 14.0f - ref : -ref;
+    const float less = F16 ? F16_UP - ref : -ref;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -366,14 +389,12 @@ struct PpWave {
         x[t][e] = __builtin_amdgcn_exp2f(fmaf(x[t][e], by, less));
         l += x[t][e];
       }
-    bool odd = false;
-    if (!whole) odd = values_odd(lv);
-    if constexpr (CT == BB_F32) {
-      add_f32(lv, x, odd);
+    if (whole || !values_odd(lv)) {
+      add<false>(lv, x);
     } else {
-      add_16(lv, x, odd);
+      add<true>(lv, x);
+      mark(lv, j0, ok0, ok1);
     }
-    if (odd) mark(lv, j0, ok0, ok1);
   }
 
   __device__ __forceinline__ bool values_odd(const char* lv) const {
@@ -397,43 +418,44 @@ struct PpWave {
     return __any(odd);
   }
 
-  __device__ __forceinline__ void add_16(const char* lv, const v16f (&x)[NT], bool odd) {
+  // The values times their weights x (ODD: those that are finite).
+  template <bool ODD>
+  __device__ __forceinline__ void add(const char* lv, const v16f (&x)[NT]) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < NT; ++t) {
+      if constexpr (CT == BB_F32) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        v4u p[NP];
+        for (int e = 0; e < 16; ++e)
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          uint32_t w[NP];
-          split2<CT, NP>(x[t][8 * s + e], x[t][8 * s + e + 1], w);
+          for (int d = 0; d < HDP / 32; ++d) {
+            float a = value(lv, t, e, d);
+            if (ODD) a = fabsf(a) < __builtin_inff() ? a : 0.0f;
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, x[t][e], o[d], 0, 0, 0);
+          }
+      } else {
 #pragma unroll
-          for (int k = 0; k < NP; ++k) p[k][e / 2] = w[k];
-        }
+        for (int s = 0; s < 2; ++s) {
+          v4u p[NP];
 #pragma unroll
-        for (int d = 0; d < HDP / 32; ++d) {
-          v4u a = values(lv, t, s, d);
-          if (odd) {
+          for (int e = 0; e < 8; e += 2) {
+            uint32_t w[NP];
+            split2<CT, NP>(x[t][8 * s + e], x[t][8 * s + e + 1], w);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) a[w] = fine_halves(a[w], odd_halves<CT>(a[w]));
+            for (int k = 0; k < NP; ++k) p[k][e / 2] = w[k];
           }
 #pragma unroll
-          for (int k = NP - 1; k >= 0; --k) o[d] = mfma32<CT>(a, p[k], o[d]);
+          for (int d = 0; d < HDP / 32; ++d) {
+            v4u a = values(lv, t, s, d);
+            if constexpr (ODD) {
+#pragma unroll
+              for (int w = 0; w < 4; ++w) a[w] = fine_halves(a[w], odd_halves<CT>(a[w]));
+            }
+#pragma unroll
+            for (int k = NP - 1; k >= 0; --k) o[d] = mfma32<CT>(a, p[k], o[d]);
+          }
         }
       }
-  }
-
-  __device__ __forceinline__ void add_f32(const char* lv, const v16f (&x)[NT], bool odd) {
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-#pragma unroll
-        for (int d = 0; d < HDP / 32; ++d) {
-          float a = value(lv, t, e, d);
-          if (odd) a = fabsf(a) < __builtin_inff() ? a : 0.0f;
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, x[t][e], o[d], 0, 0, 0);
-        }
+    }
   }
 
   // NaN for the sums that a value which is not finite belongs to: how many each row sees of them, by the same products.
@@ -445,17 +467,13 @@ struct PpWave {
       for (int e = 0; e < 16; ++e) n[e] = 0.0f;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        uint32_t see = 0;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int k = 8 * (e / 4) + 4 * half + e % 4;
-          see |= (((t ? ok1 : ok0) >> k & 1) && sees(j0 + 32 * t + k) ? 1u : 0u) << e;
-        }
+        const uint32_t see = seen(j0 + 32 * t, t ? ok1 : ok0) >> 4 * half;
+        const auto bit = [&](int e) { return see >> (8 * (e / 4) + e % 4) & 1; };
         if constexpr (CT == BB_F32) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const float a = fabsf(value(lv, t, e, d)) < __builtin_inff() ? 0.0f : 1.0f;
-            n = __builtin_amdgcn_mfma_f32_32x32x2f32(a, (float)(see >> e & 1), n, 0, 0, 0);
+            n = __builtin_amdgcn_mfma_f32_32x32x2f32(a, (float)bit(e), n, 0, 0, 0);
           }
         } else {
           constexpr uint32_t ONE = CT == BB_BF16 ? 0x3f80u : 0x3c00u;
@@ -465,7 +483,7 @@ struct PpWave {
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
               a[w] = odd_halves<CT>(a[w]);
-              p[w] = (see >> (8 * s + 2 * w) & 1 ? ONE : 0u) | (see >> (8 * s + 2 * w + 1) & 1 ? ONE << 16 : 0u);
+              p[w] = (bit(8 * s + 2 * w) ? ONE : 0u) | (bit(8 * s + 2 * w + 1) ? ONE << 16 : 0u);
             }
             n = mfma32<CT>(a, p, n);
           }
@@ -481,7 +499,7 @@ template <int CT, int NQ, int NP, int HDP, int WR, bool KV4>
 __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>::WAVES))
     k_paged_prompt(PromptQuery pq, PagedView kv, PagedSeqs sq, PromptPlan pl) {
   typedef PpShape<CT, NQ, NP, HDP, WR, KV4> S;
-  __shared__ __align__(16) char s_tiles[S::NBUF][S::BUF];
+  __shared__ __align__(1024) char s_tiles[S::LDS];
   __shared__ uint32_t s_ok[2][4];
   const int tid = threadIdx.x, lane = tid & 63;
   const int kvh = blockIdx.x % pl.n_kv, rest = blockIdx.x / pl.n_kv;
@@ -554,15 +572,20 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>
 
   if (u0 < u1) {
     w.find(kt.at(u0));
-    uint32_t ok = w.load();
+    uint32_t ok = w.load(s_tiles);
     if (u0 + 1 < u1) w.find(kt.at(u0 + 1));
-    w.put(s_tiles[0]);
+    w.put(s_tiles);
     if (lane == 0) s_ok[0][w.wv] = ok;
+    landed();
     __syncthreads();
     for (int u = u0; u < u1; ++u) {
       const int buf = S::NBUF == 2 ? (u - u0) & 1 : 0, flag = (u - u0) & 1;
-      if (u + 1 < u1) {
-        ok = w.load();
+      const char* tiles = s_tiles + buf * S::BUF;
+      char* next = s_tiles + (S::NBUF == 2 ? buf ^ 1 : 0) * S::BUF;
+      // (one buffer: other tiles than 4-bit ones come when all waves are done with this one)
+      constexpr bool EARLY = S::NBUF == 2 || KV4;
+      if (EARLY && u + 1 < u1) {
+        ok = w.load(next);
         if (u + 2 < u1) w.find(kt.at(u + 2));
       }
       uint32_t ok0, ok1 = ~0u;
@@ -578,11 +601,16 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>
       }
       ok0 = __builtin_amdgcn_readfirstlane(ok0);
       ok1 = __builtin_amdgcn_readfirstlane(ok1);
-      w.tile(s_tiles[buf], s_tiles[buf] + S::KT * S::KS, kt.at(u) * S::KT + w.wk * S::BN, ok0, ok1);
+      w.tile(tiles, tiles + S::KT * S::ROW, kt.at(u) * S::KT + w.wk * S::BN, ok0, ok1);
       if (u + 1 < u1) {
         if constexpr (S::NBUF == 1) __syncthreads();
-        w.put(s_tiles[S::NBUF == 2 ? buf ^ 1 : 0]);
+        if constexpr (!EARLY) {
+          ok = w.load(s_tiles);
+          if (u + 2 < u1) w.find(kt.at(u + 2));
+        }
+        w.put(next);
         if (lane == 0) s_ok[flag ^ 1][w.wv] = ok;
+        landed();
       }
       __syncthreads();
     }
@@ -591,8 +619,7 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>
 
   // the sums of the waves that share rows
   if constexpr (S::WK > 1) {
-    constexpr int LD = HDP + 4;
-    static_assert(S::WK * 32 * WR * (LD * 4 + 8) <= S::NBUF * S::BUF, "the sums fit the tiles' place");
+    constexpr int LD = S::LD;
     float* so = reinterpret_cast<float*>(s_tiles);
     float2* sm = reinterpret_cast<float2*>(so + 4 * 32 * LD);
     if (w.half == 0) sm[w.wv * 32 + w.col] = make_float2(w.m, w.l);
@@ -631,7 +658,7 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>
       }
   }
   if (mine >= rows) return;
-  const float up = CT == BB_F16 ? 14.0f : 0.0f;
+  const float up = CT == BB_F16 ? F16_UP : 0.0f;
   if (kp.used == 1) {
     const bool none = w.m == NEG_INF && w.l == 0.0f;
     const float f = none ? 0.0f : 1.0f / w.l;
@@ -718,7 +745,7 @@ size_t prompt_ws(const PromptCut& c, int n_kv, int hd) {
 template <int CT, int NQ, int NP, int HDP, int WR, bool KV4>
 hipError_t prompt_of(hipStream_t st, const PromptQuery& q, const PagedView& kv, const PagedSeqs& sq, PromptPlan pl) {
   typedef PpShape<CT, NQ, NP, HDP, WR, KV4> S;
-  if constexpr (S::BUF * S::NBUF > 160 * 1024) {
+  if constexpr (S::LDS > 159 * 1024) {
     return hipErrorInvalidValue;
   } else {
     // (no more parts than the table's width has of the least size)
@@ -730,7 +757,7 @@ hipError_t prompt_of(hipStream_t st, const PromptQuery& q, const PagedView& kv, 
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || pl.parts == 1) return e;
     BB_LAUNCH(k_prompt_join, dim3(pl.n_tiles * pl.n_kv, S::BM / (PP_THREADS / 64)), dim3(PP_THREADS), 0, st, q, kv.hd,
-              S::BM, pl, CT == BB_F16 ? 14.0f : 0.0f);
+              S::BM, pl, CT == BB_F16 ? F16_UP : 0.0f);
     return hipGetLastError();
   }
 }
