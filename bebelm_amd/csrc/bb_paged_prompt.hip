@@ -10,6 +10,7 @@ namespace bb {
 namespace {
 
 constexpr int PP_THREADS = 256;
+#define BB_INLINE __attribute__((always_inline))
 // Weights go up to 2^SLACK, as f16 to 2^(SLACK + F16_UP) = 2^14, whose range then costs at most 2^-33 of the largest.
 constexpr float SLACK = 6.0f, F16_UP = 8.0f;
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -29,13 +30,13 @@ struct PpShape {
   static constexpr int ROW = HDP * SZ, PPR = ROW / 16;
   __device__ static __forceinline__ int k_swap(int r) { return PPR == 8 ? r >> 1 & 7 : r & 15; }
   __device__ static __forceinline__ int v_swap(int r) {
-    return SZ == 4 ? (r >> 2 & 1) << 3 : PPR == 8 ? (r >> 1 & 1) << 2 : (r & 3) << 2;
+    return SZ == 4 ? (r >> 2 & 1) << 3 : (PPR == 8 ? (r >> 1 & 1) << 2 : (r & 3) << 2) | (r >> 2 & 3);
   }
   static constexpr int BUF = 2 * KT * ROW;
-  static constexpr int NBUF = 2 * BUF <= 158 * 1024 ? 2 : 1;
+  // (two of them: an iteration reads the keys of the next tile and the values of its own)
   static constexpr int LD = HDP + 4;                                        // a row of the waves' sums, in the same place
   static constexpr int SUMS = WK > 1 ? 4 * 32 * (LD * 4 + 8) : 0;
-  static constexpr int LDS = NBUF * BUF > SUMS ? NBUF * BUF : SUMS;
+  static constexpr int LDS = 2 * BUF > SUMS ? 2 * BUF : SUMS;
   static constexpr int RPW = KT / 4;  // rows a wave brings
   // pieces of 16 bytes in LDS that a lane brings of keys (and of values); of a 4-bit cache, units of UE elements
   static constexpr int NPC = RPW * PPR / 64;
@@ -52,6 +53,18 @@ __device__ __forceinline__ void to_lds(const char* from, char* lds) {
   typedef __attribute__((address_space(1))) const uint32_t* global_u32;
   typedef __attribute__((address_space(3))) uint32_t* lds_u32;
   __builtin_amdgcn_global_load_lds((global_u32)(from), (lds_u32)(lds), 16, 0, 0);
+}
+__device__ __forceinline__ uint32_t lds_at(const char* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)(p);
+}
+template <class T>
+__device__ __forceinline__ T read_lds(uint32_t at) {
+  return *(const __attribute__((address_space(3))) T*)(uintptr_t)(at);
+}
+// (an address that is made again for every tile: dozens that follow from it would each take a register otherwise)
+__device__ __forceinline__ uint32_t fresh(uint32_t a) {
+  asm volatile("" : "+v"(a));
+  return a;
 }
 // All of a wave's loads into LDS are there, for the waves behind the barrier that follows.
 __device__ __forceinline__ void landed() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
@@ -90,7 +103,8 @@ __device__ __forceinline__ float tanh_of(float y) {
   const float e = __builtin_amdgcn_exp2f((a > 15.0f ? 15.0f : a) * (2.0f * LOG2E));
   const bool small = a < 0.6f;
   float n0 = a * (fmaf(z, 105.0f + z, 945.0f)), d0 = fmaf(z, fmaf(z, 15.0f, 420.0f), 945.0f), n1 = e - 1.0f, d1 = e + 1.0f;
-  asm("" : "+v"(n0), "+v"(d0), "+v"(n1), "+v"(d1));  // (both in line: a branch each would cost more)
+  // (both in line: a branch each would cost more; and not done where a call has no cap)
+  asm volatile("" : "+v"(n0), "+v"(d0), "+v"(n1), "+v"(d1));
   const float num = small ? n0 : n1, den = small ? d0 : d1;
   return copysignf(num * __builtin_amdgcn_rcpf(den), y);
 }
@@ -123,7 +137,13 @@ struct PpWave {
   v4u q[NQ][HDP / 16];
   v4f qf[CT == BB_F32 ? HDP / 8 : 1];
   v16f o[HDP / 32];
-  uint32_t ck[KV4 ? S::NU * S::UE / 8 : 1], cv[KV4 ? S::NU * S::UE / 8 : 1], hk[KV4 ? S::NU : 1], hv[KV4 ? S::NU : 1];
+  struct Codes {
+    uint32_t word[KV4 ? S::NU * S::UE / 8 : 1], head[KV4 ? S::NU : 1];
+  };
+  Codes ck, cv;
+  v16f x[NT];                 // scores of the tile at work (base `by` of them), then its weights
+  float by;
+  float top;                  // the largest
   int page, in;               // of the row that the lane finds for its wave (page -1: not there)
 
   __device__ __forceinline__ PpWave(const PagedView& kv_, const PromptQuery& pq_, int tid)
@@ -188,116 +208,136 @@ struct PpWave {
     }
   }
 
-  // Asks for the rows found: 4-bit ones into registers, others straight into the tiles at `lds`, 1024 bytes an
-  // instruction, each lane a piece (zeros where nothing is). Returns which of the wave's rows are there.
-  __device__ __forceinline__ uint32_t load(char* lds) {
+  // Where the row found is in the pool (elements; of 4 bits, bytes to its (page, head)).
+  struct Row {
+    int64_t at;  // -1: not there
+    int pos;     // 4 bits: its position in the page
+  };
+  __device__ __forceinline__ Row found() const {
     const bool there = (uint32_t)page < (uint32_t)kv.n_pages;
-    const uint32_t ok = (uint32_t)__ballot(there) & (~0u >> (32 - S::RPW));
+    const size_t at = (size_t)(uint32_t)page * kv.page_stride + (KV4 ? 0 : (size_t)(uint32_t)in * kv.pos_stride) + kv_off;
+    return Row{there ? (int64_t)at : -1, in};
+  }
+  // Which of the wave's rows are there.
+  static __device__ __forceinline__ uint32_t there(const Row& r) { return (uint32_t)__ballot(r.at >= 0) & (~0u >> (32 - S::RPW)); }
+
+  // Asks for the wave's rows of a tile, keys or values: 4-bit ones into registers, others straight into the tile at
+  // `lds`, 1024 bytes an instruction, each lane a piece (zeros where nothing is).
+  template <bool KEYS>
+  __device__ __forceinline__ void load(const Row& w, char* lds) {
+    const char* pool = static_cast<const char*>(KEYS ? kv.k : kv.v);
+    const uint32_t alo = (uint32_t)w.at, ahi = (uint32_t)(w.at >> 32);
+    const int own = (int)fresh((uint32_t)lane);
     if constexpr (KV4) {
-      const size_t at = there ? (size_t)(uint32_t)page * kv.page_stride + kv_off : 0;
-      const uint32_t alo = (uint32_t)at, ahi = (uint32_t)(at >> 32);
-      const int pos = there ? in : -1;
+      Codes& c = KEYS ? ck : cv;
 #pragma unroll
       for (int p = 0; p < S::NU; ++p) {
-        const int e = p * 64 + lane, r = e / S::UPR, u = e % S::UPR, d = u * S::UE;
-        const size_t base = (size_t)__shfl((int)ahi, r) << 32 | (uint32_t)__shfl((int)alo, r);
-        const int rp = __shfl(pos, r);
-        hk[p] = hv[p] = 0;
+        const int e = p * 64 + own, r = e / S::UPR, u = e % S::UPR, d = u * S::UE;
+        const int64_t base = (int64_t)((uint64_t)(uint32_t)__shfl((int)ahi, r) << 32 | (uint32_t)__shfl((int)alo, r));
+        const int rp = __shfl(w.pos, r);
+        c.head[p] = 0;
 #pragma unroll
-        for (int w = 0; w < S::UE / 8; ++w) ck[p * S::UE / 8 + w] = cv[p * S::UE / 8 + w] = 0;
-        if (rp >= 0 && d < kv.hd) {
-          const size_t codes = base + (size_t)(uint32_t)(rp * (kv.hd / 2) + d / 2);
-          const size_t head = base + (size_t)(uint32_t)kv4_head_at(kv, rp, d / 32);
-          load_words<S::UE / 8>(static_cast<const char*>(kv.k) + codes, ck + p * S::UE / 8);
-          load_words<S::UE / 8>(static_cast<const char*>(kv.v) + codes, cv + p * S::UE / 8);
-          hk[p] = *reinterpret_cast<const uint16_t*>(static_cast<const char*>(kv.k) + head);
-          hv[p] = *reinterpret_cast<const uint16_t*>(static_cast<const char*>(kv.v) + head);
+        for (int i = 0; i < S::UE / 8; ++i) c.word[p * S::UE / 8 + i] = 0;
+        if (base >= 0 && d < kv.hd) {
+          load_words<S::UE / 8>(pool + base + (size_t)(uint32_t)(rp * (kv.hd / 2) + d / 2), c.word + p * S::UE / 8);
+          c.head[p] = *reinterpret_cast<const uint16_t*>(pool + base + (size_t)(uint32_t)kv4_head_at(kv, rp, d / 32));
         }
       }
     } else {
-      const int64_t at = there ? (int64_t)((size_t)(uint32_t)page * kv.page_stride +
-                                           (size_t)(uint32_t)in * kv.pos_stride + kv_off)
-                               : -1;
-      const uint32_t alo = (uint32_t)at, ahi = (uint32_t)(at >> 32);
-      char* lk = lds + wv * S::RPW * S::ROW;
 #pragma unroll
       for (int p = 0; p < S::NPC; ++p) {
-        const int e = p * 64 + lane, r = e / S::PPR, u = e % S::PPR, rr = wv * S::RPW + r;
+        const int e = p * 64 + own, r = e / S::PPR, u = e % S::PPR, rr = wv * S::RPW + r;
         const int64_t base = (int64_t)((uint64_t)(uint32_t)__shfl((int)ahi, r) << 32 | (uint32_t)__shfl((int)alo, r));
-        const int dk = (u ^ S::k_swap(rr)) * (16 / SZ), dv = (u ^ S::v_swap(rr)) * (16 / SZ);
-        const auto from = [&](const void* pool, int d) {
-          uint64_t a = reinterpret_cast<uint64_t>(pool) + (uint64_t)(base + d) * SZ;
-          asm("" : "+v"(a));  // (a select, no branch)
-          return reinterpret_cast<const char*>(base >= 0 && d < kv.hd ? a : reinterpret_cast<uint64_t>(g_zeros));
-        };
-        to_lds(from(kv.k, dk), lk + p * 1024);
-        to_lds(from(kv.v, dv), lk + S::KT * S::ROW + p * 1024);
+        const int d = (u ^ (KEYS ? S::k_swap(rr) : S::v_swap(rr))) * (16 / SZ);
+        uint64_t a = reinterpret_cast<uint64_t>(pool) + (uint64_t)(base + d) * SZ;
+        asm("" : "+v"(a));  // (a select, no branch)
+        a = base >= 0 && d < kv.hd ? a : reinterpret_cast<uint64_t>(g_zeros);
+        to_lds(reinterpret_cast<const char*>(a), lds + wv * S::RPW * S::ROW + p * 1024);
       }
     }
-    return ok;
   }
 
-  // Puts 4-bit rows into the tiles, as the f16 values they stand for.
+  // Puts 4-bit rows into a tile, as the f16 values they stand for.
+  template <bool KEYS>
   __device__ __forceinline__ void put(char* lds) const {
     if constexpr (KV4) {
+      const Codes& c = KEYS ? ck : cv;
+      const int own = (int)fresh((uint32_t)lane);
 #pragma unroll
       for (int p = 0; p < S::NU; ++p) {
-        const int e = p * 64 + lane, r = wv * S::RPW + e / S::UPR, u = e % S::UPR;
-        const Kv4Block bk(hk[p]), bv(hv[p]);
-        char* lk = lds + r * S::ROW;
+        const int e = p * 64 + own, r = wv * S::RPW + e / S::UPR, u = e % S::UPR;
+        const Kv4Block block(c.head[p]);
 #pragma unroll
         for (int w = 0; w < S::UE / 8; ++w) {
           const int piece = u * (S::UE / 8) + w;
-          *reinterpret_cast<v4u*>(lk + (piece ^ S::k_swap(r)) * 16) = bk.natural(ck[p * S::UE / 8 + w]);
-          *reinterpret_cast<v4u*>(lk + S::KT * S::ROW + (piece ^ S::v_swap(r)) * 16) = bv.natural(cv[p * S::UE / 8 + w]);
+          *reinterpret_cast<v4u*>(lds + r * S::ROW + (piece ^ (KEYS ? S::k_swap(r) : S::v_swap(r))) * 16) =
+              block.natural(c.word[p * S::UE / 8 + w]);
         }
       }
     }
   }
 
-  // Scores of 32 keys for 32 rows: register e of lane (row, half) is key 8(e / 4) + 4·half + e % 4.
-  template <int PARTS>
-  __device__ __forceinline__ void scores(const char* lk, v16f (&x)[NT]) const {
+  // Scores of a tile: register e of lane (row, half) is key 8(e / 4) + 4·half + e % 4 of 32. between(j) is done with the
+  // products of the j-th of STEPS steps, whose keys have been asked for a step before.
+  static constexpr int STEPS = CT == BB_F32 ? HDP / 8 : HDP / 16;
+  template <int PARTS, class F>
+  __device__ __forceinline__ void scores(uint32_t lk, v16f (&y)[NT], F&& between) const {
+    const uint32_t at0 = fresh(lk + (wk * S::BN + col) * S::ROW + (half ^ S::k_swap(col)) * 16);
+    v4u a[2][NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[t][e] = 0.0f;
-      const int r = wk * S::BN + 32 * t + col;
-      const char* at = lk + r * S::ROW;
-      const int swap = S::k_swap(r);
-      if constexpr (CT == BB_F32) {
+      for (int e = 0; e < 16; ++e) y[t][e] = 0.0f;
+      a[0][t] = read_lds<v4u>(at0 + 32 * t * S::ROW);
+    }
 #pragma unroll
-        for (int j = 0; j < HDP / 8; ++j) {
-          const v4f a = *reinterpret_cast<const v4f*>(at + ((2 * j + half) ^ swap) * 16);
+    for (int j = 0; j < STEPS; ++j) {
+      if (j + 1 < STEPS)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], qf[j][e], x[t], 0, 0, 0);
-        }
-      } else {
+        for (int t = 0; t < NT; ++t) a[(j + 1) & 1][t] = read_lds<v4u>((at0 ^ 32 * (j + 1)) + 32 * t * S::ROW);
 #pragma unroll
-        for (int j = 0; j < HDP / 16; ++j) {
-          const v4u a = *reinterpret_cast<const v4u*>(at + ((2 * j + half) ^ swap) * 16);
+      for (int t = 0; t < NT; ++t) {
+        const v4u k = a[j & 1][t];
+        if constexpr (CT == BB_F32) {
 #pragma unroll
-          for (int k = PARTS - 1; k >= 0; --k) x[t] = mfma32<CT>(a, q[k][j], x[t]);
+          for (int e = 0; e < 4; ++e)
+            y[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(as_float(k[e]), qf[j][e], y[t], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int i = PARTS - 1; i >= 0; --i) y[t] = mfma32<CT>(k, q[i][j], y[t]);
         }
       }
+      between(j);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
+  // Where the lane's values begin: at the keys of its registers 0 to 3 and, 16-bit types, 4 to 7.
+  struct At {
+    uint32_t a, b;
+  };
+  __device__ __forceinline__ At values_at(uint32_t lv) const {
+    if constexpr (CT == BB_F32) {
+      const int r = 4 * half;
+      const uint32_t a = lv + (wk * S::BN + r) * S::ROW + (col / 4 ^ S::v_swap(r)) * 16 + col % 4 * 4;
+      return At{fresh(a), 0};
+    } else {
+      const int r = 4 * half + (lane & 15) / 4, piece = (lane & 16) / 8 + (lane & 2) / 2;
+      const uint32_t row = lv + (wk * S::BN + r) * S::ROW + (lane & 1) * 8;
+      return At{fresh(row + (piece ^ S::v_swap(r)) * 16), fresh(row + 8 * S::ROW + (piece ^ S::v_swap(r + 8)) * 16)};
+    }
+  }
   // Elements 32·dt + lane % 32 of the values at the keys whose weights are registers 8s..8s+7 of a tile (16-bit types).
-  __device__ __forceinline__ v4u values(const char* lv, int t, int s, int dt) const {
-    const int r = wk * S::BN + 32 * t + 16 * s + 4 * half + (lane & 15) / 4;
-    const int piece = 4 * dt + (lane & 16) / 8 + (lane & 2) / 2;
-    const char* at = lv + r * S::ROW + (piece ^ S::v_swap(r)) * 16 + (lane & 1) * 8;
+  __device__ __forceinline__ v4u values(At at, int t, int s, int dt) const {
     typedef __attribute__((address_space(3))) v4s* lds_v4s;
-    const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at));
-    const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at + 8 * S::ROW));
+    const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)((at.a ^ 64 * dt) + (32 * t + 16 * s) * S::ROW));
+    const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)((at.b ^ 64 * dt) + (32 * t + 16 * s) * S::ROW));
     const v2u x = __builtin_bit_cast(v2u, a), y = __builtin_bit_cast(v2u, b);
     return v4u{x[0], x[1], y[0], y[1]};
   }
   // (the same of an f32 cache: at the key of register e)
-  __device__ __forceinline__ float value(const char* lv, int t, int e, int dt) const {
-    const int r = wk * S::BN + 32 * t + 8 * (e / 4) + 4 * half + e % 4;
-    return *reinterpret_cast<const float*>(lv + r * S::ROW + ((8 * dt + col / 4) ^ S::v_swap(r)) * 16 + col % 4 * 4);
+  __device__ __forceinline__ float value(At at, int t, int e, int dt) const {
+    return read_lds<float>((at.a ^ 128 * dt) + (32 * t + 8 * (e / 4) + e % 4) * S::ROW);
   }
 
   // Which of 32 keys from j0 on the row sees, of those in `ok`: the bits of the lane's registers e at 8(e / 4) + e % 4.
@@ -306,45 +346,45 @@ struct PpWave {
     return ((below(i + 1 - j0) & ~below(lo - j0)) | below(prefix - j0)) & ok;
   }
 
-  // One tile: keys from j0 on, `ok` those that are there. Values that are not finite reach the rows that see them and no
-  // others: where a tile is not seen whole by all rows of the wave, its values are looked at first, and where one is
-  // not finite it counts as 0 in the sums and makes NaN of those of the rows that see it.
-  __device__ __forceinline__ void tile(const char* lk, const char* lv, int j0, uint32_t ok0, uint32_t ok1) {
-    if (j0 >= prefix && (j0 > i1 || j0 + S::BN <= first_seen(i0, pq.window))) return;
-    v16f x[NT];
-    scores<NQ>(lk, x);
+  // The scores of a tile of keys, into x.
+  template <class F>
+  __device__ __forceinline__ void score(uint32_t lk, F&& between) {
+    v16f y[NT];
+    scores<NQ>(lk, y, between);
     if constexpr (NQ > 1) {
       // a part of 0 meets an infinite key as NaN: such scores are taken from the first parts alone
       bool odd = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) odd |= x[t][e] != x[t][e];
+        for (int e = 0; e < 16; ++e) odd |= y[t][e] != y[t][e];
       if (__any(odd)) {
-        v16f y[NT];
-        scores<1>(lk, y);
+        v16f z[NT];
+        scores<1>(lk, z, [](int) {});
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (x[t][e] != x[t][e]) x[t][e] = y[t][e];
+          for (int e = 0; e < 16; ++e) y[t][e] = y[t][e] != y[t][e] ? z[t][e] : y[t][e];
       }
     }
-    const bool there = ok0 == ~0u && (NT == 1 || ok1 == ~0u);
-    const bool whole = there && ((j0 + S::BN - 1 <= i0 && j0 >= lo1) || j0 + S::BN <= prefix);
-    float by = c;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) x[t] = y[t];
+  }
+
+  // Whether all rows of the wave see all keys from j0 on, `ok` being those that are there.
+  __device__ __forceinline__ bool whole(int j0, uint32_t ok0, uint32_t ok1) const {
+    return ok0 == ~0u && (NT == 1 || ok1 == ~0u) && ((j0 + S::BN - 1 <= i0 && j0 >= lo1) || j0 + S::BN <= prefix);
+  }
+
+  // The scores capped, with their bias, hidden where the rows do not see the keys from j0 on, and the largest.
+  __device__ __forceinline__ void shape(int j0, uint32_t ok0, uint32_t ok1) {
+    by = c;
     if (pq.cap > 0.0f) {
       by = 1.0f;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[t][e] = (pq.cap * LOG2E) * tanh_of(x[t][e] * c);
-    } else if (pq.slopes) {
-      by = 1.0f;
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[t][e] *= c;
     }
     if (pq.slopes) {
       const float away = (float)(i - j0 - 4 * half);
@@ -352,9 +392,10 @@ struct PpWave {
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          x[t][e] = fmaf(-slope, fabsf(away - (float)(32 * t + 8 * (e / 4) + e % 4)), x[t][e]);
+          x[t][e] = fmaf(-slope, fabsf(away - (float)(32 * t + 8 * (e / 4) + e % 4)), x[t][e] * by);
+      by = 1.0f;
     }
-    if (!whole) {
+    if (!whole(j0, ok0, ok1)) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const uint32_t see = seen(j0 + 32 * t, t ? ok1 : ok0) >> 4 * half;
@@ -367,49 +408,63 @@ struct PpWave {
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int e = 0; e < 16; ++e) mx = fmaxf(mx, x[t][e]);
-    mx = half_max(mx) * by;
-    // (m stays until a score is SLACK past it: the sums are as exact, and seldom multiplied)
-    const bool past = mx > m + SLACK;
-    mx = past ? mx : m;
-    const float ref = mx == NEG_INF ? 0.0f : mx;
-    if (__any(past)) {
-      const float f = __builtin_amdgcn_exp2f(m - ref);
-      l *= f;
-#pragma unroll
-      for (int d = 0; d < HDP / 32; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[d][e] *= f;
-    }
+    top = half_max(mx) * by;
+  }
+
+  // The running maximum stays until a score is SLACK past it: the sums are as exact, and seldom multiplied.
+  __device__ __forceinline__ bool past() const { return __any(top > m + SLACK); }
+  __device__ __forceinline__ void raise() {
+    const float mx = top > m + SLACK ? top : m;
+    const float f = __builtin_amdgcn_exp2f(m - (mx == NEG_INF ? 0.0f : mx));
     m = mx;
-    const float less = F16 ? F16_UP - ref : -ref;
+    l *= f;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int d = 0; d < HDP / 32; ++d)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        x[t][e] = __builtin_amdgcn_exp2f(fmaf(x[t][e], by, less));
-        l += x[t][e];
+      for (int e = 0; e < 16; ++e) o[d][e] *= f;
+  }
+
+  // The weights of the tile, in 16 bits: register 2e of w[t][s][part] those of registers 8s + 2e and 8s + 2e + 1.
+  struct Weights {
+    v4u w[CT == BB_F32 ? 1 : NT][2][NP];
+    v16f f[CT == BB_F32 ? NT : 1];
+  };
+  // Those of pairs of registers lo..hi-1 (8 of each 32 keys).
+  __device__ __forceinline__ void weigh(Weights& p, int lo, int hi) {
+    const float less = (F16 ? F16_UP : 0.0f) - (m == NEG_INF ? 0.0f : m);
+#pragma unroll
+    for (int i = lo; i < hi; ++i) {
+      const int t = i / 8, e = i % 8 * 2;
+      const float a = __builtin_amdgcn_exp2f(fmaf(x[t][e], by, less)), b = __builtin_amdgcn_exp2f(fmaf(x[t][e + 1], by, less));
+      l += a;
+      l += b;
+      if constexpr (CT == BB_F32) {
+        p.f[t][e] = a;
+        p.f[t][e + 1] = b;
+      } else {
+        uint32_t w[NP];
+        split2<CT, NP>(a, b, w);
+#pragma unroll
+        for (int k = 0; k < NP; ++k) p.w[t][e / 8][k][e % 8 / 2] = w[k];
       }
-    if (whole || !values_odd(lv)) {
-      add<false>(lv, x);
-    } else {
-      add<true>(lv, x);
-      mark(lv, j0, ok0, ok1);
     }
   }
 
-  __device__ __forceinline__ bool values_odd(const char* lv) const {
+  // Whether the wave's part of a tile has values that are not finite.
+  __device__ __forceinline__ bool values_odd(uint32_t lv) const {
     bool odd = false;
+    const At at = values_at(lv);
 #pragma unroll 1
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int d = 0; d < HDP / 32; ++d) {
         if constexpr (CT == BB_F32) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) odd |= !(fabsf(value(lv, t, e, d)) < __builtin_inff());
+          for (int e = 0; e < 16; ++e) odd |= !(fabsf(value(at, t, e, d)) < __builtin_inff());
         } else {
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
-            const v4u a = values(lv, t, s, d);
+            const v4u a = values(at, t, s, d);
 #pragma unroll
             for (int w = 0; w < 4; ++w) odd |= odd_halves<CT>(a[w]) != 0;
           }
@@ -418,48 +473,40 @@ struct PpWave {
     return __any(odd);
   }
 
-  // The values times their weights x (ODD: those that are finite).
-  template <bool ODD>
-  __device__ __forceinline__ void add(const char* lv, const v16f (&x)[NT]) {
+  // The values times their weights.
+  __device__ __forceinline__ void add(uint32_t lv, const Weights& p) {
+    const At at = values_at(lv);
+    constexpr int ND = HDP / 32;
+    if constexpr (CT == BB_F32) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if constexpr (CT == BB_F32) {
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
 #pragma unroll
-          for (int d = 0; d < HDP / 32; ++d) {
-            float a = value(lv, t, e, d);
-            if (ODD) a = fabsf(a) < __builtin_inff() ? a : 0.0f;
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, x[t][e], o[d], 0, 0, 0);
-          }
-      } else {
+          for (int d = 0; d < ND; ++d)
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(value(at, t, e, d), p.f[t][e], o[d], 0, 0, 0);
+    } else {
+      v4u a[2][ND];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          v4u p[NP];
+      for (int d = 0; d < ND; ++d) a[0][d] = values(at, 0, 0, d);
 #pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            uint32_t w[NP];
-            split2<CT, NP>(x[t][8 * s + e], x[t][8 * s + e + 1], w);
+      for (int g = 0; g < 2 * NT; ++g) {
+        if (g + 1 < 2 * NT)
 #pragma unroll
-            for (int k = 0; k < NP; ++k) p[k][e / 2] = w[k];
-          }
+          for (int d = 0; d < ND; ++d) a[(g + 1) & 1][d] = values(at, (g + 1) / 2, (g + 1) % 2, d);
 #pragma unroll
-          for (int d = 0; d < HDP / 32; ++d) {
-            v4u a = values(lv, t, s, d);
-            if constexpr (ODD) {
+        for (int d = 0; d < ND; ++d)
 #pragma unroll
-              for (int w = 0; w < 4; ++w) a[w] = fine_halves(a[w], odd_halves<CT>(a[w]));
-            }
-#pragma unroll
-            for (int k = NP - 1; k >= 0; --k) o[d] = mfma32<CT>(a, p[k], o[d]);
-          }
-        }
+          for (int k = NP - 1; k >= 0; --k) o[d] = mfma32<CT>(a[g & 1][d], p.w[g / 2][g % 2][k], o[d]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
 
-  // NaN for the sums that a value which is not finite belongs to: how many each row sees of them, by the same products.
-  __device__ __forceinline__ void mark(const char* lv, int j0, uint32_t ok0, uint32_t ok1) {
+  // Which sums a value that is not finite belongs to, among those a row sees of a tile: bit e of the lane's bad[d], by
+  // products as those of the sums, of ones.
+  __device__ __forceinline__ void mark(uint32_t* bad, uint32_t lv, int j0, uint32_t ok0, uint32_t ok1) const {
+    const At at = values_at(lv);
 #pragma unroll
     for (int d = 0; d < HDP / 32; ++d) {
       v16f n;
@@ -468,18 +515,18 @@ struct PpWave {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const uint32_t see = seen(j0 + 32 * t, t ? ok1 : ok0) >> 4 * half;
-        const auto bit = [&](int e) { return see >> (8 * (e / 4) + e % 4) & 1; };
+        const auto bit = [&](int e) BB_INLINE { return see >> (8 * (e / 4) + e % 4) & 1; };
         if constexpr (CT == BB_F32) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float a = fabsf(value(lv, t, e, d)) < __builtin_inff() ? 0.0f : 1.0f;
+            const float a = fabsf(value(at, t, e, d)) < __builtin_inff() ? 0.0f : 1.0f;
             n = __builtin_amdgcn_mfma_f32_32x32x2f32(a, (float)bit(e), n, 0, 0, 0);
           }
         } else {
           constexpr uint32_t ONE = CT == BB_BF16 ? 0x3f80u : 0x3c00u;
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
-            v4u a = values(lv, t, s, d), p;
+            v4u a = values(at, t, s, d), p;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
               a[w] = odd_halves<CT>(a[w]);
@@ -489,8 +536,27 @@ struct PpWave {
           }
         }
       }
+      uint32_t bits = 0;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) o[d][e] = n[e] > 0.0f ? __builtin_nanf("") : o[d][e];
+      for (int e = 0; e < 16; ++e) bits |= (n[e] > 0.0f ? 1u : 0u) << e;
+      bad[d * PP_THREADS] = bits;
+    }
+  }
+  __device__ __forceinline__ void spoil(const uint32_t* bad) {
+#pragma unroll
+    for (int d = 0; d < HDP / 32; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[d][e] = bad[d * PP_THREADS] >> e & 1 ? __builtin_nanf("") : o[d][e];
+  }
+  // The wave's share of a tile of values without those that are not finite.
+  __device__ __forceinline__ void clean(char* lv) const {
+    for (int i = wv * 64 + lane; i < S::KT * S::PPR; i += PP_THREADS) {
+      v4u* p = reinterpret_cast<v4u*>(lv + i * 16);
+      v4u a = *p;
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        a[w] = CT == BB_F32 ? (a[w] & 0x7f800000u) == 0x7f800000u ? 0u : a[w] : fine_halves(a[w], odd_halves<CT>(a[w]));
+      *p = a;
     }
   }
 };
@@ -501,6 +567,7 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>
   typedef PpShape<CT, NQ, NP, HDP, WR, KV4> S;
   __shared__ __align__(1024) char s_tiles[S::LDS];
   __shared__ uint32_t s_ok[2][4];
+  __shared__ uint32_t s_marks[2][HDP / 32][PP_THREADS];
   const int tid = threadIdx.x, lane = tid & 63;
   const int kvh = blockIdx.x % pl.n_kv, rest = blockIdx.x / pl.n_kv;
   const int part = rest % pl.parts, g = rest / pl.parts;
@@ -531,7 +598,8 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>
     return;
   }
 
-  PpWave<CT, NQ, NP, HDP, WR, KV4> w(kv, pq, tid);
+  typedef PpWave<CT, NQ, NP, HDP, WR, KV4> Wave;
+  Wave w(kv, pq, tid);
   const int raw = sq.lens[s], end = pq.seq_start ? pq.seq_start[s + 1] : s + 1;
   w.len = min(max(raw, 0), sq.max_pages * kv.page_size);
   w.prefix = pq.prefix ? min(max(pq.prefix[s], 0), w.len) : 0;
@@ -570,50 +638,109 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>
     w.c = fmaxf(w.c, 1e-37f);  // (0 times an infinite score would be NaN)
   }
 
+  // Tiles u0..u1-1. Turn u takes the scores of tile u + 1 while it weighs tile u, whose values it then adds, and asks for
+  // the keys of tile u + 2 and the values of tile u + 1, which a barrier later are there. What is seldom done to
+  // the sums stands outside the loop over plain turns, which keeps them in their registers.
   if (u0 < u1) {
-    w.find(kt.at(u0));
-    uint32_t ok = w.load(s_tiles);
-    if (u0 + 1 < u1) w.find(kt.at(u0 + 1));
-    w.put(s_tiles);
-    if (lane == 0) s_ok[0][w.wv] = ok;
-    landed();
-    __syncthreads();
-    for (int u = u0; u < u1; ++u) {
-      const int buf = S::NBUF == 2 ? (u - u0) & 1 : 0, flag = (u - u0) & 1;
-      const char* tiles = s_tiles + buf * S::BUF;
-      char* next = s_tiles + (S::NBUF == 2 ? buf ^ 1 : 0) * S::BUF;
-      // (one buffer: other tiles than 4-bit ones come when all waves are done with this one)
-      constexpr bool EARLY = S::NBUF == 2 || KV4;
-      if (EARLY && u + 1 < u1) {
-        ok = w.load(next);
-        if (u + 2 < u1) w.find(kt.at(u + 2));
-      }
-      uint32_t ok0, ok1 = ~0u;
+    const int n_turns = u1 - u0;
+    const auto keys = [&](int u) BB_INLINE { return s_tiles + (u & 1) * S::BUF; };
+    const auto vals = [&](int u) BB_INLINE { return s_tiles + (u & 1) * S::BUF + S::KT * S::ROW; };
+    const auto flags = [&](int u, uint32_t& ok0, uint32_t& ok1) BB_INLINE {
+      const uint32_t* ok = s_ok[u & 1];
+      ok1 = ~0u;
       if constexpr (S::RPW == 32) {
-        ok0 = s_ok[flag][w.wk];
+        ok0 = ok[w.wk];
       } else if constexpr (S::WK == 1 && S::RPW == 16) {
-        ok0 = s_ok[flag][0] | s_ok[flag][1] << 16;
-        ok1 = s_ok[flag][2] | s_ok[flag][3] << 16;
+        ok0 = ok[0] | ok[1] << 16;
+        ok1 = ok[2] | ok[3] << 16;
       } else if constexpr (S::WK == 2) {
-        ok0 = s_ok[flag][2 * w.wk] | s_ok[flag][2 * w.wk + 1] << 16;
+        ok0 = ok[2 * w.wk] | ok[2 * w.wk + 1] << 16;
       } else {
-        ok0 = s_ok[flag][0] | s_ok[flag][1] << 8 | s_ok[flag][2] << 16 | s_ok[flag][3] << 24;
+        ok0 = ok[0] | ok[1] << 8 | ok[2] << 16 | ok[3] << 24;
       }
       ok0 = __builtin_amdgcn_readfirstlane(ok0);
       ok1 = __builtin_amdgcn_readfirstlane(ok1);
-      w.tile(tiles, tiles + S::KT * S::ROW, kt.at(u) * S::KT + w.wk * S::BN, ok0, ok1);
-      if (u + 1 < u1) {
-        if constexpr (S::NBUF == 1) __syncthreads();
-        if constexpr (!EARLY) {
-          ok = w.load(s_tiles);
-          if (u + 2 < u1) w.find(kt.at(u + 2));
-        }
-        w.put(next);
-        if (lane == 0) s_ok[flag ^ 1][w.wv] = ok;
-        landed();
-      }
+    };
+    const auto first_key = [&](int u) BB_INLINE { return kt.at(u0 + u) * S::KT + w.wk * S::BN; };
+    typename Wave::Row krow, vrow;
+    uint32_t ok0, ok1;
+    const auto bring = [&](int u) BB_INLINE {  // tile u's keys (its rows found)
+      krow = w.found();
+      const uint32_t ok = Wave::there(krow);
+      if (lane == 0) s_ok[u & 1][w.wv] = ok;
+      w.template load<true>(krow, keys(u));
+    };
+    const auto see = [&](int u) BB_INLINE {  // tile u's scores, before its turn
+      flags(u, ok0, ok1);
+      w.shape(first_key(u), ok0, ok1);
+    };
+    // Values that are not finite reach the rows that see them and no others. A tile that all rows of the block see is added
+    // as it is; one that they do not is looked at when it is there. If it has such values, the sums
+    // that they belong to are marked, the values taken out, and what is marked made NaN after the tile's turn.
+    const int last = min(r0 + S::BM, rows) - 1, b0 = index_of(r0), b1 = first_seen(index_of(last), pq.window);
+    bool marked = false;
+    const auto look = [&](int u) BB_INLINE {
+      const int j0 = kt.at(u0 + u) * S::KT;
+      if ((j0 + S::KT - 1 <= b0 && j0 >= b1) || j0 + S::KT <= w.prefix) return;
+      if (!__syncthreads_or(w.values_odd(lds_at(vals(u))))) return;
+      w.mark(&s_marks[u & 1][0][tid], lds_at(vals(u)), first_key(u), ok0, ok1);
+      marked = true;
       __syncthreads();
+      w.clean(vals(u));
+      __syncthreads();
+    };
+    const auto turn = [&](int u) BB_INLINE {
+      const bool more = u + 1 < n_turns, two = u + 2 < n_turns;
+      if (two) bring(u + 2);
+      if (more) w.template load<false>(vrow, vals(u + 1));
+      if (two) {
+        vrow = krow;
+        if (u + 3 < n_turns) w.find(kt.at(u0 + u + 3));
+      }
+      typename Wave::Weights p;
+      __builtin_amdgcn_sched_barrier(0);
+      // (behind the last tile, scores of whatever is there, for nothing)
+      w.score(lds_at(keys(u + 1)), [&](int j) BB_INLINE {
+        constexpr int PAIRS = 8 * S::NT;
+        w.weigh(p, j * PAIRS / Wave::STEPS, (j + 1) * PAIRS / Wave::STEPS);
+      });
+      w.add(lds_at(vals(u)), p);
+      if (!more) return;
+      see(u + 1);
+      if (two) w.template put<true>(keys(u));
+      w.template put<false>(vals(u + 1));
+      landed();
+      __syncthreads();
+      look(u + 1);
+    };
+
+    w.find(kt.at(u0));
+    bring(0);
+    w.template load<false>(krow, vals(0));
+    w.template put<true>(keys(0));
+    w.template put<false>(vals(0));
+    if (n_turns > 1) {
+      w.find(kt.at(u0 + 1));
+      bring(1);
+      w.template put<true>(keys(1));
+      if (n_turns > 2) w.find(kt.at(u0 + 2));
     }
+    vrow = krow;
+    landed();
+    __syncthreads();
+    w.score(lds_at(keys(0)), [](int) {});
+    see(0);
+    look(0);
+    for (int u = 0; u < n_turns;) {
+      if (w.past()) w.raise();
+      const bool spoiled = marked;
+      marked = false;
+      do {
+        turn(u++);
+      } while (u < n_turns && !spoiled && !marked && !w.past());
+      if (spoiled) w.spoil(&s_marks[u - 1 & 1][0][tid]);
+    }
+    if constexpr (S::WK > 1) __syncthreads();  // (the tiles' place is taken below)
   }
   w.l = half_sum(w.l);
 
@@ -720,15 +847,16 @@ constexpr int PARTS_MAX = 64;
 
 // The blocks of a launch, chosen from what the host knows: how many tokens and sequences there are.
 struct PromptCut {
-  bool few;  // tiles of 32 rows, the block's waves sharing its keys
+  int wr;    // waves along a tile's rows: 4, or where there are few, its keys shared out to 4 / wr waves
   int bm, n_tiles, parts;
 };
 PromptCut prompt_cut(int n_cu, int cache, size_t n_tokens, size_t n_seqs, int G, int n_kv, int hd) {
   PromptCut c;
   const int cls = pa_class(hd);
   const size_t rows = n_tokens * (size_t)G, mean = (rows + n_seqs - 1) / n_seqs;
-  c.few = mean <= 32 && !(cache == BB_F32 && cls == 256);
-  c.bm = c.few ? 32 : 128;
+  const int row_bytes = cls * (cache == BB_F32 ? 4 : 2);  // in LDS, which has to hold 128 keys and values twice
+  c.wr = mean > 64 || row_bytes > 512 ? 4 : mean > 32 || row_bytes > 256 ? 2 : 1;
+  c.bm = 32 * c.wr;
   c.n_tiles = (int)std::min(rows / c.bm + n_seqs, rows);
   const size_t blocks = (size_t)c.n_tiles * n_kv;
   const size_t at_once = (size_t)n_cu * (cls == 256 || (cache == BB_F32 && cls == 128) ? 1 : 2);
@@ -763,12 +891,18 @@ hipError_t prompt_of(hipStream_t st, const PromptQuery& q, const PagedView& kv, 
 }
 
 template <int CT, int NQ, int NP, bool KV4>
-hipError_t prompt_by(hipStream_t st, bool few, const PromptQuery& q, const PagedView& kv, const PagedSeqs& sq,
+hipError_t prompt_by(hipStream_t st, int wr, const PromptQuery& q, const PagedView& kv, const PagedSeqs& sq,
                      const PromptPlan& pl) {
+  const auto of = [&](auto hdp) {
+    constexpr int H = decltype(hdp)::value;
+    return wr == 4   ? prompt_of<CT, NQ, NP, H, 4, KV4>(st, q, kv, sq, pl)
+           : wr == 2 ? prompt_of<CT, NQ, NP, H, 2, KV4>(st, q, kv, sq, pl)
+                     : prompt_of<CT, NQ, NP, H, 1, KV4>(st, q, kv, sq, pl);
+  };
   switch (pa_class(kv.hd)) {
-    case 64: return few ? prompt_of<CT, NQ, NP, 64, 1, KV4>(st, q, kv, sq, pl) : prompt_of<CT, NQ, NP, 64, 4, KV4>(st, q, kv, sq, pl);
-    case 128: return few ? prompt_of<CT, NQ, NP, 128, 1, KV4>(st, q, kv, sq, pl) : prompt_of<CT, NQ, NP, 128, 4, KV4>(st, q, kv, sq, pl);
-    default: return few ? prompt_of<CT, NQ, NP, 256, 1, KV4>(st, q, kv, sq, pl) : prompt_of<CT, NQ, NP, 256, 4, KV4>(st, q, kv, sq, pl);
+    case 64: return of(std::integral_constant<int, 64>());
+    case 128: return of(std::integral_constant<int, 128>());
+    default: return of(std::integral_constant<int, 256>());
   }
 }
 
@@ -795,17 +929,17 @@ hipError_t launch_paged_prompt(hipStream_t st, int n_cu, int cache, const Prompt
     pl.ml = reinterpret_cast<float2*>(pl.sums + slots * kv.hd);
   }
   switch (cache) {
-    case BB_F32: return prompt_by<BB_F32, 1, 1, false>(st, c.few, q, kv, sq, pl);
+    case BB_F32: return prompt_by<BB_F32, 1, 1, false>(st, c.wr, q, kv, sq, pl);
     case BB_F16:
-      return q.dt == BB_F32 ? prompt_by<BB_F16, 2, 2, false>(st, c.few, q, kv, sq, pl)
-                            : prompt_by<BB_F16, 1, 1, false>(st, c.few, q, kv, sq, pl);
+      return q.dt == BB_F32 ? prompt_by<BB_F16, 2, 2, false>(st, c.wr, q, kv, sq, pl)
+                            : prompt_by<BB_F16, 1, 1, false>(st, c.wr, q, kv, sq, pl);
     case BB_BF16:
-      return q.dt == BB_F32   ? prompt_by<BB_BF16, 3, 3, false>(st, c.few, q, kv, sq, pl)
-             : q.dt == BB_F16 ? prompt_by<BB_BF16, 2, 2, false>(st, c.few, q, kv, sq, pl)
-                              : prompt_by<BB_BF16, 1, 1, false>(st, c.few, q, kv, sq, pl);
+      return q.dt == BB_F32   ? prompt_by<BB_BF16, 3, 3, false>(st, c.wr, q, kv, sq, pl)
+             : q.dt == BB_F16 ? prompt_by<BB_BF16, 2, 2, false>(st, c.wr, q, kv, sq, pl)
+                              : prompt_by<BB_BF16, 1, 1, false>(st, c.wr, q, kv, sq, pl);
     case BB_KV4:
-      return q.dt == BB_F32 ? prompt_by<BB_F16, 2, 2, true>(st, c.few, q, kv, sq, pl)
-                            : prompt_by<BB_F16, 1, 1, true>(st, c.few, q, kv, sq, pl);
+      return q.dt == BB_F32 ? prompt_by<BB_F16, 2, 2, true>(st, c.wr, q, kv, sq, pl)
+                            : prompt_by<BB_F16, 1, 1, true>(st, c.wr, q, kv, sq, pl);
     default: return hipErrorInvalidValue;
   }
 }
