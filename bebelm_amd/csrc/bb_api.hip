@@ -2736,7 +2736,11 @@ size_t prompt_ws(bb_ctx* c, const bb_paged_kv* kv, size_t n_heads, size_t n_seqs
   // (rows of a kv head are 31-bit numbers, threads of a launch 32-bit ones)
   need(n_tokens * n_heads / 32 + n_seqs * n_kv < ((size_t)1 << 24) && n_tokens * (n_heads / n_kv) < ((size_t)1 << 31),
        BB_ERR_RANGE, "tokens times heads beyond what one call takes");
-  return bb::paged_prompt_ws(c->n_cu, (int)kv->dtype, n_tokens, n_seqs, (int)n_heads, (int)n_kv, kv->view.hd);
+  const size_t bytes = bb::paged_prompt_ws(c->n_cu, (int)kv->dtype, n_tokens, n_seqs, (int)n_heads, (int)n_kv, kv->view.hd);
+  // (one token each may take attention of single tokens)
+  return n_tokens != n_seqs || n_seqs == 0
+             ? bytes
+             : std::max(bytes, bb::paged_attn_ws(c->n_cu, (int)n_seqs, (int)n_heads, (int)n_kv, kv->view.hd));
 }
 
 size_t paged_ws(bb_ctx* c, const bb_paged_kv* kv, size_t n_heads, size_t n_seqs) {
@@ -3049,7 +3053,6 @@ int bb_paged_attention(bb_ctx* c, const bb_paged_kv* kv, const bb_paged_seqs* sq
     const size_t B = sq->n_seqs, hd = (size_t)kv->view.hd, nh = pq->n_heads, row = nh * hd;
     const size_t eb = elem_bytes(pq->dtype, "query");
     const size_t want = paged_ws(c, kv, nh, B);
-    need(kv->dtype != BB_KV4, BB_ERR_DTYPE, "a 4-bit pool");
     need_seqs(kv, sq, loc, [&](size_t, int64_t n) {
       return pq->window > 0 && pq->window < (size_t)n ? n - (int64_t)pq->window : 0;
     });
@@ -3237,7 +3240,16 @@ int bb_paged_prompt_attention(bb_ctx* c, const bb_paged_kv* kv, const bb_paged_s
               q.prefix = pq->prefix ? static_cast<const int32_t*>(d[6]) : nullptr;
               q.seq_start = pq->seq_start ? static_cast<const int32_t*>(d[7]) : nullptr;
               q.ws = want == 0 ? nullptr : pq->workspace ? pq->workspace : ensure_ws(c, want);
+              // One token each: its own kernels, but for a window behind a prefix (they read one run of positions), and a
+              // batch past what they count.
+              const bool single = !q.seq_start && !(q.prefix && q.window > 0) &&
+                                  bb::paged_attn_fits((int)B, (int)nh, kv->view.n_kv, sq->max_pages * ps);
               launch_paged(c, cap, bb::K_PAGED_PROMPT, [&] {
+                if (single) {
+                  const bb::PagedQuery one{q.q, q.out, q.q_stride, q.out_stride, q.dt, q.n_heads, q.window,
+                                           q.scale, q.lse, q.ws, q.cap, q.slopes};
+                  return bb::launch_paged_attn(c->stream, c->n_cu, (int)kv->dtype, one, kv->view, seqs_of(sq, d[0], d[1]));
+                }
                 return bb::launch_paged_prompt(c->stream, c->n_cu, (int)kv->dtype, q, kv->view, seqs_of(sq, d[0], d[1]));
               });
             });

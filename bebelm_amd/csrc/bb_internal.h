@@ -421,6 +421,8 @@ struct PagedQuery {
   float scale;
   float* lse;
   void* ws;
+  float cap = 0.0f;  // > 0: scores are capped
+  const float* slopes = nullptr;
 };
 size_t paged_attn_ws(int n_cu, int n_seqs, int n_heads, int n_kv, int hd);
 // Whether a batch's units of work can be counted in 30 bits (cap: positions of a sequence at most).

@@ -419,7 +419,7 @@ __device__ __forceinline__ float group_sum(float x) {
   return as_float(b[0]) + as_float(b[1]);
 }
 
-// A tile's shape: CT the cache's type, HDP the head size (or the next of 64, 128, 256).
+// A tile's shape: CT the cache's type (F16 for 4 bits), HDP the head size (or the next of 64, 128, 256).
 template <int CT, int HDP>
 struct PaShape {
   static constexpr int SZ = CT == BB_F32 ? 4 : 2;
@@ -440,7 +440,11 @@ struct PaShape {
 // and not: bf16, 8 kv heads of 64, 211 and 222 us; f16, of 128, 100 and 116 us. Pages of 8, half of
 // the slots empty: 300 and 223 us (bf16, 64).
 // What is not there or not attended to is loaded as 0 (a weight of 0 times what lies there need not be 0).
-template <int CT, int NP, int HDP, bool UNI>
+// KV4: a 4-bit cache, whose pieces are made f16 (exactly) where they are used. Its words stand in pairs of elements
+// (0, 4), (1, 5), ... : q is packed the same, and o[i] are in that order. A lane's part of a key row is one piece of up to
+// 32 elements, so that it needs one block's head: instruction j takes elements 32g + 8j.. of group g (64: 16g + 8j..).
+// MOD: scores are capped or get a bias by distance.
+template <int CT, int NP, int HDP, bool UNI, bool KV4, bool MOD>
 struct PaWave {
   typedef PaShape<CT, HDP> S;
   static constexpr int NT = S::NT, NC = S::NC, NV = S::NV, VE = S::VE, PE = S::PE, KE = S::KE, SZ = S::SZ;
@@ -455,8 +459,14 @@ struct PaWave {
   float c;        // what scores are multiplied by where NP is 2
   float m, l;
   v4f o[VE];
-  v4u k[NT][NC];
-  VP v[4 * NT][NV];
+  v4u k[KV4 ? 1 : NT][KV4 ? 1 : NC];
+  VP v[KV4 ? 1 : 4 * NT][KV4 ? 1 : NV];
+  static constexpr int KW = NC < 4 ? NC : 4, KC = NC / KW;  // words of a key piece, pieces
+  uint32_t kw[KV4 ? NT : 1][KV4 ? NC : 1], kh[KV4 ? NT : 1][KV4 ? KC : 1];     // of 4 bits: words, blocks' heads
+  uint32_t vw[KV4 ? 4 * NT : 1][KV4 ? NV : 1], vh[KV4 ? 4 * NT : 1][KV4 ? NV : 1];
+  int index;           // MOD: of the query's position
+  float cap, slope;    // (base 2)
+  int pos[MOD ? NT : 1];  // of the positions whose values are loaded, the first of each 16
   uint32_t valid;  // bit 4t + r: position 16t + 4g + r of the tile whose values are loaded is attended to
   static constexpr uint32_t ALL = (1u << 4 * NT) - 1;
 
@@ -467,7 +477,15 @@ struct PaWave {
     const size_t at = (size_t)s * pq.q_stride + (size_t)(head0 + min(n, heads - 1)) * kv.hd;
 #pragma unroll
     for (int j = 0; j < NC; ++j)
-      load_vec<A, KE>(static_cast<const A*>(pq.q) + at + min((4 * j + g) * KE, kv.hd - KE), x[j]);
+      load_vec<A, KE>(static_cast<const A*>(pq.q) + at + min(first_of(j), kv.hd - KE), x[j]);
+  }
+  // The first of the elements that the lane has of the j-th instruction's keys.
+  __device__ __forceinline__ int first_of(int j) const {
+    return KV4 ? j / KW * 128 + (g * KW + j % KW) * 8 : (4 * j + g) * KE;
+  }
+  // Where o has element e of a piece.
+  static __device__ __forceinline__ constexpr int place_of(int e) {
+    return !KV4 ? e : PE == 8 ? e % 4 * 2 + e / 4 : e % 2 * 2 + e / 2;
   }
 
   __device__ __forceinline__ void start(const PagedQuery& pq, int s) {
@@ -481,11 +499,16 @@ struct PaWave {
     else load_q<__bf16>(pq, s, x);
     // scores are exponents of 2; parts that are all of an f32 take the factor in, two parts only hold q itself
     c = pq.scale * LOG2E;
+    if constexpr (MOD) {
+      if (pq.cap > 0.0f) c = pq.scale / pq.cap;
+      cap = pq.cap * LOG2E;
+      slope = pq.slopes ? pq.slopes[head0 + min(n, heads - 1)] * LOG2E : 0.0f;
+    }
     const float cq = NP == 2 ? 1.0f : c;
 #pragma unroll
     for (int j = 0; j < NC; ++j)
 #pragma unroll
-      for (int e = 0; e < KE; ++e) x[j][e] = n < heads && (4 * j + g) * KE < kv.hd ? x[j][e] * cq : 0.0f;
+      for (int e = 0; e < KE; ++e) x[j][e] = n < heads && first_of(j) < kv.hd ? x[j][e] * cq : 0.0f;
     if constexpr (CT == BB_F16) {
       float top = 0.0f;
 #pragma unroll
@@ -510,7 +533,7 @@ struct PaWave {
 #pragma unroll
         for (int e = 0; e < KE; e += 2) {
           uint32_t w[NP];
-          split2<CT, NP>(x[j][e], x[j][e + 1], w);
+          split2<CT, NP>(x[j][KV4 ? e / 2 : e], x[j][KV4 ? e / 2 + 4 : e + 1], w);
 #pragma unroll
           for (int i = 0; i < NP; ++i) q[i][j][e / 2] = w[i];
         }
@@ -520,19 +543,25 @@ struct PaWave {
 
   // Where a tile's positions are in the pool (elements; -1: not there, or not attended to): UNI, each 16, the same for
   // the wave, and how many of them from there on the page has; otherwise lane l's is position l % KT's.
+  // (Of 4 bits: where the piece of (page, head) begins, in bytes, and `in`, the position in the page.)
   struct Places {
     int key0;
     int64_t at[UNI ? NT : 1];
     int rows[UNI ? NT : 1];
+    int in[KV4 ? UNI ? NT : 1 : 1];
+    int pos[UNI ? NT : 1];
   };
   __device__ __forceinline__ void place(Places& p, int t, int key, int end) const {
     const int i = min(key, sp.len - 1), entry = page_of(kv, i), in = i - entry * kv.page_slots;
     int pg = row[entry];
     if constexpr (UNI) pg = __builtin_amdgcn_readfirstlane(pg);
     const bool there = key < end && (uint32_t)pg < (uint32_t)kv.n_pages;
-    const int64_t at = (int64_t)((size_t)(uint32_t)pg * kv.page_stride + (size_t)(uint32_t)in * kv.pos_stride + kv_off);
+    const int64_t at = (int64_t)((size_t)(uint32_t)pg * kv.page_stride +
+                                 (KV4 ? 0 : (size_t)(uint32_t)in * kv.pos_stride) + kv_off);
     p.at[t] = there ? at : -1;
     p.rows[t] = min(16, kv.page_size - in);
+    if constexpr (KV4) p.in[t] = in;
+    if constexpr (MOD && UNI) p.pos[t] = entry * kv.page_size + in;
   }
   __device__ __forceinline__ Places places(int key0, int end) const {
     Places p;
@@ -556,8 +585,113 @@ struct PaWave {
   }
   __device__ __forceinline__ uint32_t stride() const { return (uint32_t)kv.pos_stride * SZ; }
 
+  // 4 bits, UNI: the piece of (page, head) as a buffer (empty: all of it reads as 0), and the lane's words in it.
+  static constexpr uint32_t NOWHERE = 0x80000000u;
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t piece_of(const void* pool, int64_t at) const {
+    const char* base = static_cast<const char*>(pool) + (at >= 0 ? (size_t)at : 0);
+    const uint32_t bytes = at >= 0 ? (uint32_t)(kv.page_size * (kv.hd / 2 + 2 * ((kv.hd / 32 + 1) & ~1))) : 0;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, bytes, 0x00027000);
+  }
+  __device__ __forceinline__ void load_k4(const Places& p) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      int64_t at = 0;
+      int in = 0;
+      if constexpr (!UNI) {
+        at = __shfl(p.at[0], n + 16 * t);
+        in = __shfl(p.in[0], n + 16 * t);
+      } else {
+        in = p.in[t] + n;
+      }
+#pragma unroll
+      for (int c4 = 0; c4 < KC; ++c4) {
+        const int d = first_of(c4 * KW);
+        const int code = in * (kv.hd / 2) + d / 2, head = kv4_head_at(kv, in, d / 32);
+        if constexpr (UNI) {
+          const auto buf = piece_of(kv.k, p.at[t]);
+          const bool here = n < p.rows[t] && d < kv.hd;
+          const uint32_t a = here ? (uint32_t)code : NOWHERE, b = here ? (uint32_t)head : NOWHERE;
+          if constexpr (KW == 4) {
+            const v4u w = __builtin_amdgcn_raw_buffer_load_b128(buf, a, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) kw[t][c4 * KW + i] = w[i];
+          } else {
+            const v2u w = __builtin_amdgcn_raw_buffer_load_b64(buf, a, 0, 0);
+            kw[t][0] = w[0];
+            kw[t][1] = w[1];
+          }
+          kh[t][c4] = __builtin_amdgcn_raw_buffer_load_b16(buf, b, 0, 0);
+        } else {
+          kh[t][c4] = 0;
+#pragma unroll
+          for (int i = 0; i < KW; ++i) kw[t][c4 * KW + i] = 0;
+          if (at >= 0 && d < kv.hd) {
+            const char* piece = static_cast<const char*>(kv.k) + at;
+            load_words<KW>(piece + code, kw[t] + c4 * KW);
+            kh[t][c4] = *reinterpret_cast<const uint16_t*>(piece + head);
+          }
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void load_v4(const Places& p) {
+    valid = 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      int skip = 0, n_rows = 16;
+      if constexpr (UNI) {
+        const int k0 = p.key0 + 16 * t;
+        skip = max(0, sp.first - k0);
+        n_rows = min(p.rows[t], sp.len - k0);
+        if (p.at[t] >= 0) {
+          if (skip == 0 && n_rows == 16) {
+            valid |= 15u << 4 * t;
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) valid |= (4 * g + r >= skip && 4 * g + r < n_rows ? 1u : 0u) << (4 * t + r);
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        int64_t at = 0;
+        int in = 0;
+        if constexpr (!UNI) {
+          at = __shfl(p.at[0], 16 * t + 4 * g + r);
+          in = __shfl(p.in[0], 16 * t + 4 * g + r);
+          valid |= (at >= 0 ? 1u : 0u) << (4 * t + r);
+        } else {
+          in = p.in[t] + 4 * g + r;
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int d = (16 * j + n) * PE;
+          const int code = in * (kv.hd / 2) + d / 2, head = kv4_head_at(kv, in, d / 32);
+          if constexpr (UNI) {
+            const auto buf = piece_of(kv.v, p.at[t]);
+            const bool here = 4 * g + r >= skip && 4 * g + r < n_rows && d < kv.hd;
+            const uint32_t a = here ? (uint32_t)code : NOWHERE, b = here ? (uint32_t)head : NOWHERE;
+            if constexpr (PE == 8) vw[4 * t + r][j] = __builtin_amdgcn_raw_buffer_load_b32(buf, a, 0, 0);
+            else vw[4 * t + r][j] = __builtin_amdgcn_raw_buffer_load_b16(buf, a, 0, 0);
+            vh[4 * t + r][j] = __builtin_amdgcn_raw_buffer_load_b16(buf, b, 0, 0);
+          } else {
+            vw[4 * t + r][j] = vh[4 * t + r][j] = 0;
+            if (at >= 0 && d < kv.hd) {
+              const char* piece = static_cast<const char*>(kv.v) + at;
+              if constexpr (PE == 8) vw[4 * t + r][j] = *reinterpret_cast<const uint32_t*>(piece + code);
+              else vw[4 * t + r][j] = *reinterpret_cast<const uint16_t*>(piece + code);
+              vh[4 * t + r][j] = *reinterpret_cast<const uint16_t*>(piece + head);
+            }
+          }
+        }
+      }
+    }
+  }
+
   __device__ __forceinline__ void load_k(const Places& p) {
-    if constexpr (UNI) {
+    if constexpr (KV4) {
+      load_k4(p);
+    } else if constexpr (UNI) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const auto rows = rows_of(kv.k, p.at[t], p.rows[t]);
@@ -585,6 +719,14 @@ struct PaWave {
   }
 
   __device__ __forceinline__ void load_v(const Places& p) {
+    if constexpr (MOD) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) pos[t] = UNI ? p.pos[t] : p.key0 + 16 * t;
+    }
+    if constexpr (KV4) {
+      load_v4(p);
+      return;
+    }
     valid = 0;
     if constexpr (UNI) {
 #pragma unroll
@@ -645,8 +787,11 @@ struct PaWave {
           for (int e = 0; e < KE; ++e)
             x[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(as_float(k[t][j][e]), as_float(q[0][j][e]), x[t], 0, 0, 0);
         } else {
+          v4u a;
+          if constexpr (KV4) a = Kv4Block(kh[t][j / KW]).paired(kw[t][j]);
+          else a = k[t][j];
 #pragma unroll
-          for (int i = PARTS - 1; i >= 0; --i) x[t] = mfma16<CT>(k[t][j], q[i][j], x[t]);
+          for (int i = PARTS - 1; i >= 0; --i) x[t] = mfma16<CT>(a, q[i][j], x[t]);
         }
       }
   }
@@ -677,6 +822,18 @@ struct PaWave {
     if constexpr (NP == 2) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) x[t] *= c;
+    }
+    if constexpr (MOD) {
+      if (cap > 0.0f) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[t][r] = cap * tanh_of(x[t][r]);
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[t][r] = fmaf(-slope, (float)abs(index - pos[t] - 4 * g - r), x[t][r]);
     }
     if (__any(valid != ALL)) {
 #pragma unroll
@@ -725,13 +882,31 @@ struct PaWave {
 #pragma unroll
           for (int i = 0; i < NP; ++i) p[i][2 * t + r / 2] = w[i];
         }
+      VP u[KV4 ? 4 * NT : 1][KV4 ? NV : 1];
+      if constexpr (KV4) {
+#pragma unroll
+        for (int r = 0; r < 4 * NT; ++r)
+#pragma unroll
+          for (int j = 0; j < NV; ++j) {
+            const Kv4Block b(vh[r][j]);
+            if constexpr (PE == 8) {
+              u[r][j] = b.paired(vw[r][j]);
+            } else {
+              const uint32_t w = (vw[r][j] & 0xffu) | (vw[r][j] & 0xff00u) << 8;  // elements 0 1, 2 3 a half
+              u[r][j] = VP{b.pair<0>(w), b.pair<1>(w)};
+            }
+          }
+      }
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
         v4u a;
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
-          a[w] = __builtin_amdgcn_perm(v[2 * w + 1][i / PE][i % PE / 2], v[2 * w][i / PE][i % PE / 2],
+        for (int w = 0; w < 4; ++w) {
+          const auto& row0 = KV4 ? u[KV4 ? 2 * w : 0] : v[KV4 ? 0 : 2 * w];
+          const auto& row1 = KV4 ? u[KV4 ? 2 * w + 1 : 0] : v[KV4 ? 0 : 2 * w + 1];
+          a[w] = __builtin_amdgcn_perm(row1[i / PE][i % PE / 2], row0[i / PE][i % PE / 2],
                                        i % 2 ? 0x07060302u : 0x05040100u);
+        }
 #pragma unroll
         for (int j = NP - 1; j >= 0; --j) o[i] = mfma16<CT>(a, p[j], o[i]);
       }
@@ -751,8 +926,11 @@ struct PaWave {
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int e = 0; e < PE; e += 4) {
-          const int d = (16 * p + 4 * g + r) * PE + e, i = p * PE + e;
-          if (d < kv.hd) store_act(pq.out, out + d, pq.dt, v4f{o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]} * f);
+          const int d = (16 * p + 4 * g + r) * PE + e, i = p * PE;
+          if (d < kv.hd)
+            store_act(pq.out, out + d, pq.dt,
+                      v4f{o[i + place_of(e)][r], o[i + place_of(e + 1)][r], o[i + place_of(e + 2)][r],
+                          o[i + place_of(e + 3)][r]} * f);
         }
     if (g == 0 && pq.lse)
       pq.lse[(size_t)s * pq.n_heads + head0 + n] = none ? NEG_INF : (m + (__builtin_amdgcn_logf(l) - up)) * LN2;
@@ -804,7 +982,7 @@ struct SeqScan {
   }
 };
 
-template <int CT, int NP, int HDP, bool UNI>
+template <int CT, int NP, int HDP, bool UNI, bool KV4, bool MOD>
 __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQuery pq, PagedView kv,
                                                                         const int* __restrict__ table,
                                                                         const int* __restrict__ lens, size_t table_stride,
@@ -872,7 +1050,8 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
   int grp = uniform_div(u - lo, cost);
   lo += grp * cost;
 
-  PaWave<CT, NP, HDP, UNI> w(kv, lane);
+  typedef PaWave<CT, NP, HDP, UNI, KV4, MOD> Wave;
+  Wave w(kv, lane);
   const float up = CT == BB_F16 ? 14.0f : 0.0f;
   bool lds_read = false;
   int turn = 0;
@@ -897,6 +1076,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
     w.heads = min(pl.hg, pl.G - sub * pl.hg);
     w.kv_off = (size_t)kvh * kv.head_stride;
     w.sp = sp;
+    if constexpr (MOD) w.index = min(max(len, 0), max_pages * kv.page_size) - 1;
     w.start(pq, s);
     const int k0 = w.sp.base + (u0 << pl.unit);
     w.run(alone ? k0 : k0 + wv * S::KT, min(k0 + (take << pl.unit), w.sp.len), alone ? S::KT : PA_WAVES * S::KT);
@@ -927,8 +1107,8 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
 #pragma unroll
           for (int e = 0; e < S::PE; e += 4)
             *reinterpret_cast<v4f*>(to + (16 * p + 4 * w.g + r) * S::PE + e) =
-                v4f{w.o[p * S::PE + e][r], w.o[p * S::PE + e + 1][r], w.o[p * S::PE + e + 2][r],
-                    w.o[p * S::PE + e + 3][r]} * f;
+                v4f{w.o[p * S::PE + Wave::place_of(e)][r], w.o[p * S::PE + Wave::place_of(e + 1)][r],
+                    w.o[p * S::PE + Wave::place_of(e + 2)][r], w.o[p * S::PE + Wave::place_of(e + 3)][r]} * f;
     }
     __syncthreads();
     const bool whole = take == nu;
@@ -1035,7 +1215,7 @@ hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQue
   if (sq.n_seqs == 0) return hipSuccess;
   const HeadGroups g = head_groups(q.n_heads, pool.n_kv);
   const PagedCut cut = paged_cut(n_cu, sq.n_seqs, g.n_groups, pool.page_size, pool.pos_stride, sq.max_pages, q.window,
-                                 pool.hd, cache == BB_F32 ? 4 : 2);
+                                 pool.hd, cache == BB_F32 ? 4 : cache == BB_KV4 ? 1 : 2);
   const bool uni = cut.uni;
   PagedView kv = pool;
   if (uni) kv.set_slots(cut.slots);
@@ -1047,32 +1227,39 @@ hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQue
   const unsigned blocks = (unsigned)cut.blocks;
   const int cls = pa_class(kv.hd);
   const size_t lds = (size_t)PA_WAVES * pl.hg * (cls + 4) * 4;
-#define BB_PA(ct, np, hdp)                                                                                     \
-  do {                                                                                                         \
-    if (uni)                                                                                                   \
-      BB_LAUNCH((k_paged_attn<ct, np, hdp, true>), dim3(blocks), dim3(PA_THREADS), lds, st, q, kv, sq.table,   \
-                sq.lens, sq.table_stride, sq.n_seqs, sq.max_pages, pl);                                        \
-    else                                                                                                       \
-      BB_LAUNCH((k_paged_attn<ct, np, hdp, false>), dim3(blocks), dim3(PA_THREADS), lds, st, q, kv, sq.table,  \
-                sq.lens, sq.table_stride, sq.n_seqs, sq.max_pages, pl);                                        \
+#define BB_PA(ct, np, hdp, four, mod)                                                                               \
+  do {                                                                                                              \
+    if (uni)                                                                                                        \
+      BB_LAUNCH((k_paged_attn<ct, np, hdp, true, four, mod>), dim3(blocks), dim3(PA_THREADS), lds, st, q, kv, sq.table,  \
+                sq.lens, sq.table_stride, sq.n_seqs, sq.max_pages, pl);                                             \
+    else                                                                                                            \
+      BB_LAUNCH((k_paged_attn<ct, np, hdp, false, four, mod>), dim3(blocks), dim3(PA_THREADS), lds, st, q, kv, sq.table, \
+                sq.lens, sq.table_stride, sq.n_seqs, sq.max_pages, pl);                                             \
   } while (0)
-#define BB_PA_HD(ct, np)             \
-  do {                               \
-    if (cls == 64) BB_PA(ct, np, 64); \
-    else if (cls == 128) BB_PA(ct, np, 128); \
-    else BB_PA(ct, np, 256);         \
+#define BB_PA_MOD(ct, np, hdp, four)              \
+  do {                                            \
+    if (q.cap > 0.0f || q.slopes) BB_PA(ct, np, hdp, four, true); \
+    else BB_PA(ct, np, hdp, four, false);         \
   } while (0)
-  if (cache == BB_F32) BB_PA_HD(BB_F32, 1);
-  else if (cache == BB_F16) BB_PA_HD(BB_F16, 2);
-  else if (q.dt == BB_F32) BB_PA_HD(BB_BF16, 3);
-  else BB_PA_HD(BB_BF16, 2);
+#define BB_PA_HD(ct, np, four)                      \
+  do {                                              \
+    if (cls == 64) BB_PA_MOD(ct, np, 64, four);     \
+    else if (cls == 128) BB_PA_MOD(ct, np, 128, four); \
+    else BB_PA_MOD(ct, np, 256, four);              \
+  } while (0)
+  if (cache == BB_F32) BB_PA_HD(BB_F32, 1, false);
+  else if (cache == BB_KV4) BB_PA_HD(BB_F16, 2, true);
+  else if (cache == BB_F16) BB_PA_HD(BB_F16, 2, false);
+  else if (q.dt == BB_F32) BB_PA_HD(BB_BF16, 3, false);
+  else BB_PA_HD(BB_BF16, 2, false);
+#undef BB_PA_MOD
 #undef BB_PA_HD
 #undef BB_PA
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !pl.join) return e;
   const int blocks_of_row = (kv.hd + 4 * PJ_PIECES - 1) / (4 * PJ_PIECES);
   BB_LAUNCH(k_paged_join, dim3(sq.n_seqs, pl.n_groups, pl.hg * blocks_of_row), dim3(PJ_THREADS), 0, st, q, kv.hd,
-            blocks_of_row, pl, cache == BB_F16 ? 14.0f : 0.0f);
+            blocks_of_row, pl, cache == BB_F16 || cache == BB_KV4 ? 14.0f : 0.0f);
   return hipGetLastError();
 }
 

@@ -96,19 +96,6 @@ __device__ __forceinline__ uint32_t fine_halves(uint32_t w, uint32_t odd) {
   return w & ~((odd & 0xffffu ? 0xffffu : 0u) | (odd >> 16 ? 0xffff0000u : 0u));
 }
 
-// tanh, within a few units in the last place: up to 0.6 a quotient of polynomials (the continued fraction
-// y / (1 + y^2 / (3 + y^2 / (5 + y^2 / (7 + y^2 / 9)))), off by less than 1e-9 there), then (e - 1) / (e + 1), e = exp(2|y|).
-__device__ __forceinline__ float tanh_of(float y) {
-  const float a = fabsf(y), z = y * y;
-  const float e = __builtin_amdgcn_exp2f((a > 15.0f ? 15.0f : a) * (2.0f * LOG2E));
-  const bool small = a < 0.6f;
-  float n0 = a * (fmaf(z, 105.0f + z, 945.0f)), d0 = fmaf(z, fmaf(z, 15.0f, 420.0f), 945.0f), n1 = e - 1.0f, d1 = e + 1.0f;
-  // (both in line: a branch each would cost more; and not done where a call has no cap)
-  asm volatile("" : "+v"(n0), "+v"(d0), "+v"(n1), "+v"(d1));
-  const float num = small ? n0 : n1, den = small ? d0 : d1;
-  return copysignf(num * __builtin_amdgcn_rcpf(den), y);
-}
-
 // The work of a launch: n_tiles (or fewer) tiles of rows, each for n_kv heads, its keys in up to `parts` parts of
 // `least` tiles and more. The sums of parts, and for each tile and head (parts used, first row, rows and first token of
 // its sequence), where there may be several.
@@ -606,7 +593,7 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>
   w.row = sq.table + (size_t)s * sq.table_stride;
   w.kv_off = (size_t)kvh * kv.head_stride;
   const int rows = n * pl.G, r0 = it * S::BM;
-  const auto index_of = [&](int r) { return token_index(raw, end, a + r / pl.G); };
+  const auto index_of = [&](int r) { return token_index(w.len, end, a + r / pl.G); };
   const KeyTiles kt =
       key_tiles(index_of(r0), index_of(min(r0 + S::BM, rows) - 1), w.len, w.prefix, pq.window, S::KT);
   const KeyParts kp = key_parts(kt.n, pl.parts, pl.least);
@@ -616,7 +603,7 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>
 
   const int mine = r0 + 32 * w.wr + w.col, r = min(mine, rows - 1);
   const int t = a + r / pl.G, head = kvh * pl.G + r % pl.G;
-  w.i = token_index(raw, end, t);
+  w.i = token_index(w.len, end, t);
   w.lo = first_seen(w.i, pq.window);
   w.i0 = __builtin_amdgcn_readlane(w.i, 0);
   w.i1 = __builtin_amdgcn_readlane(w.i, 31);
