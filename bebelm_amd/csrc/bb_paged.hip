@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(RR_THREADS) k_paged_read(ReadRows r, PagedView
       if constexpr (std::is_same<C, Kv4Pool>::value) {
         const uint32_t word = *reinterpret_cast<const uint32_t*>(pool + at + (size_t)w.row * (kv.hd / 2) + d / 2);
         const uint32_t h = *reinterpret_cast<const uint16_t*>(pool + at + kv4_head_at(kv, w.row, d / 32));
-        const v8h y = __builtin_bit_cast(v8h, Kv4Block(h).natural(word));
+        const v8h y = __builtin_bit_cast(v8h, Kv4Blocks::of(h).natural(word, Kv4Magic()));
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = (float)y[e];
       } else {
@@ -440,9 +440,10 @@ struct PaShape {
 // and not: bf16, 8 kv heads of 64, 211 and 222 us; f16, of 128, 100 and 116 us. Pages of 8, half of
 // the slots empty: 300 and 223 us (bf16, 64).
 // What is not there or not attended to is loaded as 0 (a weight of 0 times what lies there need not be 0).
-// KV4: a 4-bit cache, whose pieces are made f16 (exactly) where they are used. Its words stand in pairs of elements
-// (0, 4), (1, 5), ... : q is packed the same, and o[i] are in that order. A lane's part of a key row is one piece of up to
-// 32 elements, so that it needs one block's head: instruction j takes elements 32g + 8j.. of group g (64: 16g + 8j..).
+// KV4: a 4-bit cache, whose pieces are made f16 (exactly) where they are used. A key word gives pairs of elements
+// (0, 4), (1, 5), ... : q is packed the same. A lane's part of a key row is one piece of up to 32 elements, so that it
+// needs one block's head: instruction j takes elements 32g + 8j.. of group g (64: 16g + 8j..). Values of two positions
+// are put side by side as half words, which then give an element of both, as the instructions want them.
 // MOD: scores are capped or get a bias by distance.
 template <int CT, int NP, int HDP, bool UNI, bool KV4, bool MOD>
 struct PaWave {
@@ -464,6 +465,7 @@ struct PaWave {
   static constexpr int KW = NC < 4 ? NC : 4, KC = NC / KW;  // words of a key piece, pieces
   uint32_t kw[KV4 ? NT : 1][KV4 ? NC : 1], kh[KV4 ? NT : 1][KV4 ? KC : 1];     // of 4 bits: words, blocks' heads
   uint32_t vw[KV4 ? 4 * NT : 1][KV4 ? NV : 1], vh[KV4 ? 4 * NT : 1][KV4 ? NV : 1];
+  Kv4Magic magic;
   int index;           // MOD: of the query's position
   float cap, slope;    // (base 2)
   int pos[MOD ? NT : 1];  // of the positions whose values are loaded, the first of each 16
@@ -482,10 +484,6 @@ struct PaWave {
   // The first of the elements that the lane has of the j-th instruction's keys.
   __device__ __forceinline__ int first_of(int j) const {
     return KV4 ? j / KW * 128 + (g * KW + j % KW) * 8 : (4 * j + g) * KE;
-  }
-  // Where o has element e of a piece.
-  static __device__ __forceinline__ constexpr int place_of(int e) {
-    return !KV4 ? e : PE == 8 ? e % 4 * 2 + e / 4 : e % 2 * 2 + e / 2;
   }
 
   __device__ __forceinline__ void start(const PagedQuery& pq, int s) {
@@ -585,64 +583,66 @@ struct PaWave {
   }
   __device__ __forceinline__ uint32_t stride() const { return (uint32_t)kv.pos_stride * SZ; }
 
-  // 4 bits, UNI: the piece of (page, head) as a buffer (empty: all of it reads as 0), and the lane's words in it.
+  // 4 bits, UNI: the codes of 16 positions, and their blocks' heads, as buffers that end with row `rows` - 1.
   static constexpr uint32_t NOWHERE = 0x80000000u;
-  __device__ __forceinline__ __amdgpu_buffer_rsrc_t piece_of(const void* pool, int64_t at) const {
-    const char* base = static_cast<const char*>(pool) + (at >= 0 ? (size_t)at : 0);
-    const uint32_t bytes = at >= 0 ? (uint32_t)(kv.page_size * (kv.hd / 2 + 2 * ((kv.hd / 32 + 1) & ~1))) : 0;
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, bytes, 0x00027000);
+  struct Rows4 {
+    __amdgpu_buffer_rsrc_t codes, heads;
+  };
+  __device__ __forceinline__ Rows4 rows4_of(const void* pool, int64_t at, int in, int rows) const {
+    const int code = kv.hd / 2, head = 2 * ((kv.hd / 32 + 1) & ~1);
+    const uint32_t n_rows = at >= 0 && rows > 0 ? (uint32_t)rows : 0;
+    const char* base = static_cast<const char*>(pool) + (n_rows ? (size_t)at : 0);
+    const char* codes = base + (n_rows ? (size_t)(uint32_t)in * code : 0);
+    const char* heads = base + (n_rows ? (size_t)(uint32_t)kv.page_size * code + (size_t)(uint32_t)in * head : 0);
+    return {__builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(codes), 0, n_rows * code, 0x00027000),
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(heads), 0, n_rows * head, 0x00027000)};
   }
   __device__ __forceinline__ void load_k4(const Places& p) {
+    const int head = 2 * ((kv.hd / 32 + 1) & ~1);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      int64_t at = 0;
-      int in = 0;
-      if constexpr (!UNI) {
-        at = __shfl(p.at[0], n + 16 * t);
-        in = __shfl(p.in[0], n + 16 * t);
-      } else {
-        in = p.in[t] + n;
-      }
 #pragma unroll
       for (int c4 = 0; c4 < KC; ++c4) {
         const int d = first_of(c4 * KW);
-        const int code = in * (kv.hd / 2) + d / 2, head = kv4_head_at(kv, in, d / 32);
         if constexpr (UNI) {
-          const auto buf = piece_of(kv.k, p.at[t]);
-          const bool here = n < p.rows[t] && d < kv.hd;
-          const uint32_t a = here ? (uint32_t)code : NOWHERE, b = here ? (uint32_t)head : NOWHERE;
+          const Rows4 buf = rows4_of(kv.k, p.at[t], p.in[t], p.rows[t]);
+          const uint32_t a = d < kv.hd ? (uint32_t)(n * (kv.hd / 2) + d / 2) : NOWHERE;
+          const uint32_t b = d < kv.hd ? (uint32_t)(n * head + d / 32 * 2) : NOWHERE;
           if constexpr (KW == 4) {
-            const v4u w = __builtin_amdgcn_raw_buffer_load_b128(buf, a, 0, 0);
+            const v4u w = __builtin_amdgcn_raw_buffer_load_b128(buf.codes, a, 0, 0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) kw[t][c4 * KW + i] = w[i];
           } else {
-            const v2u w = __builtin_amdgcn_raw_buffer_load_b64(buf, a, 0, 0);
+            const v2u w = __builtin_amdgcn_raw_buffer_load_b64(buf.codes, a, 0, 0);
             kw[t][0] = w[0];
             kw[t][1] = w[1];
           }
-          kh[t][c4] = __builtin_amdgcn_raw_buffer_load_b16(buf, b, 0, 0);
+          kh[t][c4] = __builtin_amdgcn_raw_buffer_load_b16(buf.heads, b, 0, 0);
         } else {
+          const int64_t at = __shfl(p.at[0], n + 16 * t);
+          const int in = __shfl(p.in[0], n + 16 * t);
           kh[t][c4] = 0;
 #pragma unroll
           for (int i = 0; i < KW; ++i) kw[t][c4 * KW + i] = 0;
           if (at >= 0 && d < kv.hd) {
             const char* piece = static_cast<const char*>(kv.k) + at;
-            load_words<KW>(piece + code, kw[t] + c4 * KW);
-            kh[t][c4] = *reinterpret_cast<const uint16_t*>(piece + head);
+            load_words<KW>(piece + (size_t)(uint32_t)in * (kv.hd / 2) + d / 2, kw[t] + c4 * KW);
+            kh[t][c4] = *reinterpret_cast<const uint16_t*>(piece + kv4_head_at(kv, in, d / 32));
           }
         }
       }
     }
   }
   __device__ __forceinline__ void load_v4(const Places& p) {
+    const int head = 2 * ((kv.hd / 32 + 1) & ~1);
     valid = 0;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      int skip = 0, n_rows = 16;
+      int skip = 0;
+      Rows4 buf;
       if constexpr (UNI) {
-        const int k0 = p.key0 + 16 * t;
+        const int k0 = p.key0 + 16 * t, n_rows = min(p.rows[t], sp.len - k0);
         skip = max(0, sp.first - k0);
-        n_rows = min(p.rows[t], sp.len - k0);
         if (p.at[t] >= 0) {
           if (skip == 0 && n_rows == 16) {
             valid |= 15u << 4 * t;
@@ -651,6 +651,7 @@ struct PaWave {
             for (int r = 0; r < 4; ++r) valid |= (4 * g + r >= skip && 4 * g + r < n_rows ? 1u : 0u) << (4 * t + r);
           }
         }
+        buf = rows4_of(kv.v, p.at[t], p.in[t], n_rows);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -660,27 +661,25 @@ struct PaWave {
           at = __shfl(p.at[0], 16 * t + 4 * g + r);
           in = __shfl(p.in[0], 16 * t + 4 * g + r);
           valid |= (at >= 0 ? 1u : 0u) << (4 * t + r);
-        } else {
-          in = p.in[t] + 4 * g + r;
         }
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           const int d = (16 * j + n) * PE;
-          const int code = in * (kv.hd / 2) + d / 2, head = kv4_head_at(kv, in, d / 32);
           if constexpr (UNI) {
-            const auto buf = piece_of(kv.v, p.at[t]);
-            const bool here = 4 * g + r >= skip && 4 * g + r < n_rows && d < kv.hd;
-            const uint32_t a = here ? (uint32_t)code : NOWHERE, b = here ? (uint32_t)head : NOWHERE;
-            if constexpr (PE == 8) vw[4 * t + r][j] = __builtin_amdgcn_raw_buffer_load_b32(buf, a, 0, 0);
-            else vw[4 * t + r][j] = __builtin_amdgcn_raw_buffer_load_b16(buf, a, 0, 0);
-            vh[4 * t + r][j] = __builtin_amdgcn_raw_buffer_load_b16(buf, b, 0, 0);
+            const bool here = 4 * g + r >= skip && d < kv.hd;
+            const uint32_t a = here ? (uint32_t)((4 * g + r) * (kv.hd / 2) + d / 2) : NOWHERE;
+            const uint32_t b = here ? (uint32_t)((4 * g + r) * head + d / 32 * 2) : NOWHERE;
+            if constexpr (PE == 8) vw[4 * t + r][j] = __builtin_amdgcn_raw_buffer_load_b32(buf.codes, a, 0, 0);
+            else vw[4 * t + r][j] = __builtin_amdgcn_raw_buffer_load_b16(buf.codes, a, 0, 0);
+            vh[4 * t + r][j] = __builtin_amdgcn_raw_buffer_load_b16(buf.heads, b, 0, 0);
           } else {
             vw[4 * t + r][j] = vh[4 * t + r][j] = 0;
             if (at >= 0 && d < kv.hd) {
               const char* piece = static_cast<const char*>(kv.v) + at;
-              if constexpr (PE == 8) vw[4 * t + r][j] = *reinterpret_cast<const uint32_t*>(piece + code);
-              else vw[4 * t + r][j] = *reinterpret_cast<const uint16_t*>(piece + code);
-              vh[4 * t + r][j] = *reinterpret_cast<const uint16_t*>(piece + head);
+              const char* code = piece + (size_t)(uint32_t)in * (kv.hd / 2) + d / 2;
+              if constexpr (PE == 8) vw[4 * t + r][j] = *reinterpret_cast<const uint32_t*>(code);
+              else vw[4 * t + r][j] = *reinterpret_cast<const uint16_t*>(code);
+              vh[4 * t + r][j] = *reinterpret_cast<const uint16_t*>(piece + kv4_head_at(kv, in, d / 32));
             }
           }
         }
@@ -776,6 +775,13 @@ struct PaWave {
 
   template <int PARTS>
   __device__ __forceinline__ void scores(v4f (&x)[NT]) const {
+    Kv4Blocks kb[KV4 ? NT : 1][KV4 ? KC : 1];
+    if constexpr (KV4) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int c4 = 0; c4 < KC; ++c4) kb[t][c4] = Kv4Blocks::of(kh[t][c4]);
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t) x[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -788,7 +794,7 @@ struct PaWave {
             x[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(as_float(k[t][j][e]), as_float(q[0][j][e]), x[t], 0, 0, 0);
         } else {
           v4u a;
-          if constexpr (KV4) a = Kv4Block(kh[t][j / KW]).paired(kw[t][j]);
+          if constexpr (KV4) a = kb[t][j / KW].paired(kw[t][j], magic);
           else a = k[t][j];
 #pragma unroll
           for (int i = PARTS - 1; i >= 0; --i) x[t] = mfma16<CT>(a, q[i][j], x[t]);
@@ -882,30 +888,30 @@ struct PaWave {
 #pragma unroll
           for (int i = 0; i < NP; ++i) p[i][2 * t + r / 2] = w[i];
         }
-      VP u[KV4 ? 4 * NT : 1][KV4 ? NV : 1];
-      if constexpr (KV4) {
-#pragma unroll
-        for (int r = 0; r < 4 * NT; ++r)
-#pragma unroll
-          for (int j = 0; j < NV; ++j) {
-            const Kv4Block b(vh[r][j]);
-            if constexpr (PE == 8) {
-              u[r][j] = b.paired(vw[r][j]);
-            } else {
-              const uint32_t w = (vw[r][j] & 0xffu) | (vw[r][j] & 0xff00u) << 8;  // elements 0 1, 2 3 a half
-              u[r][j] = VP{b.pair<0>(w), b.pair<1>(w)};
-            }
-          }
-      }
+      // (of 4 bits: elements 4h..4h+3 of a piece of positions 2w and 2w + 1, which come from a word made of half h of each)
+      v4u four[KV4 ? 4 : 1];
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
         v4u a;
+        if constexpr (KV4) {
+          if (i % 4 == 0) {
+            const int j = i / PE, h = i % PE / 4;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const auto& row0 = KV4 ? u[KV4 ? 2 * w : 0] : v[KV4 ? 0 : 2 * w];
-          const auto& row1 = KV4 ? u[KV4 ? 2 * w + 1 : 0] : v[KV4 ? 0 : 2 * w + 1];
-          a[w] = __builtin_amdgcn_perm(row1[i / PE][i % PE / 2], row0[i / PE][i % PE / 2],
-                                       i % 2 ? 0x07060302u : 0x05040100u);
+            for (int w = 0; w < 4; ++w) {
+              const Kv4Blocks b(__builtin_amdgcn_perm(vh[2 * w + 1][j], vh[2 * w][j], 0x05040100u));
+              const uint32_t both = __builtin_amdgcn_perm(vw[2 * w + 1][j], vw[2 * w][j], h ? 0x07060302u : 0x05040100u);
+              four[0][w] = b.template pair<0>(both, magic);
+              four[1][w] = b.template pair<1>(both, magic);
+              four[2][w] = b.template pair<2>(both, magic);
+              four[3][w] = b.template pair<3>(both, magic);
+            }
+          }
+          a = four[i % 4];
+        } else {
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            a[w] = __builtin_amdgcn_perm(v[2 * w + 1][i / PE][i % PE / 2], v[2 * w][i / PE][i % PE / 2],
+                                         i % 2 ? 0x07060302u : 0x05040100u);
         }
 #pragma unroll
         for (int j = NP - 1; j >= 0; --j) o[i] = mfma16<CT>(a, p[j], o[i]);
@@ -926,11 +932,10 @@ struct PaWave {
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int e = 0; e < PE; e += 4) {
-          const int d = (16 * p + 4 * g + r) * PE + e, i = p * PE;
+          const int d = (16 * p + 4 * g + r) * PE + e, i = p * PE + e;
           if (d < kv.hd)
             store_act(pq.out, out + d, pq.dt,
-                      v4f{o[i + place_of(e)][r], o[i + place_of(e + 1)][r], o[i + place_of(e + 2)][r],
-                          o[i + place_of(e + 3)][r]} * f);
+                      v4f{o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]} * f);
         }
     if (g == 0 && pq.lse)
       pq.lse[(size_t)s * pq.n_heads + head0 + n] = none ? NEG_INF : (m + (__builtin_amdgcn_logf(l) - up)) * LN2;
@@ -1107,8 +1112,8 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
 #pragma unroll
           for (int e = 0; e < S::PE; e += 4)
             *reinterpret_cast<v4f*>(to + (16 * p + 4 * w.g + r) * S::PE + e) =
-                v4f{w.o[p * S::PE + Wave::place_of(e)][r], w.o[p * S::PE + Wave::place_of(e + 1)][r],
-                    w.o[p * S::PE + Wave::place_of(e + 2)][r], w.o[p * S::PE + Wave::place_of(e + 3)][r]} * f;
+                v4f{w.o[p * S::PE + e][r], w.o[p * S::PE + e + 1][r], w.o[p * S::PE + e + 2][r],
+                    w.o[p * S::PE + e + 3][r]} * f;
     }
     __syncthreads();
     const bool whole = take == nu;

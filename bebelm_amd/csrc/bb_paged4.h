@@ -43,30 +43,40 @@ __device__ __forceinline__ void load_words(const char* p, uint32_t* w) {
   }
 }
 
-// A block's head as what its codes are multiplied by and what is added.
-struct Kv4Block {
+// What 16 + code is made with: a constant that stands in a vector register, as an instruction with two of them needs.
+struct Kv4Magic {
+  uint32_t bits = 0x4c004c00u;  // 16 twice
+  __device__ __forceinline__ Kv4Magic() { asm("" : "+v"(bits)); }
+};
+// The heads of two blocks (in the halves of a word), as what their codes are multiplied by and what is added.
+struct Kv4Blocks {
   v2h d, zd;
-  __device__ __forceinline__ explicit Kv4Block(uint32_t head) {
-    const _Float16 step = __builtin_bit_cast(_Float16, (uint16_t)(head & 0x7fc0u));
-    const int z = (int)(head & 63u) - (int)(head >> 9 & 64u) - 16;
-    const _Float16 add = (_Float16)(float)z * step;
-    d = v2h{step, step};
-    zd = v2h{add, add};
+  Kv4Blocks() = default;
+  __device__ __forceinline__ explicit Kv4Blocks(uint32_t heads) {
+    d = __builtin_bit_cast(v2h, heads & 0x7fc07fc0u);
+    // 1024 + 64 + z, from the 6 lower bits and the sign turned round in the 7th
+    const uint32_t low = (heads & 0x003f003fu) | 0x64006400u, sign = (heads ^ 0x80008000u) >> 9;
+    const v2h z = __builtin_bit_cast(v2h, (sign & 0x00400040u) | (low & ~0x00400040u));
+    zd = (z - v2h{(_Float16)1104.0f, (_Float16)1104.0f}) * d;
   }
-  // Elements i and i + 4 of a word's 8 (i-th and (i + 4)-th half byte).
+  // One block twice.
+  static __device__ __forceinline__ Kv4Blocks of(uint32_t head) { return Kv4Blocks(head | head << 16); }
+  // The I-th half byte of both halves of a word as the elements they stand for.
   template <int I>
-  __device__ __forceinline__ uint32_t pair(uint32_t w) const {
+  __device__ __forceinline__ uint32_t pair(uint32_t w, const Kv4Magic& m) const {
     const uint32_t at = I == 0 ? w << 6 : I == 1 ? w << 2 : I == 2 ? w >> 2 : w >> 6;  // to bits 6 to 9 of each half
-    const v2h x = __builtin_bit_cast(v2h, (at & 0x03c003c0u) | 0x4c004c00u);           // 16 + code
+    const v2h x = __builtin_bit_cast(v2h, (at & 0x03c003c0u) | m.bits);                // 16 + code
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x, d, zd));
   }
-  // A word's 8 elements in their order, and in the order 0 4 1 5 2 6 3 7.
-  __device__ __forceinline__ v4u natural(uint32_t w) const {
-    const uint32_t a = pair<0>(w), b = pair<1>(w), c = pair<2>(w), e = pair<3>(w);
+  // A word's 8 elements in their order, and in the order 0 4 1 5 2 6 3 7 (of one block twice).
+  __device__ __forceinline__ v4u natural(uint32_t w, const Kv4Magic& m) const {
+    const uint32_t a = pair<0>(w, m), b = pair<1>(w, m), c = pair<2>(w, m), e = pair<3>(w, m);
     return v4u{__builtin_amdgcn_perm(b, a, 0x05040100u), __builtin_amdgcn_perm(e, c, 0x05040100u),
                __builtin_amdgcn_perm(b, a, 0x07060302u), __builtin_amdgcn_perm(e, c, 0x07060302u)};
   }
-  __device__ __forceinline__ v4u paired(uint32_t w) const { return v4u{pair<0>(w), pair<1>(w), pair<2>(w), pair<3>(w)}; }
+  __device__ __forceinline__ v4u paired(uint32_t w, const Kv4Magic& m) const {
+    return v4u{pair<0>(w, m), pair<1>(w, m), pair<2>(w, m), pair<3>(w, m)};
+  }
 };
 
 // Whether step d (at least 0) reaches from lo to hi in 15 steps, and each of them by the offsets there are. (In f64: the

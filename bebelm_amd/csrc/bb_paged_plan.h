@@ -179,7 +179,7 @@ inline PagedCut paged_cut(int n_cu, int n_seqs, int n_groups, int page_size, siz
     cap = std::min(cap, std::min((size_t)window + pages * (c.slots - page_size), pages * c.slots) + 31);
   }
   const int blocks_max = blocks_at_once(n_cu, hd), unit_short = pa_unit_short(hd * elem_bytes);
-  c.few = c.uni ? n_cu : blocks_max;
+  c.few = c.uni && elem_bytes > 1 ? n_cu : blocks_max;
   // (pairs of one unit take a block each at most, longer ones a block for each unit)
   c.unit = cap <= (size_t)1 << unit_short ? unit_short : PA_UNIT;
   const size_t pairs = (size_t)n_seqs * n_groups, units = ((cap - 1) >> c.unit) + 1;

@@ -249,16 +249,17 @@ struct PpWave {
   __device__ __forceinline__ void put(char* lds) const {
     if constexpr (KV4) {
       const Codes& c = KEYS ? ck : cv;
+      const Kv4Magic magic;
       const int own = (int)fresh((uint32_t)lane);
 #pragma unroll
       for (int p = 0; p < S::NU; ++p) {
         const int e = p * 64 + own, r = wv * S::RPW + e / S::UPR, u = e % S::UPR;
-        const Kv4Block block(c.head[p]);
+        const Kv4Blocks block = Kv4Blocks::of(c.head[p]);
 #pragma unroll
         for (int w = 0; w < S::UE / 8; ++w) {
           const int piece = u * (S::UE / 8) + w;
           *reinterpret_cast<v4u*>(lds + r * S::ROW + (piece ^ (KEYS ? S::k_swap(r) : S::v_swap(r))) * 16) =
-              block.natural(c.word[p * S::UE / 8 + w]);
+              block.natural(c.word[p * S::UE / 8 + w], magic);
         }
       }
     }
