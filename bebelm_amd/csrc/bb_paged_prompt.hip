@@ -47,7 +47,7 @@ struct PpShape {
   static constexpr int WAVES = REGS <= 208 && LDS <= 79 * 1024 ? 2 : 1;  // of a SIMD
 };
 
-__device__ __attribute__((aligned(16))) uint32_t g_zeros[4];
+__device__ __attribute__((aligned(16))) uint32_t g_zeros[256];  // a row that is not there
 // 16 bytes of every lane from its own address to lds + 16·lane.
 __device__ __forceinline__ void to_lds(const char* from, char* lds) {
   typedef __attribute__((address_space(1))) const uint32_t* global_u32;
@@ -128,7 +128,7 @@ struct PpWave {
     uint32_t word[KV4 ? S::NU * S::UE / 8 : 1], head[KV4 ? S::NU : 1];
   };
   Codes ck, cv;
-  v16f x[NT];                 // scores of the tile at work (base `by` of them), then its weights
+  v16f x[2][NT];              // scores of the tile at work (in multiples of `by`) and of the next, by turns
   float by;
   float top;                  // the largest
   int page, in;               // of the row that the lane finds for its wave (page -1: not there)
@@ -195,7 +195,7 @@ struct PpWave {
     }
   }
 
-  // Where the row found is in the pool (elements; of 4 bits, bytes to its (page, head)).
+  // Where the row found is in the pool (bytes; of 4 bits, to its (page, head)).
   struct Row {
     int64_t at;  // -1: not there
     int pos;     // 4 bits: its position in the page
@@ -203,7 +203,7 @@ struct PpWave {
   __device__ __forceinline__ Row found() const {
     const bool there = (uint32_t)page < (uint32_t)kv.n_pages;
     const size_t at = (size_t)(uint32_t)page * kv.page_stride + (KV4 ? 0 : (size_t)(uint32_t)in * kv.pos_stride) + kv_off;
-    return Row{there ? (int64_t)at : -1, in};
+    return Row{there ? (int64_t)(KV4 ? at : at * SZ) : -1, in};
   }
   // Which of the wave's rows are there.
   static __device__ __forceinline__ uint32_t there(const Row& r) { return (uint32_t)__ballot(r.at >= 0) & (~0u >> (32 - S::RPW)); }
@@ -213,9 +213,9 @@ struct PpWave {
   template <bool KEYS>
   __device__ __forceinline__ void load(const Row& w, char* lds) {
     const char* pool = static_cast<const char*>(KEYS ? kv.k : kv.v);
-    const uint32_t alo = (uint32_t)w.at, ahi = (uint32_t)(w.at >> 32);
     const int own = (int)fresh((uint32_t)lane);
     if constexpr (KV4) {
+      const uint32_t alo = (uint32_t)w.at, ahi = (uint32_t)(w.at >> 32);
       Codes& c = KEYS ? ck : cv;
 #pragma unroll
       for (int p = 0; p < S::NU; ++p) {
@@ -231,14 +231,15 @@ struct PpWave {
         }
       }
     } else {
+      const uint64_t row = w.at >= 0 ? reinterpret_cast<uint64_t>(pool) + (uint64_t)w.at : reinterpret_cast<uint64_t>(g_zeros);
+      const uint32_t alo = (uint32_t)row, ahi = (uint32_t)(row >> 32);
 #pragma unroll
       for (int p = 0; p < S::NPC; ++p) {
         const int e = p * 64 + own, r = e / S::PPR, u = e % S::PPR, rr = wv * S::RPW + r;
-        const int64_t base = (int64_t)((uint64_t)(uint32_t)__shfl((int)ahi, r) << 32 | (uint32_t)__shfl((int)alo, r));
-        const int d = (u ^ (KEYS ? S::k_swap(rr) : S::v_swap(rr))) * (16 / SZ);
-        uint64_t a = reinterpret_cast<uint64_t>(pool) + (uint64_t)(base + d) * SZ;
-        asm("" : "+v"(a));  // (a select, no branch)
-        a = base >= 0 && d < kv.hd ? a : reinterpret_cast<uint64_t>(g_zeros);
+        uint64_t a = (uint64_t)(uint32_t)__shfl((int)ahi, r) << 32 | (uint32_t)__shfl((int)alo, r);
+        const int at = (u ^ (KEYS ? S::k_swap(rr) : S::v_swap(rr))) * 16;
+        a += (uint32_t)at;
+        if (at >= kv.hd * SZ) a = reinterpret_cast<uint64_t>(g_zeros);  // (past a head that is shorter than the tile's rows)
         to_lds(reinterpret_cast<const char*>(a), lds + wv * S::RPW * S::ROW + p * 1024);
       }
     }
@@ -334,10 +335,10 @@ struct PpWave {
     return ((below(i + 1 - j0) & ~below(lo - j0)) | below(prefix - j0)) & ok;
   }
 
-  // The scores of a tile of keys, into x.
-  template <class F>
+  // The scores of a tile of keys, into set I.
+  template <int I, class F>
   __device__ __forceinline__ void score(uint32_t lk, F&& between) {
-    v16f y[NT];
+    v16f(&y)[NT] = x[I];
     scores<NQ>(lk, y, between);
     if constexpr (NQ > 1) {
       // a part of 0 meets an infinite key as NaN: such scores are taken from the first parts alone
@@ -355,8 +356,6 @@ struct PpWave {
           for (int e = 0; e < 16; ++e) y[t][e] = y[t][e] != y[t][e] ? z[t][e] : y[t][e];
       }
     }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) x[t] = y[t];
   }
 
   // Whether all rows of the wave see all keys from j0 on, `ok` being those that are there.
@@ -364,15 +363,25 @@ struct PpWave {
     return ok0 == ~0u && (NT == 1 || ok1 == ~0u) && ((j0 + S::BN - 1 <= i0 && j0 >= lo1) || j0 + S::BN <= prefix);
   }
 
+  // cap·tanh as cap - 2cap / (exp(2y) + 1): off by at most 2^-21 of the cap (the quotient's roundings and the
+  // sum's), which is 2^-21·cap of a weight that is rounded to 16 bits. Half the instructions of tanh_of (6001 tokens, 16
+  // heads of 256, f16: the whole call 297 and 224 us).
+  static constexpr bool QUICK = CT != BB_F32 && NP == 1;
+  __device__ __forceinline__ float quick_cap(float y) const {
+    const float e = __builtin_amdgcn_exp2f(y * (2.0f * LOG2E * c)), top = pq.cap * LOG2E;
+    return fmaf(-2.0f * top, __builtin_amdgcn_rcpf(e + 1.0f), top);
+  }
   // The scores capped, with their bias, hidden where the rows do not see the keys from j0 on, and the largest.
+  template <int I>
   __device__ __forceinline__ void shape(int j0, uint32_t ok0, uint32_t ok1) {
+    v16f(&y)[NT] = x[I];
     by = c;
     if (pq.cap > 0.0f) {
       by = 1.0f;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[t][e] = (pq.cap * LOG2E) * tanh_of(x[t][e] * c);
+        for (int e = 0; e < 16; ++e) y[t][e] = QUICK ? quick_cap(y[t][e]) : (pq.cap * LOG2E) * tanh_of(y[t][e] * c);
     }
     if (pq.slopes) {
       const float away = (float)(i - j0 - 4 * half);
@@ -380,7 +389,7 @@ struct PpWave {
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          x[t][e] = fmaf(-slope, fabsf(away - (float)(32 * t + 8 * (e / 4) + e % 4)), x[t][e] * by);
+          y[t][e] = fmaf(-slope, fabsf(away - (float)(32 * t + 8 * (e / 4) + e % 4)), y[t][e] * by);
       by = 1.0f;
     }
     if (!whole(j0, ok0, ok1)) {
@@ -388,14 +397,14 @@ struct PpWave {
       for (int t = 0; t < NT; ++t) {
         const uint32_t see = seen(j0 + 32 * t, t ? ok1 : ok0) >> 4 * half;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[t][e] = see >> (8 * (e / 4) + e % 4) & 1 ? x[t][e] : NEG_INF;
+        for (int e = 0; e < 16; ++e) y[t][e] = see >> (8 * (e / 4) + e % 4) & 1 ? y[t][e] : NEG_INF;
       }
     }
     float mx = NEG_INF;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, x[t][e]);
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, y[t][e]);
     top = half_max(mx) * by;
   }
 
@@ -418,12 +427,14 @@ struct PpWave {
     v16f f[CT == BB_F32 ? NT : 1];
   };
   // Those of pairs of registers lo..hi-1 (8 of each 32 keys).
+  template <int I>
   __device__ __forceinline__ void weigh(Weights& p, int lo, int hi) {
     const float less = (F16 ? F16_UP : 0.0f) - (m == NEG_INF ? 0.0f : m);
 #pragma unroll
     for (int i = lo; i < hi; ++i) {
       const int t = i / 8, e = i % 8 * 2;
-      const float a = __builtin_amdgcn_exp2f(fmaf(x[t][e], by, less)), b = __builtin_amdgcn_exp2f(fmaf(x[t][e + 1], by, less));
+      const float a = __builtin_amdgcn_exp2f(fmaf(x[I][t][e], by, less));
+      const float b = __builtin_amdgcn_exp2f(fmaf(x[I][t][e + 1], by, less));
       l += a;
       l += b;
       if constexpr (CT == BB_F32) {
@@ -658,9 +669,9 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>
       if (lane == 0) s_ok[u & 1][w.wv] = ok;
       w.template load<true>(krow, keys(u));
     };
-    const auto see = [&](int u) BB_INLINE {  // tile u's scores, before its turn
+    const auto see = [&](int u, auto set) BB_INLINE {  // tile u's scores, before its turn
       flags(u, ok0, ok1);
-      w.shape(first_key(u), ok0, ok1);
+      w.template shape<decltype(set)::value>(first_key(u), ok0, ok1);
     };
     // Values that are not finite reach the rows that see them and no others. A tile that all rows of the block see is added
     // as it is; one that they do not is looked at when it is there. If it has such values, the sums
@@ -677,7 +688,8 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>
       w.clean(vals(u));
       __syncthreads();
     };
-    const auto turn = [&](int u) BB_INLINE {
+    const auto turn = [&](int u, auto set) BB_INLINE {
+      constexpr int I = decltype(set)::value;
       const bool more = u + 1 < n_turns, two = u + 2 < n_turns;
       if (two) bring(u + 2);
       if (more) w.template load<false>(vrow, vals(u + 1));
@@ -688,13 +700,13 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>
       typename Wave::Weights p;
       __builtin_amdgcn_sched_barrier(0);
       // (behind the last tile, scores of whatever is there, for nothing)
-      w.score(lds_at(keys(u + 1)), [&](int j) BB_INLINE {
+      w.template score<1 - I>(lds_at(keys(u + 1)), [&](int j) BB_INLINE {
         constexpr int PAIRS = 8 * S::NT;
-        w.weigh(p, j * PAIRS / Wave::STEPS, (j + 1) * PAIRS / Wave::STEPS);
+        w.template weigh<I>(p, j * PAIRS / Wave::STEPS, (j + 1) * PAIRS / Wave::STEPS);
       });
       w.add(lds_at(vals(u)), p);
       if (!more) return;
-      see(u + 1);
+      see(u + 1, std::integral_constant<int, 1 - I>());
       if (two) w.template put<true>(keys(u));
       w.template put<false>(vals(u + 1));
       landed();
@@ -716,16 +728,26 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>
     vrow = krow;
     landed();
     __syncthreads();
-    w.score(lds_at(keys(0)), [](int) {});
-    see(0);
+    const std::integral_constant<int, 0> even;
+    const std::integral_constant<int, 1> uneven;
+    w.template score<0>(lds_at(keys(0)), [](int) {});
+    see(0, even);
     look(0);
     for (int u = 0; u < n_turns;) {
       if (w.past()) w.raise();
       const bool spoiled = marked;
       marked = false;
-      do {
-        turn(u++);
-      } while (u < n_turns && !spoiled && !marked && !w.past());
+      const auto on = [&]() BB_INLINE { return u < n_turns && !spoiled && !marked && !w.past(); };
+      for (;;) {
+        turn(u++, even);
+        if (!on()) {
+#pragma unroll
+          for (int t = 0; t < S::NT; ++t) w.x[0][t] = w.x[1][t];
+          break;
+        }
+        turn(u++, uneven);
+        if (!on()) break;
+      }
       if (spoiled) w.spoil(&s_marks[u - 1 & 1][0][tid]);
     }
     if constexpr (S::WK > 1) __syncthreads();  // (the tiles' place is taken below)
