@@ -101,6 +101,7 @@ __device__ __forceinline__ uint32_t fine_halves(uint32_t w, uint32_t odd) {
 // its sequence), where there may be several.
 struct PromptPlan {
   int G, n_tiles, n_kv, parts, least;
+  bool runs;     // rows of a wave and a tile lie in one page (and fill theirs in LDS)
   float* sums;   // [tile][kv head][part][row][hd]
   float2* ml;    // [tile][kv head][part][row]: maximum (base 2), sum of weights
   int4* places;  // [tile][kv head]
@@ -131,6 +132,7 @@ struct PpWave {
   v16f x[2][NT];              // scores of the tile at work (in multiples of `by`) and of the next, by turns
   float by;
   float top;                  // the largest
+  bool runs;                  // a wave's rows of a tile lie in one page, a whole tile row each, within 2^31 bytes
   int page, in;               // of the row that the lane finds for its wave (page -1: not there)
 
   __device__ __forceinline__ PpWave(const PagedView& kv_, const PromptQuery& pq_, int tid)
@@ -199,27 +201,58 @@ struct PpWave {
   struct Row {
     int64_t at;  // -1: not there
     int pos;     // 4 bits: its position in the page
+    bool run;    // (the wave's) rows of one page, the first of which is there
   };
   __device__ __forceinline__ Row found() const {
     const bool there = (uint32_t)page < (uint32_t)kv.n_pages;
     const size_t at = (size_t)(uint32_t)page * kv.page_stride + (KV4 ? 0 : (size_t)(uint32_t)in * kv.pos_stride) + kv_off;
-    return Row{there ? (int64_t)(KV4 ? at : at * SZ) : -1, in};
+    return Row{there ? (int64_t)(KV4 ? at : at * SZ) : -1, in,
+               runs && (uint32_t)__builtin_amdgcn_readfirstlane(page) < (uint32_t)kv.n_pages};
   }
   // Which of the wave's rows are there.
   static __device__ __forceinline__ uint32_t there(const Row& r) { return (uint32_t)__ballot(r.at >= 0) & (~0u >> (32 - S::RPW)); }
 
   // Asks for the wave's rows of a tile, keys or values: 4-bit ones into registers, others straight into the tile at
-  // `lds`, 1024 bytes an instruction, each lane a piece (zeros where nothing is).
+  // `lds`, 1024 bytes an instruction, each lane a piece. Rows of one page have one address and the lanes' distances from
+  // it (those past the sequence's length are whatever is there: their scores are hidden, and look() finds values that are
+  // not finite); otherwise the lanes exchange addresses, and rows that are not there are zeros.
   template <bool KEYS>
   __device__ __forceinline__ void load(const Row& w, char* lds) {
     const char* pool = static_cast<const char*>(KEYS ? kv.k : kv.v);
-    const int own = (int)fresh((uint32_t)lane);
+    if (w.run) {
+      const uint64_t first = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(w.at >> 32)) << 32 |
+                             (uint32_t)__builtin_amdgcn_readfirstlane((int)w.at);
+      const char* base = pool + first;
+      const uint32_t mine = fresh((uint32_t)lane) & 63;
+      if constexpr (KV4) {
+        Codes& c = KEYS ? ck : cv;
+        const int in0 = __builtin_amdgcn_readfirstlane(w.pos);
+        const char* heads = base + (size_t)(uint32_t)kv4_head_at(kv, in0, 0);
+        const char* codes = base + (size_t)(uint32_t)(in0 * (kv.hd / 2));
+#pragma unroll
+        for (int p = 0; p < S::NU; ++p) {
+          const uint32_t r = mine / S::UPR + p * (64 / S::UPR), u = mine % S::UPR;
+          load_words<S::UE / 8>(codes + r * (HDP / 2) + u * (S::UE / 2), c.word + p * S::UE / 8);
+          c.head[p] = *reinterpret_cast<const uint16_t*>(heads + 2 * (r * (HDP / 32) + u * S::UE / 32));
+        }
+      } else {
+        const uint32_t step = (uint32_t)kv.pos_stride * SZ, r0 = mine / S::PPR, u = mine % S::PPR;
+#pragma unroll
+        for (int p = 0; p < S::NPC; ++p) {
+          const uint32_t r = r0 + p * (64 / S::PPR), rr = r + (wv * S::RPW & 15);
+          const uint32_t at = (u ^ (uint32_t)(KEYS ? S::k_swap((int)rr) : S::v_swap((int)rr))) * 16;
+          to_lds(base + (r * step + at), lds + wv * S::RPW * S::ROW + p * 1024);
+        }
+      }
+      return;
+    }
+    const uint32_t own = fresh((uint32_t)lane) & 63;
     if constexpr (KV4) {
       const uint32_t alo = (uint32_t)w.at, ahi = (uint32_t)(w.at >> 32);
       Codes& c = KEYS ? ck : cv;
 #pragma unroll
       for (int p = 0; p < S::NU; ++p) {
-        const int e = p * 64 + own, r = e / S::UPR, u = e % S::UPR, d = u * S::UE;
+        const int r = (int)(own / S::UPR) + p * (64 / S::UPR), u = own % S::UPR, d = u * S::UE;
         const int64_t base = (int64_t)((uint64_t)(uint32_t)__shfl((int)ahi, r) << 32 | (uint32_t)__shfl((int)alo, r));
         const int rp = __shfl(w.pos, r);
         c.head[p] = 0;
@@ -233,14 +266,26 @@ struct PpWave {
     } else {
       const uint64_t row = w.at >= 0 ? reinterpret_cast<uint64_t>(pool) + (uint64_t)w.at : reinterpret_cast<uint64_t>(g_zeros);
       const uint32_t alo = (uint32_t)row, ahi = (uint32_t)(row >> 32);
+      // an instruction brings 64 / PPR rows (or a part of one); the addresses of several are asked for at once
+      constexpr int AT_ONCE = S::NPC < 4 ? S::NPC : 4;
+      const uint32_t r0 = own / S::PPR, u = own % S::PPR;
 #pragma unroll
-      for (int p = 0; p < S::NPC; ++p) {
-        const int e = p * 64 + own, r = e / S::PPR, u = e % S::PPR, rr = wv * S::RPW + r;
-        uint64_t a = (uint64_t)(uint32_t)__shfl((int)ahi, r) << 32 | (uint32_t)__shfl((int)alo, r);
-        const int at = (u ^ (KEYS ? S::k_swap(rr) : S::v_swap(rr))) * 16;
-        a += (uint32_t)at;
-        if (at >= kv.hd * SZ) a = reinterpret_cast<uint64_t>(g_zeros);  // (past a head that is shorter than the tile's rows)
-        to_lds(reinterpret_cast<const char*>(a), lds + wv * S::RPW * S::ROW + p * 1024);
+      for (int q = 0; q < S::NPC; q += AT_ONCE) {
+        uint64_t a[AT_ONCE];
+#pragma unroll
+        for (int p = 0; p < AT_ONCE; ++p) {
+          const int r = (int)(r0 + (q + p) * (64 / S::PPR)) * 4;
+          a[p] = (uint64_t)(uint32_t)__builtin_amdgcn_ds_bpermute(r, (int)ahi) << 32 |
+                 (uint32_t)__builtin_amdgcn_ds_bpermute(r, (int)alo);
+        }
+#pragma unroll
+        for (int p = 0; p < AT_ONCE; ++p) {
+          const int r = (int)r0 + (q + p) * (64 / S::PPR) + wv * S::RPW;
+          const uint32_t at = (u ^ (uint32_t)(KEYS ? S::k_swap(r) : S::v_swap(r))) * 16;
+          a[p] += at;
+          if (at >= (uint32_t)(kv.hd * SZ)) a[p] = reinterpret_cast<uint64_t>(g_zeros);  // (past a shorter head)
+          to_lds(reinterpret_cast<const char*>(a[p]), lds + wv * S::RPW * S::ROW + (q + p) * 1024);
+        }
       }
     }
   }
@@ -251,10 +296,10 @@ struct PpWave {
     if constexpr (KV4) {
       const Codes& c = KEYS ? ck : cv;
       const Kv4Magic magic;
-      const int own = (int)fresh((uint32_t)lane);
+      const uint32_t own = fresh((uint32_t)lane) & 63;
 #pragma unroll
       for (int p = 0; p < S::NU; ++p) {
-        const int e = p * 64 + own, r = wv * S::RPW + e / S::UPR, u = e % S::UPR;
+        const int r = wv * S::RPW + (int)(own / S::UPR) + p * (64 / S::UPR), u = own % S::UPR;
         const Kv4Blocks block = Kv4Blocks::of(c.head[p]);
 #pragma unroll
         for (int w = 0; w < S::UE / 8; ++w) {
@@ -437,6 +482,7 @@ struct PpWave {
       const float b = __builtin_amdgcn_exp2f(fmaf(x[I][t][e + 1], by, less));
       l += a;
       l += b;
+      asm("" : "+v"(l));  // (here, not when all weights are there)
       if constexpr (CT == BB_F32) {
         p.f[t][e] = a;
         p.f[t][e + 1] = b;
@@ -602,6 +648,7 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>
   const int raw = sq.lens[s], end = pq.seq_start ? pq.seq_start[s + 1] : s + 1;
   w.len = min(max(raw, 0), sq.max_pages * kv.page_size);
   w.prefix = pq.prefix ? min(max(pq.prefix[s], 0), w.len) : 0;
+  w.runs = pl.runs;
   w.row = sq.table + (size_t)s * sq.table_stride;
   w.kv_off = (size_t)kvh * kv.head_stride;
   const int rows = n * pl.G, r0 = it * S::BM;
@@ -691,17 +738,20 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>
     const auto turn = [&](int u, auto set) BB_INLINE {
       constexpr int I = decltype(set)::value;
       const bool more = u + 1 < n_turns, two = u + 2 < n_turns;
-      if (two) bring(u + 2);
-      if (more) w.template load<false>(vrow, vals(u + 1));
-      if (two) {
-        vrow = krow;
-        if (u + 3 < n_turns) w.find(kt.at(u0 + u + 3));
-      }
+      const auto ask = [&](int j) BB_INLINE {  // (behind the products of a step, which go on meanwhile)
+        if (j == 0 && two) bring(u + 2);
+        if (j == 1 && more) w.template load<false>(vrow, vals(u + 1));
+        if (j == 2 && two) {
+          vrow = krow;
+          if (u + 3 < n_turns) w.find(kt.at(u0 + u + 3));
+        }
+      };
       typename Wave::Weights p;
       __builtin_amdgcn_sched_barrier(0);
       // (behind the last tile, scores of whatever is there, for nothing)
       w.template score<1 - I>(lds_at(keys(u + 1)), [&](int j) BB_INLINE {
         constexpr int PAIRS = 8 * S::NT;
+        ask(j);
         w.template weigh<I>(p, j * PAIRS / Wave::STEPS, (j + 1) * PAIRS / Wave::STEPS);
       });
       w.add(lds_at(vals(u)), p);
@@ -889,6 +939,7 @@ hipError_t prompt_of(hipStream_t st, const PromptQuery& q, const PagedView& kv, 
     // (no more parts than the table's width has of the least size)
     const size_t cap = ((size_t)sq.max_pages * kv.page_size + S::KT - 1) / S::KT;
     pl.least = std::max(1, 256 / S::KT);
+    pl.runs = kv.page_size % S::RPW == 0 && kv.hd == HDP && (size_t)S::RPW * kv.pos_stride * S::SZ < ((size_t)1 << 31);
     pl.parts = (int)std::min<size_t>(pl.parts, std::max<size_t>(1, cap / pl.least));
     const unsigned blocks = (unsigned)((size_t)pl.n_tiles * pl.n_kv * pl.parts);
     BB_LAUNCH((k_paged_prompt<CT, NQ, NP, HDP, WR, KV4>), dim3(blocks), dim3(PP_THREADS), 0, st, q, kv, sq, pl);
@@ -931,7 +982,7 @@ hipError_t launch_paged_prompt(hipStream_t st, int n_cu, int cache, const Prompt
                                const PagedSeqs& sq) {
   const int G = q.n_heads / kv.n_kv;
   const PromptCut c = prompt_cut(n_cu, cache, q.n_tokens, sq.n_seqs, G, kv.n_kv, kv.hd);
-  PromptPlan pl{G, c.n_tiles, kv.n_kv, c.parts, 1, nullptr, nullptr, nullptr};
+  PromptPlan pl{G, c.n_tiles, kv.n_kv, c.parts, 1, false, nullptr, nullptr, nullptr};
   if (c.parts > 1) {
     const size_t tiles = (size_t)c.n_tiles * kv.n_kv, slots = tiles * c.parts * c.bm;
     pl.places = static_cast<int4*>(q.ws);
