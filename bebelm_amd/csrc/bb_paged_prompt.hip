@@ -16,12 +16,18 @@ constexpr float SLACK = 6.0f, F16_UP = 8.0f;
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 
+// Where tiles come from: rows of the cache as they are; 4-bit ones, made f16; f32 ones, made sums of three bf16 parts each
+// rounded from what the ones before leave (8 bits of it: all of 24 but 2^-25).
+enum { SRC_SAME, SRC_KV4, SRC_PARTS };
+
 // A block's shape. CT: the type that tiles have in LDS; WR waves along the rows (32 each), 4 / WR along the keys.
-template <int CT, int NQ, int NP, int HDP, int WR, bool KV4>
+template <int CT, int NQ, int NP, int HDP, int WR, int SRC>
 struct PpShape {
+  static constexpr bool KV4 = SRC == SRC_KV4, PARTS = SRC == SRC_PARTS;
   static constexpr int SZ = CT == BB_F32 ? 4 : 2;
+  static constexpr int NPL = PARTS ? 3 : 1;  // parts of an element, each a plane of the tile
   static constexpr int WK = 4 / WR, BM = 32 * WR;
-  static constexpr int BN = WK > 1 || HDP * SZ >= 1024 ? 32 : 64;  // keys of a wave's tile
+  static constexpr int BN = WK > 1 || HDP * SZ >= 1024 || PARTS ? 32 : 64;  // keys of a wave's tile
   static constexpr int KT = WK * BN;                               // keys of the block's
   static constexpr int NT = BN / 32;
   // Rows in LDS: 16-byte pieces, of which row r has piece u at place u ^ k_swap(r) (keys) or u ^ v_swap(r) (values).
@@ -32,7 +38,7 @@ struct PpShape {
   __device__ static __forceinline__ int v_swap(int r) {
     return SZ == 4 ? (r >> 2 & 1) << 3 : (PPR == 8 ? (r >> 1 & 1) << 2 : (r & 3) << 2) | (r >> 2 & 3);
   }
-  static constexpr int BUF = 2 * KT * ROW;
+  static constexpr int PLANE = KT * ROW, BUF = 2 * NPL * PLANE;
   // (two of them: an iteration reads the keys of the next tile and the values of its own)
   static constexpr int LD = HDP + 4;                                        // a row of the waves' sums, in the same place
   static constexpr int SUMS = WK > 1 ? 4 * 32 * (LD * 4 + 8) : 0;
@@ -40,10 +46,11 @@ struct PpShape {
   static constexpr int RPW = KT / 4;  // rows a wave brings
   // pieces of 16 bytes in LDS that a lane brings of keys (and of values); of a 4-bit cache, units of UE elements
   static constexpr int NPC = RPW * PPR / 64;
-  static constexpr int UE = RPW * HDP / 64 < 32 ? RPW * HDP / 64 : 32, UPR = HDP / UE, NU = RPW * UPR / 64;
+  // (of f32 parts, of 8)
+  static constexpr int UE = PARTS ? 8 : RPW * HDP / 64 < 32 ? RPW * HDP / 64 : 32, UPR = HDP / UE, NU = RPW * UPR / 64;
   static constexpr int QW = CT == BB_F32 ? HDP / 2 : NQ * HDP / 4;  // registers of the query rows
   static constexpr int REGS = HDP / 2 + QW + 16 * NT + (CT == BB_F32 ? 0 : 8 * NP * NT) +
-                              (KV4 ? 2 * NU * (UE / 8 + 1) : 0);
+                              (KV4 ? 2 * NU * (UE / 8 + 1) : PARTS ? 16 * NU + 32 : 0);
   static constexpr int WAVES = REGS <= 208 && LDS <= 79 * 1024 ? 2 : 1;  // of a SIMD
 };
 
@@ -86,6 +93,19 @@ __device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
+// Two values as N bf16 parts, each rounded to the nearest.
+template <int N>
+__device__ __forceinline__ void round_parts(float a, float b, uint32_t (&w)[N]) {
+  typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const v2b r = {(__bf16)a, (__bf16)b};
+    w[i] = __builtin_bit_cast(uint32_t, r);
+    a = a - as_float(w[i] << 16);
+    b = b - as_float(w[i] & 0xffff0000u);
+  }
+}
+
 // Two 16-bit elements: those that are not finite, as 1s of the type (0: finite), and the others as they are.
 template <int CT>
 __device__ __forceinline__ uint32_t odd_halves(uint32_t w) {
@@ -107,10 +127,12 @@ struct PromptPlan {
   int4* places;  // [tile][kv head]
 };
 
-template <int CT, int NQ, int NP, int HDP, int WR, bool KV4>
+template <int CT, int NQ, int NP, int HDP, int WR, int SRC>
 struct PpWave {
-  typedef PpShape<CT, NQ, NP, HDP, WR, KV4> S;
-  static constexpr int NT = S::NT, SZ = S::SZ;
+  typedef PpShape<CT, NQ, NP, HDP, WR, SRC> S;
+  static constexpr int NT = S::NT, SZ = S::SZ, NPL = S::NPL;
+  static constexpr bool KV4 = S::KV4, PARTS = S::PARTS;
+  static constexpr int CZ = PARTS ? 4 : SZ;  // bytes of the cache's elements
   static constexpr bool F16 = CT == BB_F16;
   const PagedView& kv;
   const PromptQuery& pq;
@@ -127,6 +149,7 @@ struct PpWave {
   v16f o[HDP / 32];
   struct Codes {
     uint32_t word[KV4 ? S::NU * S::UE / 8 : 1], head[KV4 ? S::NU : 1];
+    v4u f32[PARTS ? 2 * S::NU : 1];
   };
   Codes ck, cv;
   v16f x[2][NT];              // scores of the tile at work (in multiples of `by`) and of the next, by turns
@@ -177,7 +200,8 @@ struct PpWave {
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
           uint32_t w[NQ];
-          split2<CT, NQ>(x[e], x[e + 1], w);
+          if constexpr (PARTS) round_parts(x[e], x[e + 1], w);
+          else split2<CT, NQ>(x[e], x[e + 1], w);
 #pragma unroll
           for (int k = 0; k < NQ; ++k) q[k][j][e / 2] = w[k];
         }
@@ -206,7 +230,7 @@ struct PpWave {
   __device__ __forceinline__ Row found() const {
     const bool there = (uint32_t)page < (uint32_t)kv.n_pages;
     const size_t at = (size_t)(uint32_t)page * kv.page_stride + (KV4 ? 0 : (size_t)(uint32_t)in * kv.pos_stride) + kv_off;
-    return Row{there ? (int64_t)(KV4 ? at : at * SZ) : -1, in,
+    return Row{there ? (int64_t)(KV4 ? at : at * CZ) : -1, in,
                runs && (uint32_t)__builtin_amdgcn_readfirstlane(page) < (uint32_t)kv.n_pages};
   }
   // Which of the wave's rows are there.
@@ -235,6 +259,15 @@ struct PpWave {
           load_words<S::UE / 8>(codes + r * (HDP / 2) + u * (S::UE / 2), c.word + p * S::UE / 8);
           c.head[p] = *reinterpret_cast<const uint16_t*>(heads + 2 * (r * (HDP / 32) + u * S::UE / 32));
         }
+      } else if constexpr (PARTS) {
+        Codes& c = KEYS ? ck : cv;
+        const uint32_t step = (uint32_t)kv.pos_stride * 4;
+#pragma unroll
+        for (int p = 0; p < S::NU; ++p) {
+          const uint32_t r = mine / S::UPR + p * (64 / S::UPR), u = mine % S::UPR;
+          c.f32[2 * p] = *reinterpret_cast<const v4u*>(base + (r * step + u * 32));
+          c.f32[2 * p + 1] = *reinterpret_cast<const v4u*>(base + (r * step + u * 32 + 16));
+        }
       } else {
         const uint32_t step = (uint32_t)kv.pos_stride * SZ, r0 = mine / S::PPR, u = mine % S::PPR;
 #pragma unroll
@@ -247,7 +280,20 @@ struct PpWave {
       return;
     }
     const uint32_t own = fresh((uint32_t)lane) & 63;
-    if constexpr (KV4) {
+    if constexpr (PARTS) {
+      const uint32_t alo = (uint32_t)w.at, ahi = (uint32_t)(w.at >> 32);
+      Codes& c = KEYS ? ck : cv;
+#pragma unroll
+      for (int p = 0; p < S::NU; ++p) {
+        const int r = (int)(own / S::UPR) + p * (64 / S::UPR), u = own % S::UPR;
+        const int64_t base = (int64_t)((uint64_t)(uint32_t)__shfl((int)ahi, r) << 32 | (uint32_t)__shfl((int)alo, r));
+        c.f32[2 * p] = c.f32[2 * p + 1] = v4u{0, 0, 0, 0};
+        if (base >= 0 && 8 * u < kv.hd) {
+          c.f32[2 * p] = *reinterpret_cast<const v4u*>(pool + base + u * 32);
+          c.f32[2 * p + 1] = *reinterpret_cast<const v4u*>(pool + base + u * 32 + 16);
+        }
+      }
+    } else if constexpr (KV4) {
       const uint32_t alo = (uint32_t)w.at, ahi = (uint32_t)(w.at >> 32);
       Codes& c = KEYS ? ck : cv;
 #pragma unroll
@@ -290,7 +336,7 @@ struct PpWave {
     }
   }
 
-  // Puts 4-bit rows into a tile, as the f16 values they stand for.
+  // Puts 4-bit rows into a tile, as the f16 values they stand for, and f32 rows, as their parts.
   template <bool KEYS>
   __device__ __forceinline__ void put(char* lds) const {
     if constexpr (KV4) {
@@ -309,36 +355,63 @@ struct PpWave {
         }
       }
     }
+    if constexpr (PARTS) {
+      const Codes& c = KEYS ? ck : cv;
+      const uint32_t own = fresh((uint32_t)lane) & 63;
+#pragma unroll
+      for (int p = 0; p < S::NU; ++p) {
+        const int r = wv * S::RPW + (int)(own / S::UPR) + p * (64 / S::UPR), u = own % S::UPR;
+        v4u part[3];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t w[3];
+          const v4u x = c.f32[2 * p + e / 2];
+          round_parts(as_float(x[e % 2 * 2]), as_float(x[e % 2 * 2 + 1]), w);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) part[i][e] = w[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          *reinterpret_cast<v4u*>(lds + i * S::PLANE + r * S::ROW + (u ^ (KEYS ? S::k_swap(r) : S::v_swap(r))) * 16) = part[i];
+      }
+    }
   }
 
   // Scores of a tile: register e of lane (row, half) is key 8(e / 4) + 4·half + e % 4 of 32. between(j) is done with the
   // products of the j-th of STEPS steps, whose keys have been asked for a step before.
   static constexpr int STEPS = CT == BB_F32 ? HDP / 8 : HDP / 16;
-  template <int PARTS, class F>
+  // (ALL: of all parts whose product counts, those of the first: 2^-23 of each other; otherwise of the first alone)
+  template <bool ALL, class F>
   __device__ __forceinline__ void scores(uint32_t lk, v16f (&y)[NT], F&& between) const {
     const uint32_t at0 = fresh(lk + (wk * S::BN + col) * S::ROW + (half ^ S::k_swap(col)) * 16);
-    v4u a[2][NT];
+    v4u a[2][NT][NPL];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) y[t][e] = 0.0f;
-      a[0][t] = read_lds<v4u>(at0 + 32 * t * S::ROW);
+#pragma unroll
+      for (int l = 0; l < NPL; ++l) a[0][t][l] = read_lds<v4u>(at0 + 32 * t * S::ROW + l * S::PLANE);
     }
 #pragma unroll
     for (int j = 0; j < STEPS; ++j) {
       if (j + 1 < STEPS)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) a[(j + 1) & 1][t] = read_lds<v4u>((at0 ^ 32 * (j + 1)) + 32 * t * S::ROW);
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int l = 0; l < NPL; ++l)
+            a[(j + 1) & 1][t][l] = read_lds<v4u>((at0 ^ 32 * (j + 1)) + 32 * t * S::ROW + l * S::PLANE);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const v4u k = a[j & 1][t];
         if constexpr (CT == BB_F32) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            y[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(as_float(k[e]), qf[j][e], y[t], 0, 0, 0);
+            y[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(as_float(a[j & 1][t][0][e]), qf[j][e], y[t], 0, 0, 0);
         } else {
 #pragma unroll
-          for (int i = PARTS - 1; i >= 0; --i) y[t] = mfma32<CT>(k, q[i][j], y[t]);
+          for (int i = NQ - 1; i >= 0; --i)
+#pragma unroll
+            for (int l = NPL - 1; l >= 0; --l)
+              if (ALL ? l + i < 3 : l + i == 0) y[t] = mfma32<CT>(a[j & 1][t][l], q[i][j], y[t]);
         }
       }
       between(j);
@@ -362,10 +435,11 @@ struct PpWave {
     }
   }
   // Elements 32·dt + lane % 32 of the values at the keys whose weights are registers 8s..8s+7 of a tile (16-bit types).
-  __device__ __forceinline__ v4u values(At at, int t, int s, int dt) const {
+  __device__ __forceinline__ v4u values(At at, int t, int s, int dt, int plane = 0) const {
     typedef __attribute__((address_space(3))) v4s* lds_v4s;
-    const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)((at.a ^ 64 * dt) + (32 * t + 16 * s) * S::ROW));
-    const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)((at.b ^ 64 * dt) + (32 * t + 16 * s) * S::ROW));
+    const int more = (32 * t + 16 * s) * S::ROW + plane * S::PLANE;
+    const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)((at.a ^ 64 * dt) + more));
+    const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)((at.b ^ 64 * dt) + more));
     const v2u x = __builtin_bit_cast(v2u, a), y = __builtin_bit_cast(v2u, b);
     return v4u{x[0], x[1], y[0], y[1]};
   }
@@ -384,7 +458,7 @@ struct PpWave {
   template <int I, class F>
   __device__ __forceinline__ void score(uint32_t lk, F&& between) {
     v16f(&y)[NT] = x[I];
-    scores<NQ>(lk, y, between);
+    scores<true>(lk, y, between);
     if constexpr (NQ > 1) {
       // a part of 0 meets an infinite key as NaN: such scores are taken from the first parts alone
       bool odd = false;
@@ -394,7 +468,7 @@ struct PpWave {
         for (int e = 0; e < 16; ++e) odd |= y[t][e] != y[t][e];
       if (__any(odd)) {
         v16f z[NT];
-        scores<1>(lk, z, [](int) {});
+        scores<false>(lk, z, [](int) {});
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -531,18 +605,25 @@ struct PpWave {
           for (int d = 0; d < ND; ++d)
             o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(value(at, t, e, d), p.f[t][e], o[d], 0, 0, 0);
     } else {
-      v4u a[2][ND];
+      v4u a[2][ND][NPL];
 #pragma unroll
-      for (int d = 0; d < ND; ++d) a[0][d] = values(at, 0, 0, d);
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int l = 0; l < NPL; ++l) a[0][d][l] = values(at, 0, 0, d, l);
 #pragma unroll
       for (int g = 0; g < 2 * NT; ++g) {
         if (g + 1 < 2 * NT)
 #pragma unroll
-          for (int d = 0; d < ND; ++d) a[(g + 1) & 1][d] = values(at, (g + 1) / 2, (g + 1) % 2, d);
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int l = 0; l < NPL; ++l) a[(g + 1) & 1][d][l] = values(at, (g + 1) / 2, (g + 1) % 2, d, l);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
-          for (int k = NP - 1; k >= 0; --k) o[d] = mfma32<CT>(a[g & 1][d], p.w[g / 2][g % 2][k], o[d]);
+          for (int k = NP - 1; k >= 0; --k)
+#pragma unroll
+            for (int l = NPL - 1; l >= 0; --l)
+              if (l + k < 3) o[d] = mfma32<CT>(a[g & 1][d][l], p.w[g / 2][g % 2][k], o[d]);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -595,7 +676,7 @@ struct PpWave {
   }
   // The wave's share of a tile of values without those that are not finite.
   __device__ __forceinline__ void clean(char* lv) const {
-    for (int i = wv * 64 + lane; i < S::KT * S::PPR; i += PP_THREADS) {
+    for (int i = wv * 64 + lane; i < NPL * S::KT * S::PPR; i += PP_THREADS) {
       v4u* p = reinterpret_cast<v4u*>(lv + i * 16);
       v4u a = *p;
 #pragma unroll
@@ -606,10 +687,10 @@ struct PpWave {
   }
 };
 
-template <int CT, int NQ, int NP, int HDP, int WR, bool KV4>
-__global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>::WAVES))
+template <int CT, int NQ, int NP, int HDP, int WR, int SRC>
+__global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, SRC>::WAVES))
     k_paged_prompt(PromptQuery pq, PagedView kv, PagedSeqs sq, PromptPlan pl) {
-  typedef PpShape<CT, NQ, NP, HDP, WR, KV4> S;
+  typedef PpShape<CT, NQ, NP, HDP, WR, SRC> S;
   __shared__ __align__(1024) char s_tiles[S::LDS];
   __shared__ uint32_t s_ok[2][4];
   __shared__ uint32_t s_marks[2][HDP / 32][PP_THREADS];
@@ -643,7 +724,7 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>
     return;
   }
 
-  typedef PpWave<CT, NQ, NP, HDP, WR, KV4> Wave;
+  typedef PpWave<CT, NQ, NP, HDP, WR, SRC> Wave;
   Wave w(kv, pq, tid);
   const int raw = sq.lens[s], end = pq.seq_start ? pq.seq_start[s + 1] : s + 1;
   w.len = min(max(raw, 0), sq.max_pages * kv.page_size);
@@ -690,7 +771,7 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, KV4>
   if (u0 < u1) {
     const int n_turns = u1 - u0;
     const auto keys = [&](int u) BB_INLINE { return s_tiles + (u & 1) * S::BUF; };
-    const auto vals = [&](int u) BB_INLINE { return s_tiles + (u & 1) * S::BUF + S::KT * S::ROW; };
+    const auto vals = [&](int u) BB_INLINE { return s_tiles + (u & 1) * S::BUF + S::NPL * S::PLANE; };
     const auto flags = [&](int u, uint32_t& ok0, uint32_t& ok1) BB_INLINE {
       const uint32_t* ok = s_ok[u & 1];
       ok1 = ~0u;
@@ -930,19 +1011,19 @@ size_t prompt_ws(const PromptCut& c, int n_kv, int hd) {
   return slots * ((size_t)hd * 4 + sizeof(float2)) + tiles * sizeof(int4);
 }
 
-template <int CT, int NQ, int NP, int HDP, int WR, bool KV4>
+template <int CT, int NQ, int NP, int HDP, int WR, int SRC>
 hipError_t prompt_of(hipStream_t st, const PromptQuery& q, const PagedView& kv, const PagedSeqs& sq, PromptPlan pl) {
-  typedef PpShape<CT, NQ, NP, HDP, WR, KV4> S;
+  typedef PpShape<CT, NQ, NP, HDP, WR, SRC> S;
   if constexpr (S::LDS > 159 * 1024) {
     return hipErrorInvalidValue;
   } else {
     // (no more parts than the table's width has of the least size)
     const size_t cap = ((size_t)sq.max_pages * kv.page_size + S::KT - 1) / S::KT;
     pl.least = std::max(1, 256 / S::KT);
-    pl.runs = kv.page_size % S::RPW == 0 && kv.hd == HDP && (size_t)S::RPW * kv.pos_stride * S::SZ < ((size_t)1 << 31);
+    pl.runs = kv.page_size % S::RPW == 0 && kv.hd == HDP && (size_t)S::RPW * kv.pos_stride * 4 < ((size_t)1 << 31);
     pl.parts = (int)std::min<size_t>(pl.parts, std::max<size_t>(1, cap / pl.least));
     const unsigned blocks = (unsigned)((size_t)pl.n_tiles * pl.n_kv * pl.parts);
-    BB_LAUNCH((k_paged_prompt<CT, NQ, NP, HDP, WR, KV4>), dim3(blocks), dim3(PP_THREADS), 0, st, q, kv, sq, pl);
+    BB_LAUNCH((k_paged_prompt<CT, NQ, NP, HDP, WR, SRC>), dim3(blocks), dim3(PP_THREADS), 0, st, q, kv, sq, pl);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || pl.parts == 1) return e;
     BB_LAUNCH(k_prompt_join, dim3(pl.n_tiles * pl.n_kv, S::BM / (PP_THREADS / 64)), dim3(PP_THREADS), 0, st, q, kv.hd,
@@ -951,20 +1032,31 @@ hipError_t prompt_of(hipStream_t st, const PromptQuery& q, const PagedView& kv, 
   }
 }
 
-template <int CT, int NQ, int NP, bool KV4>
+template <int CT, int NQ, int NP, int SRC>
 hipError_t prompt_by(hipStream_t st, int wr, const PromptQuery& q, const PagedView& kv, const PagedSeqs& sq,
                      const PromptPlan& pl) {
   const auto of = [&](auto hdp) {
     constexpr int H = decltype(hdp)::value;
-    return wr == 4   ? prompt_of<CT, NQ, NP, H, 4, KV4>(st, q, kv, sq, pl)
-           : wr == 2 ? prompt_of<CT, NQ, NP, H, 2, KV4>(st, q, kv, sq, pl)
-                     : prompt_of<CT, NQ, NP, H, 1, KV4>(st, q, kv, sq, pl);
+    return wr == 4   ? prompt_of<CT, NQ, NP, H, 4, SRC>(st, q, kv, sq, pl)
+           : wr == 2 ? prompt_of<CT, NQ, NP, H, 2, SRC>(st, q, kv, sq, pl)
+                     : prompt_of<CT, NQ, NP, H, 1, SRC>(st, q, kv, sq, pl);
   };
   switch (pa_class(kv.hd)) {
     case 64: return of(std::integral_constant<int, 64>());
     case 128: return of(std::integral_constant<int, 128>());
     default: return of(std::integral_constant<int, 256>());
   }
+}
+
+// An f32 cache: f32 matrix instructions, or for tiles of 128 rows and heads of up to 128 six times 16-bit ones (of the
+// products of three parts with three, those that count), a sixteenth of the time each.
+template <int NQ>
+hipError_t prompt_f32(hipStream_t st, int wr, const PromptQuery& q, const PagedView& kv, const PagedSeqs& sq,
+                      const PromptPlan& pl) {
+  const int cls = pa_class(kv.hd);
+  if (wr == 4 && cls == 64) return prompt_of<BB_BF16, NQ, 3, 64, 4, SRC_PARTS>(st, q, kv, sq, pl);
+  if (wr == 4 && cls == 128) return prompt_of<BB_BF16, NQ, 3, 128, 4, SRC_PARTS>(st, q, kv, sq, pl);
+  return prompt_by<BB_F32, 1, 1, SRC_SAME>(st, wr, q, kv, sq, pl);
 }
 
 }  // namespace
@@ -990,17 +1082,17 @@ hipError_t launch_paged_prompt(hipStream_t st, int n_cu, int cache, const Prompt
     pl.ml = reinterpret_cast<float2*>(pl.sums + slots * kv.hd);
   }
   switch (cache) {
-    case BB_F32: return prompt_by<BB_F32, 1, 1, false>(st, c.wr, q, kv, sq, pl);
+    case BB_F32: return q.dt == BB_F32 ? prompt_f32<3>(st, c.wr, q, kv, sq, pl) : prompt_f32<2>(st, c.wr, q, kv, sq, pl);
     case BB_F16:
-      return q.dt == BB_F32 ? prompt_by<BB_F16, 2, 2, false>(st, c.wr, q, kv, sq, pl)
-                            : prompt_by<BB_F16, 1, 1, false>(st, c.wr, q, kv, sq, pl);
+      return q.dt == BB_F32 ? prompt_by<BB_F16, 2, 2, SRC_SAME>(st, c.wr, q, kv, sq, pl)
+                            : prompt_by<BB_F16, 1, 1, SRC_SAME>(st, c.wr, q, kv, sq, pl);
     case BB_BF16:
-      return q.dt == BB_F32   ? prompt_by<BB_BF16, 3, 3, false>(st, c.wr, q, kv, sq, pl)
-             : q.dt == BB_F16 ? prompt_by<BB_BF16, 2, 2, false>(st, c.wr, q, kv, sq, pl)
-                              : prompt_by<BB_BF16, 1, 1, false>(st, c.wr, q, kv, sq, pl);
+      return q.dt == BB_F32   ? prompt_by<BB_BF16, 3, 3, SRC_SAME>(st, c.wr, q, kv, sq, pl)
+             : q.dt == BB_F16 ? prompt_by<BB_BF16, 2, 2, SRC_SAME>(st, c.wr, q, kv, sq, pl)
+                              : prompt_by<BB_BF16, 1, 1, SRC_SAME>(st, c.wr, q, kv, sq, pl);
     case BB_KV4:
-      return q.dt == BB_F32 ? prompt_by<BB_F16, 2, 2, true>(st, c.wr, q, kv, sq, pl)
-                            : prompt_by<BB_F16, 1, 1, true>(st, c.wr, q, kv, sq, pl);
+      return q.dt == BB_F32 ? prompt_by<BB_F16, 2, 2, SRC_KV4>(st, c.wr, q, kv, sq, pl)
+                            : prompt_by<BB_F16, 1, 1, SRC_KV4>(st, c.wr, q, kv, sq, pl);
     default: return hipErrorInvalidValue;
   }
 }
