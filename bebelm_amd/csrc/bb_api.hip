@@ -2740,14 +2740,14 @@ size_t prompt_ws(bb_ctx* c, const bb_paged_kv* kv, size_t n_heads, size_t n_seqs
   // (one token each may take attention of single tokens)
   return n_tokens != n_seqs || n_seqs == 0
              ? bytes
-             : std::max(bytes, bb::paged_attn_ws(c->n_cu, (int)n_seqs, (int)n_heads, (int)n_kv, kv->view.hd));
+             : std::max(bytes, bb::paged_attn_ws(c->n_cu, (int)kv->dtype, (int)n_seqs, (int)n_heads, (int)n_kv, kv->view.hd));
 }
 
 size_t paged_ws(bb_ctx* c, const bb_paged_kv* kv, size_t n_heads, size_t n_seqs) {
   need(n_heads >= 1 && n_heads % (size_t)kv->view.n_kv == 0, BB_ERR_ARG, "n_heads must be a multiple of n_kv_heads");
   need(n_heads < ((size_t)1 << 16), BB_ERR_RANGE, "n_heads must be below 65536");
   need(n_seqs <= PAGED_SEQS_MAX, BB_ERR_RANGE, "more than 65536 sequences");
-  return bb::paged_attn_ws(c->n_cu, (int)n_seqs, (int)n_heads, kv->view.n_kv, kv->view.hd);
+  return bb::paged_attn_ws(c->n_cu, (int)kv->dtype, (int)n_seqs, (int)n_heads, kv->view.n_kv, kv->view.hd);
 }
 
 }  // namespace

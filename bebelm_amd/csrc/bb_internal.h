@@ -424,7 +424,7 @@ struct PagedQuery {
   float cap = 0.0f;  // > 0: scores are capped
   const float* slopes = nullptr;
 };
-size_t paged_attn_ws(int n_cu, int n_seqs, int n_heads, int n_kv, int hd);
+size_t paged_attn_ws(int n_cu, int cache, int n_seqs, int n_heads, int n_kv, int hd);
 // Whether a batch's units of work can be counted in 30 bits (cap: positions of a sequence at most).
 bool paged_attn_fits(int n_seqs, int n_heads, int n_kv, size_t cap);
 hipError_t launch_paged_attn(hipStream_t s, int n_cu, int cache, const PagedQuery& q, const PagedView& kv,

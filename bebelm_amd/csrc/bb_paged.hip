@@ -445,7 +445,7 @@ struct PaShape {
 // needs one block's head: instruction j takes elements 32g + 8j.. of group g (64: 16g + 8j..). Values of two positions
 // are put side by side as half words, which then give an element of both, as the instructions want them.
 // MOD: scores are capped or get a bias by distance.
-template <int CT, int NP, int HDP, bool UNI, bool KV4, bool MOD>
+template <int CT, int NQ, int NP, int HDP, bool UNI, bool KV4, bool MOD>
 struct PaWave {
   typedef PaShape<CT, HDP> S;
   static constexpr int NT = S::NT, NC = S::NC, NV = S::NV, VE = S::VE, PE = S::PE, KE = S::KE, SZ = S::SZ;
@@ -456,8 +456,9 @@ struct PaWave {
   int head0, heads;  // head0: the first head of the group; heads: how many
   size_t kv_off;     // the kv head's offset in the pool (elements)
   SeqSpan sp;
-  v4u q[NP][NC];
-  float c;        // what scores are multiplied by where NP is 2
+  v4u q[NQ][NC];  // (NQ parts of q, NP of the weights)
+  static constexpr bool SCALED = CT != BB_F32 && NP == 2;
+  float c;        // what scores are multiplied by (SCALED; otherwise it is in q)
   float m, l;
   v4f o[VE];
   v4u k[KV4 ? 1 : NT][KV4 ? 1 : NC];
@@ -502,7 +503,7 @@ struct PaWave {
       cap = pq.cap * LOG2E;
       slope = pq.slopes ? pq.slopes[head0 + min(n, heads - 1)] * LOG2E : 0.0f;
     }
-    const float cq = NP == 2 ? 1.0f : c;
+    const float cq = SCALED ? 1.0f : c;
 #pragma unroll
     for (int j = 0; j < NC; ++j)
 #pragma unroll
@@ -530,10 +531,10 @@ struct PaWave {
       } else {
 #pragma unroll
         for (int e = 0; e < KE; e += 2) {
-          uint32_t w[NP];
-          split2<CT, NP>(x[j][KV4 ? e / 2 : e], x[j][KV4 ? e / 2 + 4 : e + 1], w);
+          uint32_t w[NQ];
+          split2<CT, NQ>(x[j][KV4 ? e / 2 : e], x[j][KV4 ? e / 2 + 4 : e + 1], w);
 #pragma unroll
-          for (int i = 0; i < NP; ++i) q[i][j][e / 2] = w[i];
+          for (int i = 0; i < NQ; ++i) q[i][j][e / 2] = w[i];
         }
       }
     }
@@ -804,8 +805,8 @@ struct PaWave {
 
   // Scores of the loaded keys, from which the keys' registers are free again.
   __device__ __forceinline__ void score(v4f (&x)[NT]) const {
-    scores<NP>(x);
-    if constexpr (NP > 1) {
+    scores<NQ>(x);
+    if constexpr (NQ > 1) {
       bool odd = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -825,7 +826,7 @@ struct PaWave {
 
   // Adds a tile: its scores x and the loaded values.
   __device__ __forceinline__ void add(v4f (&x)[NT]) {
-    if constexpr (NP == 2) {
+    if constexpr (SCALED) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) x[t] *= c;
     }
@@ -865,8 +866,12 @@ struct PaWave {
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        x[t][r] = __builtin_amdgcn_exp2f(x[t][r] - ref);
-        if constexpr (CT == BB_F16) x[t][r] *= 16384.0f;
+        if constexpr (KV4) {
+          x[t][r] = __builtin_amdgcn_exp2f(x[t][r] - (ref - 14.0f));
+        } else {
+          x[t][r] = __builtin_amdgcn_exp2f(x[t][r] - ref);
+          if constexpr (CT == BB_F16) x[t][r] *= 16384.0f;
+        }
         l += x[t][r];
       }
     if constexpr (CT == BB_F32) {
@@ -987,8 +992,8 @@ struct SeqScan {
   }
 };
 
-template <int CT, int NP, int HDP, bool UNI, bool KV4, bool MOD>
-__global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQuery pq, PagedView kv,
+template <int CT, int NQ, int NP, int HDP, bool UNI, bool KV4, bool MOD>
+__global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP, KV4)) k_paged_attn(PagedQuery pq, PagedView kv,
                                                                         const int* __restrict__ table,
                                                                         const int* __restrict__ lens, size_t table_stride,
                                                                         int n_seqs, int max_pages, PagedPlan pl) {
@@ -1055,7 +1060,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP)) k_paged_attn(PagedQ
   int grp = uniform_div(u - lo, cost);
   lo += grp * cost;
 
-  typedef PaWave<CT, NP, HDP, UNI, KV4, MOD> Wave;
+  typedef PaWave<CT, NQ, NP, HDP, UNI, KV4, MOD> Wave;
   Wave w(kv, lane);
   const float up = CT == BB_F16 ? 14.0f : 0.0f;
   bool lds_read = false;
@@ -1210,8 +1215,8 @@ void PagedView::set_slots(int n) {
   page_shift = d.shift;
 }
 
-size_t paged_attn_ws(int n_cu, int n_seqs, int n_heads, int n_kv, int hd) {
-  const size_t slots = 2 * (size_t)blocks_at_once(n_cu, hd) * head_groups(n_heads, n_kv).hg;
+size_t paged_attn_ws(int n_cu, int cache, int n_seqs, int n_heads, int n_kv, int hd) {
+  const size_t slots = 2 * (size_t)blocks_at_once(n_cu, hd, cache == BB_KV4) * head_groups(n_heads, n_kv).hg;
   return slots * ((size_t)hd * 4 + sizeof(float2)) + ((size_t)n_seqs + 2) * 4;
 }
 
@@ -1225,38 +1230,39 @@ hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQue
   PagedView kv = pool;
   if (uni) kv.set_slots(cut.slots);
   PagedPlan pl{g.G, g.split, g.hg, g.n_groups, cut.join, cut.unit, cut.few, nullptr, nullptr, nullptr};
-  const size_t slots = 2 * (size_t)blocks_at_once(n_cu, kv.hd) * pl.hg;
+  const size_t slots = 2 * (size_t)blocks_at_once(n_cu, kv.hd, cache == BB_KV4) * pl.hg;
   pl.sums = static_cast<float*>(q.ws);
   pl.ml = reinterpret_cast<float2*>(pl.sums + slots * kv.hd);
   pl.chunk = reinterpret_cast<int*>(pl.ml + slots);
   const unsigned blocks = (unsigned)cut.blocks;
   const int cls = pa_class(kv.hd);
   const size_t lds = (size_t)PA_WAVES * pl.hg * (cls + 4) * 4;
-#define BB_PA(ct, np, hdp, four, mod)                                                                               \
+#define BB_PA(ct, nq, np, hdp, four, mod)                                                                               \
   do {                                                                                                              \
     if (uni)                                                                                                        \
-      BB_LAUNCH((k_paged_attn<ct, np, hdp, true, four, mod>), dim3(blocks), dim3(PA_THREADS), lds, st, q, kv, sq.table,  \
+      BB_LAUNCH((k_paged_attn<ct, nq, np, hdp, true, four, mod>), dim3(blocks), dim3(PA_THREADS), lds, st, q, kv, sq.table,  \
                 sq.lens, sq.table_stride, sq.n_seqs, sq.max_pages, pl);                                             \
     else                                                                                                            \
-      BB_LAUNCH((k_paged_attn<ct, np, hdp, false, four, mod>), dim3(blocks), dim3(PA_THREADS), lds, st, q, kv, sq.table, \
+      BB_LAUNCH((k_paged_attn<ct, nq, np, hdp, false, four, mod>), dim3(blocks), dim3(PA_THREADS), lds, st, q, kv, sq.table, \
                 sq.lens, sq.table_stride, sq.n_seqs, sq.max_pages, pl);                                             \
   } while (0)
-#define BB_PA_MOD(ct, np, hdp, four)              \
+#define BB_PA_MOD(ct, nq, np, hdp, four)              \
   do {                                            \
-    if (q.cap > 0.0f || q.slopes) BB_PA(ct, np, hdp, four, true); \
-    else BB_PA(ct, np, hdp, four, false);         \
+    if (q.cap > 0.0f || q.slopes) BB_PA(ct, nq, np, hdp, four, true); \
+    else BB_PA(ct, nq, np, hdp, four, false);         \
   } while (0)
-#define BB_PA_HD(ct, np, four)                      \
+#define BB_PA_HD(ct, nq, np, four)                      \
   do {                                              \
-    if (cls == 64) BB_PA_MOD(ct, np, 64, four);     \
-    else if (cls == 128) BB_PA_MOD(ct, np, 128, four); \
-    else BB_PA_MOD(ct, np, 256, four);              \
+    if (cls == 64) BB_PA_MOD(ct, nq, np, 64, four);     \
+    else if (cls == 128) BB_PA_MOD(ct, nq, np, 128, four); \
+    else BB_PA_MOD(ct, nq, np, 256, four);              \
   } while (0)
-  if (cache == BB_F32) BB_PA_HD(BB_F32, 1, false);
-  else if (cache == BB_KV4) BB_PA_HD(BB_F16, 2, true);
-  else if (cache == BB_F16) BB_PA_HD(BB_F16, 2, false);
-  else if (q.dt == BB_F32) BB_PA_HD(BB_BF16, 3, false);
-  else BB_PA_HD(BB_BF16, 2, false);
+  if (cache == BB_F32) BB_PA_HD(BB_F32, 1, 1, false);
+  else if (cache == BB_KV4 && q.dt == BB_F32) BB_PA_HD(BB_F16, 2, 2, true);
+  else if (cache == BB_KV4) BB_PA_HD(BB_F16, 1, 2, true);  // (16-bit q is all in one part)
+  else if (cache == BB_F16) BB_PA_HD(BB_F16, 2, 2, false);
+  else if (q.dt == BB_F32) BB_PA_HD(BB_BF16, 3, 3, false);
+  else BB_PA_HD(BB_BF16, 2, 2, false);
 #undef BB_PA_MOD
 #undef BB_PA_HD
 #undef BB_PA

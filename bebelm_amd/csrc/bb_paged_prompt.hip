@@ -41,7 +41,7 @@ struct PpShape {
   static constexpr int PLANE = KT * ROW, BUF = 2 * NPL * PLANE;
   // (two of them: an iteration reads the keys of the next tile and the values of its own)
   static constexpr int LD = HDP + 4;                                        // a row of the waves' sums, in the same place
-  static constexpr int SUMS = WK > 1 ? 4 * 32 * (LD * 4 + 8) : 0;
+  static constexpr int SUMS = WK > 1 ? 4 * 32 * (LD * 4 + 8) : 4 * 32 * HDP * 4;
   static constexpr int LDS = 2 * BUF > SUMS ? 2 * BUF : SUMS;
   static constexpr int RPW = KT / 4;  // rows a wave brings
   // pieces of 16 bytes in LDS that a lane brings of keys (and of values); of a 4-bit cache, units of UE elements
@@ -51,7 +51,8 @@ struct PpShape {
   static constexpr int QW = CT == BB_F32 ? HDP / 2 : NQ * HDP / 4;  // registers of the query rows
   static constexpr int REGS = HDP / 2 + QW + 16 * NT + (CT == BB_F32 ? 0 : 8 * NP * NT) +
                               (KV4 ? 2 * NU * (UE / 8 + 1) : PARTS ? 16 * NU + 32 : 0);
-  static constexpr int WAVES = REGS <= 208 && LDS <= 79 * 1024 ? 2 : 1;  // of a SIMD
+  static constexpr int MOST = 160 * 1024 / (LDS + 64 * HDP + 64);  // blocks of a CU by their LDS
+  static constexpr int WAVES = REGS <= 208 && MOST >= 2 ? 2 : 1;   // of a SIMD, and blocks of a CU
 };
 
 __device__ __attribute__((aligned(16))) uint32_t g_zeros[256];  // a row that is not there
@@ -379,18 +380,22 @@ struct PpWave {
 
   // Scores of a tile: register e of lane (row, half) is key 8(e / 4) + 4·half + e % 4 of 32. between(j) is done with the
   // products of the j-th of STEPS steps, whose keys have been asked for a step before.
-  static constexpr int STEPS = CT == BB_F32 ? HDP / 8 : HDP / 16;
+  static constexpr int STEPS = HDP / 16, READS = CT == BB_F32 ? 2 : NPL;  // pieces of a step: of 16 elements, or of each part
   // (ALL: of all parts whose product counts, those of the first: 2^-23 of each other; otherwise of the first alone)
   template <bool ALL, class F>
   __device__ __forceinline__ void scores(uint32_t lk, v16f (&y)[NT], F&& between) const {
     const uint32_t at0 = fresh(lk + (wk * S::BN + col) * S::ROW + (half ^ S::k_swap(col)) * 16);
-    v4u a[2][NT][NPL];
+    const auto piece = [&](int j, int t, int l) BB_INLINE {
+      return read_lds<v4u>((CT == BB_F32 ? at0 ^ 32 * (2 * j + l) : at0 ^ 32 * j) + 32 * t * S::ROW +
+                           (CT == BB_F32 ? 0 : l * S::PLANE));
+    };
+    v4u a[2][NT][READS];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) y[t][e] = 0.0f;
 #pragma unroll
-      for (int l = 0; l < NPL; ++l) a[0][t][l] = read_lds<v4u>(at0 + 32 * t * S::ROW + l * S::PLANE);
+      for (int l = 0; l < READS; ++l) a[0][t][l] = piece(0, t, l);
     }
 #pragma unroll
     for (int j = 0; j < STEPS; ++j) {
@@ -398,14 +403,14 @@ struct PpWave {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int l = 0; l < NPL; ++l)
-            a[(j + 1) & 1][t][l] = read_lds<v4u>((at0 ^ 32 * (j + 1)) + 32 * t * S::ROW + l * S::PLANE);
+          for (int l = 0; l < READS; ++l) a[(j + 1) & 1][t][l] = piece(j + 1, t, l);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         if constexpr (CT == BB_F32) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            y[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(as_float(a[j & 1][t][0][e]), qf[j][e], y[t], 0, 0, 0);
+          for (int e = 0; e < 8; ++e)
+            y[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(as_float(a[j & 1][t][e / 4][e % 4]), qf[2 * j + e / 4][e % 4], y[t],
+                                                        0, 0, 0);
         } else {
 #pragma unroll
           for (int i = NQ - 1; i >= 0; --i)
@@ -569,27 +574,18 @@ struct PpWave {
     }
   }
 
-  // Whether the wave's part of a tile has values that are not finite.
+  // Whether the wave's share of a tile's bytes has values that are not finite (of parts, the first is it).
   __device__ __forceinline__ bool values_odd(uint32_t lv) const {
-    bool odd = false;
-    const At at = values_at(lv);
-#pragma unroll 1
-    for (int t = 0; t < NT; ++t)
+    constexpr uint32_t EXP = CT == BB_BF16 ? 0x7f807f80u : 0x7c007c00u, ONE = CT == BB_BF16 ? 0x00800080u : 0x04000400u;
+    uint32_t odd = 0;
+#pragma unroll 4
+    for (int i = wv * 64 + lane; i < S::KT * S::PPR; i += PP_THREADS) {
+      const v4u a = read_lds<v4u>(lv + i * 16);
 #pragma unroll
-      for (int d = 0; d < HDP / 32; ++d) {
-        if constexpr (CT == BB_F32) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) odd |= !(fabsf(value(at, t, e, d)) < __builtin_inff());
-        } else {
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const v4u a = values(at, t, s, d);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) odd |= odd_halves<CT>(a[w]) != 0;
-          }
-        }
-      }
-    return __any(odd);
+      for (int w = 0; w < 4; ++w)
+        odd |= CT == BB_F32 ? (a[w] & 0x7f800000u) + 0x00800000u : (a[w] & EXP) + ONE;  // (carries into the sign's place)
+    }
+    return (odd & 0x80008000u) != 0;
   }
 
   // The values times their weights.
@@ -605,25 +601,29 @@ struct PpWave {
           for (int d = 0; d < ND; ++d)
             o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(value(at, t, e, d), p.f[t][e], o[d], 0, 0, 0);
     } else {
-      v4u a[2][ND][NPL];
+      // (four of them at a time, asked for four ahead)
+      constexpr int DC = ND < 4 ? ND : 4, N = 2 * NT * ND / DC;
+      v4u a[2][DC][NPL];
+      const auto ask = [&](int i) BB_INLINE {
+        const int g = i / (ND / DC);
 #pragma unroll
-      for (int d = 0; d < ND; ++d)
+        for (int d = 0; d < DC; ++d)
 #pragma unroll
-        for (int l = 0; l < NPL; ++l) a[0][d][l] = values(at, 0, 0, d, l);
+          for (int l = 0; l < NPL; ++l) a[i & 1][d][l] = values(at, g / 2, g % 2, i % (ND / DC) * DC + d, l);
+      };
+      ask(0);
 #pragma unroll
-      for (int g = 0; g < 2 * NT; ++g) {
-        if (g + 1 < 2 * NT)
+      for (int i = 0; i < N; ++i) {
+        if (i + 1 < N) ask(i + 1);
+        const int g = i / (ND / DC);
 #pragma unroll
-          for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int l = 0; l < NPL; ++l) a[(g + 1) & 1][d][l] = values(at, (g + 1) / 2, (g + 1) % 2, d, l);
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
+        for (int d = 0; d < DC; ++d)
 #pragma unroll
           for (int k = NP - 1; k >= 0; --k)
 #pragma unroll
             for (int l = NPL - 1; l >= 0; --l)
-              if (l + k < 3) o[d] = mfma32<CT>(a[g & 1][d][l], p.w[g / 2][g % 2][k], o[d]);
+              if (l + k < 3)
+                o[i % (ND / DC) * DC + d] = mfma32<CT>(a[i & 1][d][l], p.w[g / 2][g % 2][k], o[i % (ND / DC) * DC + d]);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -698,7 +698,7 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, SRC>
   const int kvh = blockIdx.x % pl.n_kv, rest = blockIdx.x / pl.n_kv;
   const int part = rest % pl.parts, g = rest / pl.parts;
 
-  // the sequence whose tile this is (every wave by itself)
+  // the sequence whose tile this is (every wave by itself); of a sequence the tiles that see most come first
   int s = -1, it = 0, a = 0, n = 0;
   for (int b = 0, before = 0; b < sq.n_seqs; b += 64) {
     const int si = min(b + lane, sq.n_seqs - 1);
@@ -710,9 +710,7 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, SRC>
     if (past) {
       const int at = __builtin_ctzll(past);
       s = b + at;
-      const int mine = __builtin_amdgcn_readlane(tiles, at);
-      // the tiles that see most first
-      it = mine - 1 - (g - before - (__builtin_amdgcn_readlane(incl, at) - mine));
+      it = before + __builtin_amdgcn_readlane(incl, at) - 1 - g;
       a = __builtin_amdgcn_readlane(sp.first, at);
       n = __builtin_amdgcn_readlane(sp.n, at);
       break;
@@ -805,13 +803,14 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, SRC>
     // as it is; one that they do not is looked at when it is there. If it has such values, the sums
     // that they belong to are marked, the values taken out, and what is marked made NaN after the tile's turn.
     const int last = min(r0 + S::BM, rows) - 1, b0 = index_of(r0), b1 = first_seen(index_of(last), pq.window);
-    bool marked = false;
+    bool odd = false;
     const auto look = [&](int u) BB_INLINE {
       const int j0 = kt.at(u0 + u) * S::KT;
       if ((j0 + S::KT - 1 <= b0 && j0 >= b1) || j0 + S::KT <= w.prefix) return;
-      if (!__syncthreads_or(w.values_odd(lds_at(vals(u))))) return;
+      odd = __syncthreads_or(w.values_odd(lds_at(vals(u))));
+    };
+    const auto mark = [&](int u) BB_INLINE {
       w.mark(&s_marks[u & 1][0][tid], lds_at(vals(u)), first_key(u), ok0, ok1);
-      marked = true;
       __syncthreads();
       w.clean(vals(u));
       __syncthreads();
@@ -866,9 +865,10 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, SRC>
     look(0);
     for (int u = 0; u < n_turns;) {
       if (w.past()) w.raise();
-      const bool spoiled = marked;
-      marked = false;
-      const auto on = [&]() BB_INLINE { return u < n_turns && !spoiled && !marked && !w.past(); };
+      if (odd) mark(u);
+      const bool spoiled = odd;
+      odd = false;
+      const auto on = [&]() BB_INLINE { return u < n_turns && !spoiled && !odd && !w.past(); };
       for (;;) {
         turn(u++, even);
         if (!on()) {
@@ -881,7 +881,7 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, SRC>
       }
       if (spoiled) w.spoil(&s_marks[u - 1 & 1][0][tid]);
     }
-    if constexpr (S::WK > 1) __syncthreads();  // (the tiles' place is taken below)
+    __syncthreads();  // (the tiles' place is taken below)
   }
   w.l = half_sum(w.l);
 
@@ -925,73 +925,130 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, SRC>
         for (int y = 0; y < 4; ++y) w.o[d][e + y] = x[y];
       }
   }
-  if (mine >= rows) return;
   const float up = CT == BB_F16 ? F16_UP : 0.0f;
-  if (kp.used == 1) {
-    const bool none = w.m == NEG_INF && w.l == 0.0f;
-    const float f = none ? 0.0f : 1.0f / w.l;
-    const size_t at = (size_t)t * pq.out_stride + (size_t)head * kv.hd;
-#pragma unroll
-    for (int d = 0; d < HDP / 32; ++d)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        if (S::WK > 1 && (d * 4 + e / 4) % S::WK != w.wk) continue;
-        const int at0 = 32 * d + 2 * e + 4 * w.half;
-        if (at0 < kv.hd)
-          store_act(pq.out, at + at0, pq.dt, v4f{w.o[d][e], w.o[d][e + 1], w.o[d][e + 2], w.o[d][e + 3]} * f);
-      }
-    if (w.half == 0 && w.wk == 0 && pq.lse)
+  const bool all = kp.used == 1, none = w.m == NEG_INF && w.l == 0.0f;
+  const float f = !all ? 1.0f : none ? 0.0f : 1.0f / w.l;
+  const size_t slot = all ? 0 : ((size_t)(g * pl.n_kv + kvh) * pl.parts + part) * S::BM + 32 * w.wr + w.col;
+  const size_t to = all ? (size_t)t * pq.out_stride + (size_t)head * kv.hd : slot * kv.hd;
+  const auto store = [&](size_t at, const v4f& x) BB_INLINE {
+    if (all) store_act(pq.out, at, pq.dt, x);
+    else *reinterpret_cast<v4f*>(pl.sums + at) = x;
+  };
+  if (mine < rows && w.half == 0 && w.wk == 0) {
+    if (!all) pl.ml[slot] = make_float2(w.m, w.l);
+    else if (pq.lse)
       pq.lse[(size_t)t * pq.n_heads + head] = none ? NEG_INF : (w.m + (__builtin_amdgcn_logf(w.l) - up)) * LN2;
-  } else {
-    const size_t slot = ((size_t)(g * pl.n_kv + kvh) * pl.parts + part) * S::BM + 32 * w.wr + w.col;
+  }
+  if constexpr (S::WK > 1) {
+    if (mine >= rows) return;
 #pragma unroll
     for (int d = 0; d < HDP / 32; ++d)
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
-        if (S::WK > 1 && (d * 4 + e / 4) % S::WK != w.wk) continue;
+        if ((d * 4 + e / 4) % S::WK != w.wk) continue;
         const int at0 = 32 * d + 2 * e + 4 * w.half;
-        if (at0 < kv.hd)
-          *reinterpret_cast<v4f*>(pl.sums + slot * kv.hd + at0) =
-              v4f{w.o[d][e], w.o[d][e + 1], w.o[d][e + 2], w.o[d][e + 3]};
+        if (at0 < kv.hd) store(to + at0, v4f{w.o[d][e], w.o[d][e + 1], w.o[d][e + 2], w.o[d][e + 3]} * f);
       }
-    if (w.half == 0 && w.wk == 0) pl.ml[slot] = make_float2(w.m, w.l);
+  } else {
+    // by way of LDS, a wave its own rows, so that a row's stores are adjacent (straight from the registers, where a lane has 4
+    // elements of every 32 of its own row, they cost 6 us a block). Piece p of row r lies at p ^ r % 16.
+    constexpr int P4 = HDP / 4;
+    v4f* rows_at = reinterpret_cast<v4f*>(s_tiles) + w.wv * 32 * P4;
+#pragma unroll
+    for (int d = 0; d < HDP / 32; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        rows_at[w.col * P4 + ((8 * d + e / 2 + w.half) ^ (w.col & 15))] =
+            v4f{w.o[d][e], w.o[d][e + 1], w.o[d][e + 2], w.o[d][e + 3]} * f;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int left = rows - (r0 + 32 * w.wr);  // rows of the wave that are there
+    const uint32_t lo = (uint32_t)to, hi = (uint32_t)(to >> 32);
+#pragma unroll 4
+    for (int i = lane; i < 32 * P4; i += 64) {
+      const int row = i / P4, piece = i % P4;
+      const size_t at = (size_t)(uint32_t)__shfl((int)hi, row) << 32 | (uint32_t)__shfl((int)lo, row);
+      if (row < left && 4 * piece < kv.hd) store(at + 4 * piece, rows_at[row * P4 + (piece ^ (row & 15))]);
+    }
   }
 }
 
-// Adds the parts of a row (a wave), where there are several.
-__global__ void __launch_bounds__(PP_THREADS) k_prompt_join(PromptQuery pq, int hd, int bm, PromptPlan pl, float up) {
-  const int lane = threadIdx.x & 63, in = blockIdx.y * (PP_THREADS / 64) + (threadIdx.x >> 6);
+// Adds the parts of rows, where there are several: `lanes` (16, 32 or 64) lanes a row, 4 elements each.
+__global__ void __launch_bounds__(PP_THREADS) k_prompt_join(PromptQuery pq, int hd, int bm, int lanes, PromptPlan pl, float up) {
+  const int lane = threadIdx.x % lanes, in = (blockIdx.y * PP_THREADS + threadIdx.x) / lanes;
   const int4 at = pl.places[blockIdx.x];
   const int used = at.x, r = at.y + in;
-  if (used <= 1 || r >= at.z) return;
+  if (used <= 1 || in >= bm || r >= at.z) return;
   const size_t first = (size_t)blockIdx.x * pl.parts * bm + in;
+  const int d = min(4 * lane, hd - 4);
   float m = NEG_INF, l = 0.0f;
-  for (int p = 0; p < used; ++p) m = fmaxf(m, pl.ml[first + (size_t)p * bm].x);
-  const float ref = m == NEG_INF ? 0.0f : m;
   v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
   for (int p = 0; p < used; ++p) {
     const float2 ml = pl.ml[first + (size_t)p * bm];
-    const float f = __builtin_amdgcn_exp2f(ml.x - ref);
-    l += ml.y * f;
-    if (4 * lane < hd) x += *reinterpret_cast<const v4f*>(pl.sums + (first + (size_t)p * bm) * hd + 4 * lane) * f;
+    const v4f y = *reinterpret_cast<const v4f*>(pl.sums + (first + (size_t)p * bm) * hd + d);
+    const float top = fmaxf(m, ml.x), ref = top == NEG_INF ? 0.0f : top;
+    const float f0 = __builtin_amdgcn_exp2f(m - ref), f1 = __builtin_amdgcn_exp2f(ml.x - ref);
+    m = top;
+    l = l * f0 + ml.y * f1;
+    x = x * f0 + y * f1;
   }
   const int t = at.w + r / pl.G, head = (int)(blockIdx.x % pl.n_kv) * pl.G + r % pl.G;
   const bool none = m == NEG_INF && l == 0.0f;
   if (4 * lane < hd)
-    store_act(pq.out, (size_t)t * pq.out_stride + (size_t)head * hd + 4 * lane, pq.dt, x * (none ? 0.0f : 1.0f / l));
+    store_act(pq.out, (size_t)t * pq.out_stride + (size_t)head * hd + d, pq.dt, x * (none ? 0.0f : 1.0f / l));
   if (lane == 0 && pq.lse)
     pq.lse[(size_t)t * pq.n_heads + head] = none ? NEG_INF : (m + (__builtin_amdgcn_logf(l) - up)) * LN2;
 }
 
 constexpr int PARTS_MAX = 64;
 
+// f(a block's shape) by the types of the cache and of q and out, the head size and the waves along the rows (4, 2 or 1).
+//
+// A 16-bit cache takes 16-bit matrix instructions on its values as they are, a 4-bit one those of f16; the query rows are split
+// into NQ parts that are all of them (f16 ones at a power of two that puts the row's largest in 2^13..2^14: f32
+// keeps 22 bits). Weights are rounded once to what the cache has (NP = 1: bf16 by 2^-8, f16 by 2^-11 at most) where out
+// is rounded as far itself; an out with more bits has them in 2 or 3 parts. An f32 cache takes f32 instructions, or for
+// tiles of 128 rows and heads of up to 128 six times 16-bit ones (of the products of three parts with three, those that
+// count), of a sixteenth of the time each.
+template <int CT, int NQ, int NP, int SRC, class F>
+auto by_size(int cls, int wr, F& f) {
+  const auto of = [&](auto hdp) {
+    constexpr int H = decltype(hdp)::value;
+    return wr == 4   ? f(PpShape<CT, NQ, NP, H, 4, SRC>())
+           : wr == 2 ? f(PpShape<CT, NQ, NP, H, 2, SRC>())
+                     : f(PpShape<CT, NQ, NP, H, 1, SRC>());
+  };
+  return cls == 64    ? of(std::integral_constant<int, 64>())
+         : cls == 128 ? of(std::integral_constant<int, 128>())
+                      : of(std::integral_constant<int, 256>());
+}
+template <class F>
+auto with_shape(int cache, int dt, int cls, int wr, F&& f) {
+  switch (cache) {
+    case BB_F32:
+      if (wr == 4 && cls < 256) {
+        if (dt == BB_F32) return cls == 64 ? f(PpShape<BB_BF16, 3, 3, 64, 4, SRC_PARTS>()) : f(PpShape<BB_BF16, 3, 3, 128, 4, SRC_PARTS>());
+        return cls == 64 ? f(PpShape<BB_BF16, 2, 3, 64, 4, SRC_PARTS>()) : f(PpShape<BB_BF16, 2, 3, 128, 4, SRC_PARTS>());
+      }
+      return by_size<BB_F32, 1, 1, SRC_SAME>(cls, wr, f);
+    case BB_F16:
+      return dt == BB_F32 ? by_size<BB_F16, 2, 2, SRC_SAME>(cls, wr, f) : by_size<BB_F16, 1, 1, SRC_SAME>(cls, wr, f);
+    case BB_KV4:
+      return dt == BB_F32 ? by_size<BB_F16, 2, 2, SRC_KV4>(cls, wr, f) : by_size<BB_F16, 1, 1, SRC_KV4>(cls, wr, f);
+    default:
+      return dt == BB_F32   ? by_size<BB_BF16, 3, 3, SRC_SAME>(cls, wr, f)
+             : dt == BB_F16 ? by_size<BB_BF16, 2, 2, SRC_SAME>(cls, wr, f)
+                            : by_size<BB_BF16, 1, 1, SRC_SAME>(cls, wr, f);
+  }
+}
+
 // The blocks of a launch, chosen from what the host knows: how many tokens and sequences there are.
 struct PromptCut {
   int wr;    // waves along a tile's rows: 4, or where there are few, its keys shared out to 4 / wr waves
   int bm, n_tiles, parts;
 };
-PromptCut prompt_cut(int n_cu, int cache, size_t n_tokens, size_t n_seqs, int G, int n_kv, int hd) {
+PromptCut prompt_cut(int n_cu, int cache, int dt, size_t n_tokens, size_t n_seqs, int G, int n_kv, int hd) {
   PromptCut c;
   const int cls = pa_class(hd);
   const size_t rows = n_tokens * (size_t)G, mean = (rows + n_seqs - 1) / n_seqs;
@@ -999,8 +1056,9 @@ PromptCut prompt_cut(int n_cu, int cache, size_t n_tokens, size_t n_seqs, int G,
   c.wr = mean > 64 || row_bytes > 512 ? 4 : mean > 32 || row_bytes > 256 ? 2 : 1;
   c.bm = 32 * c.wr;
   c.n_tiles = (int)std::min(rows / c.bm + n_seqs, rows);
-  const size_t blocks = (size_t)c.n_tiles * n_kv;
-  const size_t at_once = (size_t)n_cu * (cls == 256 || (cache == BB_F32 && cls == 128) ? 1 : 2);
+  // keys in parts while the blocks (of sequences that are alike) fit the device at once
+  const size_t blocks = (mean + c.bm - 1) / c.bm * n_seqs * n_kv;
+  const size_t at_once = (size_t)n_cu * with_shape(cache, dt, cls, c.wr, [](auto s) { return decltype(s)::WAVES; });
   c.parts = (int)std::min<size_t>(PARTS_MAX, std::max<size_t>(1, at_once / blocks));
   return c;
 }
@@ -1012,7 +1070,7 @@ size_t prompt_ws(const PromptCut& c, int n_kv, int hd) {
 }
 
 template <int CT, int NQ, int NP, int HDP, int WR, int SRC>
-hipError_t prompt_of(hipStream_t st, const PromptQuery& q, const PagedView& kv, const PagedSeqs& sq, PromptPlan pl) {
+hipError_t prompt_of(PpShape<CT, NQ, NP, HDP, WR, SRC>, hipStream_t st, const PromptQuery& q, const PagedView& kv, const PagedSeqs& sq, PromptPlan pl) {
   typedef PpShape<CT, NQ, NP, HDP, WR, SRC> S;
   if constexpr (S::LDS > 159 * 1024) {
     return hipErrorInvalidValue;
@@ -1026,54 +1084,27 @@ hipError_t prompt_of(hipStream_t st, const PromptQuery& q, const PagedView& kv, 
     BB_LAUNCH((k_paged_prompt<CT, NQ, NP, HDP, WR, SRC>), dim3(blocks), dim3(PP_THREADS), 0, st, q, kv, sq, pl);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || pl.parts == 1) return e;
-    BB_LAUNCH(k_prompt_join, dim3(pl.n_tiles * pl.n_kv, S::BM / (PP_THREADS / 64)), dim3(PP_THREADS), 0, st, q, kv.hd,
-              S::BM, pl, CT == BB_F16 ? F16_UP : 0.0f);
+    const int lanes = HDP / 4;
+    BB_LAUNCH(k_prompt_join, dim3(pl.n_tiles * pl.n_kv, S::BM * lanes / PP_THREADS), dim3(PP_THREADS), 0, st, q, kv.hd,
+              S::BM, lanes, pl, CT == BB_F16 ? F16_UP : 0.0f);
     return hipGetLastError();
   }
-}
-
-template <int CT, int NQ, int NP, int SRC>
-hipError_t prompt_by(hipStream_t st, int wr, const PromptQuery& q, const PagedView& kv, const PagedSeqs& sq,
-                     const PromptPlan& pl) {
-  const auto of = [&](auto hdp) {
-    constexpr int H = decltype(hdp)::value;
-    return wr == 4   ? prompt_of<CT, NQ, NP, H, 4, SRC>(st, q, kv, sq, pl)
-           : wr == 2 ? prompt_of<CT, NQ, NP, H, 2, SRC>(st, q, kv, sq, pl)
-                     : prompt_of<CT, NQ, NP, H, 1, SRC>(st, q, kv, sq, pl);
-  };
-  switch (pa_class(kv.hd)) {
-    case 64: return of(std::integral_constant<int, 64>());
-    case 128: return of(std::integral_constant<int, 128>());
-    default: return of(std::integral_constant<int, 256>());
-  }
-}
-
-// An f32 cache: f32 matrix instructions, or for tiles of 128 rows and heads of up to 128 six times 16-bit ones (of the
-// products of three parts with three, those that count), a sixteenth of the time each.
-template <int NQ>
-hipError_t prompt_f32(hipStream_t st, int wr, const PromptQuery& q, const PagedView& kv, const PagedSeqs& sq,
-                      const PromptPlan& pl) {
-  const int cls = pa_class(kv.hd);
-  if (wr == 4 && cls == 64) return prompt_of<BB_BF16, NQ, 3, 64, 4, SRC_PARTS>(st, q, kv, sq, pl);
-  if (wr == 4 && cls == 128) return prompt_of<BB_BF16, NQ, 3, 128, 4, SRC_PARTS>(st, q, kv, sq, pl);
-  return prompt_by<BB_F32, 1, 1, SRC_SAME>(st, wr, q, kv, sq, pl);
 }
 
 }  // namespace
 
 size_t paged_prompt_ws(int n_cu, int cache, size_t n_tokens, size_t n_seqs, int n_heads, int n_kv, int hd) {
+  size_t most = 0;
   if (n_tokens == 0 || n_seqs == 0) return 0;
-  return prompt_ws(prompt_cut(n_cu, cache, n_tokens, n_seqs, n_heads / n_kv, n_kv, hd), n_kv, hd);
+  for (const int dt : {BB_F32, BB_F16, BB_BF16})
+    most = std::max(most, prompt_ws(prompt_cut(n_cu, cache, dt, n_tokens, n_seqs, n_heads / n_kv, n_kv, hd), n_kv, hd));
+  return most;
 }
 
-// The types: a 16-bit cache takes 16-bit matrix instructions on its values as they are, a 4-bit one those of f16; the
-// query rows are split into NQ parts that are all of them (f16 ones at a power of two that puts the row's
-// largest in 2^13..2^14: f32 keeps 22 bits). Weights are rounded once to what the cache has (NP = 1: bf16 by 2^-9, f16 by
-// 2^-12 at most) where out is rounded as far itself; an out with more bits has them in 2 or 3 parts.
 hipError_t launch_paged_prompt(hipStream_t st, int n_cu, int cache, const PromptQuery& q, const PagedView& kv,
                                const PagedSeqs& sq) {
   const int G = q.n_heads / kv.n_kv;
-  const PromptCut c = prompt_cut(n_cu, cache, q.n_tokens, sq.n_seqs, G, kv.n_kv, kv.hd);
+  const PromptCut c = prompt_cut(n_cu, cache, q.dt, q.n_tokens, sq.n_seqs, G, kv.n_kv, kv.hd);
   PromptPlan pl{G, c.n_tiles, kv.n_kv, c.parts, 1, false, nullptr, nullptr, nullptr};
   if (c.parts > 1) {
     const size_t tiles = (size_t)c.n_tiles * kv.n_kv, slots = tiles * c.parts * c.bm;
@@ -1081,20 +1112,7 @@ hipError_t launch_paged_prompt(hipStream_t st, int n_cu, int cache, const Prompt
     pl.sums = reinterpret_cast<float*>(pl.places + tiles);
     pl.ml = reinterpret_cast<float2*>(pl.sums + slots * kv.hd);
   }
-  switch (cache) {
-    case BB_F32: return q.dt == BB_F32 ? prompt_f32<3>(st, c.wr, q, kv, sq, pl) : prompt_f32<2>(st, c.wr, q, kv, sq, pl);
-    case BB_F16:
-      return q.dt == BB_F32 ? prompt_by<BB_F16, 2, 2, SRC_SAME>(st, c.wr, q, kv, sq, pl)
-                            : prompt_by<BB_F16, 1, 1, SRC_SAME>(st, c.wr, q, kv, sq, pl);
-    case BB_BF16:
-      return q.dt == BB_F32   ? prompt_by<BB_BF16, 3, 3, SRC_SAME>(st, c.wr, q, kv, sq, pl)
-             : q.dt == BB_F16 ? prompt_by<BB_BF16, 2, 2, SRC_SAME>(st, c.wr, q, kv, sq, pl)
-                              : prompt_by<BB_BF16, 1, 1, SRC_SAME>(st, c.wr, q, kv, sq, pl);
-    case BB_KV4:
-      return q.dt == BB_F32 ? prompt_by<BB_F16, 2, 2, SRC_KV4>(st, c.wr, q, kv, sq, pl)
-                            : prompt_by<BB_F16, 1, 1, SRC_KV4>(st, c.wr, q, kv, sq, pl);
-    default: return hipErrorInvalidValue;
-  }
+  return with_shape(cache, q.dt, pa_class(kv.hd), c.wr, [&](auto s) { return prompt_of(s, st, q, kv, sq, pl); });
 }
 
 }  // namespace bb
