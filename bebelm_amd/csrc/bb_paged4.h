@@ -93,16 +93,23 @@ __device__ __forceinline__ float kv4_step(float lo, float hi) {
   return d < 6.103515625e-5f ? d + UNIT : as_float(__float_as_uint(d) + 0x00080000u);
 }
 // Eight elements of a block, of which four adjacent lanes hold a quarter each, as a word of codes; `head` is the block's.
-// (x / d rounded to f32 and then to an integer is x / d rounded to an integer: the borders (n + 1/2)·d, n below 64, are f32
-// numbers, so that an x which is not on one is at least 2^-24 of itself away, and a quotient's rounding moves it less
-// than that towards one.)
+// x / d is x·r corrected once by its remainder, r = 1 / d rounded: that is the quotient rounded to f32. And rounded to f32
+// and then to an integer it is x / d rounded to an integer: the borders (n + 1/2)·d, n below 64, are f32 numbers, so that an
+// x which is not on one is at least 2^-24 of itself away, and a quotient's rounding moves it less than that towards one.
+__device__ __forceinline__ float kv4_quotient(float x, float d, float r) {
+  const float q = x * r;
+  return rintf(fmaf(fmaf(-q, d, x), r, q));
+}
 __device__ __forceinline__ uint32_t kv4_quantise(float (&x)[8], uint32_t& head) {
   bool odd = false;
-  float lo = __builtin_inff(), hi = NEG_INF;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     odd |= !(fabsf(x[i]) < __builtin_inff());
-    x[i] = fminf(fmaxf(x[i], -16384.0f), 16384.0f);
+    x[i] = __builtin_amdgcn_fmed3f(x[i], -16384.0f, 16384.0f);
+  }
+  float lo = x[0], hi = x[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
     lo = fminf(lo, x[i]);
     hi = fmaxf(hi, x[i]);
   }
@@ -120,11 +127,13 @@ __device__ __forceinline__ uint32_t kv4_quantise(float (&x)[8], uint32_t& head) 
   const float d = kv4_step(lo, hi);
   head = 0;
   if (d == 0.0f) return 0;
-  const int z = (int)rintf(lo / d);
+  const float r = 1.0f / d, zf = kv4_quotient(lo, d, r);
+  const int z = (int)zf;
   head = __builtin_bit_cast(uint16_t, (_Float16)d) | (uint32_t)(z & 63) | (z < 0 ? 0x8000u : 0u);
   uint32_t w = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w |= (uint32_t)min(max((int)rintf(x[i] / d) - z, 0), 15) << 4 * i;
+  for (int i = 0; i < 8; ++i)
+    w |= (uint32_t)__builtin_amdgcn_fmed3f(kv4_quotient(x[i], d, r) - zf, 0.0f, 15.0f) << 4 * i;
   return w;
 }
 

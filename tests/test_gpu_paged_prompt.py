@@ -43,6 +43,13 @@ def done(ctx):
     torch.cuda.synchronize()
 
 
+def on_gpu(*tensors):
+    """Copies that are there when a call on another stream begins, to be held until it is done."""
+    copies = [t.cuda() for t in tensors]
+    torch.cuda.synchronize()
+    return copies
+
+
 def i32(x):
     return torch.tensor(x, dtype=torch.int32)
 
@@ -616,10 +623,10 @@ def test_append_to_4_bits_with_norm_and_rotation(gpu_ctx, rot, interleaved):
         outs.append(out.cpu())
     assert torch.equal(*outs)
     rows, back = ([torch.empty(t, kv, hd, device="cuda") for _ in range(2)] for _ in range(2))
-    torch.cuda.synchronize()
     for pool, to in ((wide, rows), (four, back)):
-        kernels.paged_read(gpu_ctx, pool.kv, pool.table.cuda(), pool.lens.cuda(), *to, seq_start=start.cuda())
-    done(gpu_ctx)
+        table, ln, st = on_gpu(pool.table, pool.lens, start)
+        kernels.paged_read(gpu_ctx, pool.kv, table, ln, *to, seq_start=st)
+        done(gpu_ctx)
     for x, got in zip(rows, back):
         assert torch.equal(got.cpu().double(), held(x.cpu()))
 
@@ -630,9 +637,9 @@ def test_append_to_4_bits_one_token_each(gpu_ctx):
     k, v = randn(57, (5, 3, 96), F16), randn(58, (5, 3, 96), F16)
     kb, vb = (torch.full((5, 3, 96), 7.0, device="cuda") for _ in range(2))
     before = pool.k.cpu().clone()
-    torch.cuda.synchronize()
-    kernels.paged_append(gpu_ctx, pool.kv, pool.table.cuda(), pool.lens.cuda(), k.cuda(), v.cuda())
-    kernels.paged_read(gpu_ctx, pool.kv, pool.table.cuda(), pool.lens.cuda(), kb, vb)
+    table, ln, kd, vd = on_gpu(pool.table, pool.lens, k, v)
+    kernels.paged_append(gpu_ctx, pool.kv, table, ln, kd, vd)
+    kernels.paged_read(gpu_ctx, pool.kv, table, ln, kb, vb)
     done(gpu_ctx)
     for s, n in enumerate(lens):
         for got, x in ((kb, k), (vb, v)):
@@ -682,8 +689,8 @@ def test_library_pool_of_4_bits(gpu_ctx):
     done(gpu_ctx)
     assert bool((back == 0).all())
     k = randn(61, (52, 2, 64), F32)
-    kernels.paged_append(gpu_ctx, kv, table, lens, k.cuda(), k.cuda(), seq_start=start)
-    torch.cuda.synchronize()
+    kd, vd = on_gpu(k, k)
+    kernels.paged_append(gpu_ctx, kv, table, lens, kd, vd, seq_start=start)
     kernels.paged_read(gpu_ctx, kv, table, lens, None, back, seq_start=start)
     done(gpu_ctx)
     assert torch.equal(back.cpu().double(), held(k))
@@ -710,14 +717,12 @@ def test_conversations(gpu_ctx, ct, dt):
         start = None if single else i32([0] + np.cumsum(chunk).tolist()).cuda()
         q, k, v = (randn(71 + 10 * c + i, (t, n, hd), dt) for i, n in enumerate((nh, kv, kv)))
         qr, out = torch.zeros(t, nh, hd, dtype=TYPES[dt], device="cuda"), torch.zeros(t, nh, hd, dtype=TYPES[dt], device="cuda")
-        ln, table = i32(lens).cuda(), pool.table.cuda()
-        torch.cuda.synchronize()
-        kernels.paged_append(gpu_ctx, pool.kv, table, ln, k.cuda(), v.cuda(), rope=plan, seq_start=start, q=q.cuda(), q_out=qr)
-        kernels.paged_prompt_attention(gpu_ctx, pool.kv, table, ln, qr, out, seq_start=start, cap=20.0, slopes=slopes.cuda())
-        every = i32([0] + np.cumsum(lens).tolist()).cuda()
+        every = i32([0] + np.cumsum(lens).tolist())
         kb, vb = (torch.zeros(sum(lens), kv, hd, device="cuda") for _ in range(2))
-        torch.cuda.synchronize()
-        kernels.paged_read(gpu_ctx, pool.kv, table, ln, kb, vb, seq_start=every)
+        ln, table, kd, vd, qd, sd, ev = on_gpu(i32(lens), pool.table, k, v, q, slopes, every)
+        kernels.paged_append(gpu_ctx, pool.kv, table, ln, kd, vd, rope=plan, seq_start=start, q=qd, q_out=qr)
+        kernels.paged_prompt_attention(gpu_ctx, pool.kv, table, ln, qr, out, seq_start=start, cap=20.0, slopes=sd)
+        kernels.paged_read(gpu_ctx, pool.kv, table, ln, kb, vb, seq_start=ev)
         done(gpu_ctx)
         at, row = 0, 0
         for s in range(3):
@@ -854,10 +859,10 @@ def test_past_32_bits(gpu_ctx):
         q = randn(97, (700, 4, hd), BF16)
         out, kb = torch.zeros(q.shape, dtype=q.dtype, device="cuda"), torch.zeros(kk.shape, device="cuda")
         one = torch.zeros(2, 4, hd, dtype=q.dtype, device="cuda")
-        torch.cuda.synchronize()
-        kernels.paged_append(gpu_ctx, handle, table, lens, kk.cuda(), vv.cuda(), seq_start=start)
-        kernels.paged_prompt_attention(gpu_ctx, handle, table, lens, q.cuda(), out, seq_start=start)
-        kernels.paged_attention(gpu_ctx, handle, table, lens, q[[399, 699]].cuda(), one)
+        kd, vd, qd, last = on_gpu(kk, vv, q, q[[399, 699]])
+        kernels.paged_append(gpu_ctx, handle, table, lens, kd, vd, seq_start=start)
+        kernels.paged_prompt_attention(gpu_ctx, handle, table, lens, qd, out, seq_start=start)
+        kernels.paged_attention(gpu_ctx, handle, table, lens, last, one)
         kernels.paged_read(gpu_ctx, handle, table, lens, kb, seq_start=start)
         done(gpu_ctx)
         hk, hv = (held(x) if ct == KV4 else x.double() for x in (kk, vv))
@@ -868,7 +873,7 @@ def test_past_32_bits(gpu_ctx):
             close(out[a:b], want, tol, f"sequence {s}")
             close(one[s], want[-1], tol[-1], f"last token of {s}")
         handle.close()
-        del k, v
+        del k, v, kd, vd, qd
 
 
 # ---- refusals ----------------------------------------------------------------------------------------
