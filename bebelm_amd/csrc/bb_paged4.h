@@ -100,6 +100,11 @@ __device__ __forceinline__ float kv4_quotient(float x, float d, float r) {
   const float q = x * r;
   return rintf(fmaf(fmaf(-q, d, x), r, q));
 }
+// The lanes of four in another order: 0xb1 neighbours exchanged, 0x4e pairs.
+template <int ORDER>
+__device__ __forceinline__ uint32_t quad(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ORDER, 0xf, 0xf, true);
+}
 __device__ __forceinline__ uint32_t kv4_quantise(float (&x)[8], uint32_t& head) {
   bool odd = false;
 #pragma unroll
@@ -113,13 +118,13 @@ __device__ __forceinline__ uint32_t kv4_quantise(float (&x)[8], uint32_t& head) 
     lo = fminf(lo, x[i]);
     hi = fmaxf(hi, x[i]);
   }
-  int any = odd;
-#pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    lo = fminf(lo, __shfl_xor(lo, o));
-    hi = fmaxf(hi, __shfl_xor(hi, o));
-    any |= __shfl_xor(any, o);
-  }
+  uint32_t any = odd;
+  lo = fminf(lo, as_float(quad<0xb1>(__float_as_uint(lo))));
+  hi = fmaxf(hi, as_float(quad<0xb1>(__float_as_uint(hi))));
+  any |= quad<0xb1>(any);
+  lo = fminf(lo, as_float(quad<0x4e>(__float_as_uint(lo))));
+  hi = fmaxf(hi, as_float(quad<0x4e>(__float_as_uint(hi))));
+  any |= quad<0x4e>(any);
   if (any) {
     head = 0x7fc0u;
     return 0;
