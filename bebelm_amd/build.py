@@ -21,8 +21,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libbebelm_moe.so")
 SOURCES = ["bb_kernels.hip", "bb_decode.hip", "bb_prefill.hip", "bb_proj.hip", "bb_row1.hip", "bb_ops.hip",
-           "bb_paged.hip", "bb_paged_prompt.hip", "bb_api.hip", "bb_gguf.hip"]
-NO_VGPR_FORM = {"bb_paged_prompt.hip"}
+           "bb_prompt_f32.hip", "bb_prompt_f16.hip", "bb_prompt_bf16.hip", "bb_prompt_kv4.hip", "bb_paged_prompt.hip",
+           "bb_paged.hip", "bb_api.hip", "bb_gguf.hip"]
+NO_VGPR_FORM = {"bb_prompt_f32.hip", "bb_prompt_f16.hip", "bb_prompt_bf16.hip", "bb_prompt_kv4.hip"}
 ARCH = os.environ.get("BB_OFFLOAD_ARCH", "gfx950")
 
 
