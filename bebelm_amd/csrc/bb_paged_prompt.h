@@ -578,13 +578,13 @@ struct PpWave {
     }
   }
 
-  // Whether the wave's share of a tile's bytes has values that are not finite (of parts, the first is it).
+  // Whether the rows that the wave brings have values that are not finite (of parts, the first is it).
   __device__ __forceinline__ bool values_odd(uint32_t lv) const {
     constexpr uint32_t EXP = CT == BB_BF16 ? 0x7f807f80u : 0x7c007c00u, ONE = CT == BB_BF16 ? 0x00800080u : 0x04000400u;
     uint32_t odd = 0;
 #pragma unroll 4
-    for (int i = wv * 64 + lane; i < S::KT * S::PPR; i += PP_THREADS) {
-      const v4u a = read_lds<v4u>(lv + i * 16);
+    for (int i = lane; i < S::RPW * S::PPR; i += 64) {
+      const v4u a = read_lds<v4u>(lv + (wv * S::RPW * S::PPR + i) * 16);
 #pragma unroll
       for (int w = 0; w < 4; ++w)
         odd |= CT == BB_F32 ? (a[w] & 0x7f800000u) + 0x00800000u : (a[w] & EXP) + ONE;  // (carries into the sign's place)
@@ -678,10 +678,11 @@ struct PpWave {
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[d][e] = bad[d * PP_THREADS] >> e & 1 ? __builtin_nanf("") : o[d][e];
   }
-  // The wave's share of a tile of values without those that are not finite.
+  // The rows that the wave brings without values that are not finite.
   __device__ __forceinline__ void clean(char* lv) const {
-    for (int i = wv * 64 + lane; i < NPL * S::KT * S::PPR; i += PP_THREADS) {
-      v4u* p = reinterpret_cast<v4u*>(lv + i * 16);
+    for (int i = lane; i < NPL * S::RPW * S::PPR; i += 64) {
+      const int l = i / (S::RPW * S::PPR), in = i % (S::RPW * S::PPR);
+      v4u* p = reinterpret_cast<v4u*>(lv + l * S::PLANE + (wv * S::RPW * S::PPR + in) * 16);
       v4u a = *p;
 #pragma unroll
       for (int w = 0; w < 4; ++w)
@@ -697,6 +698,7 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, SRC>
   typedef PpShape<CT, NQ, NP, HDP, WR, SRC> S;
   __shared__ __align__(1024) char s_tiles[S::LDS];
   __shared__ uint32_t s_ok[2][4];
+  __shared__ uint32_t s_odd[2][4];
   __shared__ uint32_t s_marks[2][HDP / 32][PP_THREADS];
   const int tid = threadIdx.x, lane = tid & 63;
   const int kvh = blockIdx.x % pl.n_kv, rest = blockIdx.x / pl.n_kv;
@@ -808,10 +810,15 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, SRC>
     // that they belong to are marked, the values taken out, and what is marked made NaN after the tile's turn.
     const int last = min(r0 + S::BM, rows) - 1, b0 = index_of(r0), b1 = first_seen(index_of(last), pq.window);
     bool odd = false;
+    int looks = 0;
     const auto look = [&](int u) BB_INLINE {
       const int j0 = kt.at(u0 + u) * S::KT;
       if ((j0 + S::KT - 1 <= b0 && j0 >= b1) || j0 + S::KT <= w.prefix) return;
-      odd = __syncthreads_or(w.values_odd(lds_at(vals(u))));
+      const bool mine_odd = __ballot(w.values_odd(lds_at(vals(u)))) != 0;
+      uint32_t* at = s_odd[looks++ & 1];  // (two in turn: a wave that writes one again has passed a barrier behind its reads)
+      if (lane == 0) at[w.wv] = mine_odd;
+      __syncthreads();
+      odd = (at[0] | at[1] | at[2] | at[3]) != 0;
     };
     const auto mark = [&](int u) BB_INLINE {
       w.mark(&s_marks[u & 1][0][tid], lds_at(vals(u)), first_key(u), ok0, ok1);
@@ -844,7 +851,12 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, SRC>
       if (two) w.template put<true>(keys(u));
       w.template put<false>(vals(u + 1));
       landed();
-      __syncthreads();
+      if constexpr (S::WK == 4) {  // (a wave brings the keys that it takes itself; 80 tokens over 16 x 8192: 119 us, not 130)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      } else {
+        __syncthreads();
+      }
       look(u + 1);
     };
 
