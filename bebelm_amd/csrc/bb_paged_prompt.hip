@@ -56,7 +56,7 @@ PromptCut prompt_cut(int n_cu, int cache, int dt, size_t n_tokens, size_t n_seqs
   const int row_bytes = cls * (cache == BB_F32 ? 4 : 2);  // in LDS, which has to hold 128 keys and values twice
   c.wr = mean > 64 || row_bytes > 512 ? 4 : mean > 32 || row_bytes > 256 ? 2 : 1;
   c.bm = 32 * c.wr;
-  c.n_tiles = (int)std::min(rows / c.bm + n_seqs, rows);
+  c.n_tiles = (int)most_tiles(rows, c.bm, n_seqs);
   // keys in parts while the blocks (of sequences that are alike) fit the device at once
   const size_t blocks = (mean + c.bm - 1) / c.bm * n_seqs * n_kv;
   const size_t at_once = (size_t)n_cu * blocks_of_cu(cache, dt, cls, c.wr);

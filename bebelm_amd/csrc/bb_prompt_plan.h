@@ -9,6 +9,8 @@ namespace bb {
 
 // The rows of a kv head: its G query heads of each of a sequence's n tokens (below 2^31 in all), `bm` a tile.
 BB_BOTH int row_tiles(int n, int G, int bm) { return (int)(((int64_t)n * G + bm - 1) / bm); }
+// Tiles of all sequences together, at most.
+inline size_t most_tiles(size_t rows, int bm, size_t n_seqs) { return rows / bm + n_seqs < rows ? rows / bm + n_seqs : rows; }
 
 // The tokens a sequence brings: seq_start's entries, whatever they hold, as a range of the call's tokens.
 struct TokenSpan {
