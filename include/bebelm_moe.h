@@ -389,11 +389,11 @@ int bb_paged_kv_pages(const bb_paged_kv* kv, void** k, void** v);
  * bytes each, element 2i in the low half of byte i), then their blocks' heads (16 bits for each 32 elements, an
  * even number a position), and what fills it up to 16 bytes. A head holds a step d (bits 6 to 14: those of an F16
  * number whose other bits are 0) and an offset z in two's complement (bits 0 to 5 and 15); an element stands for
- * d·(code + z). Memory of zeros stands for zeros. Storing takes values past ±16384 as that, the smallest such d with
- * 15d >= max - min, 63d >= max and 47d >= -min of the block (0 for a block of zeros), z = min / d and the codes x / d - z,
- * both quotients rounded to the nearest integer (ties to even) and the codes held to 0..15: no element is off by more than
- * d / 2. A block with an element that is not finite stands for NaN. (Heads that others made may have code + z
- * past -47..63: what those stand for is rounded to F16.) */
+ * d·(code + z). Memory of zeros stands for zeros. All of the calls below take such a pool. Storing takes values past
+ * ±16384 as that, the smallest such d with 15d >= max - min, 63d >= max and 47d >= -min of the block (0 for a block of
+ * zeros), z = min / d and the codes x / d - z, both quotients rounded to the nearest integer (ties to even) and the codes
+ * held to 0..15: no element is off by more than d / 2. A block with an element that is not finite stands for NaN. (Heads
+ * that others made may have code + z past -47..63: what those stand for is rounded to F16.) */
 int bb_paged_kv4_bytes(size_t page_size, size_t head_dim, size_t* bytes);
 int bb_paged_kv_view4(bb_ctx* ctx, void* k, void* v, size_t n_pages, size_t page_size, size_t n_kv_heads,
                       size_t head_dim, size_t page_stride, size_t head_stride, bb_paged_kv** out);
@@ -493,11 +493,12 @@ int bb_paged_attention(bb_ctx* ctx, const bb_paged_kv* kv, const bb_paged_seqs* 
  * each sequence has, its last ones (NULL: one each, n_tokens = n_seqs); token t of sequence s has index
  * i = lens[s] - seq_start[s+1] + t and sees the j below lens[s] with i - window < j <= i (window 0: j <= i), and those
  * below prefix[s] (i32[n_seqs], or NULL) wherever they are: a prefix read in both directions, or with a window the first
- * positions that stay in reach. Between a prefix and a window's first position nothing is read. q and out
+ * positions that stay in reach. What lies between a prefix and a window's first position makes no difference. q and out
  * [n_tokens][n_heads][head_dim] (heads side by side, tokens q_stride and out_stride apart, not overlapping); scale 0 means
  * 1/sqrt(head_dim); lse, as in bb_paged_attention, f32[n_tokens][n_heads] or NULL. A token that sees nothing gets zeros and
  * -inf; of padding nothing is written. A value that is not finite makes not finite what it reaches, and nothing else: the
- * rows that do not see it are as if it were not there. Weights are rounded to the cache's type (F16 for BB_KV4) where out is
+ * rows that do not see it are as if it were not there (of an F32 cache, magnitudes from 3.39e38 on may count as
+ * infinite). Weights are rounded to the cache's type (F16 for BB_KV4) where out is
  * F16 on an F16 or BB_KV4 cache, or BF16; elsewhere they keep what out can hold. workspace: as in bb_paged_attention, of
  * bb_paged_prompt_attention_workspace's answer (which may be 0: then a captured call needs none). Equal calls give equal
  * bits. One call takes n_tokens·n_heads / 32 + n_seqs·n_kv_heads below 2^24 (BB_ERR_RANGE: cut the batch). */

@@ -475,6 +475,64 @@ def test_starts_that_do_not_ascend(gpu_ctx):
     check(gpu_ctx, pool, q, BF16, [5, 5, 10])
 
 
+@pytest.mark.parametrize("ct", [F32, BF16, KV4])
+def test_many_sequences(gpu_ctx, ct):
+    """More sequences than a wave looks through at once, most of them with a token or two or none, a few with prompts."""
+    r = np.random.RandomState(30)
+    bring = [int(x) for x in r.choice([0, 1, 2, 3, 70], 200, p=[0.4, 0.3, 0.15, 0.13, 0.02])]
+    bring[63:66] = [0, 0, 5]
+    bring[-1] = 1
+    lens = [n + int(r.choice([0, 1, 17, 300])) for n in bring]
+    pool = Pool(gpu_ctx, 31, lens, ct, 16, 2, 64)
+    q = randn(32, (sum(bring) + 3, 4, 64), F16)
+    check(gpu_ctx, pool, q, F16, bring, window=100, prefix=[3] * 200, padding=3)
+
+
+@pytest.mark.parametrize("ct", [F32, F16, BF16, KV4])
+def test_queries_that_are_not_finite(gpu_ctx, ct):
+    """They spoil their own rows, and no others of the same tile."""
+    pool = Pool(gpu_ctx, 33, [200], ct, 16, 1, 64)
+    for dt in (F32, BF16):
+        q = randn(34, (90, 2, 64), dt)
+        want, wl = run(gpu_ctx, pool, q, [0, 90])
+        odd = [(0, 0), (3, 1), (40, 0), (89, 1)]
+        for n, (t, h) in enumerate(odd):
+            q[t, h, 7 * n] = (NAN, INF, -INF, NAN)[n]
+        out, lse = run(gpu_ctx, pool, q, [0, 90])
+        keep = torch.ones(90, 2, dtype=torch.bool)
+        for t, h in odd:
+            keep[t, h] = False
+            assert bool(out[t, h].isnan().all()) and not bool(torch.isfinite(lse[t, h]))
+        assert torch.equal(out[keep], want[keep]) and torch.equal(lse[keep], wl[keep])
+
+
+def test_two_streams_at_once(gpu_ctx):
+    """Calls of two contexts over one pool, each with its own stream, the same workspaces call after call."""
+    pool = Pool(gpu_ctx, 35, [3000, 2500, 90], BF16, 16, 2, 64)
+    plans = [([0, 5, 9, 29], dict(cap=4.0)), ([0, 1, 2, 92], dict(window=200))]
+    queries = [randn(36 + i, (start[-1], 8, 64), BF16) for i, (start, _) in enumerate(plans)]
+    want = [run(gpu_ctx, pool, x, start, **kw) for x, (start, kw) in zip(queries, plans)]
+    streams = [torch.cuda.Stream() for _ in plans]
+    ctxs, args = [], []
+    table, lens = on_gpu(pool.table, pool.lens)
+    for x, (start, kw), stream in zip(queries, plans, streams):
+        ctx = Context(0)
+        ctx.set_stream(stream.cuda_stream)
+        ctxs.append(ctx)
+        size = max(pool.kv.prompt_workspace(8, 3, start[-1]), 16)
+        args.append((x.cuda(), torch.zeros(x.shape, dtype=x.dtype, device="cuda"), i32(start).cuda(),
+                     torch.zeros(x.shape[:2], device="cuda"), torch.empty(size, dtype=torch.uint8, device="cuda"), kw))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for ctx, (x, out, start, lse, ws, kw) in zip(ctxs, args):
+            kernels.paged_prompt_attention(ctx, pool.kv, table, lens, x, out, seq_start=start, lse=lse, workspace=ws, **kw)
+    torch.cuda.synchronize()
+    for (x, out, start, lse, ws, kw), (a, b) in zip(args, want):
+        assert torch.equal(out.cpu(), a) and torch.equal(lse.cpu(), b)
+    for ctx in ctxs:
+        ctx.close()
+
+
 # ---- one token each ---------------------------------------------------------------------------------
 @pytest.mark.parametrize("dt", [F32, F16, BF16])
 @pytest.mark.parametrize("ct", [F32, F16, BF16, KV4])
