@@ -180,17 +180,23 @@ struct PpWave {
         for (int e = 0; e < 4; ++e) qf[j][e] = d < kv.hd ? x[e] * sign : 0.0f;
       }
     } else {
+      // (all of the row is asked for before any of it is used)
+      typename RunOf<A, 8>::V in[HDP / 16][8 / RunOf<A, 8>::M];
+#pragma unroll
+      for (int j = 0; j < HDP / 16; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; e += RunOf<A, 8>::M)
+          in[j][e / RunOf<A, 8>::M] =
+              *reinterpret_cast<const typename RunOf<A, 8>::V*>(p + min(16 * j + 8 * half, kv.hd - 8) + e);
+      const auto element = [&](int j, int e) BB_INLINE { return (float)in[j][e / RunOf<A, 8>::M][e % RunOf<A, 8>::M]; };
       int up = 0;
       if constexpr (F16) {
         // the power of two that puts the row's largest in 2^13..2^14 (0 and what is not finite keep their scale)
         float top = 0.0f;
-#pragma unroll 4
-        for (int j = 0; j < HDP / 16; ++j) {
-          float x[8];
-          load_vec<A, 8>(p + min(16 * j + 8 * half, kv.hd - 8), x);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
-        }
+        for (int j = 0; j < HDP / 16; ++j)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(element(j, e)));
         top = half_max(top);
         up = top > 0.0f && top < __builtin_inff() ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
         c = ldexpf(c, -up);
@@ -199,9 +205,11 @@ struct PpWave {
       for (int j = 0; j < HDP / 16; ++j) {
         float x[8];
         const int d = 16 * j + 8 * half;
-        load_vec<A, 8>(p + min(d, kv.hd - 8), x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = d < kv.hd ? F16 ? ldexpf(x[e] * sign, up) : x[e] * sign : 0.0f;
+        for (int e = 0; e < 8; ++e) {
+          const float y = element(j, e) * sign;
+          x[e] = d < kv.hd ? F16 ? ldexpf(y, up) : y : 0.0f;
+        }
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
           uint32_t w[NQ];
