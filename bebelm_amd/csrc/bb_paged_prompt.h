@@ -67,6 +67,10 @@ struct PpShape {
                               (KV4 ? 2 * NU * (UE / 8 + 1) : PARTS ? 16 * NU + 32 : 0);
   static constexpr int MOST = 160 * 1024 / (LDS + 64 * HDP + 64);  // blocks of a CU by their LDS
   static constexpr int WAVES = REGS <= 208 && MOST >= 2 ? 2 : 1;   // of a SIMD, and blocks of a CU
+  // Shapes that are not used: tiles that do not fit, and one row of waves where its tiles leave one block a CU and query rows
+  // of one part leave the matrix cores idle (16 x 5 tokens after 8192, heads of 128, bf16: 118 us, two rows 109; 64 x 5
+  // after 2000 116 and 100; in three parts 125 and 174; one sequence 27.5 and 28.9).
+  static constexpr bool NEVER = LDS > 159 * 1024 || (WR == 1 && WAVES == 1 && NQ == 1 && SZ == 2);
 };
 
 __device__ __attribute__((aligned(16))) uint32_t g_zeros[256];  // a row that is not there
@@ -859,12 +863,7 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, SRC>
       if (two) w.template put<true>(keys(u));
       w.template put<false>(vals(u + 1));
       landed();
-      if constexpr (S::WK == 4) {  // (a wave brings the keys that it takes itself; 80 tokens over 16 x 8192: 119 us, not 130)
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-      } else {
-        __syncthreads();
-      }
+      __syncthreads();
       look(u + 1);
     };
 
@@ -1045,7 +1044,7 @@ template <int CT, int NQ, int NP, int HDP, int WR, int SRC>
 hipError_t prompt_of(PpShape<CT, NQ, NP, HDP, WR, SRC>, hipStream_t st, const PromptQuery& q, const PagedView& kv,
                      const PagedSeqs& sq, PromptPlan& pl) {
   typedef PpShape<CT, NQ, NP, HDP, WR, SRC> S;
-  if constexpr (S::LDS > 159 * 1024) {
+  if constexpr (S::NEVER) {
     return hipErrorInvalidValue;  // (prompt_cut chooses none of these)
   } else {
     // (no more parts than the table's width has of the least size)

@@ -36,12 +36,13 @@ __global__ void __launch_bounds__(PP_THREADS) k_prompt_join(PromptQuery pq, int 
 
 constexpr int PARTS_MAX = 64;
 
+// The blocks of a shape that a CU takes at once (0: it is not used).
 int blocks_of_cu(int cache, int dt, int cls, int wr) {
-  const auto waves = [](auto s) { return decltype(s)::WAVES; };
-  return cache == BB_F32   ? shape_f32(dt, cls, wr, waves)
-         : cache == BB_F16 ? shape_f16(dt, cls, wr, waves)
-         : cache == BB_KV4 ? shape_kv4(dt, cls, wr, waves)
-                           : shape_bf16(dt, cls, wr, waves);
+  const auto blocks = [](auto s) { return decltype(s)::NEVER ? 0 : decltype(s)::WAVES; };
+  return cache == BB_F32   ? shape_f32(dt, cls, wr, blocks)
+         : cache == BB_F16 ? shape_f16(dt, cls, wr, blocks)
+         : cache == BB_KV4 ? shape_kv4(dt, cls, wr, blocks)
+                           : shape_bf16(dt, cls, wr, blocks);
 }
 
 // The blocks of a launch, chosen from what the host knows: how many tokens and sequences there are.
@@ -53,8 +54,8 @@ PromptCut prompt_cut(int n_cu, int cache, int dt, size_t n_tokens, size_t n_seqs
   PromptCut c;
   const int cls = pa_class(hd);
   const size_t rows = n_tokens * (size_t)G, mean = (rows + n_seqs - 1) / n_seqs;
-  const int row_bytes = cls * (cache == BB_F32 ? 4 : 2);  // in LDS, which has to hold 128 keys and values twice
-  c.wr = mean > 64 || row_bytes > 512 ? 4 : mean > 32 || row_bytes > 256 ? 2 : 1;
+  c.wr = mean > 64 ? 4 : mean > 32 ? 2 : 1;
+  while (blocks_of_cu(cache, dt, cls, c.wr) == 0) c.wr *= 2;  // (4 always is)
   c.bm = 32 * c.wr;
   c.n_tiles = (int)most_tiles(rows, c.bm, n_seqs);
   // keys in parts while the blocks (of sequences that are alike) fit the device at once
