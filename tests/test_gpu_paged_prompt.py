@@ -475,6 +475,24 @@ def test_starts_that_do_not_ascend(gpu_ctx):
     check(gpu_ctx, pool, q, BF16, [5, 5, 10])
 
 
+@pytest.mark.parametrize("ct", [F32, F16, BF16, KV4])
+@pytest.mark.parametrize("page", [5, 16])
+def test_single_tokens_behind_values_that_are_not_finite(gpu_ctx, page, ct):
+    """Keys and values before the window (in the window's first rows of a tile too) make no difference."""
+    lens = [1, 20, 21, 33, 50, 61, 200]
+    for hd, dt in ((64, F16), (128, BF16), (256, F32)):
+        pool = Pool(gpu_ctx, 95, lens, ct, page, 1, hd)
+        q = randn(96, (len(lens), 2, hd), dt)
+        for window in (1, 7, 20):
+            for s, n in enumerate(lens):
+                for j in range(max(0, n - window)):
+                    pool.put(0, s, j, NAN)
+                    pool.put(1, s, j, INF)
+            out, lse = check(gpu_ctx, pool, q, dt, [1] * len(lens), window=window, single=True)
+            assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(lse).all())
+            pool = Pool(gpu_ctx, 95, lens, ct, page, 1, hd)
+
+
 @pytest.mark.parametrize("ct", [F32, BF16, KV4])
 def test_many_sequences(gpu_ctx, ct):
     """More sequences than a wave looks through at once, most of them with a token or two or none, a few with prompts."""
