@@ -505,7 +505,7 @@ struct PpWave {
 
   // cap·tanh as cap - 2cap / (exp(2y) + 1): off by at most 2^-21 of the cap (the quotient's roundings and the
   // sum's), which is 2^-21·cap of a weight that is rounded to 16 bits. Half the instructions of tanh_of (6001 tokens, 16
-  // heads of 256, f16: the whole call 297 and 224 us).
+  // heads of 256, f16: the whole call 297 us with that and 254 with this).
   static constexpr bool QUICK = CT != BB_F32 && NP == 1;
   __device__ __forceinline__ float quick_cap(float y) const {
     const float e = __builtin_amdgcn_exp2f(y * (2.0f * LOG2E * c)), top = pq.cap * LOG2E;
@@ -704,6 +704,26 @@ struct PpWave {
   }
 };
 
+// out[t][h] = sum_j softmax_j(x[t][h][j])·v[j], a tile of rows (the G query heads of adjacent tokens, which share a kv head) in
+// one pass over the keys that any of them sees, with the running maximum and sum of the softmax.
+//
+// The scores are made transposed, Sᵀ = K·Qᵀ, by 32x32 matrix instructions: a lane then has scores of one row, 4 adjacent keys
+// at a time, which as weights are the second operand of Oᵀ = Vᵀ·Pᵀ just where they are; Vᵀ comes from LDS by reads that
+// transpose. Nothing moves between lanes but the two halves of a row's maximum. Query rows and sums stay in
+// registers. Keys and values go to LDS without passing registers, in an order of 16-byte pieces that leaves no bank
+// conflict (4 bits and f32 parts pass them, to be made 16-bit). Tiles that all rows see skip masks; those that
+// have something to be hidden get them as bits.
+//
+// What bounds it: matrix instructions and, nearly added to them, the vector ones (a weight is a multiply-add, an
+// exponential, a sum and half a conversion). 16384 tokens from the first, 32 heads on 8 of 128, bf16: 2.26 to 2.32 ms, 950 to
+// 975 TFLOP/s, where large products reach 1120 (keys by way of registers 8.3 ms; straight to LDS, with a maximum that
+// seldom moves, 3.3; a tile's weights made while the next one's scores are, 2.8; without spills 2.7; a page's
+// rows by one address and their loads behind the first products 2.3). 5003 tokens of 7 ragged prompts, 13 tiles a block: 112 us,
+// 620 TFLOP/s; blocks begin and end (6 us) two or three times a CU, and the last are alone. Heads of 256 fill the
+// registers of a SIMD with one wave, whose vector, matrix and LDS work then follow each other: 6001 tokens with a cap and a
+// window of 1024, f16, 192 to 200 us, 420 TFLOP/s. From 4 bits (2048 tokens after 8192, heads of 128) 380 us, 745
+// TFLOP/s: 150 vector instructions a tile and wave make f16 of the codes. 5 tokens of each of 16 sequences after 8192: 108 us,
+// 5.0 TB/s of cache.
 template <int CT, int NQ, int NP, int HDP, int WR, int SRC>
 __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, SRC>::WAVES))
     k_paged_prompt(PromptQuery pq, PagedView kv, PagedSeqs sq, PromptPlan pl) {
@@ -1003,8 +1023,10 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, SRC>
 // into NQ parts that are all of them (f16 ones at a power of two that puts the row's largest in 2^13..2^14: f32
 // keeps 22 bits). Weights are rounded once to what the cache has (NP = 1: bf16 by 2^-8, f16 by 2^-11 at most) where out
 // is rounded as far itself; an out with more bits has them in 2 or 3 parts. An f32 cache takes f32 instructions, or for
-// tiles of 128 rows and heads of up to 128 six times 16-bit ones (of the products of three parts with three, those that
-// count), of a sixteenth of the time each.
+// tiles of 128 rows and heads of up to 128 (more parts do not fit LDS) six times 16-bit ones (of the products of three
+// parts with three, those that count), of a sixteenth of the time each: 512 tokens after 1536, heads of 64, 67 us instead of
+// 104, 17 tokens 8.3 instead of 13.4. Few rows leave such a tile mostly empty: 8 x 5 tokens after 8192, heads of 64, 118
+// us, with f32 instructions and the keys shared out 68.
 template <int CT, int NQ, int NP, int SRC, class F>
 auto by_size(int cls, int wr, F& f) {
   const auto of = [&](auto hdp) {
