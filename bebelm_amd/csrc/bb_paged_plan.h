@@ -81,8 +81,9 @@ constexpr int PA_LONG = 16;
 
 // Waves of a SIMD that fit: 128, 256, 512 registers each. (The forms with heads of up to 64 fill theirs: f32 queries on a
 // bf16 cache, and all 16-bit caches of odd pages, spill 12 to 24 of them, at a pair's beginning and end, none in the loop
-// over tiles. 4-bit tiles take fewer: with two waves a SIMD instead of three, heads of 128, 161.0 us instead of 160.2.)
-constexpr int pa_waves(int hdp, bool four = false) { return hdp == 64 ? 4 : hdp == 128 ? (four ? 3 : 2) : four ? 2 : 1; }
+// over tiles. 4-bit tiles take fewer, and
+// heads of 256 fit twice; three waves with heads of 128, 64 sequences of 8192, 141 us, two 138.)
+constexpr int pa_waves(int hdp, bool four = false) { return hdp == 64 ? 4 : hdp == 128 || four ? 2 : 1; }
 constexpr int pa_class(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 inline int blocks_at_once(int n_cu, int hd, bool four = false) { return n_cu * pa_waves(pa_class(hd), four); }
 
@@ -179,7 +180,9 @@ inline PagedCut paged_cut(int n_cu, int n_seqs, int n_groups, int page_size, siz
     cap = std::min(cap, std::min((size_t)window + pages * (c.slots - page_size), pages * c.slots) + 31);
   }
   const int blocks_max = blocks_at_once(n_cu, hd, elem_bytes == 1), unit_short = pa_unit_short(hd * elem_bytes);
-  c.few = c.uni ? n_cu : blocks_max;
+  // (4 bits want all the waves for their instructions: 64 sequences of 8192, heads of 128, 140 us and 178 with one block a CU,
+  // of 64, 94 and 150)
+  c.few = c.uni && elem_bytes > 1 ? n_cu : blocks_max;
   // (pairs of one unit take a block each at most, longer ones a block for each unit)
   c.unit = cap <= (size_t)1 << unit_short ? unit_short : PA_UNIT;
   const size_t pairs = (size_t)n_seqs * n_groups, units = ((cap - 1) >> c.unit) + 1;
