@@ -260,8 +260,8 @@ hipError_t rope_rows_of(hipStream_t s, const RopeRows& r, const RopeTurns& t, co
 }
 
 // The keys and values of tokens' positions, as they are in the pool, a run of 8 elements a thread: a block per token (few
-// tokens: several), whose first wave finds the place. 5003 tokens of 8 kv heads of 128 from 4 bits to bf16 (26 MB): 12.3 us;
-// a wave for each token, four runs a lane at once, 12.8 and for 48 tokens 3.9 instead of 2.9.
+// tokens: several), whose first wave finds the place. Bound by its bytes: 5003 tokens of 8 kv heads of 128 from 4 bits to
+// f32 (47 MB) 12.3 us, 3.8 TB/s; a wave for each token, four runs a lane at once, 12.8 and for 48 tokens 3.9 instead of 2.9.
 template <class A, class C>
 __global__ void __launch_bounds__(RR_THREADS) k_paged_read(ReadRows r, PagedView kv, PagedSeqs sq, int per) {
   __shared__ RowPlace place;
