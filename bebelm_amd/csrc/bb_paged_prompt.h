@@ -7,6 +7,7 @@
 #include "bb_paged4.h"
 #include "bb_paged_device.h"
 #include "bb_prompt_plan.h"
+#include "bb_prompt_turns.h"
 
 namespace bb {
 
@@ -24,7 +25,6 @@ struct PromptPlan {
 namespace {
 
 constexpr int PP_THREADS = 256;
-#define BB_INLINE __attribute__((always_inline))
 // Weights go up to 2^SLACK, as f16 to 2^(SLACK + F16_UP) = 2^14, whose range then costs at most 2^-33 of the largest.
 constexpr float SLACK = 6.0f, F16_UP = 8.0f;
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -704,6 +704,96 @@ struct PpWave {
   }
 };
 
+// A block's steps, a wave's share of them, for PromptTurns.
+template <int CT, int NQ, int NP, int HDP, int WR, int SRC>
+struct PpBlock {
+  typedef PpShape<CT, NQ, NP, HDP, WR, SRC> S;
+  typedef PpWave<CT, NQ, NP, HDP, WR, SRC> Wave;
+  Wave& w;
+  const KeyTiles& kt;
+  char* const tiles;
+  uint32_t (&s_ok)[2][4];
+  uint32_t (&s_odd)[2][4];
+  uint32_t (&s_marks)[2][HDP / 32][PP_THREADS];
+  const int u0, b0, b1;  // b0, b1: the least that all rows of the block see is up to b0, from b1 on
+  typename Wave::Row krow, vrow;
+  uint32_t ok0, ok1;
+
+  __device__ BB_INLINE char* keys_of(int u) const { return tiles + (u & 1) * S::BUF; }
+  __device__ BB_INLINE char* vals_of(int u) const { return tiles + (u & 1) * S::BUF + S::NPL * S::PLANE; }
+  __device__ BB_INLINE int first_key(int u) const { return kt.at(u0 + u) * S::KT + w.wk * S::BN; }
+  __device__ BB_INLINE void flags(int u) {
+    const uint32_t* ok = s_ok[u & 1];
+    ok1 = ~0u;
+    if constexpr (S::RPW == 32) {
+      ok0 = ok[w.wk];
+    } else if constexpr (S::WK == 1 && S::RPW == 16) {
+      ok0 = ok[0] | ok[1] << 16;
+      ok1 = ok[2] | ok[3] << 16;
+    } else if constexpr (S::WK == 2) {
+      ok0 = ok[2 * w.wk] | ok[2 * w.wk + 1] << 16;
+    } else {
+      ok0 = ok[0] | ok[1] << 8 | ok[2] << 16 | ok[3] << 24;
+    }
+    ok0 = __builtin_amdgcn_readfirstlane(ok0);
+    ok1 = __builtin_amdgcn_readfirstlane(ok1);
+  }
+
+  __device__ BB_INLINE void find(int u) { w.find(kt.at(u0 + u)); }
+  __device__ BB_INLINE void keys(int u) {
+    krow = w.found();
+    const uint32_t ok = Wave::there(krow);
+    if (w.lane == 0) s_ok[u & 1][w.wv] = ok;
+    w.template load<true>(krow, keys_of(u));
+  }
+  __device__ BB_INLINE void pass() { vrow = krow; }
+  __device__ BB_INLINE void values(int u) { w.template load<false>(vrow, vals_of(u)); }
+  __device__ BB_INLINE void put_keys(int u) { w.template put<true>(keys_of(u)); }
+  __device__ BB_INLINE void put_values(int u) { w.template put<false>(vals_of(u)); }
+  __device__ BB_INLINE void landed() { bb::landed(); }
+  __device__ BB_INLINE void barrier() { __syncthreads(); }
+  template <int I>
+  __device__ BB_INLINE void score(int u, Set<I>) {
+    w.template score<I>(lds_at(keys_of(u)), [](int) {});
+  }
+  template <int I>
+  __device__ BB_INLINE void see(int u, Set<I>) {
+    flags(u);
+    w.template shape<I>(first_key(u), ok0, ok1);
+  }
+  template <int I, class F>
+  __device__ BB_INLINE void products(int u, Set<I>, F&& ask) {
+    typename Wave::Weights p;
+    __builtin_amdgcn_sched_barrier(0);
+    // (behind the last tile, scores of whatever is there, for nothing)
+    w.template score<1 - I>(lds_at(keys_of(u + 1)), [&](int j) BB_INLINE {
+      constexpr int PAIRS = 8 * S::NT;
+      ask(j);
+      w.template weigh<I>(p, j * PAIRS / Wave::STEPS, (j + 1) * PAIRS / Wave::STEPS);
+    });
+    w.add(lds_at(vals_of(u)), p);
+  }
+  __device__ BB_INLINE bool shared(int u) const {
+    const int j0 = kt.at(u0 + u) * S::KT;
+    return (j0 + S::KT - 1 <= b0 && j0 >= b1) || j0 + S::KT <= w.prefix;
+  }
+  __device__ BB_INLINE bool odd(int u) const { return __ballot(w.values_odd(lds_at(vals_of(u)))) != 0; }
+  __device__ BB_INLINE void tell(int at, bool mine) {
+    if (w.lane == 0) s_odd[at][w.wv] = mine;
+  }
+  __device__ BB_INLINE bool told(int at) const { return (s_odd[at][0] | s_odd[at][1] | s_odd[at][2] | s_odd[at][3]) != 0; }
+  __device__ BB_INLINE uint32_t* marks(int u) const { return &s_marks[u & 1][0][threadIdx.x]; }
+  __device__ BB_INLINE void mark(int u) { w.mark(marks(u), lds_at(vals_of(u)), first_key(u), ok0, ok1); }
+  __device__ BB_INLINE void clean(int u) { w.clean(vals_of(u)); }
+  __device__ BB_INLINE void spoil(int u) { w.spoil(marks(u)); }
+  __device__ BB_INLINE bool past() const { return w.past(); }
+  __device__ BB_INLINE void raise() { w.raise(); }
+  __device__ BB_INLINE void last() {
+#pragma unroll
+    for (int t = 0; t < S::NT; ++t) w.x[0][t] = w.x[1][t];
+  }
+};
+
 // out[t][h] = sum_j softmax_j(x[t][h][j])·v[j], a tile of rows (the G query heads of adjacent tokens, which share a kv head) in
 // one pass over the keys that any of them sees, with the running maximum and sum of the softmax.
 //
@@ -801,130 +891,12 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, SRC>
     w.c = fmaxf(w.c, 1e-37f);  // (0 times an infinite score would be NaN)
   }
 
-  // Tiles u0..u1-1. Turn u takes the scores of tile u + 1 while it weighs tile u, whose values it then adds, and asks for
-  // the keys of tile u + 2 and the values of tile u + 1, which a barrier later are there. What is seldom done to
-  // the sums stands outside the loop over plain turns, which keeps them in their registers.
+  // Tiles u0..u1-1 (bb_prompt_turns.h).
   if (u0 < u1) {
-    const int n_turns = u1 - u0;
-    const auto keys = [&](int u) BB_INLINE { return s_tiles + (u & 1) * S::BUF; };
-    const auto vals = [&](int u) BB_INLINE { return s_tiles + (u & 1) * S::BUF + S::NPL * S::PLANE; };
-    const auto flags = [&](int u, uint32_t& ok0, uint32_t& ok1) BB_INLINE {
-      const uint32_t* ok = s_ok[u & 1];
-      ok1 = ~0u;
-      if constexpr (S::RPW == 32) {
-        ok0 = ok[w.wk];
-      } else if constexpr (S::WK == 1 && S::RPW == 16) {
-        ok0 = ok[0] | ok[1] << 16;
-        ok1 = ok[2] | ok[3] << 16;
-      } else if constexpr (S::WK == 2) {
-        ok0 = ok[2 * w.wk] | ok[2 * w.wk + 1] << 16;
-      } else {
-        ok0 = ok[0] | ok[1] << 8 | ok[2] << 16 | ok[3] << 24;
-      }
-      ok0 = __builtin_amdgcn_readfirstlane(ok0);
-      ok1 = __builtin_amdgcn_readfirstlane(ok1);
-    };
-    const auto first_key = [&](int u) BB_INLINE { return kt.at(u0 + u) * S::KT + w.wk * S::BN; };
-    typename Wave::Row krow, vrow;
-    uint32_t ok0, ok1;
-    const auto bring = [&](int u) BB_INLINE {  // tile u's keys (its rows found)
-      krow = w.found();
-      const uint32_t ok = Wave::there(krow);
-      if (lane == 0) s_ok[u & 1][w.wv] = ok;
-      w.template load<true>(krow, keys(u));
-    };
-    const auto see = [&](int u, auto set) BB_INLINE {  // tile u's scores, before its turn
-      flags(u, ok0, ok1);
-      w.template shape<decltype(set)::value>(first_key(u), ok0, ok1);
-    };
-    // Values that are not finite reach the rows that see them and no others. A tile that all rows of the block see is added
-    // as it is; one that they do not is looked at when it is there. If it has such values, the sums
-    // that they belong to are marked, the values taken out, and what is marked made NaN after the tile's turn.
-    const int last = min(r0 + S::BM, rows) - 1, b0 = index_of(r0), b1 = first_seen(index_of(last), pq.window);
-    bool odd = false;
-    int looks = 0;
-    const auto look = [&](int u) BB_INLINE {
-      const int j0 = kt.at(u0 + u) * S::KT;
-      if ((j0 + S::KT - 1 <= b0 && j0 >= b1) || j0 + S::KT <= w.prefix) return;
-      const bool mine_odd = __ballot(w.values_odd(lds_at(vals(u)))) != 0;
-      uint32_t* at = s_odd[looks++ & 1];  // (two in turn: a wave that writes one again has passed a barrier behind its reads)
-      if (lane == 0) at[w.wv] = mine_odd;
-      __syncthreads();
-      odd = (at[0] | at[1] | at[2] | at[3]) != 0;
-    };
-    const auto mark = [&](int u) BB_INLINE {
-      w.mark(&s_marks[u & 1][0][tid], lds_at(vals(u)), first_key(u), ok0, ok1);
-      __syncthreads();
-      w.clean(vals(u));
-      __syncthreads();
-    };
-    const auto turn = [&](int u, auto set) BB_INLINE {
-      constexpr int I = decltype(set)::value;
-      const bool more = u + 1 < n_turns, two = u + 2 < n_turns;
-      const auto ask = [&](int j) BB_INLINE {  // (behind the products of a step, which go on meanwhile)
-        if (j == 0 && two) bring(u + 2);
-        if (j == 1 && more) w.template load<false>(vrow, vals(u + 1));
-        if (j == 2 && two) {
-          vrow = krow;
-          if (u + 3 < n_turns) w.find(kt.at(u0 + u + 3));
-        }
-      };
-      typename Wave::Weights p;
-      __builtin_amdgcn_sched_barrier(0);
-      // (behind the last tile, scores of whatever is there, for nothing)
-      w.template score<1 - I>(lds_at(keys(u + 1)), [&](int j) BB_INLINE {
-        constexpr int PAIRS = 8 * S::NT;
-        ask(j);
-        w.template weigh<I>(p, j * PAIRS / Wave::STEPS, (j + 1) * PAIRS / Wave::STEPS);
-      });
-      w.add(lds_at(vals(u)), p);
-      if (!more) return;
-      see(u + 1, std::integral_constant<int, 1 - I>());
-      if (two) w.template put<true>(keys(u));
-      w.template put<false>(vals(u + 1));
-      landed();
-      __syncthreads();
-      look(u + 1);
-    };
-
-    w.find(kt.at(u0));
-    bring(0);
-    w.template load<false>(krow, vals(0));
-    w.template put<true>(keys(0));
-    w.template put<false>(vals(0));
-    if (n_turns > 1) {
-      w.find(kt.at(u0 + 1));
-      bring(1);
-      w.template put<true>(keys(1));
-      if (n_turns > 2) w.find(kt.at(u0 + 2));
-    }
-    vrow = krow;
-    landed();
-    __syncthreads();
-    const std::integral_constant<int, 0> even;
-    const std::integral_constant<int, 1> uneven;
-    w.template score<0>(lds_at(keys(0)), [](int) {});
-    see(0, even);
-    look(0);
-    for (int u = 0; u < n_turns;) {
-      if (w.past()) w.raise();
-      if (odd) mark(u);
-      const bool spoiled = odd;
-      odd = false;
-      const auto on = [&]() BB_INLINE { return u < n_turns && !spoiled && !odd && !w.past(); };
-      for (;;) {
-        turn(u++, even);
-        if (!on()) {
-#pragma unroll
-          for (int t = 0; t < S::NT; ++t) w.x[0][t] = w.x[1][t];
-          break;
-        }
-        turn(u++, uneven);
-        if (!on()) break;
-      }
-      if (spoiled) w.spoil(&s_marks[u - 1 & 1][0][tid]);
-    }
-    __syncthreads();  // (the tiles' place is taken below)
+    const int last = min(r0 + S::BM, rows) - 1;
+    typedef PpBlock<CT, NQ, NP, HDP, WR, SRC> Block;
+    Block b{w, kt, s_tiles, s_ok, s_odd, s_marks, u0, index_of(r0), first_seen(index_of(last), pq.window), {}, {}, 0, 0};
+    PromptTurns<Block>(b, u1 - u0).run();
   }
   w.l = half_sum(w.l);
 
