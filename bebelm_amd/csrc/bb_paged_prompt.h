@@ -504,9 +504,11 @@ struct PpWave {
   }
 
   // cap·tanh as cap - 2cap / (exp(2y) + 1): off by at most 2^-21 of the cap (the quotient's roundings and the
-  // sum's), which is 2^-21·cap of a weight that is rounded to 16 bits. Half the instructions of tanh_of (6001 tokens, 16
-  // heads of 256, f16: the whole call 297 us with that and 254 with this).
+  // sum's), however small the score. Up to a cap of QUICK_CAP that is 2^-15 of a weight, an eighth of the half step by which f16
+  // rounds it, and of the log sum; larger ones take tanh_of, which is off by a few steps of the score itself. It has half the
+  // instructions of tanh_of (6001 tokens, 16 heads of 256, f16: the whole call 297 us with that and 254 with this).
   static constexpr bool QUICK = CT != BB_F32 && NP == 1;
+  static constexpr float QUICK_CAP = 64.0f;
   __device__ __forceinline__ float quick_cap(float y) const {
     const float e = __builtin_amdgcn_exp2f(y * (2.0f * LOG2E * c)), top = pq.cap * LOG2E;
     return fmaf(-2.0f * top, __builtin_amdgcn_rcpf(e + 1.0f), top);
@@ -518,10 +520,17 @@ struct PpWave {
     by = c;
     if (pq.cap > 0.0f) {
       by = 1.0f;
+      if (QUICK && pq.cap <= QUICK_CAP) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) y[t][e] = QUICK ? quick_cap(y[t][e]) : (pq.cap * LOG2E) * tanh_of(y[t][e] * c);
+          for (int e = 0; e < 16; ++e) y[t][e] = quick_cap(y[t][e]);
+      } else {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) y[t][e] = (pq.cap * LOG2E) * tanh_of(y[t][e] * c);
+      }
     }
     if (pq.slopes) {
       const float away = (float)(i - j0 - 4 * half);
