@@ -3234,7 +3234,7 @@ int bb_paged_prompt_attention(bb_ctx* c, const bb_paged_kv* kv, const bb_paged_s
               q.n_tokens = (int)T;
               q.window = pq->window < ((size_t)1 << 31) ? (int)pq->window : 0;  // (lengths are below 2^31)
               q.scale = pq->scale != 0.0f ? pq->scale : 1.0f / std::sqrt((float)hd);
-              q.cap = pq->cap;
+              q.cap = bb::ScoreCap::of(pq->cap);
               q.lse = nl ? static_cast<float*>(d[4]) : nullptr;
               q.slopes = pq->slopes ? static_cast<const float*>(d[5]) : nullptr;
               q.prefix = pq->prefix ? static_cast<const int32_t*>(d[6]) : nullptr;

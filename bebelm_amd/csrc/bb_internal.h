@@ -3,9 +3,11 @@
 #define BB_INTERNAL_H
 #include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>
+#include <float.h>
 #include <stddef.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <string>
 #include <vector>
 
@@ -413,6 +415,18 @@ hipError_t launch_paged_read(hipStream_t s, int dtype, int cache, const ReadRows
 // dtype of q, k, v and q_out; cache: the pool's dtype (n_kv > 0).
 hipError_t launch_rope_rows(hipStream_t s, int dtype, int cache, const RopeRows& r, const RopeTurns& t,
                             const PagedView& kv, const PagedSeqs& seqs);
+// A cap of scores in base 2: cap·log2(e), and the reciprocal of that, both held to finite numbers (top 0: none).
+struct ScoreCap {
+  float top = 0.0f, inv = 0.0f;
+  static ScoreCap of(float cap) {
+    ScoreCap c;
+    if (cap > 0.0f) {
+      c.top = (float)std::min((double)cap * 1.4426950408889634, (double)FLT_MAX);
+      c.inv = (float)std::min(0.6931471805599453 / (double)cap, (double)FLT_MAX);
+    }
+    return c;
+  }
+};
 struct PagedQuery {
   const void* q;
   void* out;
@@ -421,7 +435,7 @@ struct PagedQuery {
   float scale;
   float* lse;
   void* ws;
-  float cap = 0.0f;  // > 0: scores are capped
+  ScoreCap cap;
   const float* slopes = nullptr;
 };
 size_t paged_attn_ws(int n_cu, int cache, int n_seqs, int n_heads, int n_kv, int hd);
@@ -435,7 +449,8 @@ struct PromptQuery {
   void* out;
   size_t q_stride, out_stride;
   int dt, n_heads, n_tokens, window;
-  float scale, cap;
+  float scale;
+  ScoreCap cap;
   const float* slopes;
   const int32_t *prefix, *seq_start;
   float* lse;

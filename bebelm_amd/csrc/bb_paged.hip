@@ -474,7 +474,8 @@ struct PaWave {
   uint32_t vw[KV4 ? 4 * NT : 1][KV4 ? NV : 1], vh[KV4 ? 4 * NT : 1][KV4 ? NV : 1];
   Kv4Magic magic;
   int index;           // MOD: of the query's position
-  float cap, slope;    // (base 2)
+  ScoreCap cap;
+  float slope;         // (base 2)
   int pos[MOD ? NT : 1];  // of the positions whose values are loaded, the first of each 16
   uint32_t valid;  // bit 4t + r: position 16t + 4g + r of the tile whose values are loaded is attended to
   static constexpr uint32_t ALL = (1u << 4 * NT) - 1;
@@ -505,8 +506,7 @@ struct PaWave {
     // scores are exponents of 2; parts that are all of an f32 take the factor in, two parts only hold q itself
     c = pq.scale * LOG2E;
     if constexpr (MOD) {
-      if (pq.cap > 0.0f) c = pq.scale / pq.cap;
-      cap = pq.cap * LOG2E;
+      cap = pq.cap;
       slope = pq.slopes ? pq.slopes[head0 + min(n, heads - 1)] * LOG2E : 0.0f;
     }
     const float cq = SCALED ? 1.0f : c;
@@ -836,11 +836,11 @@ struct PaWave {
       for (int t = 0; t < NT; ++t) x[t] *= c;
     }
     if constexpr (MOD) {
-      if (cap > 0.0f) {
+      if (cap.top > 0.0f) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x[t][r] = cap * tanh_of(x[t][r]);
+          for (int r = 0; r < 4; ++r) x[t][r] = capped(x[t][r], cap);
       }
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -1259,7 +1259,7 @@ hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQue
   } while (0)
 #define BB_PA_MOD(ct, nq, np, hdp, four)              \
   do {                                            \
-    if (q.cap > 0.0f || q.slopes) BB_PA(ct, nq, np, hdp, four, true); \
+    if (q.cap.top > 0.0f || q.slopes) BB_PA(ct, nq, np, hdp, four, true); \
     else BB_PA(ct, nq, np, hdp, four, false);         \
   } while (0)
 #define BB_PA_HD(ct, nq, np, four)                      \

@@ -134,17 +134,19 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
-// tanh, within a few units in the last place: up to 0.6 a quotient of polynomials (the continued fraction
-// y / (1 + y^2 / (3 + y^2 / (5 + y^2 / (7 + y^2 / 9)))), off by less than 1e-9 there), then (e - 1) / (e + 1), e = exp(2|y|).
-__device__ __forceinline__ float tanh_of(float y) {
-  const float a = fabsf(y), z = y * y;
+// cap·tanh(s / cap) of a score s (base 2), within a few units in the last place of itself whatever the cap. With y = s / cap, up
+// to 0.6, s times a quotient of polynomials (tanh(y) / y by the continued fraction
+// 1 / (1 + y^2 / (3 + y^2 / (5 + y^2 / (7 + y^2 / 9)))), off by less than 1e-9 there), then cap·(e - 1) / (e + 1),
+// e = exp(2|y|). (Past a cap of 2.3e38, base 2's largest number stands for it.)
+__device__ __forceinline__ float capped(float s, const ScoreCap& cap) {
+  const float y = s * cap.inv, a = fabsf(y), z = y * y;
   const float e = __builtin_amdgcn_exp2f((a > 15.0f ? 15.0f : a) * (2.0f * LOG2E));
   const bool small = a < 0.6f;
-  float n0 = a * (fmaf(z, 105.0f + z, 945.0f)), d0 = fmaf(z, fmaf(z, 15.0f, 420.0f), 945.0f), n1 = e - 1.0f, d1 = e + 1.0f;
+  float n0 = fmaf(z, 105.0f + z, 945.0f), d0 = fmaf(z, fmaf(z, 15.0f, 420.0f), 945.0f), n1 = e - 1.0f, d1 = e + 1.0f;
   // (both in line: a branch each would cost more; and not done where a call has no cap)
   asm volatile("" : "+v"(n0), "+v"(d0), "+v"(n1), "+v"(d1));
   const float num = small ? n0 : n1, den = small ? d0 : d1;
-  return copysignf(num * __builtin_amdgcn_rcpf(den), y);
+  return (small ? s : copysignf(cap.top, s)) * (num * __builtin_amdgcn_rcpf(den));
 }
 
 }  // namespace

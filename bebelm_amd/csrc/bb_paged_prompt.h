@@ -505,31 +505,34 @@ struct PpWave {
 
   // cap·tanh as cap - 2cap / (exp(2y) + 1): off by at most 2^-21 of the cap (the quotient's roundings and the
   // sum's), however small the score. Up to a cap of QUICK_CAP that is 2^-15 of a weight, an eighth of the half step by which f16
-  // rounds it, and of the log sum; larger ones take tanh_of, which is off by a few steps of the score itself. It has half the
-  // instructions of tanh_of (6001 tokens, 16 heads of 256, f16: the whole call 297 us with that and 254 with this).
+  // rounds it, and of the log sum; larger ones take capped(), which is off by a few steps of the score itself. It has half the
+  // instructions of that (6001 tokens, 16 heads of 256, f16: the whole call 297 us with that and 254 with this).
   static constexpr bool QUICK = CT != BB_F32 && NP == 1;
   static constexpr float QUICK_CAP = 64.0f;
-  __device__ __forceinline__ float quick_cap(float y) const {
-    const float e = __builtin_amdgcn_exp2f(y * (2.0f * LOG2E * c)), top = pq.cap * LOG2E;
-    return fmaf(-2.0f * top, __builtin_amdgcn_rcpf(e + 1.0f), top);
+  // (y·twice: two capless scores by the cap, as an exponent of 2)
+  __device__ __forceinline__ float quick_cap(float y, float twice) const {
+    const float e = __builtin_amdgcn_exp2f(y * twice);
+    return fmaf(-2.0f * pq.cap.top, __builtin_amdgcn_rcpf(e + 1.0f), pq.cap.top);
   }
   // The scores capped, with their bias, hidden where the rows do not see the keys from j0 on, and the largest.
   template <int I>
   __device__ __forceinline__ void shape(int j0, uint32_t ok0, uint32_t ok1) {
     v16f(&y)[NT] = x[I];
     by = c;
-    if (pq.cap > 0.0f) {
+    if (pq.cap.top > 0.0f) {
       by = 1.0f;
-      if (QUICK && pq.cap <= QUICK_CAP) {
+      if (QUICK && pq.cap.top <= QUICK_CAP * LOG2E) {
+        // (finite: 0 times it is 0)
+        const float twice = fminf(c * (pq.cap.inv * (2.0f * LOG2E)), 3.0e38f);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) y[t][e] = quick_cap(y[t][e]);
+          for (int e = 0; e < 16; ++e) y[t][e] = quick_cap(y[t][e], twice);
       } else {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) y[t][e] = (pq.cap * LOG2E) * tanh_of(y[t][e] * c);
+          for (int e = 0; e < 16; ++e) y[t][e] = capped(y[t][e] * c, pq.cap);
       }
     }
     if (pq.slopes) {
@@ -884,7 +887,7 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, SRC>
   w.i1 = __builtin_amdgcn_readlane(w.i, 31);
   w.lo1 = __builtin_amdgcn_readlane(w.lo, 31);
   w.slope = pq.slopes ? pq.slopes[head] * LOG2E : 0.0f;
-  w.c = pq.cap > 0.0f ? fabsf(pq.scale) / pq.cap : fabsf(pq.scale) * LOG2E;
+  w.c = fabsf(pq.scale) * LOG2E;
   w.m = NEG_INF;
   w.l = 0.0f;
 #pragma unroll
@@ -897,7 +900,7 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, SRC>
     if (pq.dt == BB_F32) w.template load_q<float>(at, sign);
     else if (pq.dt == BB_F16) w.template load_q<_Float16>(at, sign);
     else w.template load_q<__bf16>(at, sign);
-    w.c = fmaxf(w.c, 1e-37f);  // (0 times an infinite score would be NaN)
+    w.c = fmaxf(w.c, 1e-45f);  // (0 times an infinite score would be NaN)
   }
 
   // Tiles u0..u1-1 (bb_prompt_turns.h).
