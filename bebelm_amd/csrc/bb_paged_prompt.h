@@ -561,9 +561,10 @@ struct PpWave {
   }
 
   // The running maximum stays until a score is SLACK past it: the sums are as exact, and seldom multiplied.
-  __device__ __forceinline__ bool past() const { return __any(top > m + SLACK); }
+  // (by the difference: m + SLACK may be rounded to a maximum two steps of 4 or one of 8 away, whose weight f16 does not hold)
+  __device__ __forceinline__ bool past() const { return __any(top - m > SLACK); }
   __device__ __forceinline__ void raise() {
-    const float mx = top > m + SLACK ? top : m;
+    const float mx = top - m > SLACK ? top : m;
     const float f = __builtin_amdgcn_exp2f(m - (mx == NEG_INF ? 0.0f : mx));
     m = mx;
     l *= f;
@@ -571,6 +572,26 @@ struct PpWave {
     for (int d = 0; d < HDP / 32; ++d)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[d][e] *= f;
+  }
+
+  // A weight is 2^(x·by - m) by one multiply-add: what -m + F16_UP is rounded by, and m was as a product, goes into the
+  // exponent, of all of a row's weights alike while m stays. From FAR on, where that may be 2^-7, a row's scores are made
+  // differences from m beforehand, of the product that m was taken of, and its m is 0 while they are weighed. (Each row by its own
+  // m: one that did so for a neighbour's sake would have weights of two kinds.)
+  static constexpr float FAR = 65536.0f;
+  __device__ __forceinline__ bool far_row() const { return fabsf(m) >= FAR && m != NEG_INF; }
+  __device__ __forceinline__ bool far() const { return __any(far_row()); }
+  __device__ __forceinline__ float near() {
+    const float kept = m;
+    if (far_row()) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[0][t][e] = x[0][t][e] * by - m;
+      by = 1.0f;
+      m = 0.0f;
+    }
+    return kept;
   }
 
   // The weights of the tile, in 16 bits: register 2e of w[t][s][part] those of registers 8s + 2e and 8s + 2e + 1.
@@ -800,6 +821,10 @@ struct PpBlock {
   __device__ BB_INLINE void spoil(int u) { w.spoil(marks(u)); }
   __device__ BB_INLINE bool past() const { return w.past(); }
   __device__ BB_INLINE void raise() { w.raise(); }
+  __device__ BB_INLINE bool far() const { return w.far(); }
+  // (m in the place of the next tile's marks, which are made after back())
+  __device__ BB_INLINE void near(int u) { *marks(u + 1) = __float_as_uint(w.near()); }
+  __device__ BB_INLINE void back(int u) { w.m = as_float(*marks(u + 1)); }
   __device__ BB_INLINE void last() {
 #pragma unroll
     for (int t = 0; t < S::NT; ++t) w.x[0][t] = w.x[1][t];

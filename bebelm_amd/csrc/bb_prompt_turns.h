@@ -26,7 +26,8 @@ namespace bb {
 // products(u, set, ask): tile u's scores weighed and its values added, tile u + 1's scores made, in between
 // ask(0), ask(1), ask(2); shared(u): all rows of the block see all of the tile; odd(u): the wave brought values that
 // are not finite, which tell() and told() make known to all; mark(u), clean(u), spoil(u): those taken out. past(): a
-// score is past the running maximum's slack; raise(); last(set): the scores of set 1 become those of set 0.
+// score is past the running maximum's slack; raise(); far(): the maximum is too large for weights as they are made
+// otherwise; near(u), back(u): before and after the turn of such scores. last(): the scores of set 1 become those of set 0.
 template <int I>
 struct Set {
   static constexpr int value = I;
@@ -100,6 +101,8 @@ struct PromptTurns {
     begin();
     for (int u = 0; u < n;) {
       if (b.past()) b.raise();
+      const bool far = b.far();
+      if (far) b.near(u);
       if (odd) {
         b.mark(u);
         b.barrier();
@@ -108,7 +111,7 @@ struct PromptTurns {
       }
       const bool spoiled = odd;
       odd = false;
-      const auto on = [&]() BB_INLINE { return u < n && !spoiled && !odd && !b.past(); };
+      const auto on = [&]() BB_INLINE { return u < n && !spoiled && !far && !odd && !b.past(); };
       for (;;) {
         turn(u++, Set<0>());
         if (!on()) {
@@ -119,6 +122,7 @@ struct PromptTurns {
         if (!on()) break;
       }
       if (spoiled) b.spoil(u - 1);
+      if (far) b.back(u - 1);
     }
     b.barrier();  // (the tiles' place is taken behind it)
   }

@@ -500,10 +500,11 @@ int bb_paged_attention(bb_ctx* ctx, const bb_paged_kv* kv, const bb_paged_seqs* 
  * -inf; of padding nothing is written. A value that is not finite makes not finite what it reaches, and nothing else: the
  * rows that do not see it are as if it were not there (of an F32 cache, magnitudes from 3.39e38 on may count as
  * infinite). Weights are rounded to the cache's type (F16 for BB_KV4) where out is
- * F16 on an F16 or BB_KV4 cache, or BF16; elsewhere they keep what out can hold. Capped scores are off by some steps of
- * themselves, and by 2^-21 of the cap (lse too) where weights are rounded and the cap is at most 64. workspace: as in
- * bb_paged_attention, of bb_paged_prompt_attention_workspace's answer (which may be 0: then a captured call needs none).
- * Equal calls give equal bits. One call takes n_tokens·n_heads / 32 + n_seqs·n_kv_heads below 2^24 (BB_ERR_RANGE: cut the batch). */
+ * F16 on an F16 or BB_KV4 cache, or BF16; elsewhere they keep what out can hold. On an F16 or BB_KV4 cache, elements of a
+ * query below 2^-38 of the largest of its head may count as 0. Capped scores are off by some steps of themselves, and by 2^-21
+ * of the cap (lse too) where weights are rounded and the cap is at most 64. workspace: as in bb_paged_attention, of
+ * bb_paged_prompt_attention_workspace's answer (which may be 0: then a captured call needs none). Equal calls give equal
+ * bits. One call takes n_tokens·n_heads / 32 + n_seqs·n_kv_heads below 2^24 (BB_ERR_RANGE: cut the batch). */
 typedef struct {
   size_t n_tokens;
   uint32_t dtype; /* of q and out */

@@ -28,7 +28,7 @@ typedef std::map<int, std::vector<Event>> Memory;
 struct Case {
   int n, waves_rows;              // tiles; waves along the rows (4, 2, 1)
   bool registers;                 // tiles that pass registers (4 bits, f32 parts)
-  std::vector<int> shared, odd, past;  // by tile; odd: bit w: wave w's rows hold such values
+  std::vector<int> shared, odd, past, far;  // by tile; odd: bit w: wave w's rows hold such values
 };
 
 struct Wave {
@@ -104,8 +104,19 @@ struct Wave {
   void mark(int u) { tile(VALS, u, false, false); }
   void clean(int u) { tile(VALS, u, true, true); }
   void spoil(int) {}
-  bool past() { return weighed + 1 < c.n && c.past[weighed + 1] >> wv & 1; }
+  bool past() { wrong |= kept >= 0; return weighed + 1 < c.n && c.past[weighed + 1] >> wv & 1; }
   void raise() {}
+  // (a maximum kept in a place of the wave's own while a turn is made; in set 0)
+  int kept = -1;
+  bool far() { return weighed + 1 < c.n && c.far[weighed + 1] >> wv & 1; }
+  void near(int u) {
+    wrong |= kept >= 0 || scored[0] != u;
+    kept = u;
+  }
+  void back(int u) {
+    wrong |= kept != u || weighed != u;
+    kept = -1;
+  }
   void last() { scored[0] = scored[1]; }
 };
 
@@ -113,12 +124,13 @@ int main(int argc, char** argv) {
   std::mt19937 g(std::atoi(argv[1]));
   long races = 0, stale = 0, wrong = 0, cases = 0, looks = 0, plain = 0;
   for (int it = 0; it < 4000; ++it) {
-    Case c{1 + (int)(g() %% 7), 1 << g() %% 3, (g() & 1) != 0, {}, {}, {}};
+    Case c{1 + (int)(g() %% 7), 1 << g() %% 3, (g() & 1) != 0, {}, {}, {}, {}};
     const int kind = g() %% 4;
     for (int u = 0; u < c.n; ++u) {
       c.shared.push_back(kind == 0 || (kind != 1 && (g() & 1)));
       c.odd.push_back(kind < 3 && g() %% 3 ? 0 : g() & 15);
       c.past.push_back(g() & 1 ? 0 : g() & 15);
+      c.far.push_back(g() %% 3 ? 0 : g() & 15);
     }
     Memory mem;
     std::vector<int> passed;
@@ -127,7 +139,7 @@ int main(int argc, char** argv) {
       PromptTurns<Wave>(wave, c.n).run();
       for (int two = 0; two < 2; ++two)
         for (int r = 0; r < wave.rows; ++r) wave.at(KEYS, two, r, true, -1), wave.at(VALS, two, r, true, -1);
-      wrong += wave.wrong || wave.weighed != c.n - 1 || !wave.there;
+      wrong += wave.wrong || wave.weighed != c.n - 1 || wave.kept >= 0 || !wave.there;
       passed.push_back(wave.passed);
     }
     for (int p : passed) wrong += p != passed[0];   // (a barrier that not all waves reach)
