@@ -389,6 +389,10 @@ hipError_t launch_rope_rows(hipStream_t s, int dtype, int cache, const RopeRows&
 namespace {
 
 constexpr int PA_WAVES = 4, PA_THREADS = 64 * PA_WAVES;
+// What f16 weights are scaled up by, so that their range costs little (a power of 2): times 2^14, or for 4 bits in the difference
+// itself, an instruction less. A maximum from 2^25 on is a multiple of 4 or more, by which the difference is rounded: of 14 that
+// may make 16, which f16 does not hold; of 7 at most 8. It costs 2^-32 of the largest weight.
+constexpr float F16_SCALE = 14.0f, KV4_UP = 7.0f;
 
 // A kv head's G query heads: `split` groups of `hg` (the last may have fewer).
 struct PagedPlan {
@@ -878,7 +882,7 @@ struct PaWave {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         if constexpr (KV4) {
-          x[t][r] = __builtin_amdgcn_exp2f(x[t][r] - (ref - 14.0f));
+          x[t][r] = __builtin_amdgcn_exp2f(x[t][r] - (ref - KV4_UP));
         } else {
           x[t][r] = __builtin_amdgcn_exp2f(x[t][r] - ref);
           if constexpr (CT == BB_F16) x[t][r] *= 16384.0f;
@@ -1073,7 +1077,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_waves(HDP, KV4)) k_paged_attn(P
 
   typedef PaWave<CT, NQ, NP, HDP, UNI, KV4, MOD> Wave;
   Wave w(kv, lane);
-  const float up = CT == BB_F16 ? 14.0f : 0.0f;
+  const float up = KV4 ? KV4_UP : CT == BB_F16 ? F16_SCALE : 0.0f;
   bool lds_read = false;
   int turn = 0;
   // the run's pairs: group grp of sequence s, whose cost begins at lo
@@ -1283,7 +1287,7 @@ hipError_t launch_paged_attn(hipStream_t st, int n_cu, int cache, const PagedQue
   if (e != hipSuccess || !pl.join) return e;
   const int blocks_of_row = (kv.hd + 4 * PJ_PIECES - 1) / (4 * PJ_PIECES);
   BB_LAUNCH(k_paged_join, dim3(sq.n_seqs, pl.n_groups, pl.hg * blocks_of_row), dim3(PJ_THREADS), 0, st, q, kv.hd,
-            blocks_of_row, pl, cache == BB_F16 || cache == BB_KV4 ? 14.0f : 0.0f);
+            blocks_of_row, pl, cache == BB_KV4 ? KV4_UP : cache == BB_F16 ? F16_SCALE : 0.0f);
   return hipGetLastError();
 }
 

@@ -126,3 +126,18 @@ def test_large_scores(gpu_ctx, order, dt, ct):
                 check_levels(gpu_ctx, pool, history, q, dt, [130, 30], scale, **kw)
             for n in (2, 9, 17):
                 check_levels(gpu_ctx, few, behind, q[:n], dt, [n], scale)
+
+
+@pytest.mark.parametrize("order", ["any", "rising", "falling"])
+@pytest.mark.parametrize("dt,ct", [(F16, F16), (BF16, BF16), (F16, KV4), (F32, KV4), (F32, F32), (F32, BF16)])
+def test_large_scores_of_single_tokens(gpu_ctx, order, dt, ct):
+    """The same, one token each."""
+    print("large, single", order, dt, ct, flush=True)
+    for hd, heads in ((64, 4), (128, 2), (256, 2)):
+        pool, history = levels(gpu_ctx, 140, [140, 33, 1400], ct, 1, hd, order)
+        q = torch.zeros(3, heads, hd)
+        q[:, :, 5] = 8.0 * 2.0 ** -torch.arange(heads)   # (heads that pass 2^16 at different positions)
+        q = q.to(TYPES[dt])
+        for scale in (1e4, 2e4, 3e6, 5e6, 1.1e7, 1.7e7, 3e7, 1e8, 1e10, -1e10, 1e20, 1e30, 5e36):
+            for kw in (dict(), dict(window=20), dict(slopes=torch.zeros(heads))):
+                check_levels(gpu_ctx, pool, history, q, dt, [1, 1, 1], scale, single=True, **kw)
