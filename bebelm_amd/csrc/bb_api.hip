@@ -3176,10 +3176,10 @@ int bb_paged_prompt_attention(bb_ctx* c, const bb_paged_kv* kv, const bb_paged_s
     const size_t want = prompt_ws(c, kv, nh, B, T);
     if (loc == BB_LOC_HOST && pq->seq_start && B > 0) need_starts(pq->seq_start, B, T);
     need_seqs(kv, sq, loc, [&](size_t s, int64_t n) {
-      // (pages of positions between a prefix and the first token's window may be missing)
+      // (pages of positions between a prefix and the first token's window may be missing; all of them where there is no token)
       const int64_t bring = tokens_of(pq->seq_start, s, n), prefix = pq->prefix ? std::min<int64_t>(pq->prefix[s], n) : 0;
       need(prefix >= 0, BB_ERR_RANGE, "a prefix must not be negative");
-      for (size_t i = 0; i * ps < (size_t)prefix; ++i) {
+      for (size_t i = 0; bring > 0 && i * ps < (size_t)prefix; ++i) {
         const int32_t pg = sq->page_table[s * sq->table_stride + i];
         need(pg >= 0 && pg < kv->view.n_pages, BB_ERR_RANGE,
              "sequence " + std::to_string(s) + ": page " + std::to_string(pg) + " is not in the pool");
