@@ -359,7 +359,7 @@ hipError_t launch_rope_rows(hipStream_t s, int dtype, int cache, const RopeRows&
 //
 // 64 sequences of 8192, 32 query on 8 kv heads of 128, f16: 357 to 368 us, 5.8 to 6.0 TB/s; one sequence of 9001, of 64,
 // bf16: 13 us, of which 4 are the second launch and 3 pass until the first keys are asked for. The former over 4 bits, 604 MB
-// of cache: 132 to 138 us, 4.4 to 4.6 TB/s; there the vector instructions that make f16 values of codes and weights of
+// of cache: 130 to 142 us, 4.3 to 4.6 TB/s; there the vector instructions that make f16 values of codes and weights of
 // scores (some 310 a tile of 32 positions) take as long as the bytes. Scores with a cap or a bias: 34 ragged
 // sequences of up to 16384, 8 kv heads of 64, bf16, 28 us, capped or not.
 //

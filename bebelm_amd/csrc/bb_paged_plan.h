@@ -80,9 +80,10 @@ constexpr int PA_ALONE = 2;
 constexpr int PA_LONG = 16;
 
 // Waves of a SIMD that fit: 128, 256, 512 registers each. (The forms with heads of up to 64 fill theirs: f32 queries on a
-// bf16 cache, and all 16-bit caches of odd pages, spill 12 to 24 of them, at a pair's beginning and end, none in the loop
-// over tiles. 4-bit tiles take fewer, and
-// heads of 256 fit twice; three waves with heads of 128, 64 sequences of 8192, 141 us, two 138.)
+// bf16 cache and all 16-bit caches of odd pages spill 12 to 24 of them, capped or biased scores 2 to 30, at a pair's beginning
+// and end; in the loop over tiles only 3, of f32 queries with such scores on a bf16 cache of odd pages. 4-bit tiles take fewer, and
+// heads of 256 fit twice, but with f32 queries: 56 to 63 are spilled, 13 to 32 brought back for each tile, not measured
+// against one wave; three waves with heads of 128, 64 sequences of 8192, 141 us, two 138.)
 constexpr int pa_waves(int hdp, bool four = false) { return hdp == 64 ? 4 : hdp == 128 || four ? 2 : 1; }
 constexpr int pa_class(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 inline int blocks_at_once(int n_cu, int hd, bool four = false) { return n_cu * pa_waves(pa_class(hd), four); }

@@ -1,6 +1,6 @@
 // bb_paged_prompt.h — attention of several new tokens per sequence over a paged cache: prompts, chunks of
 // them, drafts to verify (include/bebelm_moe.h states the operator). The reference has no counterpart. The kernels, which
-// one source file for each type of cache instantiates (bb_prompt_*.hip), and how a launch is cut.
+// one source file for each type of cache instantiates (bb_prompt_*.hip); bb_paged_prompt.hip cuts a launch.
 #ifndef BB_PAGED_PROMPT_H
 #define BB_PAGED_PROMPT_H
 #include <algorithm>
@@ -150,7 +150,7 @@ struct PpWave {
   size_t kv_off;
   int len, prefix;
   int i, lo;                  // the row's token's index, and what it sees first
-  int i0, i1, lo1;            // of the wave's first row, of its last
+  int i0, lo1;                // the index of the wave's first row, what its last sees first
   float c, slope;             // what scores are multiplied by; the bias of a step of distance (base 2)
   float m, l;
   v4u q[NQ][HDP / 16];
@@ -842,14 +842,14 @@ struct PpBlock {
 // have something to be hidden get them as bits.
 //
 // What bounds it: matrix instructions and, nearly added to them, the vector ones (a weight is a multiply-add, an
-// exponential, a sum and half a conversion). 16384 tokens from the first, 32 heads on 8 of 128, bf16: 2.26 to 2.32 ms, 950 to
-// 975 TFLOP/s, where large products reach 1120 (keys by way of registers 8.3 ms; straight to LDS, with a maximum that
+// exponential, a sum and half a conversion). 16384 tokens from the first, 32 heads on 8 of 128, bf16: 2.23 to 2.49 ms by the card, 880 to
+// 985 TFLOP/s, where large products reach 1120 (keys by way of registers 8.3 ms; straight to LDS, with a maximum that
 // seldom moves, 3.3; a tile's weights made while the next one's scores are, 2.8; without spills 2.7; a page's
-// rows by one address and their loads behind the first products 2.3). 5003 tokens of 7 ragged prompts, 13 tiles a block: 112 us,
-// 620 TFLOP/s; blocks begin and end (6 us) two or three times a CU, and the last are alone. Heads of 256 fill the
+// rows by one address and their loads behind the first products 2.3). 5003 tokens of 7 ragged prompts, 13 tiles a block: 111 to 119 us,
+// 590 to 630 TFLOP/s; blocks begin and end (6 us) two or three times a CU, and the last are alone. Heads of 256 fill the
 // registers of a SIMD with one wave, whose vector, matrix and LDS work then follow each other: 6001 tokens with a cap and a
-// window of 1024, f16, 192 to 200 us, 420 TFLOP/s. From 4 bits (2048 tokens after 8192, heads of 128) 380 us, 745
-// TFLOP/s: 150 vector instructions a tile and wave make f16 of the codes. 5 tokens of each of 16 sequences after 8192: 108 us,
+// window of 1024, f16, 191 to 203 us, 410 to 440 TFLOP/s. From 4 bits (2048 tokens after 8192, heads of 128) 374 to 408 us, 690 to
+// 755 TFLOP/s: 150 vector instructions a tile and wave make f16 of the codes. 5 tokens of each of 16 sequences after 8192: 108 us,
 // 5.0 TB/s of cache.
 template <int CT, int NQ, int NP, int HDP, int WR, int SRC>
 __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, SRC>::WAVES))
@@ -909,7 +909,6 @@ __global__ void __launch_bounds__(PP_THREADS, (PpShape<CT, NQ, NP, HDP, WR, SRC>
   w.i = token_index(w.len, end, t);
   w.lo = first_seen(w.i, pq.window);
   w.i0 = __builtin_amdgcn_readlane(w.i, 0);
-  w.i1 = __builtin_amdgcn_readlane(w.i, 31);
   w.lo1 = __builtin_amdgcn_readlane(w.lo, 31);
   w.slope = pq.slopes ? pq.slopes[head] * LOG2E : 0.0f;
   w.c = fabsf(pq.scale) * LOG2E;

@@ -437,7 +437,8 @@ class PagedKv:
         return n.value
 
     def prompt_workspace(self, n_heads, n_seqs, n_tokens):
-        """Bytes of device memory that kernels.paged_prompt_attention needs (its workspace argument)."""
+        """Bytes of device memory that kernels.paged_prompt_attention needs for a batch of these numbers (its workspace
+        argument; 0: none). Fewer tokens may need more: a tensor for several batches is of the largest answer."""
         n = ctypes.c_size_t()
         check(lib().bb_paged_prompt_attention_workspace(self.ctx.handle, self.handle, n_heads, n_seqs, n_tokens,
                                                         ctypes.byref(n)))

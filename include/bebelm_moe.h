@@ -502,9 +502,11 @@ int bb_paged_attention(bb_ctx* ctx, const bb_paged_kv* kv, const bb_paged_seqs* 
  * infinite). Weights are rounded to the cache's type (F16 for BB_KV4) where out is
  * F16 on an F16 or BB_KV4 cache, or BF16; elsewhere they keep what out can hold. On an F16 or BB_KV4 cache, elements of a
  * query below 2^-38 of the largest of its head may count as 0. Capped scores are off by some steps of themselves, and by 2^-21
- * of the cap (lse too) where weights are rounded and the cap is at most 64. workspace: as in bb_paged_attention, of
- * bb_paged_prompt_attention_workspace's answer (which may be 0: then a captured call needs none). Equal calls give equal
- * bits. One call takes n_tokens·n_heads / 32 + n_seqs·n_kv_heads below 2^24 (BB_ERR_RANGE: cut the batch). */
+ * of the cap (lse too) where weights are rounded and the cap is at most 64. With seq_start NULL and no window behind a
+ * prefix, roundings and sums are those of bb_paged_attention. workspace: as in bb_paged_attention, of
+ * bb_paged_prompt_attention_workspace's answer for the call's own numbers (which may be 0: then a captured call needs none;
+ * fewer tokens may need more, their keys being shared out to more blocks, so that a workspace for several batches is of the
+ * largest of their answers). Equal calls give equal bits. One call takes n_tokens·n_heads / 32 + n_seqs·n_kv_heads below 2^24 (BB_ERR_RANGE: cut the batch). */
 typedef struct {
   size_t n_tokens;
   uint32_t dtype; /* of q and out */
