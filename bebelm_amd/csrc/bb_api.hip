@@ -2727,6 +2727,9 @@ int64_t tokens_of(const int32_t* start, size_t s, int64_t n) {
   return bring;
 }
 
+// (times log2(e) it has to stay finite: a score of 0 would be NaN)
+void need_scale(float scale) { need(std::fabs(scale) < 0x1p127f, BB_ERR_ARG, "scale must be finite, below 2^127"); }
+
 size_t prompt_ws(bb_ctx* c, const bb_paged_kv* kv, size_t n_heads, size_t n_seqs, size_t n_tokens) {
   const size_t n_kv = (size_t)kv->view.n_kv;
   need(n_heads >= 1 && n_heads % n_kv == 0, BB_ERR_ARG, "n_heads must be a multiple of n_kv_heads");
@@ -3056,7 +3059,7 @@ int bb_paged_attention(bb_ctx* c, const bb_paged_kv* kv, const bb_paged_seqs* sq
     need_seqs(kv, sq, loc, [&](size_t, int64_t n) {
       return pq->window > 0 && pq->window < (size_t)n ? n - (int64_t)pq->window : 0;
     });
-    need(std::isfinite(pq->scale), BB_ERR_ARG, "scale must be finite");
+    need_scale(pq->scale);
     if (B == 0) return;
     need(bb::paged_attn_fits((int)B, (int)nh, kv->view.n_kv, sq->max_pages * (size_t)kv->view.page_size), BB_ERR_RANGE,
          "sequences times heads times positions beyond what one call counts");
@@ -3188,7 +3191,7 @@ int bb_paged_prompt_attention(bb_ctx* c, const bb_paged_kv* kv, const bb_paged_s
       return bring == 0 ? n : pq->window > 0 && pq->window < reach ? (int64_t)(reach - pq->window) : 0;
     });
     if (!pq->seq_start) need(T == B, BB_ERR_SHAPE, "without seq_start every sequence has one token");
-    need(std::isfinite(pq->scale), BB_ERR_ARG, "scale must be finite");
+    need_scale(pq->scale);
     need(std::isfinite(pq->cap) && pq->cap >= 0.0f, BB_ERR_ARG, "cap must be finite and not negative");
     if (T == 0 || B == 0) return;
     need(pq->q && pq->out, BB_ERR_ARG, "null query or output");

@@ -460,8 +460,8 @@ int bb_paged_read(bb_ctx* ctx, const bb_paged_kv* kv, const bb_paged_seqs* seqs,
 /* One query token per sequence over its cached positions (attention_decode for every sequence):
  *   out[s][h] = sum_j softmax_j(scale·q[s][h]·k[j][h / (n_heads/n_kv_heads)])·v[j][...]
  * for max(0, lens[s] - window) <= j < lens[s] (window 0: all). q and out [n_seqs][n_heads][head_dim]
- * (heads side by side, sequences q_stride and out_stride apart, not overlapping); scale 0 means
- * 1/sqrt(head_dim). lse (f32[n_seqs][n_heads], or NULL) gets the natural logarithm of the softmax sums. A
+ * (heads side by side, sequences q_stride and out_stride apart, not overlapping); scale (below 2^127)
+ * 0 means 1/sqrt(head_dim). lse (f32[n_seqs][n_heads], or NULL) gets the natural logarithm of the softmax sums. A
  * sequence with no position to attend to, and a head all of whose scores are -inf, gets zeros and
  * -inf. workspace: device memory of workspace_bytes >= bb_paged_attention_workspace's answer, for this
  * call alone while it runs; NULL takes the context's, which a captured call may not (a graph keeps the
@@ -495,8 +495,8 @@ int bb_paged_attention(bb_ctx* ctx, const bb_paged_kv* kv, const bb_paged_seqs* 
  * i = lens[s] - seq_start[s+1] + t and sees the j below lens[s] with i - window < j <= i (window 0: j <= i), and those
  * below prefix[s] (i32[n_seqs], or NULL) wherever they are: a prefix read in both directions, or with a window the first
  * positions that stay in reach. What lies between a prefix and a window's first position makes no difference. q and out
- * [n_tokens][n_heads][head_dim] (heads side by side, tokens q_stride and out_stride apart, not overlapping); scale 0 means
- * 1/sqrt(head_dim); lse, as in bb_paged_attention, f32[n_tokens][n_heads] or NULL. A token that sees nothing gets zeros and
+ * [n_tokens][n_heads][head_dim] (heads side by side, tokens q_stride and out_stride apart, not overlapping); scale (below 2^127)
+ * 0 means 1/sqrt(head_dim); lse, as in bb_paged_attention, f32[n_tokens][n_heads] or NULL. A token that sees nothing gets zeros and
  * -inf; of padding nothing is written. A value that is not finite makes not finite what it reaches, and nothing else: the
  * rows that do not see it are as if it were not there (of an F32 cache, magnitudes from 3.39e38 on may count as
  * infinite). Weights are rounded to the cache's type (F16 for BB_KV4) where out is
